@@ -52,7 +52,8 @@ enum {
 
 enum { UMSX_ACT_SILU = 0, UMSX_ACT_SWIGLU_OAI = 1 }; /* F32Activation, tools/engine/f32_experts.hpp:11 */
 
-enum { UMSX_DTYPE_F32 = 0, UMSX_DTYPE_BF16 = 1 };
+/* F16 and E4M3 are types of the products over caller-owned weights below; the layer entry points take F32 and BF16 */
+enum { UMSX_DTYPE_F32 = 0, UMSX_DTYPE_BF16 = 1, UMSX_DTYPE_F16 = 2, UMSX_DTYPE_E4M3 = 3 };
 
 enum { UMSX_PROJ_GATE_UP = 0, UMSX_PROJ_GATE = 1, UMSX_PROJ_UP = 2, UMSX_PROJ_DOWN = 3 };
 
@@ -372,6 +373,64 @@ void umsx_gguf_experts_free(umsx_gguf_experts *experts);
  * Mxfp4NativeCudaDown's constructor, quantized_cuda.hpp:38-50). */
 umsx_status umsx_moe_create_gguf(const umsx_moe_desc *desc, const char *first_shard, int layer, int device,
                                  size_t reserve_bytes, umsx_moe **out);
+
+/* ---- Products over caller-owned expert weights (no counterpart in the reference, whose experts are
+ * ggml-quantised) --------------------------------------------------------------------------------
+ * For experts that are not MXFP4 or Q8_0: 16-bit weights that are trained or not quantised yet, and
+ * e4m3 weights with one fp32 scale per block of 128 x 128.  All pointers are device pointers of the
+ * calling thread's current device; the calls are asynchronous on `stream`, allocate nothing, keep
+ * nothing between calls, synchronise nothing and can be captured into a graph.  Calls on several
+ * streams or threads do not disturb one another.  Strides count elements; the last dimension of every
+ * matrix is contiguous.  Bases and strides that are multiples of 16 bytes run on the tensor cores, any
+ * others on a slower kernel.  An output must not overlap an input.
+ *
+ * Rows are grouped by expert: rows offsets[e] .. offsets[e+1] - 1 belong to expert e (offsets: int32
+ * [experts + 1], on the device, ascending; values outside 0..rows are clamped to it).  Groups may be
+ * empty; rows before the first and behind the last group are neither read nor written.
+ * experts <= 1024; n, k <= 2^24; rows <= 2^31 - 16.
+ *
+ * umsx_group_rows: the grouping of a router's picks.  ids [tokens][top_k] as umsx_route gives them; ids
+ * outside 0..experts-1 (the -1 of masked picks) belong to no group.  The sort is stable (rows of one
+ * expert in the order of tokens, then ranks).  offsets [experts + 1]; row_token [tokens * top_k]: the
+ * token of every row (0 behind the last group); row_of_job [tokens][top_k]: the row of every pick, -1
+ * for one that belongs to no group. */
+umsx_status umsx_group_rows(const int32_t *ids, int tokens, int top_k, int experts, int32_t *offsets,
+                            int32_t *row_token, int32_t *row_of_job, umsx_stream stream);
+
+/* out[r] = w[e] x[r] for every row r of expert e: x [rows][k], w [experts][n][k] (both BF16 or both F16,
+ * `dtype`), out [rows][n] (F32, BF16 or F16).  fp32 accumulation, rounded once.  The product of
+ * umsx_mul_mat_id for 16-bit weights and rows in expert order. */
+umsx_status umsx_grouped_mm(const void *x, int64_t ldx, const void *w, int64_t ldw, int64_t w_stride,
+                            const int32_t *offsets, int experts, int64_t rows, int n, int k, int dtype, void *out,
+                            int64_t ldo, int out_dtype, umsx_stream stream);
+/* Its gradients: dx[r] = sum_n dy[r][n] w[e][n] for the rows of the groups (dx [rows][k]), and
+ * dw[e] = sum over the rows r of expert e of dy[r] x[r]^T (dw [experts][n][k]; zero for an expert without
+ * rows).  Sums run in a fixed order: the same call gives the same bits. */
+umsx_status umsx_grouped_mm_dx(const void *dy, int64_t lddy, const void *w, int64_t ldw, int64_t w_stride,
+                               const int32_t *offsets, int experts, int64_t rows, int n, int k, int dtype, void *dx,
+                               int64_t lddx, int out_dtype, umsx_stream stream);
+umsx_status umsx_grouped_mm_dw(const void *dy, int64_t lddy, const void *x, int64_t ldx, const int32_t *offsets,
+                               int experts, int64_t rows, int n, int k, int dtype, void *dw, int64_t lddw,
+                               int64_t dw_stride, int out_dtype, umsx_stream stream);
+
+/* Values to e4m3 codes with an fp32 scale per block of block_rows x 128 values: block_rows 1 for the rows
+ * of activations, 128 for weight matrices; blocks at the right and lower edge may be smaller.
+ * scale = max(amax / 448, 2^-126) with amax over the block's finite values, code = the e4m3 value nearest
+ * to x / scale (ties to even); inf and NaN become the NaN code.  x [matrices][rows][cols] (F32, BF16 or
+ * F16), q the same shape, one byte each; scale of block (i, j) of matrix m at scales[m * s_stride +
+ * i * s_row + j * s_blk]. */
+umsx_status umsx_fp8_quantize(const void *x, int64_t ldx, int64_t x_stride, int x_dtype, int matrices, int64_t rows,
+                              int cols, int block_rows, void *q, int64_t ldq, int64_t q_stride, float *scales,
+                              int64_t s_row, int64_t s_blk, int64_t s_stride, umsx_stream stream);
+
+/* umsx_grouped_mm for e4m3 operands: x [rows][k] with a scale per row and block of 128 of k
+ * (xs[r * xs_row + b * xs_blk]), w [experts][n][k] with a scale per 128 x 128 block
+ * (ws[e * ws_stride + (i / 128) * ws_row + b * ws_blk]); out[r][i] = sum_b xs ws (sum over the block's
+ * products, fp32) in fp32, rounded once.  offsets NULL with experts = 1: one matrix product of all rows. */
+umsx_status umsx_fp8_grouped_mm(const void *x, int64_t ldx, const float *xs, int64_t xs_row, int64_t xs_blk,
+                                const void *w, int64_t ldw, int64_t w_stride, const float *ws, int64_t ws_row,
+                                int64_t ws_blk, int64_t ws_stride, const int32_t *offsets, int experts, int64_t rows,
+                                int n, int k, void *out, int64_t ldo, int out_dtype, umsx_stream stream);
 
 /* Number of this library's kernels launched by the calling thread since load (graph replays count
  * every kernel they contain). */

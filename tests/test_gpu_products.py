@@ -1,0 +1,504 @@
+"""Row grouping, ragged 16-bit products with their gradients, and block-scaled e4m3 products against plain
+64-bit forms (needs a B200).
+
+Tolerances, element by element: a sum of C products accumulated in fp32 in any order is off by at most
+C * 2^-23 * sum|a b| (one ulp for every addition, truncated or rounded; products of 16- and 8-bit operands are exact in
+fp32), the scales of an e4m3 product add three more roundings per block, and the result is rounded once to the
+output's type: eps / 2 of the value, or half the smallest subnormal step.
+"""
+import pytest
+
+from tests.helpers import U
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16, E4M3 = torch.float32, torch.bfloat16, torch.float16, torch.float8_e4m3fn
+SUB = {F32: 2.0 ** -149, BF16: 2.0 ** -133, F16: 2.0 ** -24}
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _rand(gen, *shape, dtype=BF16):
+    return torch.randn(shape, generator=gen, device="cuda").to(dtype)
+
+
+def _close(got, want, size, terms, what):
+    """got (rounded) against want and size = sum|a b| (both fp64)."""
+    half = torch.finfo(got.dtype).eps / 2
+    acc = (terms + 8) * 2.0 ** -23 * size
+    tol = acc + half * (want.abs() + acc) + SUB[got.dtype]
+    off = (got.double() - want).abs()
+    bad = ~(off <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((off / tol)[bad].max())} x tolerance"
+
+
+def _offsets(counts, start=0):
+    return torch.tensor([start] + [start + sum(counts[:i + 1]) for i in range(len(counts))], dtype=torch.int32, device="cuda")
+
+
+def _spans(offsets):
+    o = offsets.tolist()
+    return list(enumerate(zip(o[:-1], o[1:])))
+
+
+# group sizes, rows before the first and behind the last group
+RAGGED = [
+    ([1], 0, 0),
+    ([0, 3, 0, 1, 0], 0, 0),
+    ([0, 0, 0], 0, 5),
+    ([7, 9, 16, 17, 1], 2, 3),
+    ([1] * 8 + [0] * 120, 0, 0),
+    ([33, 0, 129, 64, 255, 256, 257, 1], 0, 70),
+    ([700, 13], 1, 0),
+]
+# n, k: tensor-core sizes, sizes that end inside a tile, odd ones that only the general kernel takes
+WIDTHS = [(128, 64), (256, 256), (384, 512), (72, 200), (136, 1032), (17, 33), (1, 1), (1000, 8), (8, 136), (130, 128)]
+
+
+def _case(counts, before, behind, n, k, dtype, seed, pad=0):
+    """x, dy, w, offsets; rows outside the groups hold NaN, which must reach nothing.  pad: columns between rows."""
+    g = _gen(seed)
+    rows = before + sum(counts) + behind
+    x = torch.full((rows, k + pad), float("nan"), dtype=dtype, device="cuda")[:, :k]
+    dy = torch.full((rows, n + pad), float("nan"), dtype=dtype, device="cuda")[:, :n]
+    a, b = before, before + sum(counts)
+    x[a:b] = _rand(g, b - a, k, dtype=dtype)
+    dy[a:b] = _rand(g, b - a, n, dtype=dtype)
+    w = torch.empty(len(counts), n, k + pad, dtype=dtype, device="cuda")[:, :, :k]
+    w.copy_(_rand(g, len(counts), n, k, dtype=dtype))
+    return x, dy, w, _offsets(counts, before)
+
+
+def _check_all(counts, before, behind, n, k, dtype, out, seed, pad=0):
+    x, dy, w, off = _case(counts, before, behind, n, k, dtype, seed, pad)
+    rows = x.shape[0]
+    y = torch.full((rows, n), 7.0, dtype=out, device="cuda")
+    dx = torch.full((rows, k), -3.0, dtype=out, device="cuda")
+    dw = torch.full((len(counts), n, k), float("nan"), dtype=out, device="cuda")
+    assert U.grouped_mm(x, w, off, out=y) is y
+    assert U.grouped_mm_dx(dy, w, off, out=dx) is dx
+    assert U.grouped_mm_dw(dy, x, off, out=dw) is dw
+    a, b = before, before + sum(counts)
+    for t, keep in ((y, 7.0), (dx, -3.0)):
+        assert torch.all(t[:a] == keep) and torch.all(t[b:] == keep), "rows outside the groups were written"
+    for e, (i, j) in _spans(off):
+        xe, dye, we = x[i:j].double(), dy[i:j].double(), w[e].double()
+        _close(y[i:j], xe @ we.T, xe.abs() @ we.abs().T, k, f"y of expert {e}")
+        _close(dx[i:j], dye @ we, dye.abs() @ we.abs(), n, f"dx of expert {e}")
+        _close(dw[e], dye.T @ xe, dye.abs().T @ xe.abs(), j - i, f"dw of expert {e}")
+
+
+@pytest.mark.parametrize("n,k", WIDTHS)
+@pytest.mark.parametrize("ragged", range(len(RAGGED)))
+def test_products_and_gradients(ragged, n, k):
+    dtype = BF16 if (ragged + n) % 2 else F16
+    out = (F32, dtype, BF16)[(ragged + k) % 3]
+    _check_all(*RAGGED[ragged], n, k, dtype, out, seed=100 * ragged + n)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("out", [F32, BF16, F16])
+@pytest.mark.parametrize("pad", [0, 8, 3])
+def test_types_and_strides(dtype, out, pad):
+    _check_all([40, 0, 5, 300], 1, 2, 192, 320, dtype, out, seed=7, pad=pad)
+
+
+def test_wide_outputs_and_many_experts():
+    """1024 experts, most of them empty; and an n above any tile count of one wave."""
+    counts = [0] * 1024
+    for e in range(0, 1024, 37):
+        counts[e] = 1 + e % 5
+    _check_all(counts, 0, 0, 64, 64, BF16, BF16, seed=3)
+    _check_all([65, 3], 0, 0, 20000, 64, BF16, F32, seed=4)
+
+
+def test_gradients_against_differences():
+    """dx and dw are the derivatives of sum(y * dy): directional differences of the 64-bit product of nudged operands."""
+    x, dy, w, off = _case([5, 0, 12], 0, 0, 40, 24, BF16, seed=11)
+    dx, dw = U.grouped_mm_dx(dy, w, off, out_dtype=F32).double(), U.grouped_mm_dw(dy, x, off).double()
+
+    def loss(xd, wd):
+        return sum((xd[i:j] @ wd[e].T * dy[i:j].double()).sum() for e, (i, j) in _spans(off))
+
+    g = _gen(5)
+    vx, vw = torch.randn(x.shape, generator=g, device="cuda").double(), torch.randn(w.shape, generator=g, device="cuda").double()
+    xd, wd, h = x.double(), w.double(), 2.0 ** -10
+    # the loss is linear in each operand: central differences are exact but for fp64 rounding
+    want_x = (loss(xd + h * vx, wd) - loss(xd - h * vx, wd)) / (2 * h)
+    want_w = (loss(xd, wd + h * vw) - loss(xd, wd - h * vw)) / (2 * h)
+    # each gradient entry is off by at most (terms + 8) 2^-23 sum|a b| + half an ulp
+    ax = sum((dy[i:j].double().abs() @ w[e].double().abs() * vx[i:j].abs()).sum() for e, (i, j) in _spans(off))
+    aw = sum((dy[i:j].double().abs().T @ x[i:j].double().abs() * vw[e].abs()).sum() for e, (i, j) in _spans(off))
+    assert abs((dx * vx).sum() - want_x) <= 50 * 2.0 ** -23 * ax
+    assert abs((dw * vw).sum() - want_w) <= 50 * 2.0 ** -23 * aw
+
+
+def test_non_finite_values_stay_in_their_rows():
+    x, dy, w, off = _case([20, 300, 7], 0, 0, 128, 256, BF16, seed=2)
+    clean = U.grouped_mm(x, w, off)
+    x2 = x.clone()
+    x2[25, 3], x2[319, 0] = float("nan"), float("inf")
+    y = U.grouped_mm(x2, w, off)
+    rows = [r for r in range(x.shape[0]) if r not in (25, 319)]
+    assert torch.equal(y[rows], clean[rows]) and torch.isnan(y[25]).all() and not torch.isfinite(y[319]).any()
+    dw, dw2 = U.grouped_mm_dw(dy, x, off), U.grouped_mm_dw(dy, x2, off)
+    assert torch.equal(dw[0], dw2[0]) and torch.equal(dw[2], dw2[2])
+    assert torch.isnan(dw2[1][:, 3]).all() and torch.equal(dw[1][:, 4:], dw2[1][:, 4:])
+    w2 = w.clone()
+    w2[1] = float("nan")
+    y = U.grouped_mm(x, w2, off)
+    assert torch.equal(y[:20], clean[:20]) and torch.equal(y[320:], clean[320:]) and torch.isnan(y[20:320]).all()
+
+
+def test_bad_offsets_stay_inside_the_matrices():
+    """Offsets outside 0..rows are clamped, descending ones give empty groups: nothing outside is touched."""
+    x, dy, w, _ = _case([30, 30], 0, 0, 64, 64, BF16, seed=9)
+    for o in ([0, 30, 1000], [-50, 30, 60], [60, 20, 60], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1]):
+        off = torch.tensor(o, dtype=torch.int32, device="cuda")
+        y = torch.zeros(62, 64, dtype=F32, device="cuda")
+        U.grouped_mm(x, w, off, out=y[1:61])
+        U.grouped_mm_dw(dy, x, off)
+        U.grouped_mm_dx(dy, w, off)
+        torch.cuda.synchronize()
+        assert not y[0].any() and not y[61].any()
+
+
+# ---- e4m3 ------------------------------------------------------------------------------------------
+
+
+def _round_e4m3(v):
+    a = v.abs()
+    step = torch.exp2(torch.floor(torch.log2(torch.clamp(a, min=2.0 ** -6))) - 3)
+    return torch.sign(v) * torch.clamp(torch.round(a / step) * step, max=448.0)
+
+
+def _blocks(v):
+    return -(-v // 128)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("shape", [(1, 1), (3, 128), (5, 130), (128, 64), (129, 257), (300, 2880), (2, 131, 200), (3, 1, 77)])
+def test_quantize(dtype, block_rows, shape):
+    g = _gen(shape[-1])
+    x = (torch.randn(shape, generator=g, device="cuda") * torch.exp(3 * torch.randn(shape[:-1] + (1,), generator=g, device="cuda")))
+    x = x.to(dtype)
+    x[..., 0] = 0
+    q, s = U.fp8_quantize(x, block_rows)
+    assert q.dtype == E4M3 and q.shape == x.shape and s.shape == shape[:-2] + (-(-shape[-2] // block_rows), _blocks(shape[-1]))
+    rows, cols = shape[-2:]
+    x3, q3, s3 = x.float().reshape(-1, rows, cols), q.float().reshape(-1, rows, cols), s.reshape((-1,) + s.shape[-2:])
+    for i in range(s.shape[-2]):
+        for j in range(s.shape[-1]):
+            xb = x3[:, i * block_rows:(i + 1) * block_rows, j * 128:(j + 1) * 128]
+            # the fp32 divisions, as documented: a 64-bit quotient of fp32 values rounds to fp32 as theirs does
+            # (torch divides an fp32 CUDA tensor by a number through its reciprocal, which is one ulp off)
+            fine = torch.isfinite(xb)  # some rows overflow fp16
+            want = torch.clamp(torch.where(fine, xb, 0).abs().amax((1, 2)).double() / 448.0, min=2.0 ** -126).float()
+            assert torch.equal(s3[:, i, j], want)
+            qb = q3[:, i * block_rows:(i + 1) * block_rows, j * 128:(j + 1) * 128]
+            exact = _round_e4m3((torch.where(fine, xb, 0).double() / want.double()[:, None, None]).float().double()).float()
+            assert torch.equal(torch.isnan(qb), ~fine) and torch.equal(torch.where(fine, qb, 0), exact)
+        if i >= 8:
+            break
+
+
+def test_quantize_edges():
+    """Zeros, subnormals, the largest floats, and non-finite values beside finite ones."""
+    x = torch.zeros(6, 256, device="cuda")
+    x[1, :128] = 1e-45
+    x[2] = torch.finfo(F32).max
+    x[3, 5], x[3, 6], x[3, 7], x[3, 8] = float("inf"), float("nan"), -float("inf"), 2.0
+    x[4, 200] = -448.0
+    x[5] = 2.0 ** -126
+    q, s = U.fp8_quantize(x)
+    assert torch.isfinite(s).all() and (s >= 2.0 ** -126).all()
+    assert not q[0].float().any() and not q[1].float().any()
+    assert (q[2].float() == 448).all()
+    assert torch.isnan(q[3, 5:8].float()).all() and q[3, 8].float() == 448 and not q[3, 9:].float().any()
+    assert s[4, 1] == 1 and q[4, 200].float() == -448
+    assert (q[5].float() == 1).all()
+
+
+def test_quantize_strides_and_given_outputs():
+    g = _gen(1)
+    big = torch.randn(70, 3 * 400, generator=g, device="cuda", dtype=F32).to(BF16)
+    x = big[3:53, 405:405 + 300]  # rows that start at odd offsets
+    q0, s0 = U.fp8_quantize(x.contiguous())
+    store = torch.full((52, 320), 99, dtype=torch.uint8, device="cuda")
+    q = store[1:51, 7:307].view(E4M3)
+    scales = torch.zeros(50, 5, device="cuda")[:, 1:4]
+    U.fp8_quantize(x, q=q, scales=scales)
+    assert torch.equal(q.float(), q0.float()) and torch.equal(scales, s0)
+    assert (store[0] == 99).all() and (store[51] == 99).all() and (store[:, :7] == 99).all() and (store[:, 307:] == 99).all()
+
+
+def _fp8_case(counts, before, behind, n, k, seed, pad=0):
+    g = _gen(seed)
+    rows, e = before + sum(counts) + behind, len(counts)
+    x = torch.full((rows, k + pad), 0x7F, dtype=torch.uint8, device="cuda")[:, :k].view(E4M3)  # NaN outside the groups
+    a, b = before, before + sum(counts)
+    x[a:b] = (100 * torch.randn(b - a, k, generator=g, device="cuda")).clamp(-448, 448).to(E4M3)
+    w = torch.empty(e, n, k + pad, dtype=torch.uint8, device="cuda")[:, :, :k].view(E4M3)
+    w.copy_((100 * torch.randn(e, n, k, generator=g, device="cuda")).clamp(-448, 448).to(E4M3))
+    xs = torch.exp(torch.randn(_blocks(k), rows, generator=g, device="cuda")).t() * 0.01
+    ws = torch.exp(torch.randn(e, _blocks(n), _blocks(k), generator=g, device="cuda")) * 0.001
+    return x, xs, w, ws, _offsets(counts, before)
+
+
+def _fp8_want(x, xs, w, ws):
+    j = torch.arange(x.shape[1], device="cuda") // 128
+    i = torch.arange(w.shape[0], device="cuda") // 128
+    xd, wd = x.to(F32).double() * xs.double()[:, j], w.to(F32).double() * ws.double()[i][:, j]
+    return xd @ wd.T, xd.abs() @ wd.abs().T
+
+
+FP8_WIDTHS = [(128, 128), (256, 512), (384, 64), (72, 208), (136, 1040), (17, 33), (1, 1), (1000, 16), (130, 2880), (2816, 144)]
+
+
+@pytest.mark.parametrize("n,k", FP8_WIDTHS)
+@pytest.mark.parametrize("ragged", range(len(RAGGED)))
+def test_fp8_grouped(ragged, n, k):
+    counts, before, behind = RAGGED[ragged]
+    x, xs, w, ws, off = _fp8_case(counts, before, behind, n, k, seed=10 * ragged + n)
+    out = (BF16, F32, F16)[(ragged + n) % 3]
+    y = torch.full((x.shape[0], n), 5.0, dtype=out, device="cuda")
+    assert U.fp8_grouped_mm(x, xs, w, ws, off, out=y) is y
+    a, b = before, before + sum(counts)
+    assert (y[:a] == 5).all() and (y[b:] == 5).all()
+    for e, (i, j) in _spans(off):
+        want, size = _fp8_want(x[i:j], xs[i:j], w[e], ws[e])
+        _close(y[i:j], want, size, k, f"expert {e}")
+
+
+@pytest.mark.parametrize("rows", [0, 1, 2, 8, 9, 31, 64, 200, 1025])
+@pytest.mark.parametrize("n,k", [(128, 128), (700, 1056), (24, 129), (2816, 2048)])
+@pytest.mark.parametrize("pad", [0, 16])
+def test_fp8_dense(rows, n, k, pad):
+    x, xs, w, ws, _ = _fp8_case([rows], 0, 0, n, k, seed=rows + n, pad=pad)
+    for scales in (xs, xs.contiguous()):  # either layout of the rows' scales
+        for out in (F32, BF16):
+            y = U.fp8_mm(x, scales, w[0], ws[0], out_dtype=out)
+            assert y.shape == (rows, n) and y.dtype == out
+            if rows:
+                want, size = _fp8_want(x, xs, w[0], ws[0])
+                _close(y, want, size, k, "y")
+
+
+def test_fp8_non_finite_codes_stay_in_their_rows():
+    x, xs, w, ws, off = _fp8_case([20, 300, 7], 0, 0, 128, 256, seed=2)
+    clean = U.fp8_grouped_mm(x, xs, w, ws, off)
+    bad = x.view(torch.uint8).clone()
+    bad[25, 3] = 0x7F
+    y = U.fp8_grouped_mm(bad.view(E4M3), xs, w, ws, off)
+    rows = [r for r in range(x.shape[0]) if r != 25]
+    assert torch.equal(y[rows], clean[rows]) and torch.isnan(y[25]).all()
+
+
+# ---- grouping -----------------------------------------------------------------------------------------
+
+
+def _group_want(ids, experts):
+    flat = ids.flatten().long().cpu()
+    key = torch.where((flat < 0) | (flat >= experts), experts, flat)
+    order = torch.argsort(key, stable=True)
+    off = torch.zeros(experts + 1, dtype=torch.int64)
+    off[1:] = torch.bincount(key, minlength=experts + 1)[:experts].cumsum(0)
+    rows = int(off[-1])
+    token = order // ids.shape[1]
+    token[rows:] = 0
+    job = torch.full((flat.numel(),), -1, dtype=torch.int64)
+    job[order[:rows]] = torch.arange(rows)
+    return off, token, job.view(ids.shape)
+
+
+@pytest.mark.parametrize("tokens,top_k,experts", [(0, 4, 8), (1, 1, 1), (1, 8, 128), (5, 3, 7), (16, 8, 128), (128, 8, 60),
+                                                  (129, 8, 60), (1000, 1, 1024), (4096, 8, 1024), (513, 6, 64), (70000, 8, 256)])
+@pytest.mark.parametrize("kind", ["even", "masked", "one", "none"])
+def test_group_rows(tokens, top_k, experts, kind):
+    g = _gen(tokens + experts)
+    ids = torch.randint(0, experts, (tokens, top_k), generator=g, device="cuda", dtype=torch.int32)
+    if kind == "masked":
+        ids = torch.where(torch.rand(ids.shape, generator=g, device="cuda") < 0.6, -1, ids)
+        if tokens > 3:
+            ids[1, 0], ids[2, 0], ids[3, 0] = experts, 2 ** 31 - 1, -2 ** 31
+    elif kind == "one":
+        ids[:] = experts - 1
+    elif kind == "none":
+        ids[:] = -1
+    got = U.group_rows(ids, experts)
+    for name, a, b in zip(("offsets", "row_token", "row_of_job"), got, _group_want(ids, experts)):
+        assert a.dtype == torch.int32
+        assert torch.equal(a.cpu().long(), b), name
+
+
+# ---- use -------------------------------------------------------------------------------------------------
+
+
+def test_refusals():
+    x, dy, w, off = _case([3, 4], 0, 0, 64, 32, BF16, seed=1)
+    xq, xs, wq, ws, _ = _fp8_case([3, 4], 0, 0, 64, 32, seed=1)
+    bad = [
+        lambda: U.grouped_mm(x.float(), w, off), lambda: U.grouped_mm(x, w.half(), off), lambda: U.grouped_mm(x[:, :16], w, off),
+        lambda: U.grouped_mm(x, w, off[:2]), lambda: U.grouped_mm(x, w, off.long()), lambda: U.grouped_mm(x, w, off.cpu()),
+        lambda: U.grouped_mm(x.t(), w, off), lambda: U.grouped_mm(x, w.transpose(1, 2), off),
+        lambda: U.grouped_mm(x, w, off, out_dtype=torch.float64), lambda: U.grouped_mm(x, w, off, out=torch.empty(7, 63, device="cuda")),
+        lambda: U.grouped_mm(x, w, off, out=torch.empty(7, 64)), lambda: U.grouped_mm(x[:1].expand(7, 32), w, off),
+        lambda: U.grouped_mm(x, w[:1].expand(2, 64, 32), off),
+        lambda: U.grouped_mm_dx(x, w, off), lambda: U.grouped_mm_dw(dy[:3], x, off), lambda: U.grouped_mm_dw(dy, x, off[0]),
+        lambda: U.grouped_mm_dw(dy, x.half(), off), lambda: U.grouped_mm_dw(dy, x, off[:1]),
+        lambda: U.fp8_mm(x, xs, wq[0], ws[0]), lambda: U.fp8_mm(xq, xs.double(), wq[0], ws[0]), lambda: U.fp8_mm(xq, xs[:3], wq[0], ws[0]),
+        lambda: U.fp8_mm(xq, xs, wq, ws), lambda: U.fp8_grouped_mm(xq, xs, wq, ws, None), lambda: U.fp8_grouped_mm(xq, xs, wq, ws[:1], off),
+        lambda: U.fp8_quantize(x[0]), lambda: U.fp8_quantize(x, 64), lambda: U.fp8_quantize(x.t()), lambda: U.fp8_quantize(xq),
+        lambda: U.fp8_quantize(x, q=xq[:3]), lambda: U.fp8_quantize(x, scales=xs[:3]),
+        lambda: U.group_rows(off, 4), lambda: U.group_rows(off[None].long(), 4), lambda: U.group_rows(off[None], 0),
+        lambda: U.group_rows(off[None], 2000), lambda: U.group_rows(torch.zeros(4, 4, dtype=torch.int32, device="cuda").t()[:, :2], 4),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(U.UmsxError) as e:
+            call()
+        assert e.value.status == U.EINVAL, i
+
+
+def _expert_layer(x, ids, weights, gate_up, down, experts):
+    """An expert layer as a user builds it from the e4m3 operators; returns its output [tokens, width] in fp32."""
+    off, row_token, row_of_job = U.group_rows(ids, experts)
+    xq, xs = U.fp8_quantize(x)
+    xs_rows = xs.t()[:, row_token].t()
+    h = U.fp8_grouped_mm(xq.view(torch.uint8)[row_token].view(E4M3), xs_rows, *gate_up, off)
+    gate, up = h.float().chunk(2, dim=1)
+    a = (torch.nn.functional.silu(gate) * up).to(BF16)
+    y = U.fp8_grouped_mm(*U.fp8_quantize(a), *down, off, out_dtype=F32)
+    jobs = y[row_of_job.clamp(min=0)]
+    jobs = torch.where((row_of_job < 0)[..., None], 0.0, jobs)
+    return U.combine(jobs, weights)
+
+
+def test_expert_layer_of_e4m3_weights():
+    """Router, grouping, quantiser, both products and the combine in a row, as they are used; against the same layer in
+    64 bits on the operands' exact values.  The activations are rounded to bf16 once and to e4m3 twice on the way, which
+    the 64-bit layer repeats, so that what is left is the accumulation and rounding of each step."""
+    T, H, I, E, K = 37, 256, 192, 8, 2
+    g = _gen(21)
+    x = _rand(g, T, H)
+    rw = torch.randn(E, H, generator=g, device="cuda") * 0.1
+    ids, weights, _ = U.route_static(x, rw, None, E, K, U.ROUTE_SOFTMAX_TOPK_NORM)
+    ids[5, 1] = -1
+    gu = U.fp8_quantize(torch.randn(E, 2 * I, H, generator=g, device="cuda") * 0.05, 128)
+    dn = U.fp8_quantize(torch.randn(E, H, I, generator=g, device="cuda") * 0.05, 128)
+    got = _expert_layer(x, ids, weights, gu, dn, E)
+    xq, xs = U.fp8_quantize(x)
+    want = torch.zeros(T, H, dtype=torch.float64, device="cuda")
+    tol = torch.zeros(T, H, dtype=torch.float64, device="cuda")
+    for t in range(T):
+        for r in range(K):
+            e = int(ids[t, r])
+            if e < 0:
+                continue
+            h, _ = _fp8_want(xq[t:t + 1], xs[t:t + 1], gu[0][e], gu[1][e])
+            a = (torch.nn.functional.silu(h[:, :I]) * h[:, I:])
+            y, size = _fp8_want(*U.fp8_quantize(a.to(BF16).contiguous()), dn[0][e], dn[1][e])
+            wt = float(weights[t, r])
+            want[t] += wt * y[0]
+            # h is rounded to bf16 on the way (2^-8 of gate and of up; silu's slope is at most 1.1 and |silu| <= |gate|,
+            # so a is off by at most 3.2 * 2^-8 of itself plus the rounding of a, 2^-8), and a code may then land one
+            # step off, 2^-3 of the value: every term of y is off by at most 2^-3 + 5 * 2^-8 of itself.
+            tol[t] += wt * size[0] * (2.0 ** -3 + 5 * 2.0 ** -8)
+    off = (got.double() - want).abs()
+    assert (off <= tol).all()
+    assert (got.double() - want).norm() <= 0.05 * want.norm()
+
+
+def test_layer_of_16_bit_weights_with_gradients():
+    """Grouping, forward and both gradients in a row: the chain rule through two products, against autograd in 64 bits."""
+    T, H, I, E, K = 50, 128, 96, 6, 2
+    g = _gen(4)
+    ids = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(t))[:K] for t in range(T)]).int().cuda()
+    ids[3, 0] = -1
+    off, row_token, row_of_job = U.group_rows(ids, E)
+    x = _rand(g, T, H)
+    w1, w2 = _rand(g, E, I, H) * 0.125, _rand(g, E, H, I) * 0.125
+    xr = x[row_token]
+    h = U.grouped_mm(xr, w1, off, out_dtype=F32)
+    hb = h.to(BF16)
+    y = U.grouped_mm(hb, w2, off, out_dtype=F32)
+    dy = _rand(g, T * K, H)
+    dh = U.grouped_mm_dx(dy, w2, off)
+    dw2 = U.grouped_mm_dw(dy, hb, off)
+    dw1 = U.grouped_mm_dw(dh, xr, off)
+    n = int(off[-1])
+    for e, (i, j) in _spans(off):
+        xe, he, dye, dhe = (t[i:j].double() for t in (xr, hb, dy, dh))
+        _close(h[i:j], xe @ w1[e].double().T, xe.abs() @ w1[e].double().abs().T, H, "h")
+        _close(y[i:j], he @ w2[e].double().T, he.abs() @ w2[e].double().abs().T, I, "y")
+        _close(dh[i:j], dye @ w2[e].double(), dye.abs() @ w2[e].double().abs(), H, "dh")
+        _close(dw2[e], dye.T @ he, dye.abs().T @ he.abs(), j - i, "dw2")
+        _close(dw1[e], dhe.T @ xe, dhe.abs().T @ xe.abs(), j - i, "dw1")
+    assert n == T * K - 1
+
+
+def test_same_bits_twice_and_on_another_stream():
+    x, dy, w, off = _case([300, 0, 41, 77], 0, 3, 256, 384, BF16, seed=6)
+    xq, xs, wq, ws, _ = _fp8_case([300, 0, 41, 77], 0, 3, 256, 384, seed=6)
+
+    def run(stream=None):
+        y = torch.zeros(x.shape[0], 256, dtype=F32, device="cuda")
+        z = torch.zeros_like(y)
+        dx = torch.zeros(x.shape[0], 384, dtype=F32, device="cuda")
+        torch.cuda.synchronize()
+        return (U.grouped_mm(x, w, off, out=y, stream=stream), U.grouped_mm_dx(dy, w, off, out=dx, stream=stream),
+                U.grouped_mm_dw(dy, x, off, stream=stream), U.fp8_grouped_mm(xq, xs, wq, ws, off, out=z, stream=stream))
+
+    first = run()
+    side, side2 = torch.cuda.Stream(), torch.cuda.Stream()
+    a, b = run(side), run(side2)  # two calls at once
+    torch.cuda.synchronize()
+    for p, q, r in zip(first, a, b):
+        assert torch.equal(p, q) and torch.equal(p, r)
+
+
+def test_captured_and_replayed():
+    """All operators in one graph, replayed on new inputs and new group sizes in the same buffers."""
+    E, n, k, T, K = 6, 192, 256, 40, 2
+    g = _gen(8)
+    ids = torch.randint(0, E, (T, K), generator=g, device="cuda", dtype=torch.int32)
+    x, w = _rand(g, T, k), _rand(g, E, n, k)
+    dy = _rand(g, T * K, n)
+    wq, ws = U.fp8_quantize(w, 128)
+
+    def step():
+        off, tok, job = U.group_rows(ids, E)
+        xr = x[tok]
+        y = U.grouped_mm(xr, w, off, out_dtype=F32)
+        dx = U.grouped_mm_dx(dy, w, off)
+        dw = U.grouped_mm_dw(dy, xr, off)
+        xq, xs = U.fp8_quantize(xr)
+        z = U.fp8_grouped_mm(xq, xs, wq, ws, off)
+        return [off, tok, job, y, dx, dw, z]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (1, 2, 3):
+        g2 = _gen(seed)
+        ids.copy_(torch.randint(0, E if seed < 3 else 1, (T, K), generator=g2, device="cuda", dtype=torch.int32))
+        x.copy_(_rand(g2, T, k))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+
+
+def test_launches_are_counted():
+    x, dy, w, off = _case([3], 0, 0, 64, 64, BF16, seed=1)
+    before = U.kernel_launches()
+    U.grouped_mm(x, w, off)
+    U.fp8_quantize(x)
+    assert U.kernel_launches() >= before + 2

@@ -6,4 +6,5 @@ The directory name is not a Python identifier, so __graft_entry__.load_package()
 registers it as `umsx_b200`.
 """
 from . import configs, umsx  # noqa: F401
-from .umsx import MoeLayer, MoeStack, UmsxError, combine, kernel_launches, lib, load_gguf_experts  # noqa: F401
+from .umsx import (MoeLayer, MoeStack, UmsxError, combine, fp8_grouped_mm, fp8_mm, fp8_quantize, group_rows,  # noqa: F401
+                   grouped_mm, grouped_mm_dw, grouped_mm_dx, kernel_launches, lib, load_gguf_experts)

@@ -1,0 +1,58 @@
+// Ragged products over the caller's own expert weights: what the entry points
+// (umsx_products.cu) hand to the kernels.
+//
+// Every direction is one form: out[r][f] = sum_c R[r][c] * F[f][c].
+//   forward  r: rows of the group, f: n, c: k    R = x,        F = w[e]
+//   dx       r: rows of the group, f: k, c: n    R = dy,       F = w[e] transposed
+//   dw       r: n, f: k, c: rows of the group    R = dy transposed, F = x transposed
+// so that f is contiguous in the output and w is read as it lies in memory.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/umsx.h"
+
+namespace umsx {
+
+enum ProductMode { kForward = 0, kGradInput = 1, kGradWeight = 2 };
+
+constexpr int kMaxGroups = 1024;
+constexpr int kScaleBlock = 128;  // values that share one scale of an e4m3 operand
+
+struct Product {
+    ProductMode mode;
+    int dtype;      // operands: UMSX_DTYPE_BF16, _F16 or _E4M3
+    int out_dtype;  // UMSX_DTYPE_F32, _BF16 or _F16
+    int groups;
+    int64_t rows;  // of x and dy
+    int n, k;
+    const int32_t *offsets;  // [groups + 1], or null: one group of all rows
+    const void *x, *dy, *w;  // [rows][k], [rows][n], [groups][n][k]; strides in elements, the last is 1
+    int64_t ldx, lddy, ldw, w_stride;
+    const float *xs, *ws;  // e4m3: xs(row, block of k), ws(group, block of n, block of k)
+    int64_t xs_row, xs_blk, ws_row, ws_blk, ws_group;
+    void *out;  // forward [rows][n], dx [rows][k], dw [groups][n][k]
+    int64_t ldo, out_stride;
+
+    int features() const { return mode == kForward ? n : k; }
+};
+
+#ifdef __CUDACC__
+// Rows [a, b) of group g.  Offsets are clamped to the matrix, so that wrong ones cannot lead outside it.
+__device__ __forceinline__ void group_bounds(const int32_t *offsets, int g, int64_t rows, int &a, int &b) {
+    if (!offsets) {
+        a = 0;
+        b = (int)rows;
+        return;
+    }
+    const int top = (int)rows;
+    a = min(max(__ldg(offsets + g), 0), top);
+    b = min(max(__ldg(offsets + g + 1), a), top);
+}
+#endif
+
+// Each returns the number of kernels launched, -1 when the driver refuses something.
+int launch_product_any(const Product &p, int sms, cudaStream_t s);
+
+}  // namespace umsx

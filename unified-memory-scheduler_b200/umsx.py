@@ -7,6 +7,8 @@ Mirrors the reference's expert interfaces (paths inside appatalks/unified-memory
   MoeLayer.expert_down_q8 Mxfp4NativeCudaDown::execute (tools/engine/quantized_cuda.cu:413-453)
   MoeLayer.mul_mat_id     ggml MUL_MAT_ID with -1 masked ids (hybrid patch :617-621)
   combine                 ExpertPlan::execute's rank-order combine (tools/engine/expert_dispatch.cpp:77-87)
+and adds the products over caller-owned 16-bit and e4m3 expert weights (group_rows, grouped_mm and its
+gradients, fp8_quantize, fp8_mm, fp8_grouped_mm), which have no counterpart there.
 Errors raise UmsxError carrying the C status, as the reference raises
 std::invalid_argument / std::runtime_error.  Device buffers are torch CUDA
 tensors (plumbing only); there is no CPU fallback: without libumsx.so or a GPU
@@ -25,7 +27,8 @@ STATUS_NAMES = ["OK", "EINVAL", "ENOTRESIDENT", "EOOM", "ETIMEOUT", "EDEVICE", "
 QUANT_Q8_0, QUANT_MXFP4 = 8, 39
 ROUTE_TOPK_SOFTMAX, ROUTE_SOFTMAX_TOPK_NORM, ROUTE_SOFTMAX_TOPK = 0, 1, 2
 ACT_SILU, ACT_SWIGLU_OAI = 0, 1
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16, DTYPE_E4M3 = range(4)
+SCALE_BLOCK = 128  # values of a row that share one scale of an e4m3 operand
 BANK_LFU, BANK_LRU = 0, 1
 BANK_STAT_NAMES = ("dispatches", "demands", "hits", "misses", "admissions", "evictions", "transient", "halvings",
                    "upload_bytes")
@@ -45,6 +48,8 @@ EXPORTS = ["umsx_moe_create", "umsx_moe_create_synthetic", "umsx_moe_destroy", "
            "umsx_ep_prefill_connect", "umsx_ep_prefill_forward", "umsx_ep_prefill_forward_host", "umsx_ep_prefill_loads",
            "umsx_ep_prefill_status", "umsx_ep_prefill_destroy",
            "umsx_gguf_load_experts", "umsx_gguf_experts_free", "umsx_moe_create_gguf",
+           "umsx_group_rows", "umsx_grouped_mm", "umsx_grouped_mm_dx", "umsx_grouped_mm_dw", "umsx_fp8_quantize",
+           "umsx_fp8_grouped_mm",
            "umsx_kernel_launches", "umsx_last_error", "umsx_version"]
 
 
@@ -84,7 +89,7 @@ def lib():
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(f"{LIB_PATH} is not built; run __graft_entry__.build()")
     L = C.CDLL(LIB_PATH)
-    vp, i32, sz, u64 = C.c_void_p, C.c_int, C.c_size_t, C.c_uint64
+    vp, i32, i64, sz, u64 = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_uint64
     sig = {
         "umsx_moe_create": (i32, [C.POINTER(Desc), C.POINTER(Weights), i32, sz, C.POINTER(vp)]),
         "umsx_moe_create_synthetic": (i32, [C.POINTER(Desc), u64, C.c_uint32, C.c_float, C.c_float, C.c_float, i32, sz,
@@ -134,6 +139,13 @@ def lib():
         "umsx_gguf_load_experts": (i32, [C.c_char_p, i32, vp, i32, i32, C.POINTER(GgufExpertsC)]),
         "umsx_gguf_experts_free": (None, [C.POINTER(GgufExpertsC)]),
         "umsx_moe_create_gguf": (i32, [C.POINTER(Desc), C.c_char_p, i32, i32, sz, C.POINTER(vp)]),
+        "umsx_group_rows": (i32, [vp, i32, i32, i32, vp, vp, vp, vp]),
+        "umsx_grouped_mm": (i32, [vp, i64, vp, i64, i64, vp, i32, i64, i32, i32, i32, vp, i64, i32, vp]),
+        "umsx_grouped_mm_dx": (i32, [vp, i64, vp, i64, i64, vp, i32, i64, i32, i32, i32, vp, i64, i32, vp]),
+        "umsx_grouped_mm_dw": (i32, [vp, i64, vp, i64, vp, i32, i64, i32, i32, i32, vp, i64, i64, i32, vp]),
+        "umsx_fp8_quantize": (i32, [vp, i64, i64, i32, i32, i64, i32, i32, vp, i64, i64, vp, i64, i64, i64, vp]),
+        "umsx_fp8_grouped_mm": (i32, [vp, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, i64, vp, i32, i64, i32, i32,
+                                      vp, i64, i32, vp]),
         "umsx_kernel_launches": (u64, []),
         "umsx_last_error": (C.c_char_p, []),
         "umsx_version": (i32, []),
@@ -221,6 +233,225 @@ def route_static(x, router_w, router_b, experts: int, top_k: int, routing: int, 
     check(lib().umsx_route_static(_ptr(x), _dtype_code(x), T, _ptr(router_w), _ptr(router_b), H, experts, top_k,
                                   routing, routed_scale, _ptr(ids), _ptr(w), _ptr(counts), _stream(stream)))
     return ids, w, counts
+
+
+# ---- products over caller-owned expert weights --------------------------------------------------------
+
+_CODES = {}  # torch dtype -> UMSX_DTYPE_*, filled on first use (torch is imported lazily)
+
+
+def _codes():
+    if not _CODES:
+        import torch
+        _CODES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16,
+                       torch.float8_e4m3fn: DTYPE_E4M3})
+    return _CODES
+
+
+def _need(ok: bool, message: str):
+    if not ok:
+        raise UmsxError(EINVAL, message)
+
+
+def _matrix(name, t, dim, dtypes, like=None):
+    """Checks one CUDA operand: its rank, type, contiguous last dimension, and the device of `like`."""
+    _need(t.is_cuda, f"{name} must be a CUDA tensor")
+    _need(like is None or t.device == like.device, f"{name} must be on the device of the other tensors")
+    _need(t.dim() == dim, f"{name} must have {dim} dimensions, got {t.dim()}")
+    _need(t.dtype in dtypes, f"{name} has type {t.dtype}")
+    _need(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}'s last dimension must be contiguous")
+
+
+def _offsets_arg(offsets, experts, like):
+    import torch
+    _need(offsets.is_cuda and offsets.device == like.device, "offsets must be on the device of the other tensors")
+    _need(offsets.dtype == torch.int32 and offsets.shape == (experts + 1,) and offsets.is_contiguous(),
+          f"offsets must be a contiguous int32 tensor of {experts + 1} values")
+
+
+def _ld(t, dim=-2):
+    """Row (or matrix) stride; a dimension of one has no stride of its own, so it gets the least one."""
+    if t.shape[dim] > 1:
+        return t.stride(dim)
+    return t.shape[-1] if dim == -2 else t.shape[-1] + (t.shape[-2] - 1) * _ld(t)
+
+
+def _out_arg(name, out, shape, dtype, like, default):
+    """`out`, checked, or a new tensor of `dtype` (`default` where that is None)."""
+    import torch
+    if out is None:
+        dtype = default if dtype is None else dtype
+        _need(dtype in (torch.float32, torch.bfloat16, torch.float16), f"{name} cannot have type {dtype}")
+        return torch.empty(shape, dtype=dtype, device=like.device)
+    _need(dtype is None or dtype == out.dtype, f"{name} has type {out.dtype}, not {dtype}")
+    _matrix(name, out, len(shape), (torch.float32, torch.bfloat16, torch.float16), like)
+    _need(tuple(out.shape) == tuple(shape), f"{name} must have shape {tuple(shape)}, got {tuple(out.shape)}")
+    return out
+
+
+class _On:
+    """The tensors' device as the current one for a call, with the given stream or that device's current one."""
+
+    __slots__ = ("before", "index", "stream")
+
+    def __init__(self, t, stream):
+        import torch
+        self.index = t.device.index
+        self.before = torch.cuda.current_device()
+        self.stream = C.c_void_p(torch.cuda.current_stream(self.index).cuda_stream) if stream is None else _stream(stream)
+
+    def __enter__(self):
+        if self.before != self.index:
+            import torch
+            torch.cuda.set_device(self.index)
+        return self.stream
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            import torch
+            torch.cuda.set_device(self.before)
+
+
+def group_rows(ids, experts: int, stream=None):
+    """Sorts a router's picks into one run of rows per expert (umsx_group_rows).  ids: int32 CUDA
+    [tokens, top_k]; picks outside 0..experts-1 (the -1 of masked ones) belong to no run.  Returns
+    (offsets [experts + 1], row_token [tokens * top_k], row_of_job [tokens, top_k]), all int32:
+    x[row_token] are the rows in expert order, y[row_of_job] the results back in pick order (-1
+    marks a pick without a row)."""
+    import torch
+    _matrix("ids", ids, 2, (torch.int32,))
+    _need(ids.is_contiguous(), "ids must be contiguous")
+    _need(1 <= experts <= 1024, "experts must be 1..1024")
+    tokens, top_k = ids.shape
+    offsets = torch.empty(experts + 1, dtype=torch.int32, device=ids.device)
+    row_token = torch.empty(tokens * top_k, dtype=torch.int32, device=ids.device)
+    row_of_job = torch.empty((tokens, top_k), dtype=torch.int32, device=ids.device)
+    with _On(ids, stream) as s:
+        check(lib().umsx_group_rows(ids.data_ptr(), tokens, top_k, experts, offsets.data_ptr(), row_token.data_ptr(),
+                                    row_of_job.data_ptr(), s))
+    return offsets, row_token, row_of_job
+
+
+def grouped_mm(x, w, offsets, out=None, out_dtype=None, stream=None):
+    """out[r] = x[r] @ w[e].T for the rows r of every expert e (umsx_grouped_mm): x [rows, k] and w
+    [experts, n, k] both bfloat16 or both float16, offsets int32 [experts + 1]; out [rows, n] float32,
+    bfloat16 or float16 (default: x's type).  Rows outside the groups are not written."""
+    import torch
+    _matrix("x", x, 2, (torch.bfloat16, torch.float16))
+    _matrix("w", w, 3, (x.dtype,), x)
+    experts, n, k = w.shape
+    _need(x.shape[1] == k, f"x has {x.shape[1]} columns, w has {k}")
+    _offsets_arg(offsets, experts, x)
+    out = _out_arg("out", out, (x.shape[0], n), out_dtype, x, x.dtype)
+    with _On(x, stream) as s:
+        check(lib().umsx_grouped_mm(x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ld(w, -3), offsets.data_ptr(), experts,
+                                    x.shape[0], n, k, _codes()[x.dtype], out.data_ptr(), _ld(out),
+                                    _codes()[out.dtype], s))
+    return out
+
+
+def grouped_mm_dx(dy, w, offsets, out=None, out_dtype=None, stream=None):
+    """The gradient of grouped_mm's rows (umsx_grouped_mm_dx): dx[r] = dy[r] @ w[e], dy [rows, n], w
+    [experts, n, k], dx [rows, k] (default: dy's type).  Rows outside the groups are not written."""
+    import torch
+    _matrix("dy", dy, 2, (torch.bfloat16, torch.float16))
+    _matrix("w", w, 3, (dy.dtype,), dy)
+    experts, n, k = w.shape
+    _need(dy.shape[1] == n, f"dy has {dy.shape[1]} columns, w has {n} rows")
+    _offsets_arg(offsets, experts, dy)
+    out = _out_arg("out", out, (dy.shape[0], k), out_dtype, dy, dy.dtype)
+    with _On(dy, stream) as s:
+        check(lib().umsx_grouped_mm_dx(dy.data_ptr(), _ld(dy), w.data_ptr(), _ld(w), _ld(w, -3), offsets.data_ptr(),
+                                       experts, dy.shape[0], n, k, _codes()[dy.dtype], out.data_ptr(), _ld(out),
+                                       _codes()[out.dtype], s))
+    return out
+
+
+def grouped_mm_dw(dy, x, offsets, out=None, out_dtype=None, stream=None):
+    """The gradient of grouped_mm's weights (umsx_grouped_mm_dw): dw[e] = dy[rows of e].T @ x[rows of e],
+    [experts, n, k] (default: float32); zero for an expert without rows."""
+    import torch
+    _matrix("dy", dy, 2, (torch.bfloat16, torch.float16))
+    _matrix("x", x, 2, (dy.dtype,), dy)
+    _need(dy.shape[0] == x.shape[0], f"dy has {dy.shape[0]} rows, x has {x.shape[0]}")
+    n, k, experts = dy.shape[1], x.shape[1], offsets.shape[0] - 1 if offsets.dim() == 1 else 0
+    _need(experts >= 1, "offsets must hold at least two values")
+    _offsets_arg(offsets, experts, dy)
+    out = _out_arg("out", out, (experts, n, k), out_dtype, dy, torch.float32)
+    with _On(dy, stream) as s:
+        check(lib().umsx_grouped_mm_dw(dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), offsets.data_ptr(), experts,
+                                       dy.shape[0], n, k, _codes()[dy.dtype], out.data_ptr(), _ld(out), _ld(out, -3),
+                                       _codes()[out.dtype], s))
+    return out
+
+
+def fp8_quantize(x, block_rows: int = 1, q=None, scales=None, stream=None):
+    """x [rows, cols] or [matrices, rows, cols] (float32, bfloat16 or float16) as float8_e4m3fn codes with
+    one float32 scale per block of block_rows (1 or 128) x 128 values (umsx_fp8_quantize): (q, scales) with
+    x ~ q * scale.  Scales of rows (block_rows 1) are laid out one block of columns after another, as the
+    products read them: their shape is [.., rows, blocks], their last stride is the long one."""
+    import torch
+    _need(x.dim() in (2, 3), f"x must have 2 or 3 dimensions, got {x.dim()}")
+    _need(block_rows in (1, SCALE_BLOCK), "block_rows must be 1 or 128")
+    _matrix("x", x, x.dim(), (torch.float32, torch.bfloat16, torch.float16))
+    rows, cols = x.shape[-2:]
+    lead, br, bc = tuple(x.shape[:-2]), -(-rows // block_rows), -(-cols // SCALE_BLOCK)
+    if q is None:
+        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
+    _matrix("q", q, x.dim(), (torch.float8_e4m3fn,), x)
+    _need(q.shape == x.shape, f"q must have x's shape {tuple(x.shape)}, got {tuple(q.shape)}")
+    if scales is None:
+        scales = torch.empty(lead + ((bc, br) if block_rows == 1 else (br, bc)), dtype=torch.float32, device=x.device)
+        scales = scales.transpose(-1, -2) if block_rows == 1 else scales
+    _need(scales.is_cuda and scales.device == x.device and scales.dtype == torch.float32,
+          "scales must be float32 and on x's device")
+    _need(tuple(scales.shape) == lead + (br, bc), f"scales must have shape {lead + (br, bc)}, got {tuple(scales.shape)}")
+    m3 = x.dim() == 3
+    with _On(x, stream) as s:
+        check(lib().umsx_fp8_quantize(x.data_ptr(), _ld(x), x.stride(0) if m3 else 0, _codes()[x.dtype],
+                                      x.shape[0] if m3 else 1, rows, cols, block_rows, q.data_ptr(), _ld(q),
+                                      _ld(q, -3) if m3 else 0, scales.data_ptr(), scales.stride(-2), scales.stride(-1),
+                                      scales.stride(0) if m3 else 0, s))
+    return q, scales
+
+
+def _fp8_product(x, xs, w, ws, offsets, out, out_dtype, stream):
+    import torch
+    grouped = offsets is not None
+    _matrix("x", x, 2, (torch.float8_e4m3fn,))
+    _matrix("w", w, 3 if grouped else 2, (torch.float8_e4m3fn,), x)
+    n, k = w.shape[-2:]
+    _need(x.shape[1] == k, f"x has {x.shape[1]} columns, w has {k}")
+    bn, bk = -(-n // SCALE_BLOCK), -(-k // SCALE_BLOCK)
+    for name, t, shape in (("xs", xs, (x.shape[0], bk)), ("ws", ws, tuple(w.shape[:-2]) + (bn, bk))):
+        _need(t.is_cuda and t.device == x.device and t.dtype == torch.float32, f"{name} must be float32 and on x's device")
+        _need(tuple(t.shape) == shape, f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    experts = w.shape[0] if grouped else 1
+    if grouped:
+        _offsets_arg(offsets, experts, x)
+    out = _out_arg("out", out, (x.shape[0], n), out_dtype, x, torch.bfloat16)
+    with _On(x, stream) as s:
+        check(lib().umsx_fp8_grouped_mm(
+            x.data_ptr(), _ld(x), xs.data_ptr(), xs.stride(0), xs.stride(1), w.data_ptr(), _ld(w),
+            _ld(w, -3) if grouped else 0, ws.data_ptr(), ws.stride(-2), ws.stride(-1), ws.stride(0) if grouped else 0,
+            offsets.data_ptr() if grouped else None, experts, x.shape[0], n, k, out.data_ptr(), _ld(out),
+            _codes()[out.dtype], s))
+    return out
+
+
+def fp8_mm(x, xs, w, ws, out=None, out_dtype=None, stream=None):
+    """out = (x * xs) @ (w * ws).T for e4m3 operands (umsx_fp8_grouped_mm without offsets): x [rows, k] with
+    scales xs [rows, ceil(k/128)], w [n, k] with scales ws [ceil(n/128), ceil(k/128)], as fp8_quantize
+    gives them; out [rows, n] (default bfloat16)."""
+    return _fp8_product(x, xs, w, ws, None, out, out_dtype, stream)
+
+
+def fp8_grouped_mm(x, xs, w, ws, offsets, out=None, out_dtype=None, stream=None):
+    """grouped_mm for e4m3 operands (umsx_fp8_grouped_mm): x [rows, k] with scales [rows, ceil(k/128)], w
+    [experts, n, k] with scales [experts, ceil(n/128), ceil(k/128)]; out [rows, n] (default bfloat16).
+    Rows outside the groups are not written."""
+    _need(offsets is not None, "offsets must be given")
+    return _fp8_product(x, xs, w, ws, offsets, out, out_dtype, stream)
 
 
 def load_gguf_experts(first_shard: str, layer: int, ids, dequantize: bool = True) -> dict:
