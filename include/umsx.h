@@ -432,6 +432,11 @@ umsx_status umsx_fp8_grouped_mm(const void *x, int64_t ldx, const float *xs, int
                                 int64_t ws_blk, int64_t ws_stride, const int32_t *offsets, int experts, int64_t rows,
                                 int n, int k, void *out, int64_t ldo, int out_dtype, umsx_stream stream);
 
+/* Status of the products above on the current device: synchronises the stream, then reads and clears the
+ * device's status word.  UMSX_ETIMEOUT if a bounded wait inside one of their kernels gave up since the last
+ * query (after about a second; its output is then not complete), else UMSX_OK. */
+umsx_status umsx_products_status(umsx_stream stream);
+
 /* Number of this library's kernels launched by the calling thread since load (graph replays count
  * every kernel they contain). */
 uint64_t umsx_kernel_launches(void);

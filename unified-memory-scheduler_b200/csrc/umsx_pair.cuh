@@ -1,0 +1,179 @@
+// tcgen05 / TMA building blocks for kernels that run on one CTA or on a CTA pair (CG = 1 or 2), in
+// addition to umsx_tc.cuh.
+//
+// In a pair (a cluster of two CTAs) one MMA of M = 256 takes 128 rows of A and half the rows of B from
+// each CTA's shared memory, at the same offsets, and leaves 128 rows of D in each CTA's tensor memory.
+// The even CTA (the leader) issues it; the barriers that its operands complete live with the leader.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "umsx_device.cuh"
+#include "umsx_tc.cuh"
+
+namespace umsx {
+namespace tc {
+
+template <int CG>
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t *dst_smem, uint32_t ncols) {
+    if constexpr (CG == 1) {
+        tmem_alloc(dst_smem, ncols);
+        tmem_relinquish();
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)), "r"(ncols)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+}
+template <int CG>
+__device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t ncols) {
+    if constexpr (CG == 1) tmem_dealloc(taddr, ncols);
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+
+enum MmaKind { kKindF16 = 0, kKindF8 = 1 };
+
+// D (+)= A * B^T for one slice of 32 bytes of K; issued by one thread (of the leader).
+template <int CG, MmaKind KIND>
+__device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+#define UMSX_MMA(group, kind, mask)                                                                              \
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                               \
+                 "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), \
+                 "l"(b_desc), "r"(idesc), "r"(accumulate)                                                        \
+                 : "memory")
+    if constexpr (CG == 1 && KIND == kKindF16) UMSX_MMA("1", "f16", );
+    else if constexpr (CG == 2 && KIND == kKindF16) UMSX_MMA("2", "f16", );
+    else if constexpr (CG == 1) UMSX_MMA("1", "f8f6f4", );
+    else UMSX_MMA("2", "f8f6f4", );
+#undef UMSX_MMA
+}
+
+// Arrive on `bar` (of both CTAs of a pair, at the same offset) once every MMA issued so far has completed.
+template <int CG>
+__device__ __forceinline__ void pair_commit(uint64_t *bar) {
+    if constexpr (CG == 1) mma_commit(bar);
+    else
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+                smem_u32(bar)),
+            "h"((uint16_t)3)
+            : "memory");
+}
+
+// The leader's copy of a shared-memory object, as a shared::cluster address.
+__device__ __forceinline__ uint32_t leader_addr(const void *p) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+    return a;
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync_all() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+// Tiled TMA loads into this CTA that complete on the barrier at shared::cluster address `bar` (this CTA's, or its leader's).
+template <int CG>
+__device__ __forceinline__ void pair_tma_2d(void *dst, const void *tmap, int x, int y, uint32_t bar) {
+    if constexpr (CG == 1)
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+                     "[%4];" ::"r"(smem_u32(dst)),
+                     "l"(tmap), "r"(x), "r"(y), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+                     "{%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+                     "l"(tmap), "r"(x), "r"(y), "r"(bar)
+                     : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void pair_tma_3d(void *dst, const void *tmap, int x, int y, int z, uint32_t bar) {
+    if constexpr (CG == 1)
+        asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+                     "%4}], [%5];" ::"r"(smem_u32(dst)),
+                     "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
+                     "{%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+                     "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
+                     : "memory");
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle, 1024-byte atoms of eight 128-byte lines.
+//   K-major:  a line is 128 bytes of K of one row; atoms of eight rows follow one another
+//   MN-major: a line is 64 16-bit values of M (or N) at one k; atoms of eight k follow one another,
+//             the next 64 values of M (or N) start `block` bytes on
+__device__ __forceinline__ uint64_t operand_desc(const void *p, bool mn_major, uint32_t block) {
+    const uint64_t addr = smem_u32(p);
+    return ((addr & 0x3FFFFull) >> 4) | ((uint64_t)(mn_major ? block >> 4 : 1u) << 16) | (64ull << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+
+// Instruction descriptor: fp32 accumulators; a_fmt, b_fmt: kind::f16 0 f16, 1 bf16; kind::f8f6f4 0 e4m3.
+__host__ __device__ constexpr uint32_t operand_idesc(int fmt, bool a_mn, bool b_mn, int M, int N) {
+    return (1u << 4) | ((uint32_t)fmt << 7) | ((uint32_t)fmt << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
+           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// 32 consecutive fp32 columns of this warp's 32 TMEM lanes; complete after tmem_wait_ld(r).
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+}
+// The loads so far are complete; `r` is an operand so that no use of it moves above the wait.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+          "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+          "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+          "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+        :
+        : "memory");
+}
+
+// ---- bounded waits -----------------------------------------------------------------------------
+//
+// About a second; then the wait marks its CTA as given up (every later wait of the CTA returns at once, so
+// that the kernel ends) and records it in `err`.
+constexpr long long kPairWaitCycles = 2000000000ll;
+
+__device__ __forceinline__ bool pair_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up, uint32_t *err) {
+    const uint32_t a = smem_u32(bar);
+    long long t0 = 0;
+    while (true) {
+        uint32_t done;
+        asm volatile(
+            "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+            : "=r"(done)
+            : "r"(a), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if (*gave_up) return false;
+        const long long t = clock64();
+        if (!t0) t0 = t;
+        if (t - t0 > kPairWaitCycles) {
+            *gave_up = 1;
+            atomicOr(err, 1u);
+            return false;
+        }
+    }
+}
+
+}  // namespace tc
+}  // namespace umsx

@@ -193,7 +193,8 @@ umsx_status run_product(const Product &p, umsx_stream stream) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return fail(UMSX_EDEVICE, std::string("device query: ") + cudaGetErrorString(e));
-    const int n = launch_product_any(p, sms, static_cast<cudaStream_t>(stream));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int n = product_tc_takes(p) ? launch_product_tc(p, sms, s) : launch_product_any(p, sms, s);
     if (n < 0) return fail(UMSX_EDEVICE, "the product's kernel could not be set up");
     record_launches((uint64_t)n);
     e = cudaGetLastError();
@@ -281,6 +282,17 @@ umsx_status umsx_fp8_grouped_mm(const void *x, int64_t ldx, const float *xs, int
     if (rows == 0) return UMSX_OK;
     if (!x || !xs || !w || !ws || !out) return fail(UMSX_EINVAL, "null buffer");
     return run_product(p, stream);
+}
+
+umsx_status umsx_products_status(umsx_stream stream) {
+    uint32_t *word = product_err_word(), v = 0;
+    if (!word) return fail(UMSX_EDEVICE, "the device's status word has no address");
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    cudaError_t e = cudaMemcpyAsync(&v, word, sizeof v, cudaMemcpyDeviceToHost, s);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(s);
+    if (e == cudaSuccess && v) e = cudaMemsetAsync(word, 0, sizeof v, s);
+    if (e != cudaSuccess) return fail(UMSX_EDEVICE, std::string("products status: ") + cudaGetErrorString(e));
+    return v ? fail(UMSX_ETIMEOUT, "a bounded wait of a product's kernel gave up: its output is not complete") : UMSX_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,442 @@
+// Ragged products of 16-bit operands on the tensor cores (tcgen05), forward and both gradients.
+//
+// out[r][f] = sum_c R[r][c] F[f][c] with the FEATURES as the MMA's M (128 per CTA, TMEM lanes) and the
+// group's ROWS as its N.  N goes in steps of 16 (a CTA pair: 32), so a group of 140 rows costs 144 and not 256:
+// with the rows as M, ragged groups would be padded to 128.  The rows of a group are split into equal
+// tiles of at most 256.
+//
+//   forward  F = w (K-major), R = x (K-major)           contraction k
+//   dx       F = w (MN-major: k is contiguous), R = dy  contraction n
+//   dw       F = x, R = dy, both MN-major               contraction: the group's rows
+//
+// One persistent CTA (pair) per SM (pair); CTA i takes tiles i, i + grid, ... of the list (group, feature
+// tile, row tile), which every CTA derives from the offsets, so there is no scheduler state and the order of
+// sums is fixed.  Roles: warp 0 TMA, warp 1 MMA, warps 2-9 epilogue, warp 10 (dw) the group's ragged end.
+// Two accumulators of 256 columns: the epilogue drains one while the MMA fills the other.
+//
+// dw's contraction ends inside a block of 64 rows; the rows behind it belong to the next group.  Warp
+// 10 zeroes them in both operands (a zero in one would leave 0 * NaN) up to the next multiple of 16, where
+// the MMAs stop.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <mutex>
+
+#include "umsx_device.cuh"
+#include "umsx_internal.h"
+#include "umsx_pair.cuh"
+#include "umsx_products.h"
+
+namespace umsx {
+
+__device__ uint32_t g_product_err;  // a bounded wait gave up (umsx_products_status)
+
+namespace {
+
+constexpr int kBF = 128, kBC = 64;  // features per CTA, contraction per stage
+constexpr int kRowsMax = 256;       // rows of a tile (of a pair: 128 in each CTA)
+constexpr int kRowBox = 32;         // rows of one K-major TMA box
+constexpr int kThreads = 352, kEpilogueWarps = 8;
+constexpr uint32_t kTmemCols = 512;
+
+struct TcParams {
+    int groups, features, contraction, out_rows, out_dtype, fmt;
+    int64_t rows;
+    const int32_t *offsets;
+    void *out;
+    int64_t ldo, out_group;
+};
+
+template <int CG, int MODE>
+struct Shape {
+    static constexpr bool kFMn = MODE != kForward, kRMn = MODE == kGradWeight;
+    static constexpr int kBytesF = kBF * kBC * 2, kBytesR = kRowsMax / CG * kBC * 2;
+    static constexpr int kStages = CG == 1 ? 4 : 6;
+    static constexpr size_t kSmem = 1024 + (size_t)kStages * (kBytesF + kBytesR);
+};
+
+// One tile of the list: rows [row0, row0 + rows) x features [f0, f0 + 128 * CG) of group g.
+struct Tile {
+    int g, f0, row0, rows, c0, c_len;  // c0: first contraction index (dw: a row of x and dy)
+    int n;                             // rows rounded up to the MMA's N
+};
+
+template <int CG, int MODE>
+struct Tiles {
+    const int *start, *prefix;  // shared memory: bounds of the groups (start, end interleaved), tiles before group g
+    int groups, f_tiles, features, contraction, out_rows;
+
+    __device__ static int row_tiles(int rows) { return (rows + kRowsMax - 1) / kRowsMax; }
+
+    __device__ Tile get(int t) const {
+        int lo = 0, hi = groups;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (prefix[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        const int a = start[2 * lo], m = start[2 * lo + 1] - a;
+        const int all = MODE == kGradWeight ? out_rows : m, rt = row_tiles(all);
+        const int local = t - prefix[lo], i = local % rt, j = local / rt;
+        // equal tiles, in steps of the MMA's N
+        constexpr int kStep = 16 * CG;
+        const int size = min(kRowsMax, ((all + rt - 1) / rt + kStep - 1) / kStep * kStep);
+        Tile x;
+        x.g = lo;
+        x.f0 = j * kBF * CG;
+        x.row0 = i * size;
+        x.rows = max(0, min(size, all - x.row0));
+        x.n = (x.rows + kStep - 1) / kStep * kStep;
+        if (MODE == kGradWeight) {
+            x.c0 = a;
+            x.c_len = m;
+        } else {
+            x.row0 += a;
+            x.c0 = 0;
+            x.c_len = contraction;
+        }
+        return x;
+    }
+};
+
+template <int CG, int MODE>
+__global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constant__ CUtensorMap map_f,
+                                                            const __grid_constant__ CUtensorMap map_r, const TcParams p) {
+    using S = Shape<CG, MODE>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sF = smem, *sR = smem + S::kStages * S::kBytesF;
+    __shared__ __align__(8) uint64_t full[S::kStages], ready[S::kStages], empty[S::kStages], d_full[2], d_empty[2];
+    __shared__ uint32_t tmem_s;
+    __shared__ int gave_up;
+    __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = CG == 1 ? 0 : tc::cluster_rank();
+    const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
+
+    for (int g = tid; g < p.groups; g += kThreads) group_bounds(p.offsets, g, p.rows, bounds[2 * g], bounds[2 * g + 1]);
+    if (tid == 0) {
+        gave_up = 0;
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&ready[s], CG);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&d_full[b], 1);
+            mbar_init(&d_empty[b], CG * kEpilogueWarps);
+        }
+    }
+    if (warp == 1) tc::pair_tmem_alloc<CG>(&tmem_s, kTmemCols);
+    __syncthreads();
+    const int f_tiles = (p.features + kBF * CG - 1) / (kBF * CG);
+    if (warp == 0) {
+        int carry = 0;
+        for (int g0 = 0; g0 < p.groups; g0 += 32) {
+            const int g = g0 + lane;
+            int tiles = 0;
+            if (g < p.groups)
+                tiles = f_tiles * Tiles<CG, MODE>::row_tiles(MODE == kGradWeight ? p.out_rows : bounds[2 * g + 1] - bounds[2 * g]);
+            int incl = tiles;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(kFull, incl, o);
+                if (lane >= o) incl += v;
+            }
+            if (g < p.groups) prefix[g] = carry + incl - tiles;
+            carry += __shfl_sync(kFull, incl, 31);
+        }
+        if (lane == 0) prefix[p.groups] = carry;
+    }
+    tc::fence_before_sync();
+    if constexpr (CG == 1) __syncthreads();
+    else tc::cluster_sync_all();  // barriers are initialised before the peer's copies and arrivals reach them
+    tc::fence_after_sync();
+    const uint32_t tmem = tmem_s;
+    const int total = prefix[p.groups];
+    const Tiles<CG, MODE> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int t = cluster; t < total && ok; t += clusters) {
+                const Tile x = tiles.get(t);
+                const int kb = (x.c_len + kBC - 1) / kBC;
+                if (!x.rows) continue;
+                const int half = x.n / CG;  // rows of this CTA's part of R
+                const int boxes = S::kRMn ? (half + 63) / 64 : (half + kRowBox - 1) / kRowBox;
+                const uint32_t bytes = S::kBytesF + boxes * (S::kRMn ? 64 : kRowBox) * kBC * 2;
+                const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
+                for (int kk = 0; kk < kb; ++kk, ++it) {
+                    const int s = it % S::kStages;
+                    if (!(ok = tc::pair_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
+                    uint32_t bar = smem_u32(&full[s]);
+                    if (MODE == kGradWeight || CG == 1) {
+                        mbar_expect_tx(&full[s], bytes);  // each CTA's own; warp 10 passes it on
+                    } else {
+                        if (rank == 0) mbar_expect_tx(&full[s], CG * bytes);
+                        bar = tc::leader_addr(&full[s]);
+                    }
+                    const int c = x.c0 + kk * kBC;
+                    uint8_t *dF = sF + s * S::kBytesF, *dR = sR + s * S::kBytesR;
+                    if constexpr (MODE == kForward) {
+                        tc::pair_tma_3d<CG>(dF, &map_f, c, f0, x.g, bar);
+                    } else {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            if constexpr (MODE == kGradInput) tc::pair_tma_3d<CG>(dF + h * 8192, &map_f, f0 + 64 * h, c, x.g, bar);
+                            else tc::pair_tma_2d<CG>(dF + h * 8192, &map_f, f0 + 64 * h, c, bar);
+                        }
+                    }
+                    for (int b = 0; b < boxes; ++b) {
+                        if constexpr (S::kRMn) tc::pair_tma_2d<CG>(dR + b * 8192, &map_r, r0 + 64 * b, c, bar);
+                        else tc::pair_tma_2d<CG>(dR + b * kRowBox * 128, &map_r, c, r0 + kRowBox * b, bar);
+                    }
+                }
+            }
+            // A CTA must not exit under copies in flight: each stage's last one, again bounded (a wait at all only
+            // where the MMAs gave up before they read them).
+            if (MODE == kGradWeight || rank == 0)
+                for (uint32_t back = 1; back <= (uint32_t)S::kStages && back <= it; ++back)
+                    mbar_wait_bounded(&full[(it - back) % S::kStages], ((it - back) / S::kStages) & 1u, tc::kPairWaitCycles / 8);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            uint32_t it = 0, n_item = 0;
+            bool ok = true;
+            for (int t = cluster; t < total && ok; t += clusters) {
+                const Tile x = tiles.get(t);
+                const int kb = (x.c_len + kBC - 1) / kBC;
+                if (!x.rows || !kb) continue;
+                const uint32_t idesc = tc::operand_idesc(p.fmt, S::kFMn, S::kRMn, kBF * CG, x.n);
+                const uint32_t buf = n_item & 1u, d_tm = tmem + buf * kRowsMax;
+                if (!(ok = tc::pair_wait(&d_empty[buf], ((n_item >> 1) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
+                tc::fence_after_sync();
+                for (int kk = 0; kk < kb; ++kk, ++it) {
+                    const int s = it % S::kStages;
+                    if (!(ok = tc::pair_wait(MODE == kGradWeight ? &ready[s] : &full[s], (it / S::kStages) & 1u, &gave_up,
+                                             &g_product_err)))
+                        break;
+                    tc::fence_after_sync();
+                    const uint64_t df = tc::operand_desc(sF + s * S::kBytesF, S::kFMn, 8192);
+                    const uint64_t dr = tc::operand_desc(sR + s * S::kBytesR, S::kRMn, 8192);
+                    // 16 of the contraction per MMA: 32 bytes along K, or two atoms of eight lines
+                    const int steps = min(kBC / 16, (x.c_len - kk * kBC + 15) / 16);
+                    for (int j = 0; j < steps; ++j)
+                        tc::pair_mma<CG, tc::kKindF16>(d_tm, df + j * (S::kFMn ? 128 : 2), dr + j * (S::kRMn ? 128 : 2), idesc,
+                                                       (kk | j) != 0);
+                    tc::pair_commit<CG>(&empty[s]);
+                }
+                if (ok) tc::pair_commit<CG>(&d_full[buf]);
+                ++n_item;
+            }
+        }
+    } else if (warp < 2 + kEpilogueWarps) {
+        const int quad = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes 32 * quad.., columns in turn of 32
+        uint32_t n_item = 0;
+        bool ok = true;
+        for (int t = cluster; t < total && ok; t += clusters) {
+            const Tile x = tiles.get(t);
+            if (!x.rows) continue;
+            const int f = x.f0 + (int)rank * kBF + quad * 32 + lane;
+            const bool on = f < p.features;
+            const int64_t base = (MODE == kGradWeight ? x.g * p.out_group : 0) + (int64_t)x.row0 * p.ldo;
+            const uint32_t buf = n_item & 1u;
+            const bool zero = x.c_len == 0;
+            if (!zero) {
+                ok = tc::pair_wait(&d_full[buf], (n_item >> 1) & 1u, &gave_up, &g_product_err);
+                if (!(ok = __all_sync(kFull, ok))) break;
+                tc::fence_after_sync();
+                ++n_item;
+            }
+            for (int c0 = part * 32; c0 < x.rows; c0 += 64) {
+                uint32_t v[32];
+                if (!zero) {
+                    tc::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + buf * kRowsMax + c0, v);
+                    tc::tmem_wait_ld(v);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0;
+                }
+                const int n = min(32, x.rows - c0);
+                if (p.out_dtype == UMSX_DTYPE_F32) {
+                    float *o = static_cast<float *>(p.out) + base + (int64_t)c0 * p.ldo + f;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (on && j < n) o[j * p.ldo] = __uint_as_float(v[j]);
+                } else {
+                    uint16_t *o = static_cast<uint16_t *>(p.out) + base + (int64_t)c0 * p.ldo + f;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) {
+                        const float a = __uint_as_float(v[j]);
+                        const uint16_t h = p.out_dtype == UMSX_DTYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(a))
+                                                                         : __half_as_ushort(__float2half_rn(a));
+                        if (on && j < n) o[j * p.ldo] = h;
+                    }
+                }
+            }
+            if (!zero) {
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 1) tc::mbar_arrive(&d_empty[buf]);
+                    else tc::arrive_at(tc::leader_addr(&d_empty[buf]));
+                }
+            }
+        }
+    } else if (MODE == kGradWeight) {
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = cluster; t < total && ok; t += clusters) {
+            const Tile x = tiles.get(t);
+            const int kb = (x.c_len + kBC - 1) / kBC;
+            if (!x.rows) continue;
+            const int half = x.n / CG, boxes = (half + 63) / 64;
+            for (int kk = 0; kk < kb; ++kk, ++it) {
+                const int s = it % S::kStages;
+                ok = tc::pair_wait(&full[s], (it / S::kStages) & 1u, &gave_up, &g_product_err);
+                if (!(ok = __all_sync(kFull, ok))) break;
+                const int valid = x.c_len - kk * kBC;
+                if (valid < kBC && (valid & 15)) {
+                    // lines (one contraction row each) from `valid` up to the last multiple of 16 that the MMAs read
+                    const int lines = 16 - (valid & 15);
+                    for (int i = lane; i < (2 + boxes) * lines * 8; i += 32) {
+                        const int box = i / (lines * 8), rest = i - box * lines * 8;
+                        uint8_t *b = box < 2 ? sF + s * S::kBytesF + box * 8192 : sR + s * S::kBytesR + (box - 2) * 8192;
+                        *reinterpret_cast<uint4 *>(b + (valid + (rest >> 3)) * 128 + (rest & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    tc::fence_proxy_async();
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 1) tc::mbar_arrive(&ready[s]);
+                    else tc::arrive_at(tc::leader_addr(&ready[s]));
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    if constexpr (CG == 1) __syncthreads();
+    else tc::cluster_sync_all();  // the peer's shared and tensor memory are no longer in use
+    tc::fence_after_sync();
+    if (warp == 1) tc::pair_tmem_dealloc<CG>(tmem, kTmemCols);
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                 const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encoder() {
+    static EncodeTiled fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void *q = nullptr;
+        cudaDriverEntryPointQueryResult r{};
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &q, cudaEnableDefault, &r) == cudaSuccess &&
+            r == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeTiled>(q);
+    });
+    return fn;
+}
+
+// A tensor map over a matrix of 128-byte box lines: dims (inner, lines[, matrices]), strides in bytes.
+bool encode(CUtensorMap *m, int dtype, const void *base, int rank, uint64_t inner, uint64_t lines, uint64_t matrices,
+            uint64_t line_bytes, uint64_t matrix_bytes, uint32_t box_lines) {
+    EncodeTiled enc = encoder();
+    if (!enc) return false;
+    const CUtensorMapDataType t = dtype == UMSX_DTYPE_BF16  ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                  : dtype == UMSX_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                            : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const cuuint64_t dims[3] = {inner, lines, matrices};
+    const cuuint64_t strides[2] = {line_bytes, matrix_bytes};
+    const cuuint32_t box[3] = {dtype == UMSX_DTYPE_E4M3 ? 128u : 64u, box_lines, 1};
+    const cuuint32_t step[3] = {1, 1, 1};
+    return enc(m, t, (cuuint32_t)rank, const_cast<void *>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int CG, int MODE>
+int launch(const CUtensorMap &mf, const CUtensorMap &mr, const TcParams &t, int64_t tiles_most, int sms, cudaStream_t s) {
+    auto *kernel = k_product_tc<CG, MODE>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<CG, MODE>::kSmem) != cudaSuccess)
+        return -1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(CG * std::max<int64_t>(1, std::min<int64_t>(tiles_most, sms / CG))));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = Shape<CG, MODE>::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CG;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, mf, mr, t) == cudaSuccess ? 1 : -1;
+}
+
+template <int CG>
+int launch_mode(const Product &p, const CUtensorMap &mf, const CUtensorMap &mr, const TcParams &t, int sms, cudaStream_t s) {
+    const int64_t ft = (p.features() + kBF * CG - 1) / (kBF * CG);
+    const int64_t rt = p.mode == kGradWeight ? (int64_t)p.groups * ((p.n + kRowsMax - 1) / kRowsMax)
+                                             : p.rows / kRowsMax + std::min<int64_t>(p.groups, p.rows);
+    if (p.mode == kForward) return launch<CG, kForward>(mf, mr, t, ft * rt, sms, s);
+    if (p.mode == kGradInput) return launch<CG, kGradInput>(mf, mr, t, ft * rt, sms, s);
+    return launch<CG, kGradWeight>(mf, mr, t, ft * rt, sms, s);
+}
+
+bool aligned(const void *p, int64_t stride, int size) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
+}
+
+}  // namespace
+
+bool product_tc_takes(const Product &p) {
+    if (p.dtype == UMSX_DTYPE_E4M3) return false;
+    if (p.x && !aligned(p.x, p.ldx, 2)) return false;
+    if (p.dy && !aligned(p.dy, p.lddy, 2)) return false;
+    if (p.w && (!aligned(p.w, p.ldw, 2) || (p.groups > 1 && p.w_stride % 8))) return false;
+    return p.rows > 0;
+}
+
+int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
+    CUtensorMap mf, mr;
+    bool ok;
+    if (p.mode == kGradWeight) {
+        ok = encode(&mf, p.dtype, p.x, 2, p.k, p.rows, 1, p.ldx * 2, 0, kBC) &&
+             encode(&mr, p.dtype, p.dy, 2, p.n, p.rows, 1, p.lddy * 2, 0, kBC);
+    } else {
+        const uint64_t ws = p.groups > 1 ? p.w_stride * 2 : p.ldw * 2;
+        ok = encode(&mf, p.dtype, p.w, 3, p.k, p.n, p.groups, p.ldw * 2, ws, p.mode == kForward ? kBF : kBC) &&
+             encode(&mr, p.dtype, p.mode == kForward ? p.x : p.dy, 2, p.mode == kForward ? p.k : p.n, p.rows, 1,
+                    (p.mode == kForward ? p.ldx : p.lddy) * 2, 0, kRowBox);
+    }
+    if (!ok) return -1;
+    TcParams t{};
+    t.groups = p.groups;
+    t.features = p.features();
+    t.contraction = p.mode == kForward ? p.k : p.n;
+    t.out_rows = p.n;
+    t.out_dtype = p.out_dtype;
+    t.fmt = p.dtype == UMSX_DTYPE_BF16 ? 1 : 0;
+    t.rows = p.rows;
+    t.offsets = p.offsets;
+    t.out = p.out;
+    t.ldo = p.ldo;
+    t.out_group = p.out_stride;
+    // CG = 2 for wide outputs
+    return p.features() > kBF ? launch_mode<2>(p, mf, mr, t, sms, s) : launch_mode<1>(p, mf, mr, t, sms, s);
+}
+
+uint32_t *product_err_word() {
+    void *a = nullptr;
+    return cudaGetSymbolAddress(&a, g_product_err) == cudaSuccess ? static_cast<uint32_t *>(a) : nullptr;
+}
+
+}  // namespace umsx
