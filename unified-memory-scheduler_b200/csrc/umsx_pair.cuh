@@ -125,16 +125,19 @@ __host__ __device__ constexpr uint32_t operand_idesc(int fmt, bool a_mn, bool b_
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// 32 consecutive fp32 columns of this warp's 32 TMEM lanes; complete after tmem_wait_ld(r).
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
+// 32 consecutive fp32 columns of this warp's 32 TMEM lanes, in the fragment order of 8 x 8 matrices: r[16h + 4i + 2u + j]
+// is lane 16h + 8u + (thread / 4), column 8i + 2 (thread % 4) + j.  Complete after tmem_wait_ld(r).
+__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&r)[32]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+        asm volatile(
+            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+            "%15}, [%16];"
+            : "=r"(r[16 * h]), "=r"(r[16 * h + 1]), "=r"(r[16 * h + 2]), "=r"(r[16 * h + 3]), "=r"(r[16 * h + 4]),
+              "=r"(r[16 * h + 5]), "=r"(r[16 * h + 6]), "=r"(r[16 * h + 7]), "=r"(r[16 * h + 8]), "=r"(r[16 * h + 9]),
+              "=r"(r[16 * h + 10]), "=r"(r[16 * h + 11]), "=r"(r[16 * h + 12]), "=r"(r[16 * h + 13]), "=r"(r[16 * h + 14]),
+              "=r"(r[16 * h + 15])
+            : "r"(taddr + ((uint32_t)(16 * h) << 16)));
 }
 // The loads so far are complete; `r` is an operand so that no use of it moves above the wait.
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
@@ -145,6 +148,14 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
           "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
         :
         : "memory");
+}
+
+// Four 8 x 8 matrices of 16-bit values in fragment order, transposed, to the 16-byte rows that the lanes name
+// (lanes 8m .. 8m + 7: the rows of matrix m).
+__device__ __forceinline__ void stmatrix_trans4(void *row, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(smem_u32(row)), "r"(a), "r"(b),
+                 "r"(c), "r"(d)
+                 : "memory");
 }
 
 // ---- bounded waits -----------------------------------------------------------------------------

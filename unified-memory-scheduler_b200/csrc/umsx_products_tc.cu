@@ -43,7 +43,7 @@ constexpr int kThreads = 352, kEpilogueWarps = 8;
 constexpr uint32_t kTmemCols = 512;
 
 struct TcParams {
-    int groups, features, contraction, out_rows, out_dtype, fmt;
+    int groups, features, contraction, out_rows, out_dtype, fmt, vec;
     int64_t rows;
     const int32_t *offsets;
     void *out;
@@ -55,7 +55,7 @@ struct Shape {
     static constexpr bool kFMn = MODE != kForward, kRMn = MODE == kGradWeight;
     static constexpr int kBytesF = kBF * kBC * 2, kBytesR = kRowsMax / CG * kBC * 2;
     static constexpr int kStages = CG == 1 ? 4 : 6;
-    static constexpr size_t kSmem = 1024 + (size_t)kStages * (kBytesF + kBytesR);
+    static constexpr size_t kSmem = 1024 + (size_t)kStages * (kBytesF + kBytesR) + kEpilogueWarps * 32 * 80 /* staging */;
 };
 
 // One tile of the list: rows [row0, row0 + rows) x features [f0, f0 + 128 * CG) of group g.
@@ -101,6 +101,73 @@ struct Tiles {
         return x;
     }
 };
+
+// ---- epilogue ---------------------------------------------------------------------------------
+//
+// A warp holds 32 features (its TMEM lanes) x 32 rows in fragment order.  16-bit outputs are transposed through
+// shared memory (stmatrix), so that a lane stores 16 bytes of one row: one store instruction instead of eight.
+constexpr int kStageRow = 80;                       // bytes of a staged row: 64 of data; 80 spreads eight rows over all banks
+constexpr int kStageBytes = 32 * kStageRow;         // one warp's staging
+struct OutTile {
+    void *out;
+    int64_t at, ldo;  // element of the warp's first feature in the tile's first row
+    int dtype, features, rows;  // valid features of the warp's 32, valid rows of the tile
+    bool vec;         // 16-byte stores: base and rows are aligned, features is a multiple of 8 from an aligned start
+};
+
+__device__ __forceinline__ uint32_t pack16(uint32_t lo, uint32_t hi, int dtype) {
+    const float a = __uint_as_float(lo), b = __uint_as_float(hi);
+    if (dtype == UMSX_DTYPE_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// Rows c0 .. c0 + 31 of the tile from v (fragment order).
+__device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, int lane, int c0, const uint32_t (&v)[32]) {
+    if (o.dtype == UMSX_DTYPE_F32) {
+        float *p = static_cast<float *>(o.out) + o.at + (int64_t)(c0 + 2 * (lane & 3)) * o.ldo + (lane >> 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const bool on = c0 + 8 * i + 2 * (lane & 3) + j < o.rows;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    if (on && 8 * q + (lane >> 2) < o.features)
+                        p[(8 * i + j) * o.ldo + 8 * q] = __uint_as_float(v[16 * (q >> 1) + 4 * i + 2 * (q & 1) + j]);
+            }
+        return;
+    }
+    __syncwarp();  // the previous chunk has been read out of the staging
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t m[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            m[q] = pack16(v[16 * (q >> 1) + 4 * i + 2 * (q & 1)], v[16 * (q >> 1) + 4 * i + 2 * (q & 1) + 1], o.dtype);
+        tc::stmatrix_trans4(stage + (8 * i + (lane & 7)) * kStageRow + (lane >> 3) * 16, m[0], m[1], m[2], m[3]);
+    }
+    __syncwarp();
+    uint16_t *p = static_cast<uint16_t *>(o.out) + o.at;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 8 * i + (lane >> 2), f = 8 * (lane & 3);
+        if (c0 + row >= o.rows || f >= o.features) continue;
+        const uint4 w = *reinterpret_cast<const uint4 *>(stage + row * kStageRow + f * 2);
+        uint16_t *d = p + (int64_t)(c0 + row) * o.ldo + f;
+        if (o.vec && f + 8 <= o.features) {
+            *reinterpret_cast<uint4 *>(d) = w;
+        } else {
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(&w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (f + j < o.features) d[j] = h[j];
+        }
+    }
+}
 
 template <int CG, int MODE>
 __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constant__ CUtensorMap map_f,
@@ -238,14 +305,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
         }
     } else if (warp < 2 + kEpilogueWarps) {
         const int quad = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes 32 * quad.., columns in turn of 32
+        uint8_t *stage = smem + S::kStages * (S::kBytesF + S::kBytesR) + (warp - 2) * kStageBytes;
         uint32_t n_item = 0;
         bool ok = true;
         for (int t = cluster; t < total && ok; t += clusters) {
             const Tile x = tiles.get(t);
             if (!x.rows) continue;
-            const int f = x.f0 + (int)rank * kBF + quad * 32 + lane;
-            const bool on = f < p.features;
-            const int64_t base = (MODE == kGradWeight ? x.g * p.out_group : 0) + (int64_t)x.row0 * p.ldo;
+            const int f = x.f0 + (int)rank * kBF + quad * 32;
+            const OutTile o{p.out, (MODE == kGradWeight ? x.g * p.out_group : 0) + (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype,
+                            p.features - f, x.rows, p.vec != 0};
             const uint32_t buf = n_item & 1u;
             const bool zero = x.c_len == 0;
             if (!zero) {
@@ -257,28 +325,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             for (int c0 = part * 32; c0 < x.rows; c0 += 64) {
                 uint32_t v[32];
                 if (!zero) {
-                    tc::tmem_ld32(tmem + ((uint32_t)(quad * 32) << 16) + buf * kRowsMax + c0, v);
+                    tc::tmem_ld_frag32(tmem + ((uint32_t)(quad * 32) << 16) + buf * kRowsMax + c0, v);
                     tc::tmem_wait_ld(v);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = 0;
                 }
-                const int n = min(32, x.rows - c0);
-                if (p.out_dtype == UMSX_DTYPE_F32) {
-                    float *o = static_cast<float *>(p.out) + base + (int64_t)c0 * p.ldo + f;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (on && j < n) o[j * p.ldo] = __uint_as_float(v[j]);
-                } else {
-                    uint16_t *o = static_cast<uint16_t *>(p.out) + base + (int64_t)c0 * p.ldo + f;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const float a = __uint_as_float(v[j]);
-                        const uint16_t h = p.out_dtype == UMSX_DTYPE_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(a))
-                                                                         : __half_as_ushort(__float2half_rn(a));
-                        if (on && j < n) o[j * p.ldo] = h;
-                    }
-                }
+                store_chunk(o, stage, lane, c0, v);
             }
             if (!zero) {
                 tc::fence_before_sync();
@@ -430,6 +483,7 @@ int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
     t.out = p.out;
     t.ldo = p.ldo;
     t.out_group = p.out_stride;
+    t.vec = aligned(p.out, p.ldo, 2) && p.out_stride % 8 == 0;
     // CG = 2 for wide outputs
     return p.features() > kBF ? launch_mode<2>(p, mf, mr, t, sms, s) : launch_mode<1>(p, mf, mr, t, sms, s);
 }
