@@ -41,6 +41,7 @@ constexpr int kRowsMax = 256;       // rows of a tile (of a pair: 128 in each CT
 constexpr int kRowBox = 32;         // rows of one K-major TMA box
 constexpr int kThreads = 352, kEpilogueWarps = 8;
 constexpr uint32_t kTmemCols = 512;
+constexpr int kStageRow = 80;  // bytes of a staged output row: 64 of data; 80 spreads eight rows over all banks
 
 struct TcParams {
     int groups, features, contraction, out_rows, out_dtype, fmt, vec;
@@ -55,7 +56,7 @@ struct Shape {
     static constexpr bool kFMn = MODE != kForward, kRMn = MODE == kGradWeight;
     static constexpr int kBytesF = kBF * kBC * 2, kBytesR = kRowsMax / CG * kBC * 2;
     static constexpr int kStages = CG == 1 ? 4 : 6;
-    static constexpr size_t kSmem = 1024 + (size_t)kStages * (kBytesF + kBytesR) + kEpilogueWarps * 32 * 80 /* staging */;
+    static constexpr size_t kSmem = 1024 + (size_t)kStages * (kBytesF + kBytesR) + kEpilogueWarps * 32 * kStageRow;
 };
 
 // One tile of the list: rows [row0, row0 + rows) x features [f0, f0 + 128 * CG) of group g.
@@ -102,12 +103,31 @@ struct Tiles {
     }
 };
 
+// Tiles before every group, by one warp.
+template <int CG, int MODE>
+__device__ __forceinline__ void tile_prefix(const int *bounds, int *prefix, int groups, int f_tiles, int out_rows, int lane) {
+    int carry = 0;
+    for (int g0 = 0; g0 < groups; g0 += 32) {
+        const int g = g0 + lane;
+        int tiles = 0;
+        if (g < groups)
+            tiles = f_tiles * Tiles<CG, MODE>::row_tiles(MODE == kGradWeight ? out_rows : bounds[2 * g + 1] - bounds[2 * g]);
+        int incl = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(kFull, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (g < groups) prefix[g] = carry + incl - tiles;
+        carry += __shfl_sync(kFull, incl, 31);
+    }
+    if (lane == 0) prefix[groups] = carry;
+}
+
 // ---- epilogue ---------------------------------------------------------------------------------
 //
 // A warp holds 32 features (its TMEM lanes) x 32 rows in fragment order.  16-bit outputs are transposed through
 // shared memory (stmatrix), so that a lane stores 16 bytes of one row: one store instruction instead of eight.
-constexpr int kStageRow = 80;                       // bytes of a staged row: 64 of data; 80 spreads eight rows over all banks
-constexpr int kStageBytes = 32 * kStageRow;         // one warp's staging
 struct OutTile {
     void *out;
     int64_t at, ldo;  // element of the warp's first feature in the tile's first row
@@ -125,7 +145,8 @@ __device__ __forceinline__ uint32_t pack16(uint32_t lo, uint32_t hi, int dtype) 
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Rows c0 .. c0 + 31 of the tile from v (fragment order).
+// Rows c0 .. c0 + 31 of the tile from v (fragment order), through a staging of ROWS rows.
+template <int ROWS>
 __device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, int lane, int c0, const uint32_t (&v)[32]) {
     if (o.dtype == UMSX_DTYPE_F32) {
         float *p = static_cast<float *>(o.out) + o.at + (int64_t)(c0 + 2 * (lane & 3)) * o.ldo + (lane >> 2);
@@ -141,30 +162,35 @@ __device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, in
             }
         return;
     }
-    __syncwarp();  // the previous chunk has been read out of the staging
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t m[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-            m[q] = pack16(v[16 * (q >> 1) + 4 * i + 2 * (q & 1)], v[16 * (q >> 1) + 4 * i + 2 * (q & 1) + 1], o.dtype);
-        tc::stmatrix_trans4(stage + (8 * i + (lane & 7)) * kStageRow + (lane >> 3) * 16, m[0], m[1], m[2], m[3]);
-    }
-    __syncwarp();
     uint16_t *p = static_cast<uint16_t *>(o.out) + o.at;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = 8 * i + (lane >> 2), f = 8 * (lane & 3);
-        if (c0 + row >= o.rows || f >= o.features) continue;
-        const uint4 w = *reinterpret_cast<const uint4 *>(stage + row * kStageRow + f * 2);
-        uint16_t *d = p + (int64_t)(c0 + row) * o.ldo + f;
-        if (o.vec && f + 8 <= o.features) {
-            *reinterpret_cast<uint4 *>(d) = w;
-        } else {
-            const uint16_t *h = reinterpret_cast<const uint16_t *>(&w);
+    for (int r0 = 0; r0 < 32; r0 += ROWS) {
+        __syncwarp();  // the previous rows have been read out of the staging
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (f + j < o.features) d[j] = h[j];
+        for (int i = 0; i < ROWS / 8; ++i) {
+            uint32_t m[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int e = 16 * (q >> 1) + 4 * (r0 / 8 + i) + 2 * (q & 1);
+                m[q] = pack16(v[e], v[e + 1], o.dtype);
+            }
+            tc::stmatrix_trans4(stage + (8 * i + (lane & 7)) * kStageRow + (lane >> 3) * 16, m[0], m[1], m[2], m[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < ROWS / 8; ++i) {
+            const int row = 8 * i + (lane >> 2), f = 8 * (lane & 3);
+            if (c0 + r0 + row >= o.rows || f >= o.features) continue;
+            const uint4 w = *reinterpret_cast<const uint4 *>(stage + row * kStageRow + f * 2);
+            uint16_t *d = p + (int64_t)(c0 + r0 + row) * o.ldo + f;
+            if (o.vec && f + 8 <= o.features) {
+                *reinterpret_cast<uint4 *>(d) = w;
+            } else {
+                const uint16_t *h = reinterpret_cast<const uint16_t *>(&w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (f + j < o.features) d[j] = h[j];
+            }
         }
     }
 }
@@ -201,24 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     if (warp == 1) tc::pair_tmem_alloc<CG>(&tmem_s, kTmemCols);
     __syncthreads();
     const int f_tiles = (p.features + kBF * CG - 1) / (kBF * CG);
-    if (warp == 0) {
-        int carry = 0;
-        for (int g0 = 0; g0 < p.groups; g0 += 32) {
-            const int g = g0 + lane;
-            int tiles = 0;
-            if (g < p.groups)
-                tiles = f_tiles * Tiles<CG, MODE>::row_tiles(MODE == kGradWeight ? p.out_rows : bounds[2 * g + 1] - bounds[2 * g]);
-            int incl = tiles;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(kFull, incl, o);
-                if (lane >= o) incl += v;
-            }
-            if (g < p.groups) prefix[g] = carry + incl - tiles;
-            carry += __shfl_sync(kFull, incl, 31);
-        }
-        if (lane == 0) prefix[p.groups] = carry;
-    }
+    if (warp == 0) tile_prefix<CG, MODE>(bounds, prefix, p.groups, f_tiles, p.out_rows, lane);
     tc::fence_before_sync();
     if constexpr (CG == 1) __syncthreads();
     else tc::cluster_sync_all();  // barriers are initialised before the peer's copies and arrivals reach them
@@ -305,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
         }
     } else if (warp < 2 + kEpilogueWarps) {
         const int quad = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes 32 * quad.., columns in turn of 32
-        uint8_t *stage = smem + S::kStages * (S::kBytesF + S::kBytesR) + (warp - 2) * kStageBytes;
+        uint8_t *stage = smem + S::kStages * (S::kBytesF + S::kBytesR) + (warp - 2) * 32 * kStageRow;
         uint32_t n_item = 0;
         bool ok = true;
         for (int t = cluster; t < total && ok; t += clusters) {
@@ -331,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = 0;
                 }
-                store_chunk(o, stage, lane, c0, v);
+                store_chunk<32>(o, stage, lane, c0, v);
             }
             if (!zero) {
                 tc::fence_before_sync();
@@ -377,6 +386,249 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     tc::fence_before_sync();
     if constexpr (CG == 1) __syncthreads();
     else tc::cluster_sync_all();  // the peer's shared and tensor memory are no longer in use
+    tc::fence_after_sync();
+    if (warp == 1) tc::pair_tmem_dealloc<CG>(tmem, kTmemCols);
+}
+
+// ---- e4m3 operands with a scale per block of 128 -------------------------------------------------
+//
+// out[r][f] = sum_b xs[r][b] ws[f / 128][b] D_b[r][f] with D_b the product over block b of the contraction.  A stage
+// is one block: its MMAs start a fresh accumulator, and the epilogue warps add it, times the scales, to fp32
+// sums in registers.  The scale is one per column of the accumulator (a row of x) and CTA (128 features: one
+// block of w), so warps 2-3 put xs * ws of a stage's rows into shared memory and a thread multiplies
+// pairs of columns with one packed FMA.  A block's MMAs take 512 cycles at 256 rows; its
+// promotion about 110 issue slots in each of the eight warps, two warps to a scheduler, so the MMAs bound it.
+// The sums need 128 registers a thread; warps 0-3 give theirs up (72 + 2 * 208 of 3 * 168 per thread and warpgroup).
+
+constexpr int kThreadsF8 = 384, kScaleSlots = 4;
+
+struct F8Params {
+    TcParams t;
+    const float *xs, *ws;
+    int64_t xs_row, xs_blk, ws_row, ws_blk, ws_group;
+};
+
+template <int CG>
+struct ShapeF8 {
+    static constexpr int kBC8 = 128;  // contraction per stage, in bytes too
+    static constexpr int kBytesF = kBF * kBC8, kBytesR = kRowsMax / CG * kBC8;
+    static constexpr int kStages = CG == 1 ? 4 : 6;
+    static constexpr size_t kOperands = (size_t)kStages * (kBytesF + kBytesR);
+    static constexpr size_t kSmem = 1024 + kOperands + kEpilogueWarps * 16 * kStageRow + kScaleSlots * kRowsMax * sizeof(float);
+};
+
+__device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t)lo | ((uint64_t)hi << 32); }
+__device__ __forceinline__ void fma2(uint64_t &acc, uint64_t a, uint64_t b) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+
+template <int CG>
+__global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_constant__ CUtensorMap map_f,
+                                                              const __grid_constant__ CUtensorMap map_r, const F8Params fp) {
+    using S = ShapeF8<CG>;
+    const TcParams &p = fp.t;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sF = smem, *sR = smem + S::kStages * S::kBytesF;
+    float *sScale = reinterpret_cast<float *>(smem + S::kOperands);  // [slot][row of the tile]
+    uint8_t *staging = smem + S::kOperands + kScaleSlots * kRowsMax * sizeof(float);
+    __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[2], d_empty[2], sc_full[kScaleSlots],
+        sc_empty[kScaleSlots];
+    __shared__ uint32_t tmem_s;
+    __shared__ int gave_up;
+    __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = CG == 1 ? 0 : tc::cluster_rank();
+    const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
+
+    for (int g = tid; g < p.groups; g += kThreadsF8) group_bounds(p.offsets, g, p.rows, bounds[2 * g], bounds[2 * g + 1]);
+    if (tid == 0) {
+        gave_up = 0;
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(&d_full[b], 1);
+            mbar_init(&d_empty[b], CG * kEpilogueWarps);
+        }
+        for (int s = 0; s < kScaleSlots; ++s) {
+            mbar_init(&sc_full[s], 1);
+            mbar_init(&sc_empty[s], kEpilogueWarps);
+        }
+    }
+    if (warp == 1) tc::pair_tmem_alloc<CG>(&tmem_s, kTmemCols);
+    __syncthreads();
+    const int f_tiles = (p.features + kBF * CG - 1) / (kBF * CG);
+    if (warp == 0) tile_prefix<CG, kForward>(bounds, prefix, p.groups, f_tiles, p.out_rows, lane);
+    tc::fence_before_sync();
+    if constexpr (CG == 1) __syncthreads();
+    else tc::cluster_sync_all();
+    tc::fence_after_sync();
+    const uint32_t tmem = tmem_s;
+    const int total = prefix[p.groups], kb = (p.contraction + S::kBC8 - 1) / S::kBC8;
+    const Tiles<CG, kForward> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            if (lane == 0) {
+                uint32_t it = 0;
+                bool ok = true;
+                for (int t = cluster; t < total && ok; t += clusters) {
+                    const Tile x = tiles.get(t);
+                    if (!x.rows) continue;
+                    const int half = x.n / CG, boxes = (half + kRowBox - 1) / kRowBox;
+                    const uint32_t bytes = S::kBytesF + boxes * kRowBox * S::kBC8;
+                    const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
+                    for (int kk = 0; kk < kb; ++kk, ++it) {
+                        const int s = it % S::kStages;
+                        if (!(ok = tc::pair_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
+                        uint32_t bar = smem_u32(&full[s]);
+                        if (rank == 0) mbar_expect_tx(&full[s], CG * bytes);
+                        if (CG > 1) bar = tc::leader_addr(&full[s]);
+                        tc::pair_tma_3d<CG>(sF + s * S::kBytesF, &map_f, kk * S::kBC8, f0, x.g, bar);
+                        for (int b = 0; b < boxes; ++b)
+                            tc::pair_tma_2d<CG>(sR + s * S::kBytesR + b * kRowBox * S::kBC8, &map_r, kk * S::kBC8, r0 + kRowBox * b, bar);
+                    }
+                }
+                if (rank == 0)  // as in k_product_tc: no exit under copies in flight
+                    for (uint32_t back = 1; back <= (uint32_t)S::kStages && back <= it; ++back)
+                        mbar_wait_bounded(&full[(it - back) % S::kStages], ((it - back) / S::kStages) & 1u, tc::kPairWaitCycles / 8);
+            }
+        } else if (warp == 1) {
+            if (lane == 0 && rank == 0) {
+                uint32_t it = 0;
+                bool ok = true;
+                for (int t = cluster; t < total && ok; t += clusters) {
+                    const Tile x = tiles.get(t);
+                    if (!x.rows) continue;
+                    const uint32_t idesc = tc::operand_idesc(0, false, false, kBF * CG, x.n);
+                    for (int kk = 0; kk < kb; ++kk, ++it) {
+                        const int s = it % S::kStages;
+                        const uint32_t buf = it & 1u, d_tm = tmem + buf * kRowsMax;
+                        if (!(ok = tc::pair_wait(&d_empty[buf], ((it >> 1) & 1u) ^ 1u, &gave_up, &g_product_err) &&
+                                   tc::pair_wait(&full[s], (it / S::kStages) & 1u, &gave_up, &g_product_err)))
+                            break;
+                        tc::fence_after_sync();
+                        const uint64_t df = tc::operand_desc(sF + s * S::kBytesF, false, 0);
+                        const uint64_t dr = tc::operand_desc(sR + s * S::kBytesR, false, 0);
+                        const int steps = min(S::kBC8 / 32, (p.contraction - kk * S::kBC8 + 31) / 32);
+                        for (int j = 0; j < steps; ++j)
+                            tc::pair_mma<CG, tc::kKindF8>(d_tm, df + 2 * j, dr + 2 * j, idesc, j != 0);
+                        tc::pair_commit<CG>(&empty[s]);
+                        tc::pair_commit<CG>(&d_full[buf]);
+                    }
+                }
+            }
+        } else {
+            // ---- scales: warps 2 and 3 take turns; each loads its next stage's before it waits for a slot ----
+            uint32_t it = 0;
+            bool ok = true;
+            for (int t = cluster; t < total && ok; t += clusters) {
+                const Tile x = tiles.get(t);
+                if (!x.rows) continue;
+                const int f0 = x.f0 + (int)rank * kBF;
+                const float *ws = fp.ws + x.g * fp.ws_group + (int64_t)(f0 / kScaleBlock) * fp.ws_row;
+                const float *xs = fp.xs + (int64_t)(x.row0 + lane) * fp.xs_row;
+                const bool on = f0 < p.features;  // the pair's second half may lie behind the last feature
+                float v[8], w = 0.0f;
+                auto fetch = [&](int kk) {
+                    if (kk >= kb) return;
+                    w = on ? __ldg(ws + kk * fp.ws_blk) : 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        v[i] = lane + 32 * i < x.rows ? __ldg(xs + (int64_t)(32 * i) * fp.xs_row + kk * fp.xs_blk) : 0.0f;
+                };
+                int kk = (int)((it ^ (uint32_t)warp) & 1u);  // the first stage of this tile with it + kk of this warp's parity
+                fetch(kk);
+                for (; kk < kb; kk += 2) {
+                    const uint32_t i_ = it + kk, slot = i_ % kScaleSlots;
+                    float s8[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s8[i] = v[i] * w;
+                    fetch(kk + 2);
+                    ok = tc::pair_wait(&sc_empty[slot], ((i_ / kScaleSlots) & 1u) ^ 1u, &gave_up, &g_product_err);
+                    if (!(ok = __all_sync(kFull, ok))) break;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sScale[slot * kRowsMax + lane + 32 * i] = s8[i];
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&sc_full[slot]);
+                }
+                it += kb;
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        const int quad = warp & 3, part = (warp - 4) >> 2;  // TMEM lanes 32 * quad.., chunks of 32 columns in turn
+        uint8_t *stage = staging + (warp - 4) * 16 * kStageRow;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = cluster; t < total && ok; t += clusters) {
+            const Tile x = tiles.get(t);
+            if (!x.rows) continue;
+            uint64_t acc[4][16];  // chunk, [16-lane half][8 columns][8-lane half] pairs of columns: 0.0f
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[c][i] = 0;
+            for (int kk = 0; kk < kb; ++kk, ++it) {
+                const uint32_t buf = it & 1u, slot = it % kScaleSlots;
+                ok = tc::pair_wait(&d_full[buf], (it >> 1) & 1u, &gave_up, &g_product_err) &&
+                     tc::pair_wait(&sc_full[slot], (it / kScaleSlots) & 1u, &gave_up, &g_product_err);
+                if (!(ok = __all_sync(kFull, ok))) break;
+                tc::fence_after_sync();
+                const float *sc = sScale + slot * kRowsMax + 2 * (lane & 3);
+                const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + buf * kRowsMax;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const int c0 = (2 * c + part) * 32;
+                    if (c0 < x.n) {
+                        uint32_t v[32];
+                        tc::tmem_ld_frag32(src + c0, v);
+                        tc::tmem_wait_ld(v);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint64_t s2 = *reinterpret_cast<const uint64_t *>(sc + c0 + 8 * i);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const int e = 16 * (q >> 1) + 4 * i + 2 * (q & 1);
+                                fma2(acc[c][e >> 1], pack2(v[e], v[e + 1]), s2);
+                            }
+                        }
+                    }
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    if constexpr (CG == 1) tc::mbar_arrive(&d_empty[buf]);
+                    else tc::arrive_at(tc::leader_addr(&d_empty[buf]));
+                    tc::mbar_arrive(&sc_empty[slot]);
+                }
+            }
+            if (!ok) break;
+            const int f = x.f0 + (int)rank * kBF + quad * 32;
+            const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, x.rows, p.vec != 0};
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int c0 = (2 * c + part) * 32;
+                if (c0 < x.rows) {
+                    uint32_t v[32];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        v[2 * i] = (uint32_t)acc[c][i];
+                        v[2 * i + 1] = (uint32_t)(acc[c][i] >> 32);
+                    }
+                    store_chunk<16>(o, stage, lane, c0, v);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    if constexpr (CG == 1) __syncthreads();
+    else tc::cluster_sync_all();
     tc::fence_after_sync();
     if (warp == 1) tc::pair_tmem_dealloc<CG>(tmem, kTmemCols);
 }
@@ -444,6 +696,26 @@ int launch_mode(const Product &p, const CUtensorMap &mf, const CUtensorMap &mr, 
     return launch<CG, kGradWeight>(mf, mr, t, ft * rt, sms, s);
 }
 
+template <int CG>
+int launch_f8(const CUtensorMap &mf, const CUtensorMap &mr, const F8Params &fp, int sms, cudaStream_t s) {
+    auto *kernel = k_product_f8<CG>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ShapeF8<CG>::kSmem) != cudaSuccess) return -1;
+    const int64_t ft = (fp.t.features + kBF * CG - 1) / (kBF * CG);
+    const int64_t rt = fp.t.rows / kRowsMax + std::min<int64_t>(fp.t.groups, fp.t.rows);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(CG * std::max<int64_t>(1, std::min<int64_t>(ft * rt, sms / CG))));
+    cfg.blockDim = dim3(kThreadsF8);
+    cfg.dynamicSmemBytes = ShapeF8<CG>::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = CG;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, mf, mr, fp) == cudaSuccess ? 1 : -1;
+}
+
 bool aligned(const void *p, int64_t stride, int size) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && stride * size % 16 == 0;
 }
@@ -451,10 +723,10 @@ bool aligned(const void *p, int64_t stride, int size) {
 }  // namespace
 
 bool product_tc_takes(const Product &p) {
-    if (p.dtype == UMSX_DTYPE_E4M3) return false;
-    if (p.x && !aligned(p.x, p.ldx, 2)) return false;
-    if (p.dy && !aligned(p.dy, p.lddy, 2)) return false;
-    if (p.w && (!aligned(p.w, p.ldw, 2) || (p.groups > 1 && p.w_stride % 8))) return false;
+    const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2;
+    if (p.x && !aligned(p.x, p.ldx, size)) return false;
+    if (p.dy && !aligned(p.dy, p.lddy, size)) return false;
+    if (p.w && (!aligned(p.w, p.ldw, size) || (p.groups > 1 && p.w_stride * size % 16))) return false;
     return p.rows > 0;
 }
 
@@ -465,10 +737,11 @@ int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
         ok = encode(&mf, p.dtype, p.x, 2, p.k, p.rows, 1, p.ldx * 2, 0, kBC) &&
              encode(&mr, p.dtype, p.dy, 2, p.n, p.rows, 1, p.lddy * 2, 0, kBC);
     } else {
-        const uint64_t ws = p.groups > 1 ? p.w_stride * 2 : p.ldw * 2;
-        ok = encode(&mf, p.dtype, p.w, 3, p.k, p.n, p.groups, p.ldw * 2, ws, p.mode == kForward ? kBF : kBC) &&
+        const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2;
+        const uint64_t ws = (p.groups > 1 ? p.w_stride : p.ldw) * size;
+        ok = encode(&mf, p.dtype, p.w, 3, p.k, p.n, p.groups, p.ldw * size, ws, p.mode == kForward ? kBF : kBC) &&
              encode(&mr, p.dtype, p.mode == kForward ? p.x : p.dy, 2, p.mode == kForward ? p.k : p.n, p.rows, 1,
-                    (p.mode == kForward ? p.ldx : p.lddy) * 2, 0, kRowBox);
+                    (p.mode == kForward ? p.ldx : p.lddy) * size, 0, kRowBox);
     }
     if (!ok) return -1;
     TcParams t{};
@@ -484,6 +757,10 @@ int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
     t.ldo = p.ldo;
     t.out_group = p.out_stride;
     t.vec = aligned(p.out, p.ldo, 2) && p.out_stride % 8 == 0;
+    if (p.dtype == UMSX_DTYPE_E4M3) {
+        const F8Params fp{t, p.xs, p.ws, p.xs_row, p.xs_blk, p.ws_row, p.ws_blk, p.ws_group};
+        return p.features() > kBF ? launch_f8<2>(mf, mr, fp, sms, s) : launch_f8<1>(mf, mr, fp, sms, s);
+    }
     // CG = 2 for wide outputs
     return p.features() > kBF ? launch_mode<2>(p, mf, mr, t, sms, s) : launch_mode<1>(p, mf, mr, t, sms, s);
 }
