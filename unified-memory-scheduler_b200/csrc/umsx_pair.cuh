@@ -77,7 +77,13 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// Arrival at a barrier of the pair.  It orders tensor-memory reads (tcgen05 fences around it) but publishes no
+// writes to the other CTA, so it needs no cluster scope, whose fence would wait for every store in flight.
 __device__ __forceinline__ void arrive_at(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+// The same, publishing this thread's writes to the other CTA.
+__device__ __forceinline__ void publish_at(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
@@ -125,29 +131,21 @@ __host__ __device__ constexpr uint32_t operand_idesc(int fmt, bool a_mn, bool b_
            ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// 32 consecutive fp32 columns of this warp's 32 TMEM lanes, in the fragment order of 8 x 8 matrices: r[16h + 4i + 2u + j]
-// is lane 16h + 8u + (thread / 4), column 8i + 2 (thread % 4) + j.  Complete after tmem_wait_ld(r).
-__device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&r)[32]) {
+// 16 consecutive fp32 columns of this warp's 32 TMEM lanes, in the fragment order of 8 x 8 matrices: r[8h + 4i + 2u + j]
+// is lane 16h + 8u + (thread / 4), column 8i + 2 (thread % 4) + j.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-        asm volatile(
-            "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-            "%15}, [%16];"
-            : "=r"(r[16 * h]), "=r"(r[16 * h + 1]), "=r"(r[16 * h + 2]), "=r"(r[16 * h + 3]), "=r"(r[16 * h + 4]),
-              "=r"(r[16 * h + 5]), "=r"(r[16 * h + 6]), "=r"(r[16 * h + 7]), "=r"(r[16 * h + 8]), "=r"(r[16 * h + 9]),
-              "=r"(r[16 * h + 10]), "=r"(r[16 * h + 11]), "=r"(r[16 * h + 12]), "=r"(r[16 * h + 13]), "=r"(r[16 * h + 14]),
-              "=r"(r[16 * h + 15])
-            : "r"(taddr + ((uint32_t)(16 * h) << 16)));
-}
-// The loads so far are complete; `r` is an operand so that no use of it moves above the wait.
-__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[32]) {
+        asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(r[8 * h]), "=r"(r[8 * h + 1]), "=r"(r[8 * h + 2]), "=r"(r[8 * h + 3]), "=r"(r[8 * h + 4]),
+                       "=r"(r[8 * h + 5]), "=r"(r[8 * h + 6]), "=r"(r[8 * h + 7])
+                     : "r"(taddr + ((uint32_t)(16 * h) << 16)));
+    // the values are operands of the wait, so that no use of them moves above it
     asm volatile("tcgen05.wait::ld.sync.aligned;"
-        : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
-          "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
-          "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
-          "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
-        :
-        : "memory");
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                   "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
 }
 
 // Four 8 x 8 matrices of 16-bit values in fragment order, transposed, to the 16-byte rows that the lanes name
@@ -158,22 +156,40 @@ __device__ __forceinline__ void stmatrix_trans4(void *row, uint32_t a, uint32_t 
                  : "memory");
 }
 
+// True in one lane of a converged warp.  The copies and MMAs are issued under it and not under a test of the
+// lane: their operands then stay in uniform registers (four MMAs took 490 cycles to issue under `lane == 0`).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(p));
+    return p != 0;
+}
+
 // ---- bounded waits -----------------------------------------------------------------------------
 //
 // About a second; then the wait marks its CTA as given up (every later wait of the CTA returns at once, so
 // that the kernel ends) and records it in `err`.
 constexpr long long kPairWaitCycles = 2000000000ll;
 
+// ACROSS: the barrier hands over what the other CTA's threads wrote (publish_at); an acquire of cluster scope
+// costs about 200 cycles even where the phase is complete, so the other waits stay at this CTA's scope.
+template <bool ACROSS = false>
 __device__ __forceinline__ bool pair_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up, uint32_t *err) {
     const uint32_t a = smem_u32(bar);
     long long t0 = 0;
     while (true) {
         uint32_t done;
-        asm volatile(
-            "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-            : "=r"(done)
-            : "r"(a), "r"(parity)
-            : "memory");
+        if constexpr (ACROSS)
+            asm volatile(
+                "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
+                : "=r"(done)
+                : "r"(a), "r"(parity)
+                : "memory");
+        else
+            asm volatile(
+                "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
+                : "=r"(done)
+                : "r"(a), "r"(parity), "r"(1000000u)
+                : "memory");
         if (done) return true;
         if (*gave_up) return false;
         const long long t = clock64();
@@ -184,6 +200,12 @@ __device__ __forceinline__ bool pair_wait(uint64_t *bar, uint32_t parity, volati
             return false;
         }
     }
+}
+
+// The same by a whole warp: one answer for all lanes.
+template <bool ACROSS = false>
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up, uint32_t *err) {
+    return __all_sync(kFull, pair_wait<ACROSS>(bar, parity, gave_up, err));
 }
 
 }  // namespace tc

@@ -16,7 +16,7 @@
 //
 // dw's contraction ends inside a block of 64 rows; the rows behind it belong to the next group.  Warp
 // 10 zeroes them in both operands (a zero in one would leave 0 * NaN) up to the next multiple of 16, where
-// the MMAs stop.
+// the MMAs stop.  Only that last stage of a tile goes through it: handing every stage on cost 1.8 K cycles a stage.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -56,7 +56,7 @@ struct Shape {
     static constexpr bool kFMn = MODE != kForward, kRMn = MODE == kGradWeight;
     static constexpr int kBytesF = kBF * kBC * 2, kBytesR = kRowsMax / CG * kBC * 2;
     static constexpr int kStages = CG == 1 ? 4 : 6;
-    static constexpr size_t kSmem = 1024 + (size_t)kStages * (kBytesF + kBytesR) + kEpilogueWarps * 32 * kStageRow;
+    static constexpr size_t kSmem = 1024 + (size_t)kStages * (kBytesF + kBytesR) + kEpilogueWarps * 16 * kStageRow;
 };
 
 // One tile of the list: rows [row0, row0 + rows) x features [f0, f0 + 128 * CG) of group g.
@@ -126,7 +126,7 @@ __device__ __forceinline__ void tile_prefix(const int *bounds, int *prefix, int 
 
 // ---- epilogue ---------------------------------------------------------------------------------
 //
-// A warp holds 32 features (its TMEM lanes) x 32 rows in fragment order.  16-bit outputs are transposed through
+// A warp holds 32 features (its TMEM lanes) x 16 rows in fragment order.  16-bit outputs are transposed through
 // shared memory (stmatrix), so that a lane stores 16 bytes of one row: one store instruction instead of eight.
 struct OutTile {
     void *out;
@@ -145,52 +145,48 @@ __device__ __forceinline__ uint32_t pack16(uint32_t lo, uint32_t hi, int dtype) 
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// Rows c0 .. c0 + 31 of the tile from v (fragment order), through a staging of ROWS rows.
-template <int ROWS>
-__device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, int lane, int c0, const uint32_t (&v)[32]) {
+// Rows c0 .. c0 + 15 of the tile from v (fragment order), through the warp's staging of 16 rows.
+__device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, int lane, int c0, const uint32_t (&v)[16]) {
     if (o.dtype == UMSX_DTYPE_F32) {
         float *p = static_cast<float *>(o.out) + o.at + (int64_t)(c0 + 2 * (lane & 3)) * o.ldo + (lane >> 2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 const bool on = c0 + 8 * i + 2 * (lane & 3) + j < o.rows;
 #pragma unroll
                 for (int q = 0; q < 4; ++q)
                     if (on && 8 * q + (lane >> 2) < o.features)
-                        p[(8 * i + j) * o.ldo + 8 * q] = __uint_as_float(v[16 * (q >> 1) + 4 * i + 2 * (q & 1) + j]);
+                        p[(8 * i + j) * o.ldo + 8 * q] = __uint_as_float(v[8 * (q >> 1) + 4 * i + 2 * (q & 1) + j]);
             }
         return;
     }
+    __syncwarp();  // the previous rows have been read out of the staging
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint32_t m[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int e = 8 * (q >> 1) + 4 * i + 2 * (q & 1);
+            m[q] = pack16(v[e], v[e + 1], o.dtype);
+        }
+        tc::stmatrix_trans4(stage + (8 * i + (lane & 7)) * kStageRow + (lane >> 3) * 16, m[0], m[1], m[2], m[3]);
+    }
+    __syncwarp();
     uint16_t *p = static_cast<uint16_t *>(o.out) + o.at;
 #pragma unroll
-    for (int r0 = 0; r0 < 32; r0 += ROWS) {
-        __syncwarp();  // the previous rows have been read out of the staging
+    for (int i = 0; i < 2; ++i) {
+        const int row = 8 * i + (lane >> 2), f = 8 * (lane & 3);
+        if (c0 + row >= o.rows || f >= o.features) continue;
+        const uint4 w = *reinterpret_cast<const uint4 *>(stage + row * kStageRow + f * 2);
+        uint16_t *d = p + (int64_t)(c0 + row) * o.ldo + f;
+        if (o.vec && f + 8 <= o.features) {
+            *reinterpret_cast<uint4 *>(d) = w;
+        } else {
+            const uint16_t *h = reinterpret_cast<const uint16_t *>(&w);
 #pragma unroll
-        for (int i = 0; i < ROWS / 8; ++i) {
-            uint32_t m[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int e = 16 * (q >> 1) + 4 * (r0 / 8 + i) + 2 * (q & 1);
-                m[q] = pack16(v[e], v[e + 1], o.dtype);
-            }
-            tc::stmatrix_trans4(stage + (8 * i + (lane & 7)) * kStageRow + (lane >> 3) * 16, m[0], m[1], m[2], m[3]);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < ROWS / 8; ++i) {
-            const int row = 8 * i + (lane >> 2), f = 8 * (lane & 3);
-            if (c0 + r0 + row >= o.rows || f >= o.features) continue;
-            const uint4 w = *reinterpret_cast<const uint4 *>(stage + row * kStageRow + f * 2);
-            uint16_t *d = p + (int64_t)(c0 + r0 + row) * o.ldo + f;
-            if (o.vec && f + 8 <= o.features) {
-                *reinterpret_cast<uint4 *>(d) = w;
-            } else {
-                const uint16_t *h = reinterpret_cast<const uint16_t *>(&w);
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (f + j < o.features) d[j] = h[j];
-            }
+            for (int j = 0; j < 8; ++j)
+                if (f + j < o.features) d[j] = h[j];
         }
     }
 }
@@ -200,9 +196,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                                                             const __grid_constant__ CUtensorMap map_r, const TcParams p) {
     using S = Shape<CG, MODE>;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     uint8_t *sF = smem, *sR = smem + S::kStages * S::kBytesF;
-    __shared__ __align__(8) uint64_t full[S::kStages], ready[S::kStages], empty[S::kStages], d_full[2], d_empty[2];
+    __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[2], d_empty[2];
+    // dw, a tile's ragged last stage: its copies to this CTA, and both CTAs' zeroing
+    __shared__ __align__(8) uint64_t tail[S::kStages], fixed[S::kStages];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up;
     __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
@@ -216,7 +214,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
         gave_up = 0;
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&ready[s], CG);
+            mbar_init(&tail[s], 1);
+            mbar_init(&fixed[s], CG);
             mbar_init(&empty[s], 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -237,26 +236,30 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     const Tiles<CG, MODE> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t it = 0;
-            bool ok = true;
-            for (int t = cluster; t < total && ok; t += clusters) {
-                const Tile x = tiles.get(t);
-                const int kb = (x.c_len + kBC - 1) / kBC;
-                if (!x.rows) continue;
-                const int half = x.n / CG;  // rows of this CTA's part of R
-                const int boxes = S::kRMn ? (half + 63) / 64 : (half + kRowBox - 1) / kRowBox;
-                const uint32_t bytes = S::kBytesF + boxes * (S::kRMn ? 64 : kRowBox) * kBC * 2;
-                const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
-                for (int kk = 0; kk < kb; ++kk, ++it) {
-                    const int s = it % S::kStages;
-                    if (!(ok = tc::pair_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
-                    uint32_t bar = smem_u32(&full[s]);
-                    if (MODE == kGradWeight || CG == 1) {
-                        mbar_expect_tx(&full[s], bytes);  // each CTA's own; warp 10 passes it on
+        uint32_t it = 0, tails = 0, tail_phase = 0;  // bit s: stage s holds a ragged end; uses of tail[s], mod 2
+        bool ok = true;
+        for (int t = cluster; t < total && ok; t += clusters) {
+            const Tile x = tiles.get(t);
+            const int kb = (x.c_len + kBC - 1) / kBC;
+            if (!x.rows) continue;
+            const int half = x.n / CG;  // rows of this CTA's part of R
+            const int boxes = S::kRMn ? (half + 63) / 64 : (half + kRowBox - 1) / kRowBox;
+            const uint32_t bytes = S::kBytesF + boxes * (S::kRMn ? 64 : kRowBox) * kBC * 2;
+            const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
+            for (int kk = 0; kk < kb; ++kk, ++it) {
+                const int s = it % S::kStages;
+                if (!(ok = tc::warp_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
+                const bool ragged = MODE == kGradWeight && kk == kb - 1 && (x.c_len & 15);
+                if (ragged) tails |= 1u << s, tail_phase ^= 1u << s;
+                else tails &= ~(1u << s);
+                if (tc::elect_one()) {
+                    uint32_t bar = smem_u32(ragged ? &tail[s] : &full[s]);
+                    if (ragged) {
+                        mbar_expect_tx(&tail[s], bytes);  // each CTA's own, for its warp 10
+                        if (rank == 0) tc::mbar_arrive(&full[s]);
                     } else {
                         if (rank == 0) mbar_expect_tx(&full[s], CG * bytes);
-                        bar = tc::leader_addr(&full[s]);
+                        if (CG > 1) bar = tc::leader_addr(&full[s]);
                     }
                     const int c = x.c0 + kk * kBC;
                     uint8_t *dF = sF + s * S::kBytesF, *dR = sR + s * S::kBytesR;
@@ -274,16 +277,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                         else tc::pair_tma_2d<CG>(dR + b * kRowBox * 128, &map_r, c, r0 + kRowBox * b, bar);
                     }
                 }
+                __syncwarp();
             }
-            // A CTA must not exit under copies in flight: each stage's last one, again bounded (a wait at all only
-            // where the MMAs gave up before they read them).
-            if (MODE == kGradWeight || rank == 0)
-                for (uint32_t back = 1; back <= (uint32_t)S::kStages && back <= it; ++back)
-                    mbar_wait_bounded(&full[(it - back) % S::kStages], ((it - back) / S::kStages) & 1u, tc::kPairWaitCycles / 8);
+        }
+        // A CTA must not exit under copies in flight: each stage's last one, again bounded (a wait at all only
+        // where the MMAs gave up before they read them).
+        for (uint32_t back = 1; back <= (uint32_t)S::kStages && back <= it; ++back) {
+            const uint32_t s = (it - back) % S::kStages;
+            if (tails >> s & 1u) mbar_wait_bounded(&tail[s], (tail_phase >> s & 1u) ^ 1u, tc::kPairWaitCycles / 8);
+            else if (rank == 0) mbar_wait_bounded(&full[s], ((it - back) / S::kStages) & 1u, tc::kPairWaitCycles / 8);
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            uint32_t it = 0, n_item = 0;
+        if (rank == 0) {
+            uint32_t it = 0, n_item = 0, fixed_phase = 0;
             bool ok = true;
             for (int t = cluster; t < total && ok; t += clusters) {
                 const Tile x = tiles.get(t);
@@ -291,30 +297,38 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                 if (!x.rows || !kb) continue;
                 const uint32_t idesc = tc::operand_idesc(p.fmt, S::kFMn, S::kRMn, kBF * CG, x.n);
                 const uint32_t buf = n_item & 1u, d_tm = tmem + buf * kRowsMax;
-                if (!(ok = tc::pair_wait(&d_empty[buf], ((n_item >> 1) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
+                if (!(ok = tc::warp_wait(&d_empty[buf], ((n_item >> 1) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
                 tc::fence_after_sync();
                 for (int kk = 0; kk < kb; ++kk, ++it) {
                     const int s = it % S::kStages;
-                    if (!(ok = tc::pair_wait(MODE == kGradWeight ? &ready[s] : &full[s], (it / S::kStages) & 1u, &gave_up,
-                                             &g_product_err)))
-                        break;
+                    ok = tc::warp_wait(&full[s], (it / S::kStages) & 1u, &gave_up, &g_product_err);
+                    if (MODE == kGradWeight && ok && kk == kb - 1 && (x.c_len & 15)) {
+                        ok = tc::warp_wait<(CG > 1)>(&fixed[s], fixed_phase >> s & 1u, &gave_up, &g_product_err);
+                        fixed_phase ^= 1u << s;
+                    }
+                    if (!ok) break;
                     tc::fence_after_sync();
-                    const uint64_t df = tc::operand_desc(sF + s * S::kBytesF, S::kFMn, 8192);
-                    const uint64_t dr = tc::operand_desc(sR + s * S::kBytesR, S::kRMn, 8192);
-                    // 16 of the contraction per MMA: 32 bytes along K, or two atoms of eight lines
-                    const int steps = min(kBC / 16, (x.c_len - kk * kBC + 15) / 16);
-                    for (int j = 0; j < steps; ++j)
-                        tc::pair_mma<CG, tc::kKindF16>(d_tm, df + j * (S::kFMn ? 128 : 2), dr + j * (S::kRMn ? 128 : 2), idesc,
-                                                       (kk | j) != 0);
-                    tc::pair_commit<CG>(&empty[s]);
+                    if (tc::elect_one()) {
+                        const uint64_t df = tc::operand_desc(sF + s * S::kBytesF, S::kFMn, 8192);
+                        const uint64_t dr = tc::operand_desc(sR + s * S::kBytesR, S::kRMn, 8192);
+                        // 16 of the contraction per MMA: 32 bytes along K, or two atoms of eight lines
+                        const int left = x.c_len - kk * kBC;
+#pragma unroll
+                        for (int j = 0; j < kBC / 16; ++j)
+                            if (16 * j < left)
+                                tc::pair_mma<CG, tc::kKindF16>(d_tm, df + j * (S::kFMn ? 128 : 2), dr + j * (S::kRMn ? 128 : 2), idesc,
+                                                               (kk | j) != 0);
+                        tc::pair_commit<CG>(&empty[s]);
+                        if (kk == kb - 1) tc::pair_commit<CG>(&d_full[buf]);
+                    }
+                    __syncwarp();
                 }
-                if (ok) tc::pair_commit<CG>(&d_full[buf]);
                 ++n_item;
             }
         }
     } else if (warp < 2 + kEpilogueWarps) {
-        const int quad = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes 32 * quad.., columns in turn of 32
-        uint8_t *stage = smem + S::kStages * (S::kBytesF + S::kBytesR) + (warp - 2) * 32 * kStageRow;
+        const int quad = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes 32 * quad.., columns in turns of 16
+        uint8_t *stage = smem + S::kStages * (S::kBytesF + S::kBytesR) + (warp - 2) * 16 * kStageRow;
         uint32_t n_item = 0;
         bool ok = true;
         for (int t = cluster; t < total && ok; t += clusters) {
@@ -326,21 +340,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             const uint32_t buf = n_item & 1u;
             const bool zero = x.c_len == 0;
             if (!zero) {
-                ok = tc::pair_wait(&d_full[buf], (n_item >> 1) & 1u, &gave_up, &g_product_err);
-                if (!(ok = __all_sync(kFull, ok))) break;
+                if (!(ok = tc::warp_wait(&d_full[buf], (n_item >> 1) & 1u, &gave_up, &g_product_err))) break;
                 tc::fence_after_sync();
                 ++n_item;
             }
-            for (int c0 = part * 32; c0 < x.rows; c0 += 64) {
-                uint32_t v[32];
+            for (int c0 = part * 16; c0 < x.rows; c0 += 32) {
+                uint32_t v[16];
                 if (!zero) {
-                    tc::tmem_ld_frag32(tmem + ((uint32_t)(quad * 32) << 16) + buf * kRowsMax + c0, v);
-                    tc::tmem_wait_ld(v);
+                    tc::tmem_ld_frag(tmem + ((uint32_t)(quad * 32) << 16) + buf * kRowsMax + c0, v);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0;
+                    for (int j = 0; j < 16; ++j) v[j] = 0;
                 }
-                store_chunk<32>(o, stage, lane, c0, v);
+                store_chunk(o, stage, lane, c0, v);
             }
             if (!zero) {
                 tc::fence_before_sync();
@@ -352,33 +364,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             }
         }
     } else if (MODE == kGradWeight) {
-        uint32_t it = 0;
+        uint32_t it = 0, tail_phase = 0;
         bool ok = true;
         for (int t = cluster; t < total && ok; t += clusters) {
             const Tile x = tiles.get(t);
             const int kb = (x.c_len + kBC - 1) / kBC;
             if (!x.rows) continue;
-            const int half = x.n / CG, boxes = (half + 63) / 64;
-            for (int kk = 0; kk < kb; ++kk, ++it) {
-                const int s = it % S::kStages;
-                ok = tc::pair_wait(&full[s], (it / S::kStages) & 1u, &gave_up, &g_product_err);
-                if (!(ok = __all_sync(kFull, ok))) break;
-                const int valid = x.c_len - kk * kBC;
-                if (valid < kBC && (valid & 15)) {
-                    // lines (one contraction row each) from `valid` up to the last multiple of 16 that the MMAs read
-                    const int lines = 16 - (valid & 15);
-                    for (int i = lane; i < (2 + boxes) * lines * 8; i += 32) {
-                        const int box = i / (lines * 8), rest = i - box * lines * 8;
-                        uint8_t *b = box < 2 ? sF + s * S::kBytesF + box * 8192 : sR + s * S::kBytesR + (box - 2) * 8192;
-                        *reinterpret_cast<uint4 *>(b + (valid + (rest >> 3)) * 128 + (rest & 7) * 16) = make_uint4(0, 0, 0, 0);
-                    }
-                    tc::fence_proxy_async();
-                }
-                __syncwarp();
-                if (lane == 0) {
-                    if constexpr (CG == 1) tc::mbar_arrive(&ready[s]);
-                    else tc::arrive_at(tc::leader_addr(&ready[s]));
-                }
+            it += kb;
+            if (!(x.c_len & 15)) continue;
+            const int boxes = (x.n / CG + 63) / 64, s = (it - 1) % S::kStages;
+            if (!(ok = tc::warp_wait(&tail[s], tail_phase >> s & 1u, &gave_up, &g_product_err))) break;
+            tail_phase ^= 1u << s;
+            // lines (one contraction row each) from `valid` up to the last multiple of 16 that the MMAs read
+            const int valid = x.c_len - (kb - 1) * kBC, lines = 16 - (valid & 15);
+            for (int i = lane; i < (2 + boxes) * lines * 8; i += 32) {
+                const int box = i / (lines * 8), rest = i - box * lines * 8;
+                uint8_t *b = box < 2 ? sF + s * S::kBytesF + box * 8192 : sR + s * S::kBytesR + (box - 2) * 8192;
+                *reinterpret_cast<uint4 *>(b + (valid + (rest >> 3)) * 128 + (rest & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+            tc::fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (CG == 1) tc::mbar_arrive(&fixed[s]);
+                else tc::publish_at(tc::leader_addr(&fixed[s]));
             }
         }
     }
@@ -396,11 +404,34 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
 // is one block: its MMAs start a fresh accumulator, and the epilogue warps add it, times the scales, to fp32
 // sums in registers.  The scale is one per column of the accumulator (a row of x) and CTA (128 features: one
 // block of w), so warps 2-3 put xs * ws of a stage's rows into shared memory and a thread multiplies
-// pairs of columns with one packed FMA.  A block's MMAs take 512 cycles at 256 rows; its
-// promotion about 110 issue slots in each of the eight warps, two warps to a scheduler, so the MMAs bound it.
-// The sums need 128 registers a thread; warps 0-3 give theirs up (72 + 2 * 208 of 3 * 168 per thread and warpgroup).
+// pairs of columns with one packed FMA.
+//
+// The promotion bounds the widest tiles: 256 columns take the eight warps 600 cycles (the accumulator leaves TMEM at
+// about 230 bytes a cycle, measured alone), their MMAs 512.  What it needs: the number of column chunks a compile-time
+// constant (a test per chunk costs 350 cycles a block) and 16 columns a load (with 32 the sums spill).  128 sums a
+// thread leave no room for more warps: sixteen of them with half the sums spill at 96 registers and are no faster.
+//
+// Tensor memory is a ring of four slots of 128 columns; a tile of more than 128 rows takes two.  So narrow tiles have
+// four accumulators in flight, which covers the way from the MMAs to the promotion and back.
 
-constexpr int kThreadsF8 = 384, kScaleSlots = 4;
+constexpr int kThreadsF8 = 384, kSlots = 4, kSlotCols = 128;
+
+// The ring of accumulator slots as every role walks it: the same sequence of tiles gives the same slots.
+struct SlotRing {
+    uint32_t pos = 0, full_phase = 0, empty_phase = 0;  // phases: bit s is the parity of slot s's next use
+    int slot = 0;
+    __device__ __forceinline__ void next(bool wide) {
+        if (wide) pos = (pos + 1) & ~1u;
+        slot = (int)(pos & (kSlots - 1));
+        pos += wide ? 2 : 1;
+    }
+    __device__ __forceinline__ uint32_t full() const { return (full_phase >> slot) & 1u; }
+    __device__ __forceinline__ uint32_t empty(int s) const { return ((empty_phase >> s) & 1u) ^ 1u; }
+    __device__ __forceinline__ void used(bool wide) {
+        full_phase ^= 1u << slot;
+        empty_phase ^= (wide ? 3u : 1u) << slot;
+    }
+};
 
 struct F8Params {
     TcParams t;
@@ -414,12 +445,77 @@ struct ShapeF8 {
     static constexpr int kBytesF = kBF * kBC8, kBytesR = kRowsMax / CG * kBC8;
     static constexpr int kStages = CG == 1 ? 4 : 6;
     static constexpr size_t kOperands = (size_t)kStages * (kBytesF + kBytesR);
-    static constexpr size_t kSmem = 1024 + kOperands + kEpilogueWarps * 16 * kStageRow + kScaleSlots * kRowsMax * sizeof(float);
+    static constexpr size_t kSmem = 1024 + kOperands + kEpilogueWarps * 16 * kStageRow + kSlots * kSlotCols * sizeof(float);
 };
 
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t)lo | ((uint64_t)hi << 32); }
 __device__ __forceinline__ void fma2(uint64_t &acc, uint64_t a, uint64_t b) {
     asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(a), "l"(b));
+}
+
+// What a promotion warp needs of its CTA.
+struct F8Sync {
+    uint64_t *d_full, *d_empty, *sc_empty;
+    const float *scales;
+    uint8_t *stage;
+    uint32_t lanes;  // TMEM address of the warp's lanes
+    volatile int *gave_up;
+};
+
+// One tile by one promotion warp: NCH chunks of 32 columns, from 32 * part in turns of 64.  Returns false after a wait gave up.
+template <int CG, int NCH>
+__device__ __forceinline__ bool promote_tile(const F8Sync &y, SlotRing &ring, const OutTile &o, int kb, bool wide, int part,
+                                             int lane) {
+    uint64_t acc[NCH ? 2 * NCH : 1][8];  // 16 columns, pairs of columns in fragment order: 0.0f
+#pragma unroll
+    for (int h = 0; h < 2 * NCH; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[h][i] = 0;
+    auto column = [&](int h) { return (2 * (h >> 1) + part) * 32 + 16 * (h & 1); };
+    for (int kk = 0; kk < kb; ++kk) {
+        ring.next(wide);
+        const int slot = ring.slot;
+        if (!tc::warp_wait(&y.d_full[slot], ring.full(), y.gave_up, &g_product_err)) return false;
+        tc::fence_after_sync();
+        const float *sc = y.scales + slot * kSlotCols + 2 * (lane & 3);
+        const uint32_t src = y.lanes + slot * kSlotCols;
+#pragma unroll
+        for (int h = 0; h < 2 * NCH; ++h) {
+            uint32_t v[16];
+            tc::tmem_ld_frag(src + column(h), v);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint64_t s2 = *reinterpret_cast<const uint64_t *>(sc + column(h) + 8 * i);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int e = 8 * (q >> 1) + 4 * i + 2 * (q & 1);
+                    fma2(acc[h][e >> 1], pack2(v[e], v[e + 1]), s2);
+                }
+            }
+        }
+        tc::fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+            const int slots = wide ? 2 : 1;
+            for (int s = slot; s < slot + slots; ++s) {
+                if constexpr (CG == 1) tc::mbar_arrive(&y.d_empty[s]);
+                else tc::arrive_at(tc::leader_addr(&y.d_empty[s]));
+                tc::mbar_arrive(&y.sc_empty[s]);
+            }
+        }
+        ring.used(wide);
+    }
+#pragma unroll
+    for (int h = 0; h < 2 * NCH; ++h) {
+        uint32_t v[16];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            v[2 * i] = (uint32_t)acc[h][i];
+            v[2 * i + 1] = (uint32_t)(acc[h][i] >> 32);
+        }
+        store_chunk(o, y.stage, lane, column(h), v);
+    }
+    return true;
 }
 
 template <int CG>
@@ -428,12 +524,12 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     using S = ShapeF8<CG>;
     const TcParams &p = fp.t;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     uint8_t *sF = smem, *sR = smem + S::kStages * S::kBytesF;
-    float *sScale = reinterpret_cast<float *>(smem + S::kOperands);  // [slot][row of the tile]
-    uint8_t *staging = smem + S::kOperands + kScaleSlots * kRowsMax * sizeof(float);
-    __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[2], d_empty[2], sc_full[kScaleSlots],
-        sc_empty[kScaleSlots];
+    float *scales = reinterpret_cast<float *>(smem + S::kOperands);  // [slot][column]: xs * ws
+    uint8_t *staging = smem + S::kOperands + kSlots * kSlotCols * sizeof(float);
+    // d_full: a slot's MMAs and its scales; d_empty: read by both CTAs' warps; sc_empty: by this one's
+    __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[kSlots], d_empty[kSlots], sc_empty[kSlots];
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up;
     __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
@@ -449,12 +545,9 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
-            mbar_init(&d_full[b], 1);
-            mbar_init(&d_empty[b], CG * kEpilogueWarps);
-        }
-        for (int s = 0; s < kScaleSlots; ++s) {
-            mbar_init(&sc_full[s], 1);
+        for (int s = 0; s < kSlots; ++s) {
+            mbar_init(&d_full[s], 2);
+            mbar_init(&d_empty[s], CG * kEpilogueWarps);
             mbar_init(&sc_empty[s], kEpilogueWarps);
         }
     }
@@ -470,159 +563,128 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     const int total = prefix[p.groups], kb = (p.contraction + S::kBC8 - 1) / S::kBC8;
     const Tiles<CG, kForward> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
-    if (warp < 4) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        if (warp == 0) {
-            if (lane == 0) {
-                uint32_t it = 0;
-                bool ok = true;
-                for (int t = cluster; t < total && ok; t += clusters) {
-                    const Tile x = tiles.get(t);
-                    if (!x.rows) continue;
-                    const int half = x.n / CG, boxes = (half + kRowBox - 1) / kRowBox;
-                    const uint32_t bytes = S::kBytesF + boxes * kRowBox * S::kBC8;
-                    const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
-                    for (int kk = 0; kk < kb; ++kk, ++it) {
-                        const int s = it % S::kStages;
-                        if (!(ok = tc::pair_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
-                        uint32_t bar = smem_u32(&full[s]);
-                        if (rank == 0) mbar_expect_tx(&full[s], CG * bytes);
-                        if (CG > 1) bar = tc::leader_addr(&full[s]);
-                        tc::pair_tma_3d<CG>(sF + s * S::kBytesF, &map_f, kk * S::kBC8, f0, x.g, bar);
-                        for (int b = 0; b < boxes; ++b)
-                            tc::pair_tma_2d<CG>(sR + s * S::kBytesR + b * kRowBox * S::kBC8, &map_r, kk * S::kBC8, r0 + kRowBox * b, bar);
-                    }
-                }
-                if (rank == 0)  // as in k_product_tc: no exit under copies in flight
-                    for (uint32_t back = 1; back <= (uint32_t)S::kStages && back <= it; ++back)
-                        mbar_wait_bounded(&full[(it - back) % S::kStages], ((it - back) / S::kStages) & 1u, tc::kPairWaitCycles / 8);
-            }
-        } else if (warp == 1) {
-            if (lane == 0 && rank == 0) {
-                uint32_t it = 0;
-                bool ok = true;
-                for (int t = cluster; t < total && ok; t += clusters) {
-                    const Tile x = tiles.get(t);
-                    if (!x.rows) continue;
-                    const uint32_t idesc = tc::operand_idesc(0, false, false, kBF * CG, x.n);
-                    for (int kk = 0; kk < kb; ++kk, ++it) {
-                        const int s = it % S::kStages;
-                        const uint32_t buf = it & 1u, d_tm = tmem + buf * kRowsMax;
-                        if (!(ok = tc::pair_wait(&d_empty[buf], ((it >> 1) & 1u) ^ 1u, &gave_up, &g_product_err) &&
-                                   tc::pair_wait(&full[s], (it / S::kStages) & 1u, &gave_up, &g_product_err)))
-                            break;
-                        tc::fence_after_sync();
-                        const uint64_t df = tc::operand_desc(sF + s * S::kBytesF, false, 0);
-                        const uint64_t dr = tc::operand_desc(sR + s * S::kBytesR, false, 0);
-                        const int steps = min(S::kBC8 / 32, (p.contraction - kk * S::kBC8 + 31) / 32);
-                        for (int j = 0; j < steps; ++j)
-                            tc::pair_mma<CG, tc::kKindF8>(d_tm, df + 2 * j, dr + 2 * j, idesc, j != 0);
-                        tc::pair_commit<CG>(&empty[s]);
-                        tc::pair_commit<CG>(&d_full[buf]);
-                    }
-                }
-            }
-        } else {
-            // ---- scales: warps 2 and 3 take turns; each loads its next stage's before it waits for a slot ----
-            uint32_t it = 0;
-            bool ok = true;
-            for (int t = cluster; t < total && ok; t += clusters) {
-                const Tile x = tiles.get(t);
-                if (!x.rows) continue;
-                const int f0 = x.f0 + (int)rank * kBF;
-                const float *ws = fp.ws + x.g * fp.ws_group + (int64_t)(f0 / kScaleBlock) * fp.ws_row;
-                const float *xs = fp.xs + (int64_t)(x.row0 + lane) * fp.xs_row;
-                const bool on = f0 < p.features;  // the pair's second half may lie behind the last feature
-                float v[8], w = 0.0f;
-                auto fetch = [&](int kk) {
-                    if (kk >= kb) return;
-                    w = on ? __ldg(ws + kk * fp.ws_blk) : 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        v[i] = lane + 32 * i < x.rows ? __ldg(xs + (int64_t)(32 * i) * fp.xs_row + kk * fp.xs_blk) : 0.0f;
-                };
-                int kk = (int)((it ^ (uint32_t)warp) & 1u);  // the first stage of this tile with it + kk of this warp's parity
-                fetch(kk);
-                for (; kk < kb; kk += 2) {
-                    const uint32_t i_ = it + kk, slot = i_ % kScaleSlots;
-                    float s8[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) s8[i] = v[i] * w;
-                    fetch(kk + 2);
-                    ok = tc::pair_wait(&sc_empty[slot], ((i_ / kScaleSlots) & 1u) ^ 1u, &gave_up, &g_product_err);
-                    if (!(ok = __all_sync(kFull, ok))) break;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) sScale[slot * kRowsMax + lane + 32 * i] = s8[i];
-                    __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&sc_full[slot]);
-                }
-                it += kb;
-            }
-        }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int quad = warp & 3, part = (warp - 4) >> 2;  // TMEM lanes 32 * quad.., chunks of 32 columns in turn
-        uint8_t *stage = staging + (warp - 4) * 16 * kStageRow;
+    if (warp == 0) {
         uint32_t it = 0;
         bool ok = true;
         for (int t = cluster; t < total && ok; t += clusters) {
             const Tile x = tiles.get(t);
             if (!x.rows) continue;
-            uint64_t acc[4][16];  // chunk, [16-lane half][8 columns][8-lane half] pairs of columns: 0.0f
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) acc[c][i] = 0;
+            const int half = x.n / CG, boxes = (half + kRowBox - 1) / kRowBox;
+            const uint32_t bytes = S::kBytesF + boxes * kRowBox * S::kBC8;
+            const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
             for (int kk = 0; kk < kb; ++kk, ++it) {
-                const uint32_t buf = it & 1u, slot = it % kScaleSlots;
-                ok = tc::pair_wait(&d_full[buf], (it >> 1) & 1u, &gave_up, &g_product_err) &&
-                     tc::pair_wait(&sc_full[slot], (it / kScaleSlots) & 1u, &gave_up, &g_product_err);
-                if (!(ok = __all_sync(kFull, ok))) break;
-                tc::fence_after_sync();
-                const float *sc = sScale + slot * kRowsMax + 2 * (lane & 3);
-                const uint32_t src = tmem + ((uint32_t)(quad * 32) << 16) + buf * kRowsMax;
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int c0 = (2 * c + part) * 32;
-                    if (c0 < x.n) {
-                        uint32_t v[32];
-                        tc::tmem_ld_frag32(src + c0, v);
-                        tc::tmem_wait_ld(v);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const uint64_t s2 = *reinterpret_cast<const uint64_t *>(sc + c0 + 8 * i);
-#pragma unroll
-                            for (int q = 0; q < 4; ++q) {
-                                const int e = 16 * (q >> 1) + 4 * i + 2 * (q & 1);
-                                fma2(acc[c][e >> 1], pack2(v[e], v[e + 1]), s2);
-                            }
-                        }
-                    }
+                const int s = it % S::kStages;
+                if (!(ok = tc::warp_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
+                if (tc::elect_one()) {
+                    uint32_t bar = smem_u32(&full[s]);
+                    if (rank == 0) mbar_expect_tx(&full[s], CG * bytes);
+                    if (CG > 1) bar = tc::leader_addr(&full[s]);
+                    tc::pair_tma_3d<CG>(sF + s * S::kBytesF, &map_f, kk * S::kBC8, f0, x.g, bar);
+                    for (int b = 0; b < boxes; ++b)
+                        tc::pair_tma_2d<CG>(sR + s * S::kBytesR + b * kRowBox * S::kBC8, &map_r, kk * S::kBC8, r0 + kRowBox * b, bar);
                 }
-                tc::fence_before_sync();
                 __syncwarp();
-                if (lane == 0) {
-                    if constexpr (CG == 1) tc::mbar_arrive(&d_empty[buf]);
-                    else tc::arrive_at(tc::leader_addr(&d_empty[buf]));
-                    tc::mbar_arrive(&sc_empty[slot]);
+            }
+        }
+        if (rank == 0)  // as in k_product_tc: no exit under copies in flight
+            for (uint32_t back = 1; back <= (uint32_t)S::kStages && back <= it; ++back)
+                mbar_wait_bounded(&full[(it - back) % S::kStages], ((it - back) / S::kStages) & 1u, tc::kPairWaitCycles / 8);
+    } else if (warp == 1) {
+        if (rank == 0) {
+            uint32_t it = 0;
+            SlotRing ring;
+            bool ok = true;
+            for (int t = cluster; t < total && ok; t += clusters) {
+                const Tile x = tiles.get(t);
+                if (!x.rows) continue;
+                const bool wide = x.n > kSlotCols;
+                const uint32_t idesc = tc::operand_idesc(0, false, false, kBF * CG, x.n);
+                for (int kk = 0; kk < kb; ++kk, ++it) {
+                    const int s = it % S::kStages;
+                    ring.next(wide);
+                    const int slot = ring.slot;
+                    ok = tc::warp_wait(&d_empty[slot], ring.empty(slot), &gave_up, &g_product_err) &&
+                         (!wide || tc::warp_wait(&d_empty[slot + 1], ring.empty(slot + 1), &gave_up, &g_product_err)) &&
+                         tc::warp_wait(&full[s], (it / S::kStages) & 1u, &gave_up, &g_product_err);
+                    if (!ok) break;
+                    tc::fence_after_sync();
+                    if (tc::elect_one()) {
+                        const uint64_t df = tc::operand_desc(sF + s * S::kBytesF, false, 0);
+                        const uint64_t dr = tc::operand_desc(sR + s * S::kBytesR, false, 0);
+                        const int left = p.contraction - kk * S::kBC8;
+#pragma unroll
+                        for (int j = 0; j < S::kBC8 / 32; ++j)
+                            if (32 * j < left)
+                                tc::pair_mma<CG, tc::kKindF8>(tmem + slot * kSlotCols, df + 2 * j, dr + 2 * j, idesc, j != 0);
+                        tc::pair_commit<CG>(&empty[s]);
+                        tc::pair_commit<CG>(&d_full[slot]);
+                    }
+                    __syncwarp();
+                    ring.used(wide);
                 }
             }
-            if (!ok) break;
+        }
+    } else if (warp < 4) {
+        // ---- scales: the two warps take turns; each loads its next stage's before it waits for a slot ----
+        uint32_t it = 0;
+        SlotRing ring;
+        bool ok = true;
+        for (int t = cluster; t < total && ok; t += clusters) {
+            const Tile x = tiles.get(t);
+            if (!x.rows) continue;
+            const bool wide = x.n > kSlotCols;
+            const int f0 = x.f0 + (int)rank * kBF;
+            const float *ws = fp.ws + x.g * fp.ws_group + (int64_t)(f0 / kScaleBlock) * fp.ws_row;
+            const float *xs = fp.xs + (int64_t)(x.row0 + lane) * fp.xs_row;
+            const bool on = f0 < p.features;  // the pair's second half may lie behind the last feature
+            float v[8], w = 0.0f;
+            auto fetch = [&](int kk) {
+                if (kk >= kb) return;
+                w = on ? __ldg(ws + kk * fp.ws_blk) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    v[i] = lane + 32 * i < x.rows ? __ldg(xs + (int64_t)(32 * i) * fp.xs_row + kk * fp.xs_blk) : 0.0f;
+            };
+            const int mine = (int)((it ^ (uint32_t)warp) & 1u);  // the first stage of this tile that is this warp's
+            fetch(mine);
+            for (int kk = 0; kk < kb; ++kk, ++it) {
+                ring.next(wide);
+                if ((kk & 1) == mine) {
+                    const int slot = ring.slot;
+                    float s8[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) s8[i] = v[i] * w;
+                    fetch(kk + 2);
+                    ok = tc::warp_wait(&sc_empty[slot], ring.empty(slot), &gave_up, &g_product_err) &&
+                         (!wide || tc::warp_wait(&sc_empty[slot + 1], ring.empty(slot + 1), &gave_up, &g_product_err));
+                    if (!ok) break;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (wide || i < 4) scales[slot * kSlotCols + lane + 32 * i] = s8[i];
+                    __syncwarp();
+                    if (lane == 0) tc::mbar_arrive(&d_full[slot]);
+                }
+                ring.used(wide);
+            }
+        }
+    } else {
+        const int quad = warp & 3, part = (warp - 4) >> 2;  // TMEM lanes 32 * quad.., chunks of 32 columns in turns
+        const F8Sync y{d_full, d_empty, sc_empty, scales, staging + (warp - 4) * 16 * kStageRow, tmem + ((uint32_t)(quad * 32) << 16),
+                       &gave_up};
+        SlotRing ring;
+        bool ok = true;
+        for (int t = cluster; t < total && ok; t += clusters) {
+            const Tile x = tiles.get(t);
+            if (!x.rows) continue;
+            const bool wide = x.n > kSlotCols;
             const int f = x.f0 + (int)rank * kBF + quad * 32;
             const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, x.rows, p.vec != 0};
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int c0 = (2 * c + part) * 32;
-                if (c0 < x.rows) {
-                    uint32_t v[32];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        v[2 * i] = (uint32_t)acc[c][i];
-                        v[2 * i + 1] = (uint32_t)(acc[c][i] >> 32);
-                    }
-                    store_chunk<16>(o, stage, lane, c0, v);
-                }
-            }
+            const int chunks = (x.n - 32 * part + 63) / 64;  // columns 32 * part + 64 * c that lie below n
+            if (chunks <= 0) ok = promote_tile<CG, 0>(y, ring, o, kb, wide, part, lane);
+            else if (chunks == 1) ok = promote_tile<CG, 1>(y, ring, o, kb, wide, part, lane);
+            else if (chunks == 2) ok = promote_tile<CG, 2>(y, ring, o, kb, wide, part, lane);
+            else if (chunks == 3) ok = promote_tile<CG, 3>(y, ring, o, kb, wide, part, lane);
+            else ok = promote_tile<CG, 4>(y, ring, o, kb, wide, part, lane);
         }
     }
     __syncwarp();
