@@ -53,12 +53,12 @@ __device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t a_desc, uint6
 
 // Arrive on `bar` (of both CTAs of a pair, at the same offset) once every MMA issued so far has completed.
 template <int CG>
-__device__ __forceinline__ void pair_commit(uint64_t *bar) {
-    if constexpr (CG == 1) mma_commit(bar);
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
+    if constexpr (CG == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
     else
         asm volatile(
-            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
-                smem_u32(bar)),
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
             "h"((uint16_t)3)
             : "memory");
 }
@@ -89,38 +89,44 @@ __device__ __forceinline__ void publish_at(uint32_t cluster_addr) {
 
 // Tiled TMA loads into this CTA that complete on the barrier at shared::cluster address `bar` (this CTA's, or its leader's).
 template <int CG>
-__device__ __forceinline__ void pair_tma_2d(void *dst, const void *tmap, int x, int y, uint32_t bar) {
+__device__ __forceinline__ void pair_tma_2d(uint32_t dst, const void *tmap, int x, int y, uint32_t bar) {
     if constexpr (CG == 1)
         asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-                     "[%4];" ::"r"(smem_u32(dst)),
+                     "[%4];" ::"r"(dst),
                      "l"(tmap), "r"(x), "r"(y), "r"(bar)
                      : "memory");
     else
         asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
-                     "{%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+                     "{%2, %3}], [%4];" ::"r"(dst),
                      "l"(tmap), "r"(x), "r"(y), "r"(bar)
                      : "memory");
 }
 template <int CG>
-__device__ __forceinline__ void pair_tma_3d(void *dst, const void *tmap, int x, int y, int z, uint32_t bar) {
+__device__ __forceinline__ void pair_tma_3d(uint32_t dst, const void *tmap, int x, int y, int z, uint32_t bar) {
     if constexpr (CG == 1)
         asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-                     "%4}], [%5];" ::"r"(smem_u32(dst)),
+                     "%4}], [%5];" ::"r"(dst),
                      "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
                      : "memory");
     else
         asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, "
-                     "{%2, %3, %4}], [%5];" ::"r"(smem_u32(dst)),
+                     "{%2, %3, %4}], [%5];" ::"r"(dst),
                      "l"(tmap), "r"(x), "r"(y), "r"(z), "r"(bar)
                      : "memory");
+}
+
+// The same for a barrier or buffer given by its address in this CTA.
+__device__ __forceinline__ uint32_t leader_addr(uint32_t p) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(p));
+    return a;
 }
 
 // Shared-memory matrix descriptor, 128-byte swizzle, 1024-byte atoms of eight 128-byte lines.
 //   K-major:  a line is 128 bytes of K of one row; atoms of eight rows follow one another
 //   MN-major: a line is 64 16-bit values of M (or N) at one k; atoms of eight k follow one another,
 //             the next 64 values of M (or N) start `block` bytes on
-__device__ __forceinline__ uint64_t operand_desc(const void *p, bool mn_major, uint32_t block) {
-    const uint64_t addr = smem_u32(p);
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn_major, uint32_t block) {
     return ((addr & 0x3FFFFull) >> 4) | ((uint64_t)(mn_major ? block >> 4 : 1u) << 16) | (64ull << 32) | (1ull << 46) |
            (2ull << 61);
 }
@@ -156,6 +162,13 @@ __device__ __forceinline__ void stmatrix_trans4(void *row, uint32_t a, uint32_t 
                  : "memory");
 }
 
+__device__ __forceinline__ void expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
 // True in one lane of a converged warp.  The copies and MMAs are issued under it and not under a test of the
 // lane: their operands then stay in uniform registers (four MMAs took 490 cycles to issue under `lane == 0`).
 __device__ __forceinline__ bool elect_one() {
@@ -166,47 +179,40 @@ __device__ __forceinline__ bool elect_one() {
 
 // ---- bounded waits -----------------------------------------------------------------------------
 //
-// About a second; then the wait marks its CTA as given up (every later wait of the CTA returns at once, so
-// that the kernel ends) and records it in `err`.
+// A wait that has not ended after about a second marks its CTA as given up (`gave_up`, shared memory): every other
+// wait of the CTA then returns at once, so that the kernel ends; its loops look at the mark once per tile.  One asm
+// block without results: as a function with a verdict, tested and voted on after every call, a wait for a complete
+// phase took 250 cycles instead of 50.
 constexpr long long kPairWaitCycles = 2000000000ll;
 
-// ACROSS: the barrier hands over what the other CTA's threads wrote (publish_at); an acquire of cluster scope
-// costs about 200 cycles even where the phase is complete, so the other waits stay at this CTA's scope.
-template <bool ACROSS = false>
-__device__ __forceinline__ bool pair_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up, uint32_t *err) {
-    const uint32_t a = smem_u32(bar);
-    long long t0 = 0;
-    while (true) {
-        uint32_t done;
-        if constexpr (ACROSS)
-            asm volatile(
-                "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2; selp.u32 %0, 1, 0, p; }"
-                : "=r"(done)
-                : "r"(a), "r"(parity)
-                : "memory");
-        else
-            asm volatile(
-                "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3; selp.u32 %0, 1, 0, p; }"
-                : "=r"(done)
-                : "r"(a), "r"(parity), "r"(1000000u)
-                : "memory");
-        if (done) return true;
-        if (*gave_up) return false;
-        const long long t = clock64();
-        if (!t0) t0 = t;
-        if (t - t0 > kPairWaitCycles) {
-            *gave_up = 1;
-            atomicOr(err, 1u);
-            return false;
-        }
-    }
-}
+#define UMSX_WAIT(sem)                                                                                            \
+    asm volatile(                                                                                                 \
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 g;\n\t.reg .b64 t0, t;\n\t"                                          \
+        "mbarrier.try_wait.parity" sem ".shared::cta.b64 p, [%0], %1;\n\t"                                        \
+        "@p bra DONE;\n\tmov.u64 t0, %%clock64;\n"                                                               \
+        "AGAIN:\n\tmbarrier.try_wait.parity" sem ".shared::cta.b64 p, [%0], %1;\n\t"                             \
+        "@p bra DONE;\n\tld.volatile.shared.b32 g, [%2];\n\tsetp.ne.b32 q, g, 0;\n\t@q bra DONE;\n\t"            \
+        "mov.u64 t, %%clock64;\n\tsub.s64 t, t, t0;\n\tsetp.lt.s64 q, t, %3;\n\t@q bra AGAIN;\n\t"              \
+        "st.volatile.shared.b32 [%2], 1;\nDONE:\n\t}" ::"r"(bar), "r"(parity), "r"(gave_up), "l"(kPairWaitCycles) \
+        : "memory")
 
-// The same by a whole warp: one answer for all lanes.
+// bar, gave_up: shared-memory addresses.  ACROSS: the barrier hands over what the other CTA's threads wrote
+// (publish_at); an acquire of cluster scope costs about 200 cycles more, so the other waits stay at this CTA's scope.
 template <bool ACROSS = false>
-__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, volatile int *gave_up, uint32_t *err) {
-    return __all_sync(kFull, pair_wait<ACROSS>(bar, parity, gave_up, err));
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, uint32_t gave_up) {
+    if constexpr (ACROSS) UMSX_WAIT(".acquire.cluster");
+    else UMSX_WAIT("");
 }
+#undef UMSX_WAIT
+
+// A ring position: stage and the parity of its next use.
+template <int STAGES>
+struct Ring {
+    uint32_t s = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++s == STAGES) s = 0, phase ^= 1u;
+    }
+};
 
 }  // namespace tc
 }  // namespace umsx

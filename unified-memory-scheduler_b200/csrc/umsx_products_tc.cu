@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     uint8_t *sF = smem, *sR = smem + S::kStages * S::kBytesF;
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[2], d_empty[2];
     // dw, a tile's ragged last stage: its copies to this CTA, and both CTAs' zeroing
-    __shared__ __align__(8) uint64_t tail[S::kStages], fixed[S::kStages];
+    __shared__ __align__(8) uint64_t tail[S::kStages], fixed[S::kStages], last;
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up;
     __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
@@ -218,6 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             mbar_init(&fixed[s], CG);
             mbar_init(&empty[s], 1);
         }
+        mbar_init(&last, 1);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&d_full[b], 1);
             mbar_init(&d_empty[b], CG * kEpilogueWarps);
@@ -235,10 +236,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     const int total = prefix[p.groups];
     const Tiles<CG, MODE> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
+    const uint32_t up = smem_u32(&gave_up), aF = smem_u32(sF), aR = smem_u32(sR);
+    const uint32_t b_full = smem_u32(full), b_empty = smem_u32(empty), b_dfull = smem_u32(d_full), b_dempty = smem_u32(d_empty),
+                   b_tail = smem_u32(tail), b_fixed = smem_u32(fixed);
+    volatile int *const stop = &gave_up;
+
     if (warp == 0) {
-        uint32_t it = 0, tails = 0, tail_phase = 0;  // bit s: stage s holds a ragged end; uses of tail[s], mod 2
-        bool ok = true;
-        for (int t = cluster; t < total && ok; t += clusters) {
+        tc::Ring<S::kStages> r;
+        uint32_t tails = 0, tail_phase = 0, used = 0;  // bit s: stage s holds a ragged end; uses of tail[s], mod 2; stages in use
+        for (int t = cluster; t < total && !*stop; t += clusters) {
             const Tile x = tiles.get(t);
             const int kb = (x.c_len + kBC - 1) / kBC;
             if (!x.rows) continue;
@@ -246,23 +252,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             const int boxes = S::kRMn ? (half + 63) / 64 : (half + kRowBox - 1) / kRowBox;
             const uint32_t bytes = S::kBytesF + boxes * (S::kRMn ? 64 : kRowBox) * kBC * 2;
             const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
-            for (int kk = 0; kk < kb; ++kk, ++it) {
-                const int s = it % S::kStages;
-                if (!(ok = tc::warp_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
+            for (int kk = 0; kk < kb; ++kk, r.next()) {
+                tc::wait(b_empty + 8 * r.s, r.phase ^ 1u, up);
                 const bool ragged = MODE == kGradWeight && kk == kb - 1 && (x.c_len & 15);
-                if (ragged) tails |= 1u << s, tail_phase ^= 1u << s;
-                else tails &= ~(1u << s);
+                used |= 1u << r.s;
+                if (ragged) tails |= 1u << r.s, tail_phase ^= 1u << r.s;
+                else tails &= ~(1u << r.s);
                 if (tc::elect_one()) {
-                    uint32_t bar = smem_u32(ragged ? &tail[s] : &full[s]);
+                    uint32_t bar = (ragged ? b_tail : b_full) + 8 * r.s;
                     if (ragged) {
-                        mbar_expect_tx(&tail[s], bytes);  // each CTA's own, for its warp 10
-                        if (rank == 0) tc::mbar_arrive(&full[s]);
+                        tc::expect_tx(bar, bytes);  // each CTA's own, for its warp 10
+                        if (rank == 0) tc::arrive(b_full + 8 * r.s);
                     } else {
-                        if (rank == 0) mbar_expect_tx(&full[s], CG * bytes);
-                        if (CG > 1) bar = tc::leader_addr(&full[s]);
+                        if (rank == 0) tc::expect_tx(bar, CG * bytes);
+                        if (CG > 1) bar = tc::leader_addr(bar);
                     }
                     const int c = x.c0 + kk * kBC;
-                    uint8_t *dF = sF + s * S::kBytesF, *dR = sR + s * S::kBytesR;
+                    const uint32_t dF = aF + r.s * S::kBytesF, dR = aR + r.s * S::kBytesR;
                     if constexpr (MODE == kForward) {
                         tc::pair_tma_3d<CG>(dF, &map_f, c, f0, x.g, bar);
                     } else {
@@ -282,35 +288,32 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
         }
         // A CTA must not exit under copies in flight: each stage's last one, again bounded (a wait at all only
         // where the MMAs gave up before they read them).
-        for (uint32_t back = 1; back <= (uint32_t)S::kStages && back <= it; ++back) {
-            const uint32_t s = (it - back) % S::kStages;
+        for (uint32_t s = 0; s < (uint32_t)S::kStages; ++s) {
+            if (!(used >> s & 1u)) continue;
             if (tails >> s & 1u) mbar_wait_bounded(&tail[s], (tail_phase >> s & 1u) ^ 1u, tc::kPairWaitCycles / 8);
-            else if (rank == 0) mbar_wait_bounded(&full[s], ((it - back) / S::kStages) & 1u, tc::kPairWaitCycles / 8);
+            else if (rank == 0) mbar_wait_bounded(&full[s], r.phase ^ (s >= r.s ? 1u : 0u), tc::kPairWaitCycles / 8);
         }
     } else if (warp == 1) {
         if (rank == 0) {
-            uint32_t it = 0, n_item = 0, fixed_phase = 0;
-            bool ok = true;
-            for (int t = cluster; t < total && ok; t += clusters) {
+            tc::Ring<S::kStages> r;
+            uint32_t n_item = 0, fixed_phase = 0;
+            for (int t = cluster; t < total && !*stop; t += clusters) {
                 const Tile x = tiles.get(t);
                 const int kb = (x.c_len + kBC - 1) / kBC;
                 if (!x.rows || !kb) continue;
                 const uint32_t idesc = tc::operand_idesc(p.fmt, S::kFMn, S::kRMn, kBF * CG, x.n);
                 const uint32_t buf = n_item & 1u, d_tm = tmem + buf * kRowsMax;
-                if (!(ok = tc::warp_wait(&d_empty[buf], ((n_item >> 1) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
-                tc::fence_after_sync();
-                for (int kk = 0; kk < kb; ++kk, ++it) {
-                    const int s = it % S::kStages;
-                    ok = tc::warp_wait(&full[s], (it / S::kStages) & 1u, &gave_up, &g_product_err);
-                    if (MODE == kGradWeight && ok && kk == kb - 1 && (x.c_len & 15)) {
-                        ok = tc::warp_wait<(CG > 1)>(&fixed[s], fixed_phase >> s & 1u, &gave_up, &g_product_err);
-                        fixed_phase ^= 1u << s;
+                tc::wait(b_dempty + 8 * buf, ((n_item >> 1) & 1u) ^ 1u, up);
+                for (int kk = 0; kk < kb; ++kk, r.next()) {
+                    tc::wait(b_full + 8 * r.s, r.phase, up);
+                    if (MODE == kGradWeight && kk == kb - 1 && (x.c_len & 15)) {
+                        tc::wait<(CG > 1)>(b_fixed + 8 * r.s, fixed_phase >> r.s & 1u, up);
+                        fixed_phase ^= 1u << r.s;
                     }
-                    if (!ok) break;
                     tc::fence_after_sync();
                     if (tc::elect_one()) {
-                        const uint64_t df = tc::operand_desc(sF + s * S::kBytesF, S::kFMn, 8192);
-                        const uint64_t dr = tc::operand_desc(sR + s * S::kBytesR, S::kRMn, 8192);
+                        const uint64_t df = tc::operand_desc(aF + r.s * S::kBytesF, S::kFMn, 8192);
+                        const uint64_t dr = tc::operand_desc(aR + r.s * S::kBytesR, S::kRMn, 8192);
                         // 16 of the contraction per MMA: 32 bytes along K, or two atoms of eight lines
                         const int left = x.c_len - kk * kBC;
 #pragma unroll
@@ -318,20 +321,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                             if (16 * j < left)
                                 tc::pair_mma<CG, tc::kKindF16>(d_tm, df + j * (S::kFMn ? 128 : 2), dr + j * (S::kRMn ? 128 : 2), idesc,
                                                                (kk | j) != 0);
-                        tc::pair_commit<CG>(&empty[s]);
-                        if (kk == kb - 1) tc::pair_commit<CG>(&d_full[buf]);
+                        tc::pair_commit<CG>(b_empty + 8 * r.s);
+                        if (kk == kb - 1) tc::pair_commit<CG>(b_dfull + 8 * buf);
                     }
                     __syncwarp();
                 }
                 ++n_item;
             }
+            // nor under MMAs in flight
+            if (tc::elect_one()) tc::pair_commit<CG>(smem_u32(&last));
+            mbar_wait_bounded(&last, 0, tc::kPairWaitCycles / 8);
         }
     } else if (warp < 2 + kEpilogueWarps) {
         const int quad = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes 32 * quad.., columns in turns of 16
         uint8_t *stage = smem + S::kStages * (S::kBytesF + S::kBytesR) + (warp - 2) * 16 * kStageRow;
         uint32_t n_item = 0;
-        bool ok = true;
-        for (int t = cluster; t < total && ok; t += clusters) {
+        for (int t = cluster; t < total && !*stop; t += clusters) {
             const Tile x = tiles.get(t);
             if (!x.rows) continue;
             const int f = x.f0 + (int)rank * kBF + quad * 32;
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             const uint32_t buf = n_item & 1u;
             const bool zero = x.c_len == 0;
             if (!zero) {
-                if (!(ok = tc::warp_wait(&d_full[buf], (n_item >> 1) & 1u, &gave_up, &g_product_err))) break;
+                tc::wait(b_dfull + 8 * buf, (n_item >> 1) & 1u, up);
                 tc::fence_after_sync();
                 ++n_item;
             }
@@ -358,22 +363,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
-                    if constexpr (CG == 1) tc::mbar_arrive(&d_empty[buf]);
-                    else tc::arrive_at(tc::leader_addr(&d_empty[buf]));
+                    if constexpr (CG == 1) tc::arrive(b_dempty + 8 * buf);
+                    else tc::arrive_at(tc::leader_addr(b_dempty + 8 * buf));
                 }
             }
         }
     } else if (MODE == kGradWeight) {
         uint32_t it = 0, tail_phase = 0;
-        bool ok = true;
-        for (int t = cluster; t < total && ok; t += clusters) {
+        for (int t = cluster; t < total && !*stop; t += clusters) {
             const Tile x = tiles.get(t);
             const int kb = (x.c_len + kBC - 1) / kBC;
             if (!x.rows) continue;
             it += kb;
             if (!(x.c_len & 15)) continue;
             const int boxes = (x.n / CG + 63) / 64, s = (it - 1) % S::kStages;
-            if (!(ok = tc::warp_wait(&tail[s], tail_phase >> s & 1u, &gave_up, &g_product_err))) break;
+            tc::wait(b_tail + 8 * s, tail_phase >> s & 1u, up);
             tail_phase ^= 1u << s;
             // lines (one contraction row each) from `valid` up to the last multiple of 16 that the MMAs read
             const int valid = x.c_len - (kb - 1) * kBC, lines = 16 - (valid & 15);
@@ -385,11 +389,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             tc::fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (CG == 1) tc::mbar_arrive(&fixed[s]);
-                else tc::publish_at(tc::leader_addr(&fixed[s]));
+                if constexpr (CG == 1) tc::arrive(b_fixed + 8 * s);
+                else tc::publish_at(tc::leader_addr(b_fixed + 8 * s));
             }
         }
     }
+    if (lane == 0 && *stop) atomicOr(&g_product_err, 1u);
     __syncwarp();
     tc::fence_before_sync();
     if constexpr (CG == 1) __syncthreads();
@@ -455,16 +460,15 @@ __device__ __forceinline__ void fma2(uint64_t &acc, uint64_t a, uint64_t b) {
 
 // What a promotion warp needs of its CTA.
 struct F8Sync {
-    uint64_t *d_full, *d_empty, *sc_empty;
+    uint32_t d_full, d_empty, sc_empty, gave_up;  // shared-memory addresses
+    uint32_t lanes;                               // TMEM address of the warp's lanes
     const float *scales;
     uint8_t *stage;
-    uint32_t lanes;  // TMEM address of the warp's lanes
-    volatile int *gave_up;
 };
 
-// One tile by one promotion warp: NCH chunks of 32 columns, from 32 * part in turns of 64.  Returns false after a wait gave up.
+// One tile by one promotion warp: NCH chunks of 32 columns, from 32 * part in turns of 64.
 template <int CG, int NCH>
-__device__ __forceinline__ bool promote_tile(const F8Sync &y, SlotRing &ring, const OutTile &o, int kb, bool wide, int part,
+__device__ __forceinline__ void promote_tile(const F8Sync &y, SlotRing &ring, const OutTile &o, int kb, bool wide, int part,
                                              int lane) {
     uint64_t acc[NCH ? 2 * NCH : 1][8];  // 16 columns, pairs of columns in fragment order: 0.0f
 #pragma unroll
@@ -475,7 +479,7 @@ __device__ __forceinline__ bool promote_tile(const F8Sync &y, SlotRing &ring, co
     for (int kk = 0; kk < kb; ++kk) {
         ring.next(wide);
         const int slot = ring.slot;
-        if (!tc::warp_wait(&y.d_full[slot], ring.full(), y.gave_up, &g_product_err)) return false;
+        tc::wait(y.d_full + 8 * slot, ring.full(), y.gave_up);
         tc::fence_after_sync();
         const float *sc = y.scales + slot * kSlotCols + 2 * (lane & 3);
         const uint32_t src = y.lanes + slot * kSlotCols;
@@ -498,9 +502,9 @@ __device__ __forceinline__ bool promote_tile(const F8Sync &y, SlotRing &ring, co
         if (lane == 0) {
             const int slots = wide ? 2 : 1;
             for (int s = slot; s < slot + slots; ++s) {
-                if constexpr (CG == 1) tc::mbar_arrive(&y.d_empty[s]);
-                else tc::arrive_at(tc::leader_addr(&y.d_empty[s]));
-                tc::mbar_arrive(&y.sc_empty[s]);
+                if constexpr (CG == 1) tc::arrive(y.d_empty + 8 * s);
+                else tc::arrive_at(tc::leader_addr(y.d_empty + 8 * s));
+                tc::arrive(y.sc_empty + 8 * s);
             }
         }
         ring.used(wide);
@@ -515,7 +519,6 @@ __device__ __forceinline__ bool promote_tile(const F8Sync &y, SlotRing &ring, co
         }
         store_chunk(o, y.stage, lane, column(h), v);
     }
-    return true;
 }
 
 template <int CG>
@@ -529,7 +532,7 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     float *scales = reinterpret_cast<float *>(smem + S::kOperands);  // [slot][column]: xs * ws
     uint8_t *staging = smem + S::kOperands + kSlots * kSlotCols * sizeof(float);
     // d_full: a slot's MMAs and its scales; d_empty: read by both CTAs' warps; sc_empty: by this one's
-    __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[kSlots], d_empty[kSlots], sc_empty[kSlots];
+    __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[kSlots], d_empty[kSlots], sc_empty[kSlots], last;
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up;
     __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
@@ -541,6 +544,7 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     for (int g = tid; g < p.groups; g += kThreadsF8) group_bounds(p.offsets, g, p.rows, bounds[2 * g], bounds[2 * g + 1]);
     if (tid == 0) {
         gave_up = 0;
+        mbar_init(&last, 1);
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
@@ -563,73 +567,76 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     const int total = prefix[p.groups], kb = (p.contraction + S::kBC8 - 1) / S::kBC8;
     const Tiles<CG, kForward> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
+    const uint32_t up = smem_u32(&gave_up), aF = smem_u32(sF), aR = smem_u32(sR);
+    const uint32_t b_full = smem_u32(full), b_empty = smem_u32(empty), b_dfull = smem_u32(d_full), b_dempty = smem_u32(d_empty),
+                   b_sempty = smem_u32(sc_empty);
+    volatile int *const stop = &gave_up;
+
     if (warp == 0) {
-        uint32_t it = 0;
-        bool ok = true;
-        for (int t = cluster; t < total && ok; t += clusters) {
+        tc::Ring<S::kStages> r;
+        uint32_t used = 0;  // stages in use
+        for (int t = cluster; t < total && !*stop; t += clusters) {
             const Tile x = tiles.get(t);
             if (!x.rows) continue;
             const int half = x.n / CG, boxes = (half + kRowBox - 1) / kRowBox;
             const uint32_t bytes = S::kBytesF + boxes * kRowBox * S::kBC8;
             const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
-            for (int kk = 0; kk < kb; ++kk, ++it) {
-                const int s = it % S::kStages;
-                if (!(ok = tc::warp_wait(&empty[s], ((it / S::kStages) & 1u) ^ 1u, &gave_up, &g_product_err))) break;
+            for (int kk = 0; kk < kb; ++kk, r.next()) {
+                tc::wait(b_empty + 8 * r.s, r.phase ^ 1u, up);
+                used |= 1u << r.s;
                 if (tc::elect_one()) {
-                    uint32_t bar = smem_u32(&full[s]);
-                    if (rank == 0) mbar_expect_tx(&full[s], CG * bytes);
-                    if (CG > 1) bar = tc::leader_addr(&full[s]);
-                    tc::pair_tma_3d<CG>(sF + s * S::kBytesF, &map_f, kk * S::kBC8, f0, x.g, bar);
+                    uint32_t bar = b_full + 8 * r.s;
+                    if (rank == 0) tc::expect_tx(bar, CG * bytes);
+                    if (CG > 1) bar = tc::leader_addr(bar);
+                    tc::pair_tma_3d<CG>(aF + r.s * S::kBytesF, &map_f, kk * S::kBC8, f0, x.g, bar);
                     for (int b = 0; b < boxes; ++b)
-                        tc::pair_tma_2d<CG>(sR + s * S::kBytesR + b * kRowBox * S::kBC8, &map_r, kk * S::kBC8, r0 + kRowBox * b, bar);
+                        tc::pair_tma_2d<CG>(aR + r.s * S::kBytesR + b * kRowBox * S::kBC8, &map_r, kk * S::kBC8, r0 + kRowBox * b, bar);
                 }
                 __syncwarp();
             }
         }
         if (rank == 0)  // as in k_product_tc: no exit under copies in flight
-            for (uint32_t back = 1; back <= (uint32_t)S::kStages && back <= it; ++back)
-                mbar_wait_bounded(&full[(it - back) % S::kStages], ((it - back) / S::kStages) & 1u, tc::kPairWaitCycles / 8);
+            for (uint32_t s = 0; s < (uint32_t)S::kStages; ++s)
+                if (used >> s & 1u) mbar_wait_bounded(&full[s], r.phase ^ (s >= r.s ? 1u : 0u), tc::kPairWaitCycles / 8);
     } else if (warp == 1) {
         if (rank == 0) {
-            uint32_t it = 0;
+            tc::Ring<S::kStages> r;
             SlotRing ring;
-            bool ok = true;
-            for (int t = cluster; t < total && ok; t += clusters) {
+            for (int t = cluster; t < total && !*stop; t += clusters) {
                 const Tile x = tiles.get(t);
                 if (!x.rows) continue;
                 const bool wide = x.n > kSlotCols;
                 const uint32_t idesc = tc::operand_idesc(0, false, false, kBF * CG, x.n);
-                for (int kk = 0; kk < kb; ++kk, ++it) {
-                    const int s = it % S::kStages;
+                for (int kk = 0; kk < kb; ++kk, r.next()) {
                     ring.next(wide);
                     const int slot = ring.slot;
-                    ok = tc::warp_wait(&d_empty[slot], ring.empty(slot), &gave_up, &g_product_err) &&
-                         (!wide || tc::warp_wait(&d_empty[slot + 1], ring.empty(slot + 1), &gave_up, &g_product_err)) &&
-                         tc::warp_wait(&full[s], (it / S::kStages) & 1u, &gave_up, &g_product_err);
-                    if (!ok) break;
+                    tc::wait(b_dempty + 8 * slot, ring.empty(slot), up);
+                    if (wide) tc::wait(b_dempty + 8 * slot + 8, ring.empty(slot + 1), up);
+                    tc::wait(b_full + 8 * r.s, r.phase, up);
                     tc::fence_after_sync();
                     if (tc::elect_one()) {
-                        const uint64_t df = tc::operand_desc(sF + s * S::kBytesF, false, 0);
-                        const uint64_t dr = tc::operand_desc(sR + s * S::kBytesR, false, 0);
+                        const uint64_t df = tc::operand_desc(aF + r.s * S::kBytesF, false, 0);
+                        const uint64_t dr = tc::operand_desc(aR + r.s * S::kBytesR, false, 0);
                         const int left = p.contraction - kk * S::kBC8;
 #pragma unroll
                         for (int j = 0; j < S::kBC8 / 32; ++j)
                             if (32 * j < left)
                                 tc::pair_mma<CG, tc::kKindF8>(tmem + slot * kSlotCols, df + 2 * j, dr + 2 * j, idesc, j != 0);
-                        tc::pair_commit<CG>(&empty[s]);
-                        tc::pair_commit<CG>(&d_full[slot]);
+                        tc::pair_commit<CG>(b_empty + 8 * r.s);
+                        tc::pair_commit<CG>(b_dfull + 8 * slot);
                     }
                     __syncwarp();
                     ring.used(wide);
                 }
             }
+            if (tc::elect_one()) tc::pair_commit<CG>(smem_u32(&last));  // nor under MMAs in flight
+            mbar_wait_bounded(&last, 0, tc::kPairWaitCycles / 8);
         }
     } else if (warp < 4) {
         // ---- scales: the two warps take turns; each loads its next stage's before it waits for a slot ----
         uint32_t it = 0;
         SlotRing ring;
-        bool ok = true;
-        for (int t = cluster; t < total && ok; t += clusters) {
+        for (int t = cluster; t < total && !*stop; t += clusters) {
             const Tile x = tiles.get(t);
             if (!x.rows) continue;
             const bool wide = x.n > kSlotCols;
@@ -655,38 +662,37 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
 #pragma unroll
                     for (int i = 0; i < 8; ++i) s8[i] = v[i] * w;
                     fetch(kk + 2);
-                    ok = tc::warp_wait(&sc_empty[slot], ring.empty(slot), &gave_up, &g_product_err) &&
-                         (!wide || tc::warp_wait(&sc_empty[slot + 1], ring.empty(slot + 1), &gave_up, &g_product_err));
-                    if (!ok) break;
+                    tc::wait(b_sempty + 8 * slot, ring.empty(slot), up);
+                    if (wide) tc::wait(b_sempty + 8 * slot + 8, ring.empty(slot + 1), up);
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
                         if (wide || i < 4) scales[slot * kSlotCols + lane + 32 * i] = s8[i];
                     __syncwarp();
-                    if (lane == 0) tc::mbar_arrive(&d_full[slot]);
+                    if (lane == 0) tc::arrive(b_dfull + 8 * slot);
                 }
                 ring.used(wide);
             }
         }
     } else {
         const int quad = warp & 3, part = (warp - 4) >> 2;  // TMEM lanes 32 * quad.., chunks of 32 columns in turns
-        const F8Sync y{d_full, d_empty, sc_empty, scales, staging + (warp - 4) * 16 * kStageRow, tmem + ((uint32_t)(quad * 32) << 16),
-                       &gave_up};
+        const F8Sync y{b_dfull, b_dempty, b_sempty, up, tmem + ((uint32_t)(quad * 32) << 16), scales,
+                       staging + (warp - 4) * 16 * kStageRow};
         SlotRing ring;
-        bool ok = true;
-        for (int t = cluster; t < total && ok; t += clusters) {
+        for (int t = cluster; t < total && !*stop; t += clusters) {
             const Tile x = tiles.get(t);
             if (!x.rows) continue;
             const bool wide = x.n > kSlotCols;
             const int f = x.f0 + (int)rank * kBF + quad * 32;
             const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, x.rows, p.vec != 0};
             const int chunks = (x.n - 32 * part + 63) / 64;  // columns 32 * part + 64 * c that lie below n
-            if (chunks <= 0) ok = promote_tile<CG, 0>(y, ring, o, kb, wide, part, lane);
-            else if (chunks == 1) ok = promote_tile<CG, 1>(y, ring, o, kb, wide, part, lane);
-            else if (chunks == 2) ok = promote_tile<CG, 2>(y, ring, o, kb, wide, part, lane);
-            else if (chunks == 3) ok = promote_tile<CG, 3>(y, ring, o, kb, wide, part, lane);
-            else ok = promote_tile<CG, 4>(y, ring, o, kb, wide, part, lane);
+            if (chunks <= 0) promote_tile<CG, 0>(y, ring, o, kb, wide, part, lane);
+            else if (chunks == 1) promote_tile<CG, 1>(y, ring, o, kb, wide, part, lane);
+            else if (chunks == 2) promote_tile<CG, 2>(y, ring, o, kb, wide, part, lane);
+            else if (chunks == 3) promote_tile<CG, 3>(y, ring, o, kb, wide, part, lane);
+            else promote_tile<CG, 4>(y, ring, o, kb, wide, part, lane);
         }
     }
+    if (lane == 0 && *stop) atomicOr(&g_product_err, 1u);
     __syncwarp();
     tc::fence_before_sync();
     if constexpr (CG == 1) __syncthreads();
