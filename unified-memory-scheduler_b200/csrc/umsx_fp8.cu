@@ -6,7 +6,7 @@
 //
 // 448 is the largest e4m3 value, so a block's largest entry lands on it.  The floor 2^-126 (the
 // smallest normal float) keeps the quotient finite for blocks of zeros and subnormals.  scale and
-// quotient are IEEE divisions, one rounding each, so the codes are those of the same formula on a CPU.
+// quotient are rounded once each, as IEEE divisions are, so the codes are those of the same formula on a CPU.
 // Bound: memory, (2 + 1) bytes per bf16 value plus 4 per block, read and written once.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -15,6 +15,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "umsx_device.cuh"
 #include "umsx_internal.h"
@@ -26,7 +27,7 @@ namespace {
 struct QuantParams {
     const void *x;
     int64_t ldx, x_stride;
-    int matrices, cols, vec;  // vec: rows start at multiples of 16 bytes (x) and 8 bytes (q)
+    int matrices, cols, vec;  // vec: rows start at multiples of 16 bytes (x) and of 16 (2) or 8 (1) bytes (q); 0 otherwise
     int64_t rows;
     uint8_t *q;
     int64_t ldq, q_stride;
@@ -34,115 +35,191 @@ struct QuantParams {
     int64_t s_row, s_blk, s_stride;
 };
 
+// Sixteen consecutive values of a row as they lie in memory; a 128-block is eight lanes of them.  Values stay in their
+// own type until they are scaled, which halves the registers of 16-bit inputs and doubles the warps that hide the loads.
 template <class T>
-__device__ __forceinline__ float to_f32(T v) {
-    return (float)v;
-}
+struct Sixteen {
+    static constexpr int kWords = 16 * sizeof(T) / 4;
+    uint32_t w[kWords];
 
-// Eight consecutive values of a row from column c on; zeros behind the last column.
-template <class T>
-__device__ __forceinline__ void load8(const T *row, int c, int cols, bool vec, float (&v)[8]) {
-    if (vec && c + 8 <= cols) {
-        constexpr int kVecs = 8 * sizeof(T) / 16;
-        uint4 raw[kVecs];
+    __device__ __forceinline__ void load(const T *row, int c, int cols, bool vec) {
+        if (vec && c + 16 <= cols) {
 #pragma unroll
-        for (int i = 0; i < kVecs; ++i) raw[i] = __ldg(reinterpret_cast<const uint4 *>(row + c) + i);
-        const T *e = reinterpret_cast<const T *>(raw);
+            for (int i = 0; i < kWords / 4; ++i)
+                *reinterpret_cast<uint4 *>(w + 4 * i) = __ldg(reinterpret_cast<const uint4 *>(row + c) + i);
+            return;
+        }
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_f32(e[i]);
-        return;
+            for (int i = 0; i < 16; ++i) w[i] = c + i < cols ? __ldg(reinterpret_cast<const uint32_t *>(row) + c + i) : 0u;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const unsigned short *h = reinterpret_cast<const unsigned short *>(row) + c + 2 * i;
+                w[i] = (c + 2 * i < cols ? __ldg(h) : 0u) | (c + 2 * i + 1 < cols ? (uint32_t)__ldg(h + 1) << 16 : 0u);
+            }
+        }
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? to_f32(row[c + i]) : 0.0f;
-}
-
-__device__ __forceinline__ float amax8(const float (&v)[8]) {
-    float m = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float a = fabsf(v[i]);
-        if (a < INFINITY) m = fmaxf(m, a);  // false for inf and NaN
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i]);
+        else {
+            const uint32_t h = i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) return i & 1 ? __uint_as_float(w[i >> 1] & 0xffff0000u) : bf16_bits_to_f32(h);
+            else return f16_bits_to_f32(h);
+        }
     }
-    return m;
-}
+    // Bits of |v| order like |v|; those of inf and NaN are at least kInf.  top: the largest of the sixteen (16-bit types: of the
+    // even and of the odd ones); finite: of the finite ones.
+    static constexpr uint32_t kInf = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+    __device__ __forceinline__ uint32_t top() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4) m = max(m, w[i] & 0x7fffffffu);
+            else m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+        }
+        return m;
+    }
+    __device__ __forceinline__ uint32_t finite() const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t a = sizeof(T) == 4 ? w[i] & 0x7fffffffu : (w[i >> 1] >> 16 * (i & 1)) & 0x7fffu;
+            if (a < kInf) m = max(m, a);
+        }
+        return m;
+    }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b); }
+    static __device__ __forceinline__ uint32_t one(uint32_t m) { return sizeof(T) == 4 ? m : max(m >> 16, m & 0xffffu); }
+    static __device__ __forceinline__ float as_float(uint32_t m) {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(m);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) return bf16_bits_to_f32(m);
+        else return f16_bits_to_f32(m);
+    }
+};
 
 __device__ __forceinline__ float block_scale(float amax) { return fmaxf(__fdiv_rn(amax, 448.0f), 0x1p-126f); }
 
-__device__ __forceinline__ void store8(uint8_t *row, int c, int cols, bool vec, const float (&v)[8], float scale) {
-    uint32_t w[2] = {0, 0};
+// Codes of sixteen values.  plain: every value is finite and scale >= 2^-100.  Then the quotient is Markstein's (1990):
+// with y = 1 / scale correctly rounded, q = x y and r = x - q scale (exact), q + r y rounds to x / scale, three
+// operations instead of a division's ten (with divisions the arithmetic, not memory, would bound the kernel).  Below
+// 2^-100 the residual may be subnormal and lose bits, so those blocks divide.
+template <class T>
+__device__ __forceinline__ void store16(uint8_t *row, int c, int cols, int vec, const Sixteen<T> &v, float scale, bool plain) {
+    uint32_t w[4];
+    if (plain) {
+        const float y = __frcp_rn(scale);
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        float2 t;
-        // inf / scale would saturate to 448: make it the NaN that it stands for
-        t.x = fabsf(v[i]) < INFINITY ? __fdiv_rn(v[i], scale) : __uint_as_float(0x7fc00000u);
-        t.y = fabsf(v[i + 1]) < INFINITY ? __fdiv_rn(v[i + 1], scale) : __uint_as_float(0x7fc00000u);
-        w[i >> 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(t, __NV_SATFINITE, __NV_E4M3) << (16 * ((i >> 1) & 1));
+        for (int i = 0; i < 4; ++i) {
+            float t[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x = v.value(4 * i + j), q = __fmul_rn(x, y);
+                t[j] = __fmaf_rn(__fmaf_rn(-q, scale, x), y, q);
+            }
+            w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(t[0], t[1]), __NV_SATFINITE, __NV_E4M3) |
+                   (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(t[2], t[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            w[i] = 0;
+            for (int j = 0; j < 4; ++j) {  // inf / scale would saturate to 448: make it the NaN that it stands for
+                const float x = v.value(4 * i + j), t = fabsf(x) < INFINITY ? __fdiv_rn(x, scale) : __uint_as_float(0x7fc00000u);
+                w[i] |= (uint32_t)__nv_cvt_float_to_fp8(t, __NV_SATFINITE, __NV_E4M3) << (8 * j);
+            }
+        }
     }
-    if (vec && c + 8 <= cols) {
-        *reinterpret_cast<uint2 *>(row + c) = make_uint2(w[0], w[1]);
+    if (vec && c + 16 <= cols) {
+        if (vec == 2) {
+            *reinterpret_cast<uint4 *>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            *reinterpret_cast<uint2 *>(row + c) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2 *>(row + c + 8) = make_uint2(w[2], w[3]);
+        }
         return;
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 16; ++i)
         if (c + i < cols) row[c + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
 }
 
-// 1 x 128 blocks: sixteen lanes per block, eight values each.
+// 1 x 128 blocks: eight lanes per block, a warp takes 4 * kSteps blocks of a row, all loaded before the first is used.
+constexpr int kSteps = 2;
 template <class T>
 __global__ void __launch_bounds__(256) k_quant_rows(const QuantParams p) {
-    const int nb = (p.cols + kScaleBlock - 1) / kScaleBlock, l = threadIdx.x & 15;
-    const int64_t blocks = (int64_t)p.matrices * p.rows * nb;
-    // whole warps step together: the shuffles below need both halves
-    for (int64_t i0 = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; 2 * i0 < blocks;
-         i0 += ((int64_t)gridDim.x * blockDim.x) >> 5) {
-        const int64_t i = 2 * i0 + ((threadIdx.x >> 4) & 1);
-        const bool on = i < blocks;
-        const int64_t mr = on ? i / nb : 0, mat = mr / p.rows, r = mr - mat * p.rows;
-        const int b = on ? (int)(i - mr * nb) : 0, c = b * kScaleBlock + l * 8;
-        float v[8] = {};
-        if (on) load8(static_cast<const T *>(p.x) + mat * p.x_stride + r * p.ldx, c, p.cols, p.vec, v);
-        float m = amax8(v);
+    const int l = threadIdx.x & 7, sub = (threadIdx.x >> 3) & 3;
+    const int nb = (p.cols + kScaleBlock - 1) / kScaleBlock;
+    const uint32_t segs = (nb + 4 * kSteps - 1) / (4 * kSteps);
+    const int64_t items = (int64_t)p.matrices * p.rows * segs, step = ((int64_t)gridDim.x * blockDim.x) >> 5;
+    for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < items; i += step) {
+        const int64_t mr = items < (1ll << 32) ? (uint32_t)i / segs : i / segs;
+        const int b0 = (int)(i - mr * segs) * 4 * kSteps + sub;
+        int64_t r = mr, mat = 0;
+        if (p.matrices > 1) mat = mr / p.rows, r = mr - mat * p.rows;
+        const T *x = static_cast<const T *>(p.x) + mat * p.x_stride + r * p.ldx;
+        uint8_t *q = p.q + mat * p.q_stride + r * p.ldq;
+        float *s = p.scales + mat * p.s_stride + r * p.s_row;
+        Sixteen<T> v[kSteps];
 #pragma unroll
-        for (int s = 8; s >= 1; s >>= 1) m = fmaxf(m, __shfl_xor_sync(kFull, m, s));
-        const float scale = block_scale(m);
-        if (!on) continue;
-        store8(p.q + mat * p.q_stride + r * p.ldq, c, p.cols, p.vec, v, scale);
-        if (l == 0) p.scales[mat * p.s_stride + r * p.s_row + b * p.s_blk] = scale;
+        for (int j = 0; j < kSteps; ++j) v[j].load(x, (b0 + 4 * j) * kScaleBlock + l * 16, p.cols, p.vec);
+#pragma unroll
+        for (int j = 0; j < kSteps; ++j) {
+            const int b = b0 + 4 * j;
+            uint32_t m = v[j].top();
+#pragma unroll
+            for (int o = 4; o >= 1; o >>= 1) m = Sixteen<T>::larger(m, __shfl_xor_sync(kFull, m, o));
+            m = Sixteen<T>::one(m);
+            const bool fine = m < Sixteen<T>::kInf;
+            if (__any_sync(kFull, !fine)) {
+                m = v[j].finite();
+#pragma unroll
+                for (int o = 4; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(kFull, m, o));
+            }
+            if (b >= nb) continue;
+            const float scale = block_scale(Sixteen<T>::as_float(m));
+            store16(q, b * kScaleBlock + l * 16, p.cols, p.vec, v[j], scale, fine && scale >= 0x1p-100f);
+            if (l == 0) s[b * p.s_blk] = scale;
+        }
     }
 }
 
 // 128 x 128 blocks: one CTA per block; the block stays in registers between its maximum and its codes.
 template <class T>
 __global__ void __launch_bounds__(256) k_quant_blocks(const QuantParams p) {
-    __shared__ float part[8];
+    __shared__ uint32_t part[2][8];
     const int64_t nbr = (p.rows + kScaleBlock - 1) / kScaleBlock;
     const int nb = (p.cols + kScaleBlock - 1) / kScaleBlock;
     const int64_t blocks = (int64_t)p.matrices * nbr * nb;
     for (int64_t i = blockIdx.x; i < blocks; i += gridDim.x) {
         const int64_t mbr = i / nb, mat = mbr / nbr, br = mbr - mat * nbr;
-        const int b = (int)(i - mbr * nb), c = b * kScaleBlock + (threadIdx.x & 15) * 8;
-        const int64_t r0 = br * kScaleBlock + (threadIdx.x >> 4);
-        float v[8][8], m = 0.0f;
+        const int b = (int)(i - mbr * nb), c = b * kScaleBlock + (threadIdx.x & 7) * 16;
+        const int64_t r0 = br * kScaleBlock + (threadIdx.x >> 3);
+        Sixteen<T> v[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t r = r0 + 16 * j;
-            if (r < p.rows) load8(static_cast<const T *>(p.x) + mat * p.x_stride + r * p.ldx, c, p.cols, p.vec, v[j]);
-            else
-#pragma unroll
-                for (int q = 0; q < 8; ++q) v[j][q] = 0.0f;
-            m = fmaxf(m, amax8(v[j]));
+        for (int j = 0; j < 4; ++j) {
+            const int64_t r = r0 + 32 * j;
+            v[j].load(static_cast<const T *>(p.x) + mat * p.x_stride + r * p.ldx, c, r < p.rows ? p.cols : 0, p.vec);
         }
-        m = warp_max(m);
+        uint32_t m = 0, f = 0;  // over all values, over the finite ones
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            m = max(m, Sixteen<T>::one(v[j].top()));
+            f = max(f, v[j].finite());
+        }
+        m = __reduce_max_sync(kFull, m);
+        f = __reduce_max_sync(kFull, f);
         __syncthreads();  // the previous block's readers are done with part
-        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+        if ((threadIdx.x & 31) == 0) part[0][threadIdx.x >> 5] = m, part[1][threadIdx.x >> 5] = f;
         __syncthreads();
 #pragma unroll
-        for (int w = 0; w < 8; ++w) m = fmaxf(m, part[w]);
-        const float scale = block_scale(m);
+        for (int w = 0; w < 8; ++w) m = max(m, part[0][w]), f = max(f, part[1][w]);
+        const float scale = block_scale(Sixteen<T>::as_float(f));
+        const bool plain = m < Sixteen<T>::kInf && scale >= 0x1p-100f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t r = r0 + 16 * j;
-            if (r < p.rows) store8(p.q + mat * p.q_stride + r * p.ldq, c, p.cols, p.vec, v[j], scale);
+        for (int j = 0; j < 4; ++j) {
+            const int64_t r = r0 + 32 * j;
+            if (r < p.rows) store16(p.q + mat * p.q_stride + r * p.ldq, c, p.cols, p.vec, v[j], scale, plain);
         }
         if (threadIdx.x == 0) p.scales[mat * p.s_stride + br * p.s_row + b * p.s_blk] = scale;
     }
@@ -152,8 +229,8 @@ template <class T>
 void launch_quant(const QuantParams &p, int block_rows, int sms, cudaStream_t s) {
     const int64_t nb = (p.cols + kScaleBlock - 1) / kScaleBlock;
     if (block_rows == 1) {
-        const int64_t ctas = ((int64_t)p.matrices * p.rows * nb + 15) / 16;
-        k_quant_rows<T><<<(unsigned)std::min<int64_t>(ctas, 8 * sms), 256, 0, s>>>(p);
+        const int64_t items = (int64_t)p.matrices * p.rows * ((nb + 4 * kSteps - 1) / (4 * kSteps));
+        k_quant_rows<T><<<(unsigned)std::min<int64_t>((items + 7) / 8, 64 * sms), 256, 0, s>>>(p);
     } else {
         const int64_t blocks = (int64_t)p.matrices * ((p.rows + kScaleBlock - 1) / kScaleBlock) * nb;
         k_quant_blocks<T><<<(unsigned)std::min<int64_t>(blocks, 64 * sms), 256, 0, s>>>(p);
@@ -194,8 +271,9 @@ extern "C" umsx_status umsx_fp8_quantize(const void *x, int64_t ldx, int64_t x_s
     p.matrices = matrices, p.rows = rows, p.cols = cols;
     p.q = static_cast<uint8_t *>(q), p.ldq = ldq, p.q_stride = q_stride;
     p.scales = scales, p.s_row = s_row, p.s_blk = s_blk, p.s_stride = s_stride;
-    p.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * size % 16 == 0 && x_stride * size % 16 == 0 &&
-            reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0 && q_stride % 8 == 0;
+    const uint64_t at = reinterpret_cast<uintptr_t>(q) | (uint64_t)ldq | (uint64_t)q_stride;  // multiples of a power of two?
+    if (reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * size % 16 == 0 && x_stride * size % 16 == 0)
+        p.vec = at % 16 == 0 ? 2 : at % 8 == 0 ? 1 : 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (x_dtype == UMSX_DTYPE_F32) launch_quant<float>(p, block_rows, sms, s);
     else if (x_dtype == UMSX_DTYPE_BF16) launch_quant<__nv_bfloat16>(p, block_rows, sms, s);

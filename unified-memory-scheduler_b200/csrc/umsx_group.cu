@@ -2,8 +2,8 @@
 //
 // A stable counting sort of T*k jobs by expert in ONE launch without global scratch: a cluster of
 // up to eight CTAs splits the jobs into one contiguous piece per warp; each warp counts its piece
-// per expert (lanes of equal expert find one another with match_any, so no atomics and one fixed
-// order), the counts are scanned over the warps of a CTA, over the CTAs through distributed shared
+// per expert (lanes of equal expert find one another with a ballot per bit, so no atomics and one fixed
+// order; match_any takes an SM about 50 cycles a warp and bounded the kernel), the counts are scanned over the warps of a CTA, over the CTAs through distributed shared
 // memory and over the experts, and a second walk over the piece gives every job its row.
 // Bound: two dependent walks and three barriers, so latency; the ids are read twice (the second
 // time from cache) and 8 bytes per job are written once.
@@ -22,11 +22,22 @@ namespace cg = cooperative_groups;
 namespace umsx {
 namespace {
 
-constexpr int kGroupCluster = 8;
+constexpr int kGroupCluster = 8, kBatch = 8;  // kBatch: steps of ids a warp has in flight
 constexpr int kGroupSmemMax = 200 * 1024;
 
 // Shared memory: hist[warps][E], total[E], all[E], base[E], 32 partial sums.
 size_t group_smem(int warps, int experts) { return ((size_t)(warps + 3) * experts + 32) * sizeof(int); }
+
+// Lanes of the warp that hold the same expert.
+__device__ __forceinline__ unsigned same_expert(int e, int bits) {
+    unsigned same = kFull;
+    for (int b = 0; b < bits; ++b) {
+        const bool set = e >> b & 1;
+        const unsigned v = __ballot_sync(kFull, set);
+        same &= set ? v : ~v;
+    }
+    return same;
+}
 
 __global__ void __launch_bounds__(1024) k_group_rows(const int32_t *ids, int64_t jobs, int top_k, int E, int32_t *offsets,
                                                      int32_t *row_token, int32_t *row_of_job) {
@@ -43,12 +54,24 @@ __global__ void __launch_bounds__(1024) k_group_rows(const int32_t *ids, int64_t
     const int64_t first = (int64_t)(rank * warps + warp) * per * 32;
     const int64_t last = min(first + per * 32, jobs);
     int *mine = hist + warp * E;
-    for (int64_t i = first + lane; i - lane < last; i += 32) {
-        int id = i < last ? __ldg(ids + i) : -1;
-        if (id < 0 || id >= E) id = -1;
-        const unsigned same = __match_any_sync(kFull, id);
-        if (id >= 0 && lane == __ffs(same) - 1) mine[id] += __popc(same);
-        __syncwarp();
+    const int bits = 32 - __clz(E);
+    int id[kBatch];
+    auto fetch = [&](int64_t i) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            id[j] = i + 32 * j < last ? __ldg(ids + i + 32 * j) : E;
+            if (id[j] < 0 || id[j] >= E) id[j] = E;  // of no group
+        }
+    };
+    for (int64_t i = first + lane; i - lane < last; i += 32 * kBatch) {
+        fetch(i);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (i - lane + 32 * j >= last) break;
+            const unsigned same = same_expert(id[j], bits);
+            if (id[j] < E && lane == __ffs(same) - 1) mine[id[j]] += __popc(same);
+            __syncwarp();
+        }
     }
     __syncthreads();
     // per expert: counts -> starts within the CTA
@@ -100,17 +123,23 @@ __global__ void __launch_bounds__(1024) k_group_rows(const int32_t *ids, int64_t
     }
     const int rows = carry;
     if (rank == 0 && tid == 0) offsets[E] = rows;
-    for (int64_t i = first + lane; i - lane < last; i += 32) {
-        int id = i < last ? __ldg(ids + i) : -1;
-        if (id < 0 || id >= E) id = -1;
-        const unsigned same = __match_any_sync(kFull, id);
-        int row = -1;
-        if (id >= 0) row = base[id] + mine[id] + __popc(same & ((1u << lane) - 1u));
-        __syncwarp();
-        if (id >= 0 && lane == __ffs(same) - 1) mine[id] += __popc(same);
-        __syncwarp();
-        if (i < last) row_of_job[i] = row;
-        if (row >= 0) row_token[row] = (int32_t)((uint32_t)i / (uint32_t)top_k);
+    const bool once = per <= kBatch;  // the ids are still in registers
+    for (int64_t i0 = first + lane; i0 - lane < last; i0 += 32 * kBatch) {
+        if (!once) fetch(i0);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const int64_t i = i0 + 32 * j;
+            if (i - lane >= last) break;
+            const int e = id[j];
+            const unsigned same = same_expert(e, bits);
+            int row = -1;
+            if (e < E) row = base[e] + mine[e] + __popc(same & ((1u << lane) - 1u));
+            __syncwarp();
+            if (e < E && lane == __ffs(same) - 1) mine[e] += __popc(same);
+            __syncwarp();
+            if (i < last) row_of_job[i] = row;
+            if (row >= 0) row_token[row] = (int32_t)((uint32_t)i / (uint32_t)top_k);
+        }
     }
     // rows behind the last group name token 0, so that a gather by them stays inside x
     for (int64_t r = rows + (int64_t)rank * blockDim.x + tid; r < jobs; r += (int64_t)ctas * blockDim.x) row_token[r] = 0;

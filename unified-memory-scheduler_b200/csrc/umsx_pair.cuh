@@ -63,6 +63,13 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
             : "memory");
 }
 
+// The same to the leader's barrier alone.
+template <int CG>
+__device__ __forceinline__ void leader_commit(uint32_t bar) {
+    if constexpr (CG == 1) pair_commit<1>(bar);
+    else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // The leader's copy of a shared-memory object, as a shared::cluster address.
 __device__ __forceinline__ uint32_t leader_addr(const void *p) {
     uint32_t a;

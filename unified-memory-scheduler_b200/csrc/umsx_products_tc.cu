@@ -286,12 +286,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                 __syncwarp();
             }
         }
-        // A CTA must not exit under copies in flight: each stage's last one, again bounded (a wait at all only
-        // where the MMAs gave up before they read them).
+        // A CTA must not exit before the last arrivals at its barriers, nor, where a wait gave up and the MMAs did not
+        // read them, under copies in flight.
         for (uint32_t s = 0; s < (uint32_t)S::kStages; ++s) {
             if (!(used >> s & 1u)) continue;
+            const uint32_t last_phase = r.phase ^ (s >= r.s ? 1u : 0u);
+            mbar_wait_bounded(&empty[s], last_phase, tc::kPairWaitCycles / 8);
+            if (!*stop) continue;
             if (tails >> s & 1u) mbar_wait_bounded(&tail[s], (tail_phase >> s & 1u) ^ 1u, tc::kPairWaitCycles / 8);
-            else if (rank == 0) mbar_wait_bounded(&full[s], r.phase ^ (s >= r.s ? 1u : 0u), tc::kPairWaitCycles / 8);
+            else if (rank == 0) mbar_wait_bounded(&full[s], last_phase, tc::kPairWaitCycles / 8);
         }
     } else if (warp == 1) {
         if (rank == 0) {
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                 ++n_item;
             }
             // nor under MMAs in flight
-            if (tc::elect_one()) tc::pair_commit<CG>(smem_u32(&last));
+            if (tc::elect_one()) tc::leader_commit<CG>(smem_u32(&last));
             mbar_wait_bounded(&last, 0, tc::kPairWaitCycles / 8);
         }
     } else if (warp < 2 + kEpilogueWarps) {
@@ -468,8 +471,8 @@ struct F8Sync {
 
 // One tile by one promotion warp: NCH chunks of 32 columns, from 32 * part in turns of 64.
 template <int CG, int NCH>
-__device__ __forceinline__ void promote_tile(const F8Sync &y, SlotRing &ring, const OutTile &o, int kb, bool wide, int part,
-                                             int lane) {
+__device__ __forceinline__ void promote_tile(const F8Sync &y, SlotRing &ring, const TcParams &p, const Tile &x, int f, int kb,
+                                             bool wide, int part, int lane) {
     uint64_t acc[NCH ? 2 * NCH : 1][8];  // 16 columns, pairs of columns in fragment order: 0.0f
 #pragma unroll
     for (int h = 0; h < 2 * NCH; ++h)
@@ -499,16 +502,13 @@ __device__ __forceinline__ void promote_tile(const F8Sync &y, SlotRing &ring, co
         }
         tc::fence_before_sync();
         __syncwarp();
-        if (lane == 0) {
-            const int slots = wide ? 2 : 1;
-            for (int s = slot; s < slot + slots; ++s) {
-                if constexpr (CG == 1) tc::arrive(y.d_empty + 8 * s);
-                else tc::arrive_at(tc::leader_addr(y.d_empty + 8 * s));
-                tc::arrive(y.sc_empty + 8 * s);
-            }
+        if (lane < (wide ? 4 : 2)) {  // one lane per barrier
+            const uint32_t at = 8 * (slot + (lane >> 1));
+            tc::arrive_at(lane & 1 ? y.sc_empty + at : CG == 1 ? y.d_empty + at : tc::leader_addr(y.d_empty + at));
         }
         ring.used(wide);
     }
+    const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, x.rows, p.vec != 0};
 #pragma unroll
     for (int h = 0; h < 2 * NCH; ++h) {
         uint32_t v[16];
@@ -595,9 +595,12 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
                 __syncwarp();
             }
         }
-        if (rank == 0)  // as in k_product_tc: no exit under copies in flight
-            for (uint32_t s = 0; s < (uint32_t)S::kStages; ++s)
-                if (used >> s & 1u) mbar_wait_bounded(&full[s], r.phase ^ (s >= r.s ? 1u : 0u), tc::kPairWaitCycles / 8);
+        for (uint32_t s = 0; s < (uint32_t)S::kStages; ++s) {  // as in k_product_tc: no exit before the last arrivals
+            if (!(used >> s & 1u)) continue;
+            const uint32_t last_phase = r.phase ^ (s >= r.s ? 1u : 0u);
+            mbar_wait_bounded(&empty[s], last_phase, tc::kPairWaitCycles / 8);
+            if (*stop && rank == 0) mbar_wait_bounded(&full[s], last_phase, tc::kPairWaitCycles / 8);
+        }
     } else if (warp == 1) {
         if (rank == 0) {
             tc::Ring<S::kStages> r;
@@ -629,7 +632,7 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
                     ring.used(wide);
                 }
             }
-            if (tc::elect_one()) tc::pair_commit<CG>(smem_u32(&last));  // nor under MMAs in flight
+            if (tc::elect_one()) tc::leader_commit<CG>(smem_u32(&last));  // nor under MMAs in flight
             mbar_wait_bounded(&last, 0, tc::kPairWaitCycles / 8);
         }
     } else if (warp < 4) {
@@ -683,13 +686,12 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
             if (!x.rows) continue;
             const bool wide = x.n > kSlotCols;
             const int f = x.f0 + (int)rank * kBF + quad * 32;
-            const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, x.rows, p.vec != 0};
             const int chunks = (x.n - 32 * part + 63) / 64;  // columns 32 * part + 64 * c that lie below n
-            if (chunks <= 0) promote_tile<CG, 0>(y, ring, o, kb, wide, part, lane);
-            else if (chunks == 1) promote_tile<CG, 1>(y, ring, o, kb, wide, part, lane);
-            else if (chunks == 2) promote_tile<CG, 2>(y, ring, o, kb, wide, part, lane);
-            else if (chunks == 3) promote_tile<CG, 3>(y, ring, o, kb, wide, part, lane);
-            else promote_tile<CG, 4>(y, ring, o, kb, wide, part, lane);
+            if (chunks <= 0) promote_tile<CG, 0>(y, ring, p, x, f, kb, wide, part, lane);
+            else if (chunks == 1) promote_tile<CG, 1>(y, ring, p, x, f, kb, wide, part, lane);
+            else if (chunks == 2) promote_tile<CG, 2>(y, ring, p, x, f, kb, wide, part, lane);
+            else if (chunks == 3) promote_tile<CG, 3>(y, ring, p, x, f, kb, wide, part, lane);
+            else promote_tile<CG, 4>(y, ring, p, x, f, kb, wide, part, lane);
         }
     }
     if (lane == 0 && *stop) atomicOr(&g_product_err, 1u);
