@@ -44,7 +44,7 @@ constexpr uint32_t kTmemCols = 512;
 constexpr int kStageRow = 80;  // bytes of a staged output row: 64 of data; 80 spreads eight rows over all banks
 
 struct TcParams {
-    int groups, features, contraction, out_rows, out_dtype, fmt, vec;
+    int groups, features, contraction, out_rows, out_dtype, fmt, vec, bulk;
     int64_t rows;
     const int32_t *offsets;
     void *out;
@@ -72,19 +72,21 @@ struct Tiles {
 
     __device__ static int row_tiles(int rows) { return (rows + kRowsMax - 1) / kRowsMax; }
 
-    __device__ Tile get(int t) const {
-        int lo = 0, hi = groups;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (prefix[mid] <= t) lo = mid;
-            else hi = mid;
+    // Tile t, by a converged warp that asks for ascending ones; `lo` is its group so far.
+    __device__ __forceinline__ Tile get(int t, int &lo, int lane) const {
+        while (true) {  // 32 groups a step: a binary search's dependent reads took 500 cycles of every tile
+            const unsigned below = __ballot_sync(kFull, prefix[min(lo + 1 + lane, groups)] <= t);
+            lo += __popc(below);
+            if (below != kFull) break;
         }
         const int a = start[2 * lo], m = start[2 * lo + 1] - a;
         const int all = MODE == kGradWeight ? out_rows : m, rt = row_tiles(all);
-        const int local = t - prefix[lo], i = local % rt, j = local / rt;
+        const int local = t - prefix[lo];
+        int i = 0, j = local, each = all;
+        if (rt > 1) i = local % rt, j = local / rt, each = (all + rt - 1) / rt;
         // equal tiles, in steps of the MMA's N
         constexpr int kStep = 16 * CG;
-        const int size = min(kRowsMax, ((all + rt - 1) / rt + kStep - 1) / kStep * kStep);
+        const int size = min(kRowsMax, (each + kStep - 1) / kStep * kStep);
         Tile x;
         x.g = lo;
         x.f0 = j * kBF * CG;
@@ -135,14 +137,33 @@ struct OutTile {
     bool vec;         // 16-byte stores: base and rows are aligned, features is a multiple of 8 from an aligned start
 };
 
-__device__ __forceinline__ uint32_t pack16(uint32_t lo, uint32_t hi, int dtype) {
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(uint32_t lo, uint32_t hi) {
     const float a = __uint_as_float(lo), b = __uint_as_float(hi);
-    if (dtype == UMSX_DTYPE_BF16) {
+    if constexpr (BF16) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t *>(&h);
     }
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+// 16 rows of 32 16-bit features from v (fragment order) to shared memory, row by row: rows of kStageRow bytes, or rows of 128
+// swizzled bytes of which the warp's features are chunks `chunk` to chunk + 3 (`to` at a multiple of eight rows).
+template <bool BF16, bool SWIZZLED>
+__device__ __forceinline__ void stage16(uint8_t *to, int chunk, int lane, const uint32_t (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint32_t m[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int e = 8 * (q >> 1) + 4 * i + 2 * (q & 1);
+            m[q] = pack16<BF16>(v[e], v[e + 1]);
+        }
+        const int row = 8 * i + (lane & 7);
+        tc::stmatrix_trans4(SWIZZLED ? to + row * 128 + ((chunk + (lane >> 3)) ^ (lane & 7)) * 16 : to + row * kStageRow + (lane >> 3) * 16,
+                            m[0], m[1], m[2], m[3]);
+    }
 }
 
 // Rows c0 .. c0 + 15 of the tile from v (fragment order), through the warp's staging of 16 rows.
@@ -162,16 +183,8 @@ __device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, in
         return;
     }
     __syncwarp();  // the previous rows have been read out of the staging
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        uint32_t m[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int e = 8 * (q >> 1) + 4 * i + 2 * (q & 1);
-            m[q] = pack16(v[e], v[e + 1], o.dtype);
-        }
-        tc::stmatrix_trans4(stage + (8 * i + (lane & 7)) * kStageRow + (lane >> 3) * 16, m[0], m[1], m[2], m[3]);
-    }
+    if (o.dtype == UMSX_DTYPE_BF16) stage16<true, false>(stage, 0, lane, v);
+    else stage16<false, false>(stage, 0, lane, v);
     __syncwarp();
     uint16_t *p = static_cast<uint16_t *>(o.out) + o.at;
 #pragma unroll
@@ -244,8 +257,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     if (warp == 0) {
         tc::Ring<S::kStages> r;
         uint32_t tails = 0, tail_phase = 0, used = 0;  // bit s: stage s holds a ragged end; uses of tail[s], mod 2; stages in use
+        int group = 0;
         for (int t = cluster; t < total && !*stop; t += clusters) {
-            const Tile x = tiles.get(t);
+            const Tile x = tiles.get(t, group, lane);
             const int kb = (x.c_len + kBC - 1) / kBC;
             if (!x.rows) continue;
             const int half = x.n / CG;  // rows of this CTA's part of R
@@ -300,8 +314,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
         if (rank == 0) {
             tc::Ring<S::kStages> r;
             uint32_t n_item = 0, fixed_phase = 0;
+            int group = 0;
             for (int t = cluster; t < total && !*stop; t += clusters) {
-                const Tile x = tiles.get(t);
+                const Tile x = tiles.get(t, group, lane);
                 const int kb = (x.c_len + kBC - 1) / kBC;
                 if (!x.rows || !kb) continue;
                 const uint32_t idesc = tc::operand_idesc(p.fmt, S::kFMn, S::kRMn, kBF * CG, x.n);
@@ -339,8 +354,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
         const int quad = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes 32 * quad.., columns in turns of 16
         uint8_t *stage = smem + S::kStages * (S::kBytesF + S::kBytesR) + (warp - 2) * 16 * kStageRow;
         uint32_t n_item = 0;
+        int group = 0;
         for (int t = cluster; t < total && !*stop; t += clusters) {
-            const Tile x = tiles.get(t);
+            const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
             const int f = x.f0 + (int)rank * kBF + quad * 32;
             const OutTile o{p.out, (MODE == kGradWeight ? x.g * p.out_group : 0) + (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype,
@@ -373,8 +389,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
         }
     } else if (MODE == kGradWeight) {
         uint32_t it = 0, tail_phase = 0;
+        int group = 0;
         for (int t = cluster; t < total && !*stop; t += clusters) {
-            const Tile x = tiles.get(t);
+            const Tile x = tiles.get(t, group, lane);
             const int kb = (x.c_len + kBC - 1) / kBC;
             if (!x.rows) continue;
             it += kb;
@@ -419,6 +436,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
 // constant (a test per chunk costs 350 cycles a block) and 16 columns a load (with 32 the sums spill).  128 sums a
 // thread leave no room for more warps: sixteen of them with half the sums spill at 96 registers and are no faster.
 //
+// 16-bit outputs leave through a staging of the whole tile and TMA stores of 32 or 8 rows, which drain under the next
+// tile's blocks; the last rows of a group, fewer than eight, are stored by the warps, since a box would overwrite the next
+// group's.  Stored by the promotion warps alone, all SMs at once, tiles took 5 K of their 23 K cycles (16 blocks) for it.
+//
 // Tensor memory is a ring of four slots of 128 columns; a tile of more than 128 rows takes two.  So narrow tiles have
 // four accumulators in flight, which covers the way from the MMAs to the promotion and back.
 
@@ -441,6 +462,10 @@ struct SlotRing {
     }
 };
 
+// A staged tile: two halves of 64 features, a row of a half is 128 bytes with the swizzle of the tensor map (16-byte
+// chunk c of row r at c ^ (r & 7)).
+constexpr int kHalfTile = kRowsMax * 128;
+
 struct F8Params {
     TcParams t;
     const float *xs, *ws;
@@ -451,9 +476,12 @@ template <int CG>
 struct ShapeF8 {
     static constexpr int kBC8 = 128;  // contraction per stage, in bytes too
     static constexpr int kBytesF = kBF * kBC8, kBytesR = kRowsMax / CG * kBC8;
-    static constexpr int kStages = CG == 1 ? 4 : 6;
+    static constexpr int kStages = 4;
     static constexpr size_t kOperands = (size_t)kStages * (kBytesF + kBytesR);
-    static constexpr size_t kSmem = 1024 + kOperands + kEpilogueWarps * 16 * kStageRow + kSlots * kSlotCols * sizeof(float);
+    // a pair's half stages leave room for a tile; a single CTA's (outputs of at most 128 features) do not
+    static constexpr bool kBulk = CG == 2;
+    static constexpr size_t kStaging = kBulk ? 2 * kHalfTile : kEpilogueWarps * 16 * kStageRow;
+    static constexpr size_t kSmem = 1024 + kOperands + kSlots * kSlotCols * sizeof(float) + kStaging;
 };
 
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t)lo | ((uint64_t)hi << 32); }
@@ -466,7 +494,8 @@ struct F8Sync {
     uint32_t d_full, d_empty, sc_empty, gave_up;  // shared-memory addresses
     uint32_t lanes;                               // TMEM address of the warp's lanes
     const float *scales;
-    uint8_t *stage;
+    uint8_t *staging;  // 1024-byte aligned
+    const CUtensorMap *out32, *out8;  // boxes of 64 features x 32 and x 8 rows
 };
 
 // One tile by one promotion warp: NCH chunks of 32 columns, from 32 * part in turns of 64.
@@ -508,29 +537,94 @@ __device__ __forceinline__ void promote_tile(const F8Sync &y, SlotRing &ring, co
         }
         ring.used(wide);
     }
-    const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, x.rows, p.vec != 0};
-#pragma unroll
-    for (int h = 0; h < 2 * NCH; ++h) {
-        uint32_t v[16];
+    if constexpr (NCH == 0) return;
+    auto sums = [&](int h, uint32_t (&v)[16]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             v[2 * i] = (uint32_t)acc[h][i];
             v[2 * i + 1] = (uint32_t)(acc[h][i] >> 32);
         }
-        store_chunk(o, y.stage, lane, column(h), v);
+    };
+    const int quad = (threadIdx.x >> 5) & 3;
+    if (ShapeF8<CG>::kBulk && p.bulk) {
+        tc::bulk_wait_read();
+        tc::bar_128(1 + part);  // all four warps' copies of the last tile have read the staging
+        uint8_t *to = y.staging + (quad >> 1) * kHalfTile;
+        const int chunk = (quad & 1) * 4;  // of this warp's 32 features in a row of the half
+        if (p.out_dtype == UMSX_DTYPE_BF16) {
+#pragma unroll
+            for (int h = 0; h < 2 * NCH; ++h) {
+                uint32_t v[16];
+                sums(h, v);
+                stage16<true, true>(to + column(h) * 128, chunk, lane, v);
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < 2 * NCH; ++h) {
+                uint32_t v[16];
+                sums(h, v);
+                stage16<false, true>(to + column(h) * 128, chunk, lane, v);
+            }
+        }
+        tc::fence_proxy_async();
+        tc::bar_128(1 + part);
+        const int even = x.rows & ~7, left = x.rows - even;  // rows in boxes, rows behind them
+        if (quad == 0) {
+            if (tc::elect_one()) {
+                const int f0 = f;  // of the tile's 128
+#pragma unroll
+                for (int c = 0; c < NCH; ++c)
+                    for (int half = 0; half < 2 && f0 + 64 * half < p.features; ++half) {
+                        const int r = (2 * c + part) * 32;
+                        const uint32_t src = smem_u32(y.staging) + half * kHalfTile;
+                        if (r + 32 <= even) tc::tma_store_2d(y.out32, f0 + 64 * half, x.row0 + r, src + r * 128);
+                        else
+                            for (int q = r; q < even && q < r + 32; q += 8)
+                                tc::tma_store_2d(y.out8, f0 + 64 * half, x.row0 + q, src + q * 128);
+                    }
+                tc::bulk_commit();
+            }
+            __syncwarp();
+        }
+        if (left && (even >> 5 & 1) == part) {  // in this part's chunk: four lanes to a row
+            const int row = even + (lane >> 2), fl = 8 * (lane & 3);
+            if (row < x.rows && f + fl < p.features) {
+                const uint4 w = *reinterpret_cast<const uint4 *>(to + row * 128 + ((chunk + (lane & 3)) ^ (row & 7)) * 16);
+                uint16_t *d = static_cast<uint16_t *>(p.out) + (int64_t)(x.row0 + row) * p.ldo + f + fl;
+                if (f + fl + 8 <= p.features) {
+                    *reinterpret_cast<uint4 *>(d) = w;
+                } else {
+                    const uint16_t *e = reinterpret_cast<const uint16_t *>(&w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (f + fl + j < p.features) d[j] = e[j];
+                }
+            }
+        }
+        return;
+    }
+    const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, x.rows, p.vec != 0};
+    uint8_t *own = y.staging + (quad + 4 * part) * 16 * kStageRow;
+#pragma unroll
+    for (int h = 0; h < 2 * NCH; ++h) {
+        uint32_t v[16];
+        sums(h, v);
+        store_chunk(o, own, lane, column(h), v);
     }
 }
 
 template <int CG>
 __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_constant__ CUtensorMap map_f,
-                                                              const __grid_constant__ CUtensorMap map_r, const F8Params fp) {
+                                                              const __grid_constant__ CUtensorMap map_r,
+                                                              const __grid_constant__ CUtensorMap map_o32,
+                                                              const __grid_constant__ CUtensorMap map_o8, const F8Params fp) {
     using S = ShapeF8<CG>;
     const TcParams &p = fp.t;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     uint8_t *sF = smem, *sR = smem + S::kStages * S::kBytesF;
-    float *scales = reinterpret_cast<float *>(smem + S::kOperands);  // [slot][column]: xs * ws
-    uint8_t *staging = smem + S::kOperands + kSlots * kSlotCols * sizeof(float);
+    uint8_t *staging = smem + S::kOperands;  // 1024-byte aligned
+    float *scales = reinterpret_cast<float *>(staging + S::kStaging);  // [slot][column]: xs * ws
     // d_full: a slot's MMAs and its scales; d_empty: read by both CTAs' warps; sc_empty: by this one's
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[kSlots], d_empty[kSlots], sc_empty[kSlots], last;
     __shared__ uint32_t tmem_s;
@@ -575,8 +669,9 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     if (warp == 0) {
         tc::Ring<S::kStages> r;
         uint32_t used = 0;  // stages in use
+        int group = 0;
         for (int t = cluster; t < total && !*stop; t += clusters) {
-            const Tile x = tiles.get(t);
+            const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
             const int half = x.n / CG, boxes = (half + kRowBox - 1) / kRowBox;
             const uint32_t bytes = S::kBytesF + boxes * kRowBox * S::kBC8;
@@ -605,8 +700,9 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
         if (rank == 0) {
             tc::Ring<S::kStages> r;
             SlotRing ring;
+            int group = 0;
             for (int t = cluster; t < total && !*stop; t += clusters) {
-                const Tile x = tiles.get(t);
+                const Tile x = tiles.get(t, group, lane);
                 if (!x.rows) continue;
                 const bool wide = x.n > kSlotCols;
                 const uint32_t idesc = tc::operand_idesc(0, false, false, kBF * CG, x.n);
@@ -639,8 +735,9 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
         // ---- scales: the two warps take turns; each loads its next stage's before it waits for a slot ----
         uint32_t it = 0;
         SlotRing ring;
+        int group = 0;
         for (int t = cluster; t < total && !*stop; t += clusters) {
-            const Tile x = tiles.get(t);
+            const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
             const bool wide = x.n > kSlotCols;
             const int f0 = x.f0 + (int)rank * kBF;
@@ -679,10 +776,12 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     } else {
         const int quad = warp & 3, part = (warp - 4) >> 2;  // TMEM lanes 32 * quad.., chunks of 32 columns in turns
         const F8Sync y{b_dfull, b_dempty, b_sempty, up, tmem + ((uint32_t)(quad * 32) << 16), scales,
-                       staging + (warp - 4) * 16 * kStageRow};
+                       staging, &map_o32, &map_o8};
         SlotRing ring;
-        for (int t = cluster; t < total && !*stop; t += clusters) {
-            const Tile x = tiles.get(t);
+        int group = 0;
+        for (int t = cluster; t < total; t += clusters) {
+            if (tc::bar_any_128(1 + part, *stop)) break;  // the four warps of a part meet at barriers: they stop together
+            const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
             const bool wide = x.n > kSlotCols;
             const int f = x.f0 + (int)rank * kBF + quad * 32;
@@ -693,6 +792,7 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
             else if (chunks == 3) promote_tile<CG, 3>(y, ring, p, x, f, kb, wide, part, lane);
             else promote_tile<CG, 4>(y, ring, p, x, f, kb, wide, part, lane);
         }
+        tc::bulk_wait_read();  // the copies read this CTA's shared memory
     }
     if (lane == 0 && *stop) atomicOr(&g_product_err, 1u);
     __syncwarp();
@@ -767,7 +867,8 @@ int launch_mode(const Product &p, const CUtensorMap &mf, const CUtensorMap &mr, 
 }
 
 template <int CG>
-int launch_f8(const CUtensorMap &mf, const CUtensorMap &mr, const F8Params &fp, int sms, cudaStream_t s) {
+int launch_f8(const CUtensorMap &mf, const CUtensorMap &mr, const CUtensorMap (&mo)[2], const F8Params &fp, int sms,
+              cudaStream_t s) {
     auto *kernel = k_product_f8<CG>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ShapeF8<CG>::kSmem) != cudaSuccess) return -1;
     const int64_t ft = (fp.t.features + kBF * CG - 1) / (kBF * CG);
@@ -783,7 +884,7 @@ int launch_f8(const CUtensorMap &mf, const CUtensorMap &mr, const F8Params &fp, 
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, mf, mr, fp) == cudaSuccess ? 1 : -1;
+    return cudaLaunchKernelEx(&cfg, kernel, mf, mr, mo[0], mo[1], fp) == cudaSuccess ? 1 : -1;
 }
 
 bool aligned(const void *p, int64_t stride, int size) {
@@ -827,9 +928,14 @@ int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
     t.ldo = p.ldo;
     t.out_group = p.out_stride;
     t.vec = aligned(p.out, p.ldo, 2) && p.out_stride % 8 == 0;
+    t.bulk = t.vec && p.out_dtype != UMSX_DTYPE_F32;
     if (p.dtype == UMSX_DTYPE_E4M3) {
         const F8Params fp{t, p.xs, p.ws, p.xs_row, p.xs_blk, p.ws_row, p.ws_blk, p.ws_group};
-        return p.features() > kBF ? launch_f8<2>(mf, mr, fp, sms, s) : launch_f8<1>(mf, mr, fp, sms, s);
+        CUtensorMap mo[2] = {};  // of the output, where it can have one: boxes of 32 and of 8 rows
+        if (t.bulk && (!encode(&mo[0], p.out_dtype, p.out, 2, p.n, p.rows, 1, p.ldo * 2, 0, 32) ||
+                       !encode(&mo[1], p.out_dtype, p.out, 2, p.n, p.rows, 1, p.ldo * 2, 0, 8)))
+            return -1;
+        return p.features() > kBF ? launch_f8<2>(mf, mr, mo, fp, sms, s) : launch_f8<1>(mf, mr, mo, fp, sms, s);
     }
     // CG = 2 for wide outputs
     return p.features() > kBF ? launch_mode<2>(p, mf, mr, t, sms, s) : launch_mode<1>(p, mf, mr, t, sms, s);
