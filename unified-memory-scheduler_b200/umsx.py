@@ -239,35 +239,52 @@ def route_static(x, router_w, router_b, experts: int, top_k: int, routing: int, 
 # ---- products over caller-owned expert weights --------------------------------------------------------
 
 _CODES = {}  # torch dtype -> UMSX_DTYPE_*, filled on first use (torch is imported lazily)
+_TORCH = None
+_RAW_STREAM = None  # device index -> cudaStream_t of its current stream
 
 
-def _codes():
-    if not _CODES:
+def _torch():
+    global _TORCH, _RAW_STREAM
+    if _TORCH is None:
         import torch
+        _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda index: torch.cuda.current_stream(index).cuda_stream)
         _CODES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16,
                        torch.float8_e4m3fn: DTYPE_E4M3})
-    return _CODES
+        _TORCH = torch
+    return _TORCH
 
 
-def _need(ok: bool, message: str):
-    if not ok:
-        raise UmsxError(EINVAL, message)
+def _refuse(message: str):
+    raise UmsxError(EINVAL, message)
 
 
-def _matrix(name, t, dim, dtypes, like=None):
-    """Checks one CUDA operand: its rank, type, contiguous last dimension, and the device of `like`."""
-    _need(t.is_cuda, f"{name} must be a CUDA tensor")
-    _need(like is None or t.device == like.device, f"{name} must be on the device of the other tensors")
-    _need(t.dim() == dim, f"{name} must have {dim} dimensions, got {t.dim()}")
-    _need(t.dtype in dtypes, f"{name} has type {t.dtype}")
-    _need(t.shape[-1] <= 1 or t.stride(-1) == 1, f"{name}'s last dimension must be contiguous")
+def _matrix(name, t, dim, codes, like=None):
+    """Checks one CUDA operand: its rank, type (UMSX_DTYPE_* codes), contiguous last dimension, and the device of
+    `like`.  Returns its type's code."""
+    if not t.is_cuda:
+        _refuse(f"{name} must be a CUDA tensor")
+    if like is not None and t.device != like.device:
+        _refuse(f"{name} must be on the device of the other tensors")
+    if t.dim() != dim:
+        _refuse(f"{name} must have {dim} dimensions, got {t.dim()}")
+    code = _CODES.get(t.dtype, -1)
+    if code not in codes:
+        _refuse(f"{name} has type {t.dtype}")
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        _refuse(f"{name}'s last dimension must be contiguous")
+    return code
+
+
+_SIXTEEN = (DTYPE_BF16, DTYPE_F16)
+_OUT = (DTYPE_F32, DTYPE_BF16, DTYPE_F16)
 
 
 def _offsets_arg(offsets, experts, like):
-    import torch
-    _need(offsets.is_cuda and offsets.device == like.device, "offsets must be on the device of the other tensors")
-    _need(offsets.dtype == torch.int32 and offsets.shape == (experts + 1,) and offsets.is_contiguous(),
-          f"offsets must be a contiguous int32 tensor of {experts + 1} values")
+    if offsets.dtype != _TORCH.int32 or offsets.dim() != 1 or offsets.shape[0] != experts + 1 or not offsets.is_contiguous():
+        _refuse(f"offsets must be a contiguous int32 tensor of {experts + 1} values")
+    if offsets.device != like.device:
+        _refuse("offsets must be on the device of the other tensors")
 
 
 def _ld(t, dim=-2):
@@ -277,40 +294,45 @@ def _ld(t, dim=-2):
     return t.shape[-1] if dim == -2 else t.shape[-1] + (t.shape[-2] - 1) * _ld(t)
 
 
+def _new(shape, dtype, device):
+    """torch.empty for two or three dimensions; with the strides given it costs half as much."""
+    strides = (shape[1], 1) if len(shape) == 2 else (shape[1] * shape[2], shape[2], 1)
+    return _TORCH.empty_strided(shape, strides, dtype=dtype, device=device)
+
+
 def _out_arg(name, out, shape, dtype, like, default):
-    """`out`, checked, or a new tensor of `dtype` (`default` where that is None)."""
-    import torch
+    """`out`, checked, or a new tensor of `dtype` (`default` where that is None); and its type's code."""
     if out is None:
         dtype = default if dtype is None else dtype
-        _need(dtype in (torch.float32, torch.bfloat16, torch.float16), f"{name} cannot have type {dtype}")
-        return torch.empty(shape, dtype=dtype, device=like.device)
-    _need(dtype is None or dtype == out.dtype, f"{name} has type {out.dtype}, not {dtype}")
-    _matrix(name, out, len(shape), (torch.float32, torch.bfloat16, torch.float16), like)
-    _need(tuple(out.shape) == tuple(shape), f"{name} must have shape {tuple(shape)}, got {tuple(out.shape)}")
-    return out
+        code = _CODES.get(dtype, -1)
+        if code not in _OUT:
+            _refuse(f"{name} cannot have type {dtype}")
+        return _new(shape, dtype, like.device), code
+    if dtype is not None and dtype != out.dtype:
+        _refuse(f"{name} has type {out.dtype}, not {dtype}")
+    code = _matrix(name, out, len(shape), _OUT, like)
+    if out.shape != shape:
+        _refuse(f"{name} must have shape {tuple(shape)}, got {tuple(out.shape)}")
+    return out, code
 
 
-class _On:
-    """The tensors' device as the current one for a call, with the given stream or that device's current one."""
-
-    __slots__ = ("before", "index", "stream")
-
-    def __init__(self, t, stream):
-        import torch
-        self.index = t.device.index
-        self.before = torch.cuda.current_device()
-        self.stream = C.c_void_p(torch.cuda.current_stream(self.index).cuda_stream) if stream is None else _stream(stream)
-
-    def __enter__(self):
-        if self.before != self.index:
-            import torch
-            torch.cuda.set_device(self.index)
-        return self.stream
-
-    def __exit__(self, *exc):
-        if self.before != self.index:
-            import torch
-            torch.cuda.set_device(self.before)
+def _call(entry, t, stream, *args):
+    """entry(*args, stream) on t's device, which is the current one for the call; the stream given, or that device's
+    current one."""
+    index = t.device.index
+    cuda = _TORCH.cuda
+    before = cuda.current_device()
+    if stream is None:
+        s = _RAW_STREAM(index)
+    else:
+        s = stream if isinstance(stream, int) else stream.cuda_stream
+    if before == index:
+        status = entry(*args, s)
+    else:
+        with cuda.device(index):
+            status = entry(*args, s)
+    if status:
+        check(status)
 
 
 def group_rows(ids, experts: int, stream=None):
@@ -319,17 +341,20 @@ def group_rows(ids, experts: int, stream=None):
     (offsets [experts + 1], row_token [tokens * top_k], row_of_job [tokens, top_k]), all int32:
     x[row_token] are the rows in expert order, y[row_of_job] the results back in pick order (-1
     marks a pick without a row)."""
-    import torch
-    _matrix("ids", ids, 2, (torch.int32,))
-    _need(ids.is_contiguous(), "ids must be contiguous")
-    _need(1 <= experts <= 1024, "experts must be 1..1024")
+    torch = _torch()
+    if not ids.is_cuda:
+        _refuse("ids must be a CUDA tensor")
+    if ids.dtype != torch.int32 or ids.dim() != 2 or not ids.is_contiguous():
+        _refuse("ids must be a contiguous int32 tensor [tokens, top_k]")
+    if not 1 <= experts <= 1024:
+        _refuse("experts must be 1..1024")
     tokens, top_k = ids.shape
-    offsets = torch.empty(experts + 1, dtype=torch.int32, device=ids.device)
-    row_token = torch.empty(tokens * top_k, dtype=torch.int32, device=ids.device)
-    row_of_job = torch.empty((tokens, top_k), dtype=torch.int32, device=ids.device)
-    with _On(ids, stream) as s:
-        check(lib().umsx_group_rows(ids.data_ptr(), tokens, top_k, experts, offsets.data_ptr(), row_token.data_ptr(),
-                                    row_of_job.data_ptr(), s))
+    dev, i32 = ids.device, torch.int32
+    offsets = torch.empty_strided((experts + 1,), (1,), dtype=i32, device=dev)
+    row_token = torch.empty_strided((tokens * top_k,), (1,), dtype=i32, device=dev)
+    row_of_job = torch.empty_strided((tokens, top_k), (top_k, 1), dtype=i32, device=dev)
+    _call(lib().umsx_group_rows, ids, stream, ids.data_ptr(), tokens, top_k, experts, offsets.data_ptr(),
+          row_token.data_ptr(), row_of_job.data_ptr())
     return offsets, row_token, row_of_job
 
 
@@ -337,52 +362,54 @@ def grouped_mm(x, w, offsets, out=None, out_dtype=None, stream=None):
     """out[r] = x[r] @ w[e].T for the rows r of every expert e (umsx_grouped_mm): x [rows, k] and w
     [experts, n, k] both bfloat16 or both float16, offsets int32 [experts + 1]; out [rows, n] float32,
     bfloat16 or float16 (default: x's type).  Rows outside the groups are not written."""
-    import torch
-    _matrix("x", x, 2, (torch.bfloat16, torch.float16))
-    _matrix("w", w, 3, (x.dtype,), x)
+    _torch()
+    code = _matrix("x", x, 2, _SIXTEEN)
+    _matrix("w", w, 3, (code,), x)
     experts, n, k = w.shape
-    _need(x.shape[1] == k, f"x has {x.shape[1]} columns, w has {k}")
+    rows = x.shape[0]
+    if x.shape[1] != k:
+        _refuse(f"x has {x.shape[1]} columns, w has {k}")
     _offsets_arg(offsets, experts, x)
-    out = _out_arg("out", out, (x.shape[0], n), out_dtype, x, x.dtype)
-    with _On(x, stream) as s:
-        check(lib().umsx_grouped_mm(x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ld(w, -3), offsets.data_ptr(), experts,
-                                    x.shape[0], n, k, _codes()[x.dtype], out.data_ptr(), _ld(out),
-                                    _codes()[out.dtype], s))
+    out, oc = _out_arg("out", out, (rows, n), out_dtype, x, x.dtype)
+    _call(lib().umsx_grouped_mm, x, stream, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ld(w, -3), offsets.data_ptr(),
+          experts, rows, n, k, code, out.data_ptr(), _ld(out), oc)
     return out
 
 
 def grouped_mm_dx(dy, w, offsets, out=None, out_dtype=None, stream=None):
     """The gradient of grouped_mm's rows (umsx_grouped_mm_dx): dx[r] = dy[r] @ w[e], dy [rows, n], w
     [experts, n, k], dx [rows, k] (default: dy's type).  Rows outside the groups are not written."""
-    import torch
-    _matrix("dy", dy, 2, (torch.bfloat16, torch.float16))
-    _matrix("w", w, 3, (dy.dtype,), dy)
+    _torch()
+    code = _matrix("dy", dy, 2, _SIXTEEN)
+    _matrix("w", w, 3, (code,), dy)
     experts, n, k = w.shape
-    _need(dy.shape[1] == n, f"dy has {dy.shape[1]} columns, w has {n} rows")
+    rows = dy.shape[0]
+    if dy.shape[1] != n:
+        _refuse(f"dy has {dy.shape[1]} columns, w has {n} rows")
     _offsets_arg(offsets, experts, dy)
-    out = _out_arg("out", out, (dy.shape[0], k), out_dtype, dy, dy.dtype)
-    with _On(dy, stream) as s:
-        check(lib().umsx_grouped_mm_dx(dy.data_ptr(), _ld(dy), w.data_ptr(), _ld(w), _ld(w, -3), offsets.data_ptr(),
-                                       experts, dy.shape[0], n, k, _codes()[dy.dtype], out.data_ptr(), _ld(out),
-                                       _codes()[out.dtype], s))
+    out, oc = _out_arg("out", out, (rows, k), out_dtype, dy, dy.dtype)
+    _call(lib().umsx_grouped_mm_dx, dy, stream, dy.data_ptr(), _ld(dy), w.data_ptr(), _ld(w), _ld(w, -3),
+          offsets.data_ptr(), experts, rows, n, k, code, out.data_ptr(), _ld(out), oc)
     return out
 
 
 def grouped_mm_dw(dy, x, offsets, out=None, out_dtype=None, stream=None):
     """The gradient of grouped_mm's weights (umsx_grouped_mm_dw): dw[e] = dy[rows of e].T @ x[rows of e],
     [experts, n, k] (default: float32); zero for an expert without rows."""
-    import torch
-    _matrix("dy", dy, 2, (torch.bfloat16, torch.float16))
-    _matrix("x", x, 2, (dy.dtype,), dy)
-    _need(dy.shape[0] == x.shape[0], f"dy has {dy.shape[0]} rows, x has {x.shape[0]}")
-    n, k, experts = dy.shape[1], x.shape[1], offsets.shape[0] - 1 if offsets.dim() == 1 else 0
-    _need(experts >= 1, "offsets must hold at least two values")
+    torch = _torch()
+    code = _matrix("dy", dy, 2, _SIXTEEN)
+    _matrix("x", x, 2, (code,), dy)
+    rows, n = dy.shape
+    k = x.shape[1]
+    if x.shape[0] != rows:
+        _refuse(f"dy has {rows} rows, x has {x.shape[0]}")
+    experts = offsets.shape[0] - 1 if offsets.dim() == 1 else 0
+    if experts < 1:
+        _refuse("offsets must hold at least two values")
     _offsets_arg(offsets, experts, dy)
-    out = _out_arg("out", out, (experts, n, k), out_dtype, dy, torch.float32)
-    with _On(dy, stream) as s:
-        check(lib().umsx_grouped_mm_dw(dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), offsets.data_ptr(), experts,
-                                       dy.shape[0], n, k, _codes()[dy.dtype], out.data_ptr(), _ld(out), _ld(out, -3),
-                                       _codes()[out.dtype], s))
+    out, oc = _out_arg("out", out, (experts, n, k), out_dtype, dy, torch.float32)
+    _call(lib().umsx_grouped_mm_dw, dy, stream, dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), offsets.data_ptr(), experts,
+          rows, n, k, code, out.data_ptr(), _ld(out), _ld(out, -3), oc)
     return out
 
 
@@ -391,52 +418,69 @@ def fp8_quantize(x, block_rows: int = 1, q=None, scales=None, stream=None):
     one float32 scale per block of block_rows (1 or 128) x 128 values (umsx_fp8_quantize): (q, scales) with
     x ~ q * scale.  Scales of rows (block_rows 1) are laid out one block of columns after another, as the
     products read them: their shape is [.., rows, blocks], their last stride is the long one."""
-    import torch
-    _need(x.dim() in (2, 3), f"x must have 2 or 3 dimensions, got {x.dim()}")
-    _need(block_rows in (1, SCALE_BLOCK), "block_rows must be 1 or 128")
-    _matrix("x", x, x.dim(), (torch.float32, torch.bfloat16, torch.float16))
-    rows, cols = x.shape[-2:]
-    lead, br, bc = tuple(x.shape[:-2]), -(-rows // block_rows), -(-cols // SCALE_BLOCK)
+    torch = _torch()
+    dim = x.dim()
+    if dim != 2 and dim != 3:
+        _refuse(f"x must have 2 or 3 dimensions, got {dim}")
+    if block_rows != 1 and block_rows != SCALE_BLOCK:
+        _refuse("block_rows must be 1 or 128")
+    code = _matrix("x", x, dim, _OUT)
+    if dim == 2:
+        matrices, (rows, cols) = 1, x.shape
+    else:
+        matrices, rows, cols = x.shape
+    br, bc = -(-rows // block_rows), -(-cols // SCALE_BLOCK)
+    dev = x.device
     if q is None:
-        q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=x.device)
-    _matrix("q", q, x.dim(), (torch.float8_e4m3fn,), x)
-    _need(q.shape == x.shape, f"q must have x's shape {tuple(x.shape)}, got {tuple(q.shape)}")
+        q = _new((rows, cols) if dim == 2 else (matrices, rows, cols), torch.float8_e4m3fn, dev)
+        ldq, qm = cols, rows * cols
+    else:
+        _matrix("q", q, dim, (DTYPE_E4M3,), x)
+        if q.shape != x.shape:
+            _refuse(f"q must have x's shape {tuple(x.shape)}, got {tuple(q.shape)}")
+        ldq, qm = _ld(q), _ld(q, -3) if dim == 3 else 0
     if scales is None:
-        scales = torch.empty(lead + ((bc, br) if block_rows == 1 else (br, bc)), dtype=torch.float32, device=x.device)
-        scales = scales.transpose(-1, -2) if block_rows == 1 else scales
-    _need(scales.is_cuda and scales.device == x.device and scales.dtype == torch.float32,
-          "scales must be float32 and on x's device")
-    _need(tuple(scales.shape) == lead + (br, bc), f"scales must have shape {lead + (br, bc)}, got {tuple(scales.shape)}")
-    m3 = x.dim() == 3
-    with _On(x, stream) as s:
-        check(lib().umsx_fp8_quantize(x.data_ptr(), _ld(x), x.stride(0) if m3 else 0, _codes()[x.dtype],
-                                      x.shape[0] if m3 else 1, rows, cols, block_rows, q.data_ptr(), _ld(q),
-                                      _ld(q, -3) if m3 else 0, scales.data_ptr(), scales.stride(-2), scales.stride(-1),
-                                      scales.stride(0) if m3 else 0, s))
+        s_row, s_blk, sm = (1, br, br * bc) if block_rows == 1 else (bc, 1, br * bc)
+        if dim == 2:
+            scales = torch.empty_strided((br, bc), (s_row, s_blk), dtype=torch.float32, device=dev)
+        else:
+            scales = torch.empty_strided((matrices, br, bc), (sm, s_row, s_blk), dtype=torch.float32, device=dev)
+    else:
+        want = (br, bc) if dim == 2 else (matrices, br, bc)
+        if scales.device != dev or scales.dtype != torch.float32 or scales.shape != want:
+            _refuse(f"scales must be float32, on x's device and of shape {want}")
+        s_row, s_blk, sm = scales.stride(-2), scales.stride(-1), scales.stride(0) if dim == 3 else 0
+    _call(lib().umsx_fp8_quantize, x, stream, x.data_ptr(), _ld(x), x.stride(0) if dim == 3 else 0, code, matrices, rows,
+          cols, block_rows, q.data_ptr(), ldq, qm, scales.data_ptr(), s_row, s_blk, sm)
     return q, scales
 
 
 def _fp8_product(x, xs, w, ws, offsets, out, out_dtype, stream):
-    import torch
+    torch = _torch()
     grouped = offsets is not None
-    _matrix("x", x, 2, (torch.float8_e4m3fn,))
-    _matrix("w", w, 3 if grouped else 2, (torch.float8_e4m3fn,), x)
-    n, k = w.shape[-2:]
-    _need(x.shape[1] == k, f"x has {x.shape[1]} columns, w has {k}")
+    _matrix("x", x, 2, (DTYPE_E4M3,))
+    _matrix("w", w, 3 if grouped else 2, (DTYPE_E4M3,), x)
+    n, k = w.shape[-2], w.shape[-1]
+    rows = x.shape[0]
+    if x.shape[1] != k:
+        _refuse(f"x has {x.shape[1]} columns, w has {k}")
     bn, bk = -(-n // SCALE_BLOCK), -(-k // SCALE_BLOCK)
-    for name, t, shape in (("xs", xs, (x.shape[0], bk)), ("ws", ws, tuple(w.shape[:-2]) + (bn, bk))):
-        _need(t.is_cuda and t.device == x.device and t.dtype == torch.float32, f"{name} must be float32 and on x's device")
-        _need(tuple(t.shape) == shape, f"{name} must have shape {shape}, got {tuple(t.shape)}")
-    experts = w.shape[0] if grouped else 1
+    f32, dev = torch.float32, x.device
+    if xs.dtype != f32 or xs.device != dev or xs.shape != (rows, bk):
+        _refuse(f"xs must be float32, on x's device and of shape {(rows, bk)}, got {tuple(xs.shape)}")
+    want = (w.shape[0], bn, bk) if grouped else (bn, bk)
+    if ws.dtype != f32 or ws.device != dev or ws.shape != want:
+        _refuse(f"ws must be float32, on x's device and of shape {want}, got {tuple(ws.shape)}")
     if grouped:
+        experts, wm, sm = w.shape[0], _ld(w, -3), ws.stride(0)
         _offsets_arg(offsets, experts, x)
-    out = _out_arg("out", out, (x.shape[0], n), out_dtype, x, torch.bfloat16)
-    with _On(x, stream) as s:
-        check(lib().umsx_fp8_grouped_mm(
-            x.data_ptr(), _ld(x), xs.data_ptr(), xs.stride(0), xs.stride(1), w.data_ptr(), _ld(w),
-            _ld(w, -3) if grouped else 0, ws.data_ptr(), ws.stride(-2), ws.stride(-1), ws.stride(0) if grouped else 0,
-            offsets.data_ptr() if grouped else None, experts, x.shape[0], n, k, out.data_ptr(), _ld(out),
-            _codes()[out.dtype], s))
+        at = offsets.data_ptr()
+    else:
+        experts, wm, sm, at = 1, 0, 0, None
+    out, oc = _out_arg("out", out, (rows, n), out_dtype, x, torch.bfloat16)
+    _call(lib().umsx_fp8_grouped_mm, x, stream, x.data_ptr(), _ld(x), xs.data_ptr(), xs.stride(0), xs.stride(1),
+          w.data_ptr(), _ld(w), wm, ws.data_ptr(), ws.stride(-2), ws.stride(-1), sm, at, experts, rows, n, k,
+          out.data_ptr(), _ld(out), oc)
     return out
 
 
@@ -451,7 +495,8 @@ def fp8_grouped_mm(x, xs, w, ws, offsets, out=None, out_dtype=None, stream=None)
     """grouped_mm for e4m3 operands (umsx_fp8_grouped_mm): x [rows, k] with scales [rows, ceil(k/128)], w
     [experts, n, k] with scales [experts, ceil(n/128), ceil(k/128)]; out [rows, n] (default bfloat16).
     Rows outside the groups are not written."""
-    _need(offsets is not None, "offsets must be given")
+    if offsets is None:
+        _refuse("offsets must be given")
     return _fp8_product(x, xs, w, ws, offsets, out, out_dtype, stream)
 
 
