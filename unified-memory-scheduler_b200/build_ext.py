@@ -15,7 +15,7 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "..", "_build", "umsx")
 LIB = os.path.join(PKG, "libumsx.so")
 SOURCES = ["umsx_api.cu", "umsx_kernels.cu", "umsx_decode.cu", "umsx_gguf.cpp", "umsx_prefill.cu", "umsx_static.cu", "umsx_ep.cu",
-           "umsx_group.cu", "umsx_fp8.cu", "umsx_products.cu", "umsx_products_tc.cu"]
+           "umsx_group.cu", "umsx_fp8.cu", "umsx_products.cu", "umsx_products_tc.cu", "umsx_products_few.cu"]
 HEADERS = ["umsx_internal.h", "umsx_device.cuh", "umsx_mx.cuh", "umsx_tc.cuh", "umsx_products.h", "umsx_pair.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
