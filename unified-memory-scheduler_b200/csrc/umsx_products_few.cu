@@ -217,28 +217,32 @@ void launch(const FewParams &p, int nt, int64_t chunks, cudaStream_t s) {
     const dim3 grid((p.n + features - 1) / features, (unsigned)chunks);
     constexpr bool kF8 = DTYPE == UMSX_DTYPE_E4M3;  // steps in flight: what 128 registers hold
     if (nt == 1) k_product_few<DTYPE, 1, kF8 ? 3 : 4><<<grid, kWarps * 32, 0, s>>>(p);
-    else if (nt == 2) k_product_few<DTYPE, 2, 2><<<grid, kWarps * 32, 0, s>>>(p);
-    else k_product_few<DTYPE, 4, kF8 ? 1 : 2><<<grid, kWarps * 32, 0, s>>>(p);
+    else k_product_few<DTYPE, 2, 2><<<grid, kWarps * 32, 0, s>>>(p);
 }
 
 }  // namespace
 
-// Tiles of eight rows a CTA takes, or 0 where the tcgen05 kernel is to be used.
-static int few_tiles(const Product &p) {
+// Tiles of eight rows a CTA takes, or 0 where the tcgen05 kernel is to be used.  Measured with cold weights (2816 x 2048 e4m3,
+// 1536 x 2048 bf16), this kernel / the other: 3 rows an expert 82 / 78 us and 123 / 125, 6 rows 88 / 88, 8 rows (bf16) 160 / 147;
+// one matrix, which gives the other only n / 256 tiles: 8 rows 10.2 / 14.3, 32 rows 12.3 / 14.3 with two tiles of rows
+// (one: 14.3), 48 rows 14.3 / 14.3.
+static int few_tiles(const Product &p, int sms) {
     const double mean = (double)p.rows / p.groups;
-    if (mean > 16 || p.rows > 65000) return 0;
-    return mean <= 3 ? 1 : mean <= 8 ? 2 : 4;
+    const int64_t tiles = std::min<int64_t>(p.groups, p.rows) * ((p.n + 255) / 256);
+    if (p.rows > 32768) return 0;
+    if (mean <= 4) return 1;
+    return mean <= 32 && tiles <= sms / 2 ? (mean <= 8 ? 1 : 2) : 0;
 }
 
-bool product_few_takes(const Product &p) {
+bool product_few_takes(const Product &p, int sms) {
     const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2;
     const auto ok = [&](const void *b, int64_t ld) { return reinterpret_cast<uintptr_t>(b) % 16 == 0 && ld * size % 16 == 0; };
     return p.mode == kForward && p.rows > 0 && p.k * size % 16 == 0 && ok(p.x, p.ldx) && ok(p.w, p.ldw) &&
-           (p.groups == 1 || p.w_stride * size % 16 == 0) && few_tiles(p) > 0;
+           (p.groups == 1 || p.w_stride * size % 16 == 0) && few_tiles(p, sms) > 0;
 }
 
 int launch_product_few(const Product &p, int sms, cudaStream_t s) {
-    const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2, nt = few_tiles(p);
+    const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2, nt = few_tiles(p, sms);
     FewParams f{};
     f.groups = p.groups, f.n = p.n, f.k = p.k, f.out_dtype = p.out_dtype;
     f.rows = p.rows, f.offsets = p.offsets;
@@ -249,10 +253,11 @@ int launch_product_few(const Product &p, int sms, cudaStream_t s) {
     f.out = p.out, f.ldo = p.ldo;
     // chunks of 8 * nt rows: at most one that is not full for each group that has rows
     const int64_t chunks = p.offsets ? p.rows / (8 * nt) + std::min<int64_t>(p.groups, p.rows) : (p.rows + 8 * nt - 1) / (8 * nt);
-    // about two warps per resident one (16 an SM), for the blocks of 16 features that have rows
+    // As many warps as are resident (16 an SM) for the blocks of 16 features that have rows, and at most 2 KB of a row to a
+    // warp: 8 bf16 experts of 1536 features 18.5 us with two warps a block (four: 20.5), 16 tokens' 92 us (one: 98).
     const int64_t blocks = std::min<int64_t>(p.groups, p.rows) * ((p.n + kFewF - 1) / kFewF);
-    f.split = 8;
-    while (f.split > 1 && blocks * f.split > 32 * sms) f.split /= 2;
+    f.split = 1;
+    while (f.split < 8 && (2 * f.split * blocks <= 16 * sms || f.split * 2048 < p.k * size)) f.split *= 2;
     if (p.dtype == UMSX_DTYPE_BF16) launch<UMSX_DTYPE_BF16>(f, nt, chunks, s);
     else if (p.dtype == UMSX_DTYPE_F16) launch<UMSX_DTYPE_F16>(f, nt, chunks, s);
     else launch<UMSX_DTYPE_E4M3>(f, nt, chunks, s);
