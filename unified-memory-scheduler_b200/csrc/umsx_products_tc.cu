@@ -14,6 +14,10 @@
 // sums is fixed.  Roles: warp 0 TMA, warp 1 MMA, warps 2-9 epilogue, warp 10 (dw) the group's ragged end.
 // Two accumulators of 256 columns: the epilogue drains one while the MMA fills the other.
 //
+// The tensor cores add to an fp32 accumulator by truncation, whose error grows with the number of additions (2.5e-6 of the
+// result at a contraction of 2048, against 0.8e-6 of rounded fp32 sums).  Outputs in fp32 therefore get a fresh accumulator
+// every kSegment stages, which the epilogue adds up in registers; in 16-bit outputs the last rounding hides it.
+//
 // dw's contraction ends inside a block of 64 rows; the rows behind it belong to the next group.  Warp
 // 10 zeroes them in both operands (a zero in one would leave 0 * NaN) up to the next multiple of 16, where
 // the MMAs stop.  Only that last stage of a tile goes through it: handing every stage on cost 1.8 K cycles a stage.
@@ -41,10 +45,11 @@ constexpr int kRowsMax = 256;       // rows of a tile (of a pair: 128 in each CT
 constexpr int kRowBox = 32;         // rows of one K-major TMA box
 constexpr int kThreads = 352, kEpilogueWarps = 8;
 constexpr uint32_t kTmemCols = 512;
+constexpr int kSegment = 8;  // stages that share an accumulator where the output is fp32: 512 of the contraction
 constexpr int kStageRow = 80;  // bytes of a staged output row: 64 of data; 80 spreads eight rows over all banks
 
 struct TcParams {
-    int groups, features, contraction, out_rows, out_dtype, fmt, vec, bulk;
+    int groups, features, contraction, out_rows, out_dtype, fmt, vec, bulk, segment;
     int64_t rows;
     const int32_t *offsets;
     void *out;
@@ -320,9 +325,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                 const int kb = (x.c_len + kBC - 1) / kBC;
                 if (!x.rows || !kb) continue;
                 const uint32_t idesc = tc::operand_idesc(p.fmt, S::kFMn, S::kRMn, kBF * CG, x.n);
-                const uint32_t buf = n_item & 1u, d_tm = tmem + buf * kRowsMax;
-                tc::wait(b_dempty + 8 * buf, ((n_item >> 1) & 1u) ^ 1u, up);
-                for (int kk = 0; kk < kb; ++kk, r.next()) {
+                uint32_t buf = 0, d_tm = 0;
+                for (int kk = 0, in_seg = 0; kk < kb; ++kk, r.next()) {
+                    if (in_seg == 0) {
+                        buf = n_item & 1u, d_tm = tmem + buf * kRowsMax;
+                        tc::wait(b_dempty + 8 * buf, ((n_item >> 1) & 1u) ^ 1u, up);
+                        ++n_item;
+                    }
                     tc::wait(b_full + 8 * r.s, r.phase, up);
                     if (MODE == kGradWeight && kk == kb - 1 && (x.c_len & 15)) {
                         tc::wait<(CG > 1)>(b_fixed + 8 * r.s, fixed_phase >> r.s & 1u, up);
@@ -338,13 +347,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                         for (int j = 0; j < kBC / 16; ++j)
                             if (16 * j < left)
                                 tc::pair_mma<CG, tc::kKindF16>(d_tm, df + j * (S::kFMn ? 128 : 2), dr + j * (S::kRMn ? 128 : 2), idesc,
-                                                               (kk | j) != 0);
+                                                               (in_seg | j) != 0);
                         tc::pair_commit<CG>(b_empty + 8 * r.s);
-                        if (kk == kb - 1) tc::pair_commit<CG>(b_dfull + 8 * buf);
+                        if (kk == kb - 1 || in_seg == p.segment - 1) tc::pair_commit<CG>(b_dfull + 8 * buf);
                     }
                     __syncwarp();
+                    if (++in_seg == p.segment) in_seg = 0;
                 }
-                ++n_item;
             }
             // nor under MMAs in flight
             if (tc::elect_one()) tc::leader_commit<CG>(smem_u32(&last));
@@ -361,31 +370,59 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             const int f = x.f0 + (int)rank * kBF + quad * 32;
             const OutTile o{p.out, (MODE == kGradWeight ? x.g * p.out_group : 0) + (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype,
                             p.features - f, x.rows, p.vec != 0};
-            const uint32_t buf = n_item & 1u;
-            const bool zero = x.c_len == 0;
-            if (!zero) {
+            const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+            const int kb = (x.c_len + kBC - 1) / kBC, segments = kb > p.segment ? (kb + p.segment - 1) / p.segment : kb > 0;
+            // The next accumulator, and its return.
+            auto take = [&] {
+                const uint32_t buf = n_item & 1u;
                 tc::wait(b_dfull + 8 * buf, (n_item >> 1) & 1u, up);
                 tc::fence_after_sync();
                 ++n_item;
-            }
-            for (int c0 = part * 16; c0 < x.rows; c0 += 32) {
-                uint32_t v[16];
-                if (!zero) {
-                    tc::tmem_ld_frag(tmem + ((uint32_t)(quad * 32) << 16) + buf * kRowsMax + c0, v);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) v[j] = 0;
-                }
-                store_chunk(o, stage, lane, c0, v);
-            }
-            if (!zero) {
+                return buf;
+            };
+            auto give = [&](uint32_t buf) {
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
                     if constexpr (CG == 1) tc::arrive(b_dempty + 8 * buf);
                     else tc::arrive_at(tc::leader_addr(b_dempty + 8 * buf));
                 }
+            };
+            if (segments <= 1) {
+                const uint32_t buf = segments ? take() : 0;
+                for (int c0 = part * 16; c0 < x.rows; c0 += 32) {
+                    uint32_t v[16] = {};  // an expert without rows: dw is zero
+                    if (segments) tc::tmem_ld_frag(lanes + buf * kRowsMax + c0, v);
+                    store_chunk(o, stage, lane, c0, v);
+                }
+                if (segments) give(buf);
+                continue;
             }
+            float acc[kRowsMax / 32][16];
+#pragma unroll
+            for (int c = 0; c < kRowsMax / 32; ++c)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[c][j] = 0.0f;
+            for (int g = 0; g < segments; ++g) {
+                const uint32_t buf = take();
+#pragma unroll
+                for (int c = 0; c < kRowsMax / 32; ++c)
+                    if (32 * c + part * 16 < x.rows) {
+                        uint32_t v[16];
+                        tc::tmem_ld_frag(lanes + buf * kRowsMax + 32 * c + part * 16, v);
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) acc[c][j] += __uint_as_float(v[j]);
+                    }
+                give(buf);
+            }
+#pragma unroll
+            for (int c = 0; c < kRowsMax / 32; ++c)
+                if (32 * c + part * 16 < x.rows) {
+                    uint32_t v[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(acc[c][j]);
+                    store_chunk(o, stage, lane, 32 * c + part * 16, v);
+                }
         }
     } else if (MODE == kGradWeight) {
         uint32_t it = 0, tail_phase = 0;
@@ -928,6 +965,7 @@ int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
     t.ldo = p.ldo;
     t.out_group = p.out_stride;
     t.vec = aligned(p.out, p.ldo, 2) && p.out_stride % 8 == 0;
+    t.segment = p.out_dtype == UMSX_DTYPE_F32 ? kSegment : 0x7fffffff;
     t.bulk = t.vec && p.out_dtype != UMSX_DTYPE_F32;
     if (p.dtype == UMSX_DTYPE_E4M3) {
         const F8Params fp{t, p.xs, p.ws, p.xs_row, p.xs_blk, p.ws_row, p.ws_blk, p.ws_group};
