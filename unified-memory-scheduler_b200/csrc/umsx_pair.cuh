@@ -145,20 +145,26 @@ __host__ __device__ constexpr uint32_t operand_idesc(int fmt, bool a_mn, bool b_
 }
 
 // 16 consecutive fp32 columns of this warp's 32 TMEM lanes, in the fragment order of 8 x 8 matrices: r[8h + 4i + 2u + j]
-// is lane 16h + 8u + (thread / 4), column 8i + 2 (thread % 4) + j.
-__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
+// is lane 16h + 8u + (thread / 4), column 8i + 2 (thread % 4) + j.  Complete after tmem_wait_ld(r).
+__device__ __forceinline__ void tmem_ld_frag_async(uint32_t taddr, uint32_t (&r)[16]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
         asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
                      : "=r"(r[8 * h]), "=r"(r[8 * h + 1]), "=r"(r[8 * h + 2]), "=r"(r[8 * h + 3]), "=r"(r[8 * h + 4]),
                        "=r"(r[8 * h + 5]), "=r"(r[8 * h + 6]), "=r"(r[8 * h + 7])
                      : "r"(taddr + ((uint32_t)(16 * h) << 16)));
-    // the values are operands of the wait, so that no use of them moves above it
+}
+// All loads so far are complete.  The values are operands of the wait, so that no use of them moves above it.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
                    "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
                  :
                  : "memory");
+}
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t (&r)[16]) {
+    tmem_ld_frag_async(taddr, r);
+    tmem_wait_ld(r);
 }
 
 // Four 8 x 8 matrices of 16-bit values in fragment order, transposed, to the 16-byte rows that the lanes name

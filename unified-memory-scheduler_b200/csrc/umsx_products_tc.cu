@@ -84,9 +84,13 @@ struct Tiles {
             lo += __popc(below);
             if (below != kFull) break;
         }
-        const int a = start[2 * lo], m = start[2 * lo + 1] - a;
+        // A value that comes out of lane 0's register is the same in all lanes for the compiler too: the loops' counters and the
+        // descriptors made of them then live in uniform registers, where the MMAs and copies want them.
+        const auto uniform = [](int v) { return __shfl_sync(kFull, v, 0); };
+        lo = uniform(lo);
+        const int a = uniform(start[2 * lo]), m = uniform(start[2 * lo + 1]) - a;
         const int all = MODE == kGradWeight ? out_rows : m, rt = row_tiles(all);
-        const int local = t - prefix[lo];
+        const int local = t - uniform(prefix[lo]);
         int i = 0, j = local, each = all;
         if (rt > 1) i = local % rt, j = local / rt, each = (all + rt - 1) / rt;
         // equal tiles, in steps of the MMA's N
@@ -223,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     __shared__ int gave_up;
     __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
     const uint32_t rank = CG == 1 ? 0 : tc::cluster_rank();
     const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
 
@@ -250,20 +254,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     if constexpr (CG == 1) __syncthreads();
     else tc::cluster_sync_all();  // barriers are initialised before the peer's copies and arrivals reach them
     tc::fence_after_sync();
-    const uint32_t tmem = tmem_s;
-    const int total = prefix[p.groups];
+    const uint32_t tmem = __shfl_sync(kFull, tmem_s, 0);
+    const int total = __shfl_sync(kFull, prefix[p.groups], 0);
     const Tiles<CG, MODE> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
     const uint32_t up = smem_u32(&gave_up), aF = smem_u32(sF), aR = smem_u32(sR);
     const uint32_t b_full = smem_u32(full), b_empty = smem_u32(empty), b_dfull = smem_u32(d_full), b_dempty = smem_u32(d_empty),
                    b_tail = smem_u32(tail), b_fixed = smem_u32(fixed);
-    volatile int *const stop = &gave_up;
+    const auto stop = [&] { return __shfl_sync(kFull, *const_cast<volatile int *>(&gave_up), 0) != 0; };
 
     if (warp == 0) {
         tc::Ring<S::kStages> r;
         uint32_t tails = 0, tail_phase = 0, used = 0;  // bit s: stage s holds a ragged end; uses of tail[s], mod 2; stages in use
         int group = 0;
-        for (int t = cluster; t < total && !*stop; t += clusters) {
+        for (int t = cluster; t < total && !stop(); t += clusters) {
             const Tile x = tiles.get(t, group, lane);
             const int kb = (x.c_len + kBC - 1) / kBC;
             if (!x.rows) continue;
@@ -311,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             if (!(used >> s & 1u)) continue;
             const uint32_t last_phase = r.phase ^ (s >= r.s ? 1u : 0u);
             mbar_wait_bounded(&empty[s], last_phase, tc::kPairWaitCycles / 8);
-            if (!*stop) continue;
+            if (!stop()) continue;
             if (tails >> s & 1u) mbar_wait_bounded(&tail[s], (tail_phase >> s & 1u) ^ 1u, tc::kPairWaitCycles / 8);
             else if (rank == 0) mbar_wait_bounded(&full[s], last_phase, tc::kPairWaitCycles / 8);
         }
@@ -320,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             tc::Ring<S::kStages> r;
             uint32_t n_item = 0, fixed_phase = 0;
             int group = 0;
-            for (int t = cluster; t < total && !*stop; t += clusters) {
+            for (int t = cluster; t < total && !stop(); t += clusters) {
                 const Tile x = tiles.get(t, group, lane);
                 const int kb = (x.c_len + kBC - 1) / kBC;
                 if (!x.rows || !kb) continue;
@@ -364,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
         uint8_t *stage = smem + S::kStages * (S::kBytesF + S::kBytesR) + (warp - 2) * 16 * kStageRow;
         uint32_t n_item = 0;
         int group = 0;
-        for (int t = cluster; t < total && !*stop; t += clusters) {
+        for (int t = cluster; t < total && !stop(); t += clusters) {
             const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
             const int f = x.f0 + (int)rank * kBF + quad * 32;
@@ -427,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     } else if (MODE == kGradWeight) {
         uint32_t it = 0, tail_phase = 0;
         int group = 0;
-        for (int t = cluster; t < total && !*stop; t += clusters) {
+        for (int t = cluster; t < total && !stop(); t += clusters) {
             const Tile x = tiles.get(t, group, lane);
             const int kb = (x.c_len + kBC - 1) / kBC;
             if (!x.rows) continue;
@@ -451,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             }
         }
     }
-    if (lane == 0 && *stop) atomicOr(&g_product_err, 1u);
+    if (stop() && lane == 0) atomicOr(&g_product_err, 1u);
     __syncwarp();
     tc::fence_before_sync();
     if constexpr (CG == 1) __syncthreads();
@@ -468,40 +472,33 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
 // block of w), so warps 2-3 put xs * ws of a stage's rows into shared memory and a thread multiplies
 // pairs of columns with one packed FMA.
 //
-// The promotion bounds the widest tiles: 256 columns take the eight warps 600 cycles (the accumulator leaves TMEM at
-// about 230 bytes a cycle, measured alone), their MMAs 512.  What it needs: the number of column chunks a compile-time
-// constant (a test per chunk costs 350 cycles a block) and 16 columns a load (with 32 the sums spill).  128 sums a
-// thread leave no room for more warps: sixteen of them with half the sums spill at 96 registers and are no faster.
+// A tile's rows are two halves, each with MMAs, accumulators (two of 128 columns), a scale warp and four promotion
+// warps of its own, so that one half's waits and tile changes run under the other's arithmetic; with both halves in
+// one accumulator the eight warps waited together, 250 of a block's 850 cycles at 128 rows.  The promotion bounds wide
+// tiles: the accumulator leaves TMEM at about 230 bytes a cycle, 256 columns in 570 cycles, their MMAs take 512.  What it
+// needs: the number of column chunks a compile-time constant (a test per chunk costs 350 cycles a block) and, at 128
+// columns, 16 columns a load (with 32 the sums spill).
 //
 // 16-bit outputs leave through a staging of the whole tile and TMA stores of 32 or 8 rows, which drain under the next
 // tile's blocks; the last rows of a group, fewer than eight, are stored by the warps, since a box would overwrite the next
 // group's.  Stored by the promotion warps alone, all SMs at once, tiles took 5 K of their 23 K cycles (16 blocks) for it.
-//
-// Tensor memory is a ring of four slots of 128 columns; a tile of more than 128 rows takes two.  So narrow tiles have
-// four accumulators in flight, which covers the way from the MMAs to the promotion and back.
 
-constexpr int kThreadsF8 = 384, kSlots = 4, kSlotCols = 128;
-
-// The ring of accumulator slots as every role walks it: the same sequence of tiles gives the same slots.
-struct SlotRing {
-    uint32_t pos = 0, full_phase = 0, empty_phase = 0;  // phases: bit s is the parity of slot s's next use
-    int slot = 0;
-    __device__ __forceinline__ void next(bool wide) {
-        if (wide) pos = (pos + 1) & ~1u;
-        slot = (int)(pos & (kSlots - 1));
-        pos += wide ? 2 : 1;
-    }
-    __device__ __forceinline__ uint32_t full() const { return (full_phase >> slot) & 1u; }
-    __device__ __forceinline__ uint32_t empty(int s) const { return ((empty_phase >> s) & 1u) ^ 1u; }
-    __device__ __forceinline__ void used(bool wide) {
-        full_phase ^= 1u << slot;
-        empty_phase ^= (wide ? 3u : 1u) << slot;
-    }
-};
+constexpr int kThreadsF8 = 384, kHalfCols = 128, kSlots = 4, kHalfWarps = 4;
 
 // A staged tile: two halves of 64 features, a row of a half is 128 bytes with the swizzle of the tensor map (16-byte
 // chunk c of row r at c ^ (r & 7)).
 constexpr int kHalfTile = kRowsMax * 128;
+
+// Half h of a tile: columns [at, at + n) of its n, and its accumulators: slot h + 2 * (block & 1).
+struct Half {
+    int at, n;
+};
+template <int CG>
+__device__ __forceinline__ Half tile_half(int n, int h) {
+    constexpr int kStep = 16 * CG;
+    const int first = (n / 2 + kStep - 1) / kStep * kStep;
+    return h ? Half{first, n - first} : Half{0, first};
+}
 
 struct F8Params {
     TcParams t;
@@ -512,13 +509,13 @@ struct F8Params {
 template <int CG>
 struct ShapeF8 {
     static constexpr int kBC8 = 128;  // contraction per stage, in bytes too
-    static constexpr int kBytesF = kBF * kBC8, kBytesR = kRowsMax / CG * kBC8;
+    static constexpr int kBytesF = kBF * kBC8, kBytesR = kRowsMax / CG * kBC8, kBytesHalf = kBytesR / 2;
     static constexpr int kStages = 4;
     static constexpr size_t kOperands = (size_t)kStages * (kBytesF + kBytesR);
     // a pair's half stages leave room for a tile; a single CTA's (outputs of at most 128 features) do not
     static constexpr bool kBulk = CG == 2;
     static constexpr size_t kStaging = kBulk ? 2 * kHalfTile : kEpilogueWarps * 16 * kStageRow;
-    static constexpr size_t kSmem = 1024 + kOperands + kSlots * kSlotCols * sizeof(float) + kStaging;
+    static constexpr size_t kSmem = 1024 + kOperands + kSlots * kHalfCols * sizeof(float) + kStaging;
 };
 
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t)lo | ((uint64_t)hi << 32); }
@@ -535,46 +532,46 @@ struct F8Sync {
     const CUtensorMap *out32, *out8;  // boxes of 64 features x 32 and x 8 rows
 };
 
-// One tile by one promotion warp: NCH chunks of 32 columns, from 32 * part in turns of 64.
+// Half `part` of a tile by one promotion warp: NCH chunks of 32 columns.  `it`: blocks of this half so far.
 template <int CG, int NCH>
-__device__ __forceinline__ void promote_tile(const F8Sync &y, SlotRing &ring, const TcParams &p, const Tile &x, int f, int kb,
-                                             bool wide, int part, int lane) {
-    uint64_t acc[NCH ? 2 * NCH : 1][8];  // 16 columns, pairs of columns in fragment order: 0.0f
+__device__ __forceinline__ void promote_half(const F8Sync &y, uint32_t &it, const TcParams &p, const Tile &x, const Half &half,
+                                             int f, int kb, int part, int lane) {
+    uint64_t acc[2 * NCH][8];  // 16 columns, pairs of columns in fragment order: 0.0f
 #pragma unroll
     for (int h = 0; h < 2 * NCH; ++h)
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[h][i] = 0;
-    auto column = [&](int h) { return (2 * (h >> 1) + part) * 32 + 16 * (h & 1); };
-    for (int kk = 0; kk < kb; ++kk) {
-        ring.next(wide);
-        const int slot = ring.slot;
-        tc::wait(y.d_full + 8 * slot, ring.full(), y.gave_up);
+    constexpr int kTogether = NCH <= 2 ? 2 * NCH : 1;  // loads of 16 columns under one wait
+    for (int kk = 0; kk < kb; ++kk, ++it) {
+        const int slot = part + 2 * (int)(it & 1u);
+        tc::wait(y.d_full + 8 * slot, (it >> 1) & 1u, y.gave_up);
         tc::fence_after_sync();
-        const float *sc = y.scales + slot * kSlotCols + 2 * (lane & 3);
-        const uint32_t src = y.lanes + slot * kSlotCols;
+        const float *sc = y.scales + slot * kHalfCols + 2 * (lane & 3);
+        const uint32_t src = y.lanes + slot * kHalfCols;
 #pragma unroll
-        for (int h = 0; h < 2 * NCH; ++h) {
-            uint32_t v[16];
-            tc::tmem_ld_frag(src + column(h), v);
+        for (int h0 = 0; h0 < 2 * NCH; h0 += kTogether) {
+            uint32_t v[kTogether][16];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint64_t s2 = *reinterpret_cast<const uint64_t *>(sc + column(h) + 8 * i);
+            for (int j = 0; j < kTogether; ++j) tc::tmem_ld_frag_async(src + 16 * (h0 + j), v[j]);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int e = 8 * (q >> 1) + 4 * i + 2 * (q & 1);
-                    fma2(acc[h][e >> 1], pack2(v[e], v[e + 1]), s2);
+            for (int j = 0; j < kTogether; ++j) tc::tmem_wait_ld(v[j]);
+#pragma unroll
+            for (int j = 0; j < kTogether; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint64_t s2 = *reinterpret_cast<const uint64_t *>(sc + 16 * (h0 + j) + 8 * i);
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int e = 8 * (q >> 1) + 4 * i + 2 * (q & 1);
+                        fma2(acc[h0 + j][e >> 1], pack2(v[j][e], v[j][e + 1]), s2);
+                    }
                 }
-            }
         }
         tc::fence_before_sync();
         __syncwarp();
-        if (lane < (wide ? 4 : 2)) {  // one lane per barrier
-            const uint32_t at = 8 * (slot + (lane >> 1));
-            tc::arrive_at(lane & 1 ? y.sc_empty + at : CG == 1 ? y.d_empty + at : tc::leader_addr(y.d_empty + at));
-        }
-        ring.used(wide);
+        if (lane < 2)  // one lane per barrier
+            tc::arrive_at(lane ? y.sc_empty + 8 * slot : CG == 1 ? y.d_empty + 8 * slot : tc::leader_addr(y.d_empty + 8 * slot));
     }
-    if constexpr (NCH == 0) return;
     auto sums = [&](int h, uint32_t (&v)[16]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -593,14 +590,14 @@ __device__ __forceinline__ void promote_tile(const F8Sync &y, SlotRing &ring, co
             for (int h = 0; h < 2 * NCH; ++h) {
                 uint32_t v[16];
                 sums(h, v);
-                stage16<true, true>(to + column(h) * 128, chunk, lane, v);
+                stage16<true, true>(to + (half.at + 16 * h) * 128, chunk, lane, v);
             }
         } else {
 #pragma unroll
             for (int h = 0; h < 2 * NCH; ++h) {
                 uint32_t v[16];
                 sums(h, v);
-                stage16<false, true>(to + column(h) * 128, chunk, lane, v);
+                stage16<false, true>(to + (half.at + 16 * h) * 128, chunk, lane, v);
             }
         }
         tc::fence_proxy_async();
@@ -611,19 +608,19 @@ __device__ __forceinline__ void promote_tile(const F8Sync &y, SlotRing &ring, co
                 const int f0 = f;  // of the tile's 128
 #pragma unroll
                 for (int c = 0; c < NCH; ++c)
-                    for (int half = 0; half < 2 && f0 + 64 * half < p.features; ++half) {
-                        const int r = (2 * c + part) * 32;
-                        const uint32_t src = smem_u32(y.staging) + half * kHalfTile;
-                        if (r + 32 <= even) tc::tma_store_2d(y.out32, f0 + 64 * half, x.row0 + r, src + r * 128);
+                    for (int s = 0; s < 2 && f0 + 64 * s < p.features; ++s) {
+                        const int r = half.at + 32 * c;
+                        const uint32_t src = smem_u32(y.staging) + s * kHalfTile;
+                        if (r + 32 <= even) tc::tma_store_2d(y.out32, f0 + 64 * s, x.row0 + r, src + r * 128);
                         else
                             for (int q = r; q < even && q < r + 32; q += 8)
-                                tc::tma_store_2d(y.out8, f0 + 64 * half, x.row0 + q, src + q * 128);
+                                tc::tma_store_2d(y.out8, f0 + 64 * s, x.row0 + q, src + q * 128);
                     }
                 tc::bulk_commit();
             }
             __syncwarp();
         }
-        if (left && (even >> 5 & 1) == part) {  // in this part's chunk: four lanes to a row
+        if (left && even >= half.at && even < half.at + half.n) {  // in this half: four lanes to a row
             const int row = even + (lane >> 2), fl = 8 * (lane & 3);
             if (row < x.rows && f + fl < p.features) {
                 const uint4 w = *reinterpret_cast<const uint4 *>(to + row * 128 + ((chunk + (lane & 3)) ^ (row & 7)) * 16);
@@ -640,13 +637,14 @@ __device__ __forceinline__ void promote_tile(const F8Sync &y, SlotRing &ring, co
         }
         return;
     }
-    const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, x.rows, p.vec != 0};
+    // a half ends at a multiple of 16 (of 32 in a pair), its last chunk may not
+    const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, min(x.rows, half.at + half.n), p.vec != 0};
     uint8_t *own = y.staging + (quad + 4 * part) * 16 * kStageRow;
 #pragma unroll
     for (int h = 0; h < 2 * NCH; ++h) {
         uint32_t v[16];
         sums(h, v);
-        store_chunk(o, own, lane, column(h), v);
+        store_chunk(o, own, lane, half.at + 16 * h, v);
     }
 }
 
@@ -659,7 +657,7 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     const TcParams &p = fp.t;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
-    uint8_t *sF = smem, *sR = smem + S::kStages * S::kBytesF;
+    uint8_t *sF = smem, *sR = smem + S::kStages * S::kBytesF;  // a stage of R: the rows of half 0, from its middle those of half 1
     uint8_t *staging = smem + S::kOperands;  // 1024-byte aligned
     float *scales = reinterpret_cast<float *>(staging + S::kStaging);  // [slot][column]: xs * ws
     // d_full: a slot's MMAs and its scales; d_empty: read by both CTAs' warps; sc_empty: by this one's
@@ -668,7 +666,7 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     __shared__ int gave_up;
     __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
 
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
     const uint32_t rank = CG == 1 ? 0 : tc::cluster_rank();
     const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
 
@@ -682,8 +680,8 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
         }
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(&d_full[s], 2);
-            mbar_init(&d_empty[s], CG * kEpilogueWarps);
-            mbar_init(&sc_empty[s], kEpilogueWarps);
+            mbar_init(&d_empty[s], CG * kHalfWarps);
+            mbar_init(&sc_empty[s], kHalfWarps);
         }
     }
     if (warp == 1) tc::pair_tmem_alloc<CG>(&tmem_s, kTmemCols);
@@ -694,25 +692,27 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     if constexpr (CG == 1) __syncthreads();
     else tc::cluster_sync_all();
     tc::fence_after_sync();
-    const uint32_t tmem = tmem_s;
-    const int total = prefix[p.groups], kb = (p.contraction + S::kBC8 - 1) / S::kBC8;
+    const uint32_t tmem = __shfl_sync(kFull, tmem_s, 0);
+    const int total = __shfl_sync(kFull, prefix[p.groups], 0), kb = (p.contraction + S::kBC8 - 1) / S::kBC8;
     const Tiles<CG, kForward> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
     const uint32_t up = smem_u32(&gave_up), aF = smem_u32(sF), aR = smem_u32(sR);
     const uint32_t b_full = smem_u32(full), b_empty = smem_u32(empty), b_dfull = smem_u32(d_full), b_dempty = smem_u32(d_empty),
                    b_sempty = smem_u32(sc_empty);
-    volatile int *const stop = &gave_up;
+    const auto stop = [&] { return __shfl_sync(kFull, *const_cast<volatile int *>(&gave_up), 0) != 0; };
 
     if (warp == 0) {
         tc::Ring<S::kStages> r;
         uint32_t used = 0;  // stages in use
         int group = 0;
-        for (int t = cluster; t < total && !*stop; t += clusters) {
+        for (int t = cluster; t < total && !stop(); t += clusters) {
             const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
-            const int half = x.n / CG, boxes = (half + kRowBox - 1) / kRowBox;
-            const uint32_t bytes = S::kBytesF + boxes * kRowBox * S::kBC8;
-            const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
+            const Half h0 = tile_half<CG>(x.n, 0), h1 = tile_half<CG>(x.n, 1);
+            const int rows0 = h0.n / CG, rows1 = h1.n / CG;  // this CTA's rows of each half
+            const int boxes0 = (rows0 + kRowBox - 1) / kRowBox, boxes1 = (rows1 + kRowBox - 1) / kRowBox;
+            const uint32_t bytes = S::kBytesF + (boxes0 + boxes1) * kRowBox * S::kBC8;
+            const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * rows0, r1 = x.row0 + h1.at + (int)rank * rows1;
             for (int kk = 0; kk < kb; ++kk, r.next()) {
                 tc::wait(b_empty + 8 * r.s, r.phase ^ 1u, up);
                 used |= 1u << r.s;
@@ -720,9 +720,13 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
                     uint32_t bar = b_full + 8 * r.s;
                     if (rank == 0) tc::expect_tx(bar, CG * bytes);
                     if (CG > 1) bar = tc::leader_addr(bar);
-                    tc::pair_tma_3d<CG>(aF + r.s * S::kBytesF, &map_f, kk * S::kBC8, f0, x.g, bar);
-                    for (int b = 0; b < boxes; ++b)
-                        tc::pair_tma_2d<CG>(aR + r.s * S::kBytesR + b * kRowBox * S::kBC8, &map_r, kk * S::kBC8, r0 + kRowBox * b, bar);
+                    const int c = kk * S::kBC8;
+                    const uint32_t dR = aR + r.s * S::kBytesR;
+                    tc::pair_tma_3d<CG>(aF + r.s * S::kBytesF, &map_f, c, f0, x.g, bar);
+                    for (int b = 0; b < boxes0; ++b)
+                        tc::pair_tma_2d<CG>(dR + b * kRowBox * S::kBC8, &map_r, c, r0 + kRowBox * b, bar);
+                    for (int b = 0; b < boxes1; ++b)
+                        tc::pair_tma_2d<CG>(dR + S::kBytesHalf + b * kRowBox * S::kBC8, &map_r, c, r1 + kRowBox * b, bar);
                 }
                 __syncwarp();
             }
@@ -731,107 +735,108 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
             if (!(used >> s & 1u)) continue;
             const uint32_t last_phase = r.phase ^ (s >= r.s ? 1u : 0u);
             mbar_wait_bounded(&empty[s], last_phase, tc::kPairWaitCycles / 8);
-            if (*stop && rank == 0) mbar_wait_bounded(&full[s], last_phase, tc::kPairWaitCycles / 8);
+            if (stop() && rank == 0) mbar_wait_bounded(&full[s], last_phase, tc::kPairWaitCycles / 8);
         }
     } else if (warp == 1) {
         if (rank == 0) {
             tc::Ring<S::kStages> r;
-            SlotRing ring;
+            uint32_t it[2] = {0, 0};  // blocks of each half so far
             int group = 0;
-            for (int t = cluster; t < total && !*stop; t += clusters) {
+            for (int t = cluster; t < total && !stop(); t += clusters) {
                 const Tile x = tiles.get(t, group, lane);
                 if (!x.rows) continue;
-                const bool wide = x.n > kSlotCols;
-                const uint32_t idesc = tc::operand_idesc(0, false, false, kBF * CG, x.n);
+                const int n0 = tile_half<CG>(x.n, 0).n, n1 = tile_half<CG>(x.n, 1).n;
+                const uint32_t idesc0 = tc::operand_idesc(0, false, false, kBF * CG, n0);
+                const uint32_t idesc1 = tc::operand_idesc(0, false, false, kBF * CG, n1);
                 for (int kk = 0; kk < kb; ++kk, r.next()) {
-                    ring.next(wide);
-                    const int slot = ring.slot;
-                    tc::wait(b_dempty + 8 * slot, ring.empty(slot), up);
-                    if (wide) tc::wait(b_dempty + 8 * slot + 8, ring.empty(slot + 1), up);
+                    const uint64_t df = tc::operand_desc(aF + r.s * S::kBytesF, false, 0);
+                    const uint64_t dr = tc::operand_desc(aR + r.s * S::kBytesR, false, 0);
+                    const int left = p.contraction - kk * S::kBC8;
                     tc::wait(b_full + 8 * r.s, r.phase, up);
-                    tc::fence_after_sync();
-                    if (tc::elect_one()) {
-                        const uint64_t df = tc::operand_desc(aF + r.s * S::kBytesF, false, 0);
-                        const uint64_t dr = tc::operand_desc(aR + r.s * S::kBytesR, false, 0);
-                        const int left = p.contraction - kk * S::kBC8;
 #pragma unroll
-                        for (int j = 0; j < S::kBC8 / 32; ++j)
-                            if (32 * j < left)
-                                tc::pair_mma<CG, tc::kKindF8>(tmem + slot * kSlotCols, df + 2 * j, dr + 2 * j, idesc, j != 0);
-                        tc::pair_commit<CG>(b_empty + 8 * r.s);
-                        tc::pair_commit<CG>(b_dfull + 8 * slot);
+                    for (int h = 0; h < 2; ++h) {
+                        if (h && !n1) break;
+                        const int slot = h + 2 * (int)(it[h] & 1u);
+                        tc::wait(b_dempty + 8 * slot, ((it[h] >> 1) & 1u) ^ 1u, up);
+                        tc::fence_after_sync();
+                        if (tc::elect_one()) {
+#pragma unroll
+                            for (int j = 0; j < S::kBC8 / 32; ++j)
+                                if (32 * j < left)
+                                    tc::pair_mma<CG, tc::kKindF8>(tmem + slot * kHalfCols, df + 2 * j,
+                                                                  dr + h * (S::kBytesHalf >> 4) + 2 * j, h ? idesc1 : idesc0, j != 0);
+                            tc::pair_commit<CG>(b_dfull + 8 * slot);
+                            if (h || !n1) tc::pair_commit<CG>(b_empty + 8 * r.s);
+                        }
+                        __syncwarp();
+                        ++it[h];
                     }
-                    __syncwarp();
-                    ring.used(wide);
                 }
             }
             if (tc::elect_one()) tc::leader_commit<CG>(smem_u32(&last));  // nor under MMAs in flight
             mbar_wait_bounded(&last, 0, tc::kPairWaitCycles / 8);
         }
     } else if (warp < 4) {
-        // ---- scales: the two warps take turns; each loads its next stage's before it waits for a slot ----
+        // ---- scales of half warp - 2, two blocks ahead ----------------------------------------------------
+        const int h = warp - 2;
         uint32_t it = 0;
-        SlotRing ring;
         int group = 0;
-        for (int t = cluster; t < total && !*stop; t += clusters) {
+        for (int t = cluster; t < total && !stop(); t += clusters) {
             const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
-            const bool wide = x.n > kSlotCols;
-            const int f0 = x.f0 + (int)rank * kBF;
+            const Half half = tile_half<CG>(x.n, h);
+            if (!half.n) continue;
+            const int f0 = x.f0 + (int)rank * kBF, first = half.at + lane;
             const float *ws = fp.ws + x.g * fp.ws_group + (int64_t)(f0 / kScaleBlock) * fp.ws_row;
-            const float *xs = fp.xs + (int64_t)(x.row0 + lane) * fp.xs_row;
+            const float *xs = fp.xs + (int64_t)(x.row0 + first) * fp.xs_row;
             const bool on = f0 < p.features;  // the pair's second half may lie behind the last feature
-            float v[8], w = 0.0f;
-            auto fetch = [&](int kk) {
-                if (kk >= kb) return;
-                w = on ? __ldg(ws + kk * fp.ws_blk) : 0.0f;
+            float v[2][4], w[2];
+            auto fetch = [&](int kk, float (&v)[4], float &w) {
+                w = on && kk < kb ? __ldg(ws + kk * fp.ws_blk) : 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    v[i] = lane + 32 * i < x.rows ? __ldg(xs + (int64_t)(32 * i) * fp.xs_row + kk * fp.xs_blk) : 0.0f;
+                for (int i = 0; i < 4; ++i)
+                    v[i] = kk < kb && first + 32 * i < x.rows ? __ldg(xs + (int64_t)(32 * i) * fp.xs_row + kk * fp.xs_blk) : 0.0f;
             };
-            const int mine = (int)((it ^ (uint32_t)warp) & 1u);  // the first stage of this tile that is this warp's
-            fetch(mine);
-            for (int kk = 0; kk < kb; ++kk, ++it) {
-                ring.next(wide);
-                if ((kk & 1) == mine) {
-                    const int slot = ring.slot;
-                    float s8[8];
+            fetch(0, v[0], w[0]);
+            fetch(1, v[1], w[1]);
+            for (int k0 = 0; k0 < kb; k0 += 2)
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) s8[i] = v[i] * w;
-                    fetch(kk + 2);
-                    tc::wait(b_sempty + 8 * slot, ring.empty(slot), up);
-                    if (wide) tc::wait(b_sempty + 8 * slot + 8, ring.empty(slot + 1), up);
+                for (int d = 0; d < 2; ++d) {
+                    if (k0 + d >= kb) break;
+                    const int slot = h + 2 * (int)(it & 1u);
+                    float s4[4];
 #pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (wide || i < 4) scales[slot * kSlotCols + lane + 32 * i] = s8[i];
+                    for (int i = 0; i < 4; ++i) s4[i] = v[d][i] * w[d];
+                    fetch(k0 + d + 2, v[d], w[d]);
+                    tc::wait(b_sempty + 8 * slot, ((it >> 1) & 1u) ^ 1u, up);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) scales[slot * kHalfCols + lane + 32 * i] = s4[i];
                     __syncwarp();
                     if (lane == 0) tc::arrive(b_dfull + 8 * slot);
+                    ++it;
                 }
-                ring.used(wide);
-            }
         }
     } else {
-        const int quad = warp & 3, part = (warp - 4) >> 2;  // TMEM lanes 32 * quad.., chunks of 32 columns in turns
+        const int quad = warp & 3, part = (warp - 4) >> 2;  // TMEM lanes 32 * quad.., half
         const F8Sync y{b_dfull, b_dempty, b_sempty, up, tmem + ((uint32_t)(quad * 32) << 16), scales,
                        staging, &map_o32, &map_o8};
-        SlotRing ring;
+        uint32_t it = 0;
         int group = 0;
         for (int t = cluster; t < total; t += clusters) {
-            if (tc::bar_any_128(1 + part, *stop)) break;  // the four warps of a part meet at barriers: they stop together
+            if (tc::bar_any_128(1 + part, stop())) break;  // the four warps of a half meet at barriers: they stop together
             const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
-            const bool wide = x.n > kSlotCols;
-            const int f = x.f0 + (int)rank * kBF + quad * 32;
-            const int chunks = (x.n - 32 * part + 63) / 64;  // columns 32 * part + 64 * c that lie below n
-            if (chunks <= 0) promote_tile<CG, 0>(y, ring, p, x, f, kb, wide, part, lane);
-            else if (chunks == 1) promote_tile<CG, 1>(y, ring, p, x, f, kb, wide, part, lane);
-            else if (chunks == 2) promote_tile<CG, 2>(y, ring, p, x, f, kb, wide, part, lane);
-            else if (chunks == 3) promote_tile<CG, 3>(y, ring, p, x, f, kb, wide, part, lane);
-            else promote_tile<CG, 4>(y, ring, p, x, f, kb, wide, part, lane);
+            const Half half = tile_half<CG>(x.n, part);
+            const int f = x.f0 + (int)rank * kBF + quad * 32, chunks = (half.n + 31) / 32;
+            if (chunks == 0) continue;
+            if (chunks == 1) promote_half<CG, 1>(y, it, p, x, half, f, kb, part, lane);
+            else if (chunks == 2) promote_half<CG, 2>(y, it, p, x, half, f, kb, part, lane);
+            else if (chunks == 3) promote_half<CG, 3>(y, it, p, x, half, f, kb, part, lane);
+            else promote_half<CG, 4>(y, it, p, x, half, f, kb, part, lane);
         }
         tc::bulk_wait_read();  // the copies read this CTA's shared memory
     }
-    if (lane == 0 && *stop) atomicOr(&g_product_err, 1u);
+    if (stop() && lane == 0) atomicOr(&g_product_err, 1u);
     __syncwarp();
     tc::fence_before_sync();
     if constexpr (CG == 1) __syncthreads();
