@@ -27,7 +27,8 @@ namespace {
 struct QuantParams {
     const void *x;
     int64_t ldx, x_stride;
-    int matrices, cols, vec;  // vec: rows start at multiples of 16 bytes (x) and of 16 (2) or 8 (1) bytes (q); 0 otherwise
+    int matrices, cols, steps;
+    bool vec;  // rows start at multiples of 16 bytes (x) and 8 bytes (q)
     int64_t rows;
     uint8_t *q;
     int64_t ldq, q_stride;
@@ -35,28 +36,34 @@ struct QuantParams {
     int64_t s_row, s_blk, s_stride;
 };
 
-// Sixteen consecutive values of a row as they lie in memory; a 128-block is eight lanes of them.  Values stay in their
-// own type until they are scaled, which halves the registers of 16-bit inputs and doubles the warps that hide the loads.
+// A lane's 32 values of a 128-block, as pieces of 16 bytes: four lanes hold a block, piece j of lane l starts at column
+// 128 / kPieces * j + kPer * l, so that the lanes of one load are neighbours in memory.  Values stay in their own type until
+// they are scaled, which halves the registers of 16-bit inputs.  (With eight lanes to a block the work per block, a
+// division, a reciprocal, shuffles and addresses, took as many instructions as the values.)
 template <class T>
-struct Sixteen {
-    static constexpr int kWords = 16 * sizeof(T) / 4;
+struct Values {
+    static constexpr int kWords = 32 * sizeof(T) / 4, kPer = 16 / sizeof(T), kPieces = 32 / kPer;
     uint32_t w[kWords];
 
-    __device__ __forceinline__ void load(const T *row, int c, int cols, bool vec) {
-        if (vec && c + 16 <= cols) {
+    static __device__ __forceinline__ int column(int b, int l, int j) { return b * kScaleBlock + kScaleBlock / kPieces * j + kPer * l; }
+
+    // Block b's values of lane l of a row of `cols` values; zeros behind its end.
+    __device__ __forceinline__ void load(const T *row, int b, int l, int cols, bool vec) {
 #pragma unroll
-            for (int i = 0; i < kWords / 4; ++i)
-                *reinterpret_cast<uint4 *>(w + 4 * i) = __ldg(reinterpret_cast<const uint4 *>(row + c) + i);
-            return;
-        }
-        if constexpr (sizeof(T) == 4) {
+        for (int j = 0; j < kPieces; ++j) {
+            const int c = column(b, l, j);
+            if (vec && c + kPer <= cols) {
+                *reinterpret_cast<uint4 *>(w + 4 * j) = __ldg(reinterpret_cast<const uint4 *>(row + c));
+                continue;
+            }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = c + i < cols ? __ldg(reinterpret_cast<const uint32_t *>(row) + c + i) : 0u;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const unsigned short *h = reinterpret_cast<const unsigned short *>(row) + c + 2 * i;
-                w[i] = (c + 2 * i < cols ? __ldg(h) : 0u) | (c + 2 * i + 1 < cols ? (uint32_t)__ldg(h + 1) << 16 : 0u);
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (sizeof(T) == 4) {
+                    w[4 * j + i] = c + i < cols ? __ldg(reinterpret_cast<const uint32_t *>(row) + c + i) : 0u;
+                } else {
+                    const unsigned short *h = reinterpret_cast<const unsigned short *>(row) + c + 2 * i;
+                    w[4 * j + i] = (c + 2 * i < cols ? __ldg(h) : 0u) | (c + 2 * i + 1 < cols ? (uint32_t)__ldg(h + 1) << 16 : 0u);
+                }
             }
         }
     }
@@ -68,7 +75,7 @@ struct Sixteen {
             else return f16_bits_to_f32(h);
         }
     }
-    // Bits of |v| order like |v|; those of inf and NaN are at least kInf.  top: the largest of the sixteen (16-bit types: of the
+    // Bits of |v| order like |v|; those of inf and NaN are at least kInf.  top: the largest of the 32 (16-bit types: of the
     // even and of the odd ones); finite: of the finite ones.
     static constexpr uint32_t kInf = sizeof(T) == 4 ? 0x7f800000u : std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
     __device__ __forceinline__ uint32_t top() const {
@@ -83,7 +90,7 @@ struct Sixteen {
     __device__ __forceinline__ uint32_t finite() const {
         uint32_t m = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < 32; ++i) {
             const uint32_t a = sizeof(T) == 4 ? w[i] & 0x7fffffffu : (w[i >> 1] >> 16 * (i & 1)) & 0x7fffu;
             if (a < kInf) m = max(m, a);
         }
@@ -98,31 +105,50 @@ struct Sixteen {
     }
 };
 
-__device__ __forceinline__ float block_scale(float amax) { return fmaxf(__fdiv_rn(amax, 448.0f), 0x1p-126f); }
+// x / d as an IEEE division rounds it, Markstein's way (1990): with y = 1 / d correctly rounded, q = x y and r = x - q d
+// (exact), q + r y rounds to x / d.  Three operations instead of ten, which would bound the kernel; not for quotients or
+// residuals that may be subnormal.
+__device__ __forceinline__ float quotient(float x, float d, float y) {
+    const float q = __fmul_rn(x, y);
+    return __fmaf_rn(__fmaf_rn(-q, d, x), y, q);
+}
+constexpr float kPlain = 0x1p-90f;  // smallest block maximum for it
 
-// Codes of sixteen values.  plain: every value is finite and scale >= 2^-100.  Then the quotient is Markstein's (1990):
-// with y = 1 / scale correctly rounded, q = x y and r = x - q scale (exact), q + r y rounds to x / scale, three
-// operations instead of a division's ten (with divisions the arithmetic, not memory, would bound the kernel).  Below
-// 2^-100 the residual may be subnormal and lose bits, so those blocks divide.
+// The same for two values at once (packed fp32 operations); yy, dd: y and -d in both halves.
+__device__ __forceinline__ uint64_t twice(float v) { return (uint64_t)__float_as_uint(v) << 32 | __float_as_uint(v); }
+__device__ __forceinline__ float2 quotients(float a, float b, uint64_t dd, uint64_t yy) {
+    uint64_t x, q, r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(q) : "l"(x), "l"(yy));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(q), "l"(dd), "l"(x));
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(q) : "l"(r), "l"(yy), "l"(q));
+    float2 t;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(t.x), "=f"(t.y) : "l"(q));
+    return t;
+}
+
+__device__ __forceinline__ float block_scale(float amax) {
+    if (amax >= kPlain) return quotient(amax, 448.0f, 1.0f / 448.0f);
+    return fmaxf(__fdiv_rn(amax, 448.0f), 0x1p-126f);
+}
+
+// Codes of a lane's values.  plain: every value is finite and the block's maximum at least kPlain; a value far below
+// it may have a subnormal residual, but then rounds to the code zero either way.
 template <class T>
-__device__ __forceinline__ void store16(uint8_t *row, int c, int cols, int vec, const Sixteen<T> &v, float scale, bool plain) {
-    uint32_t w[4];
+__device__ __forceinline__ void store_codes(uint8_t *row, int b, int l, int cols, bool vec, const Values<T> &v, float scale, bool plain) {
+    uint32_t w[8];
     if (plain) {
-        const float y = __frcp_rn(scale);
+        const uint64_t yy = twice(__frcp_rn(scale)), dd = twice(-scale);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float t[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float x = v.value(4 * i + j), q = __fmul_rn(x, y);
-                t[j] = __fmaf_rn(__fmaf_rn(-q, scale, x), y, q);
-            }
-            w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(t[0], t[1]), __NV_SATFINITE, __NV_E4M3) |
-                   (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(t[2], t[3]), __NV_SATFINITE, __NV_E4M3) << 16;
+        for (int i = 0; i < 8; ++i) {
+            const float2 a = quotients(v.value(4 * i), v.value(4 * i + 1), dd, yy);
+            const float2 b = quotients(v.value(4 * i + 2), v.value(4 * i + 3), dd, yy);
+            w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
+                   (uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16;
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
             w[i] = 0;
             for (int j = 0; j < 4; ++j) {  // inf / scale would saturate to 448: make it the NaN that it stands for
                 const float x = v.value(4 * i + j), t = fabsf(x) < INFINITY ? __fdiv_rn(x, scale) : __uint_as_float(0x7fc00000u);
@@ -130,55 +156,54 @@ __device__ __forceinline__ void store16(uint8_t *row, int c, int cols, int vec, 
             }
         }
     }
-    if (vec && c + 16 <= cols) {
-        if (vec == 2) {
-            *reinterpret_cast<uint4 *>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-            *reinterpret_cast<uint2 *>(row + c) = make_uint2(w[0], w[1]);
-            *reinterpret_cast<uint2 *>(row + c + 8) = make_uint2(w[2], w[3]);
-        }
-        return;
-    }
+    constexpr int kPer = Values<T>::kPer;
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (c + i < cols) row[c + i] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+    for (int j = 0; j < Values<T>::kPieces; ++j) {
+        const int c = Values<T>::column(b, l, j);
+        if (vec && c + kPer <= cols) {
+            if constexpr (kPer == 8) *reinterpret_cast<uint2 *>(row + c) = make_uint2(w[2 * j], w[2 * j + 1]);
+            else *reinterpret_cast<uint32_t *>(row + c) = w[j];
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (c + i < cols) row[c + i] = (uint8_t)(w[(kPer * j + i) >> 2] >> (8 * (i & 3)));
+    }
 }
 
-// 1 x 128 blocks: eight lanes per block, a warp takes 4 * kSteps blocks of a row, all loaded before the first is used.
-constexpr int kSteps = 2;
+// 1 x 128 blocks: four lanes per block, a warp takes p.steps times eight blocks of a row, the next ones loaded before
+// these are used.
 template <class T>
 __global__ void __launch_bounds__(256) k_quant_rows(const QuantParams p) {
-    const int l = threadIdx.x & 7, sub = (threadIdx.x >> 3) & 3;
+    const int l = threadIdx.x & 3, sub = (threadIdx.x >> 2) & 7;
     const int nb = (p.cols + kScaleBlock - 1) / kScaleBlock;
-    const uint32_t segs = (nb + 4 * kSteps - 1) / (4 * kSteps);
+    const uint32_t segs = (nb + 8 * p.steps - 1) / (8 * p.steps);
     const int64_t items = (int64_t)p.matrices * p.rows * segs, step = ((int64_t)gridDim.x * blockDim.x) >> 5;
     for (int64_t i = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 5; i < items; i += step) {
         const int64_t mr = items < (1ll << 32) ? (uint32_t)i / segs : i / segs;
-        const int b0 = (int)(i - mr * segs) * 4 * kSteps + sub;
+        const int b0 = (int)(i - mr * segs) * 8 * p.steps + sub, b1 = min(nb, b0 - sub + 8 * p.steps);
         int64_t r = mr, mat = 0;
         if (p.matrices > 1) mat = mr / p.rows, r = mr - mat * p.rows;
         const T *x = static_cast<const T *>(p.x) + mat * p.x_stride + r * p.ldx;
         uint8_t *q = p.q + mat * p.q_stride + r * p.ldq;
         float *s = p.scales + mat * p.s_stride + r * p.s_row;
-        Sixteen<T> v[kSteps];
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) v[j].load(x, (b0 + 4 * j) * kScaleBlock + l * 16, p.cols, p.vec);
-#pragma unroll
-        for (int j = 0; j < kSteps; ++j) {
-            const int b = b0 + 4 * j;
-            uint32_t m = v[j].top();
-#pragma unroll
-            for (int o = 4; o >= 1; o >>= 1) m = Sixteen<T>::larger(m, __shfl_xor_sync(kFull, m, o));
-            m = Sixteen<T>::one(m);
-            const bool fine = m < Sixteen<T>::kInf;
+        Values<T> v, next;
+        next.load(x, b0, l, p.cols, p.vec);
+        for (int b = b0; b - sub < b1; b += 8) {  // whole warps: lanes behind the last block hold zeros
+            v = next;
+            if (b - sub + 8 < b1) next.load(x, b + 8, l, p.cols, p.vec);
+            uint32_t m = v.top();
+            m = Values<T>::larger(m, __shfl_xor_sync(kFull, m, 2));
+            m = Values<T>::one(Values<T>::larger(m, __shfl_xor_sync(kFull, m, 1)));
+            const bool fine = m < Values<T>::kInf;
             if (__any_sync(kFull, !fine)) {
-                m = v[j].finite();
-#pragma unroll
-                for (int o = 4; o >= 1; o >>= 1) m = max(m, __shfl_xor_sync(kFull, m, o));
+                m = v.finite();
+                m = max(m, __shfl_xor_sync(kFull, m, 2));
+                m = max(m, __shfl_xor_sync(kFull, m, 1));
             }
-            if (b >= nb) continue;
-            const float scale = block_scale(Sixteen<T>::as_float(m));
-            store16(q, b * kScaleBlock + l * 16, p.cols, p.vec, v[j], scale, fine && scale >= 0x1p-100f);
+            if (b >= b1) continue;
+            const float amax = Values<T>::as_float(m), scale = block_scale(amax);
+            store_codes(q, b, l, p.cols, p.vec, v, scale, fine && amax >= kPlain);
             if (l == 0) s[b * p.s_blk] = scale;
         }
     }
@@ -193,18 +218,18 @@ __global__ void __launch_bounds__(256) k_quant_blocks(const QuantParams p) {
     const int64_t blocks = (int64_t)p.matrices * nbr * nb;
     for (int64_t i = blockIdx.x; i < blocks; i += gridDim.x) {
         const int64_t mbr = i / nb, mat = mbr / nbr, br = mbr - mat * nbr;
-        const int b = (int)(i - mbr * nb), c = b * kScaleBlock + (threadIdx.x & 7) * 16;
-        const int64_t r0 = br * kScaleBlock + (threadIdx.x >> 3);
-        Sixteen<T> v[4];
+        const int b = (int)(i - mbr * nb), l = threadIdx.x & 3;
+        const int64_t r0 = br * kScaleBlock + (threadIdx.x >> 2);
+        Values<T> v[2];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = r0 + 32 * j;
-            v[j].load(static_cast<const T *>(p.x) + mat * p.x_stride + r * p.ldx, c, r < p.rows ? p.cols : 0, p.vec);
+        for (int j = 0; j < 2; ++j) {
+            const int64_t r = r0 + 64 * j;
+            v[j].load(static_cast<const T *>(p.x) + mat * p.x_stride + r * p.ldx, b, l, r < p.rows ? p.cols : 0, p.vec);
         }
         uint32_t m = 0, f = 0;  // over all values, over the finite ones
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            m = max(m, Sixteen<T>::one(v[j].top()));
+        for (int j = 0; j < 2; ++j) {
+            m = max(m, Values<T>::one(v[j].top()));
             f = max(f, v[j].finite());
         }
         m = __reduce_max_sync(kFull, m);
@@ -214,22 +239,25 @@ __global__ void __launch_bounds__(256) k_quant_blocks(const QuantParams p) {
         __syncthreads();
 #pragma unroll
         for (int w = 0; w < 8; ++w) m = max(m, part[0][w]), f = max(f, part[1][w]);
-        const float scale = block_scale(Sixteen<T>::as_float(f));
-        const bool plain = m < Sixteen<T>::kInf && scale >= 0x1p-100f;
+        const float amax = Values<T>::as_float(f), scale = block_scale(amax);
+        const bool plain = m < Values<T>::kInf && amax >= kPlain;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int64_t r = r0 + 32 * j;
-            if (r < p.rows) store16(p.q + mat * p.q_stride + r * p.ldq, c, p.cols, p.vec, v[j], scale, plain);
+        for (int j = 0; j < 2; ++j) {
+            const int64_t r = r0 + 64 * j;
+            if (r < p.rows) store_codes(p.q + mat * p.q_stride + r * p.ldq, b, l, p.cols, p.vec, v[j], scale, plain);
         }
         if (threadIdx.x == 0) p.scales[mat * p.s_stride + br * p.s_row + b * p.s_blk] = scale;
     }
 }
 
 template <class T>
-void launch_quant(const QuantParams &p, int block_rows, int sms, cudaStream_t s) {
-    const int64_t nb = (p.cols + kScaleBlock - 1) / kScaleBlock;
+void launch_quant(QuantParams p, int block_rows, int sms, cudaStream_t s) {
+    const int64_t nb = (p.cols + kScaleBlock - 1) / kScaleBlock, rows = (int64_t)p.matrices * p.rows;
     if (block_rows == 1) {
-        const int64_t items = (int64_t)p.matrices * p.rows * ((nb + 4 * kSteps - 1) / (4 * kSteps));
+        // eight blocks a warp where that leaves warps idle, otherwise up to 32
+        p.steps = 1;
+        while (p.steps < 4 && rows * ((nb + 16 * p.steps - 1) / (16 * p.steps)) >= 64 * sms) p.steps *= 2;
+        const int64_t items = rows * ((nb + 8 * p.steps - 1) / (8 * p.steps));
         k_quant_rows<T><<<(unsigned)std::min<int64_t>((items + 7) / 8, 64 * sms), 256, 0, s>>>(p);
     } else {
         const int64_t blocks = (int64_t)p.matrices * ((p.rows + kScaleBlock - 1) / kScaleBlock) * nb;
@@ -271,9 +299,8 @@ extern "C" umsx_status umsx_fp8_quantize(const void *x, int64_t ldx, int64_t x_s
     p.matrices = matrices, p.rows = rows, p.cols = cols;
     p.q = static_cast<uint8_t *>(q), p.ldq = ldq, p.q_stride = q_stride;
     p.scales = scales, p.s_row = s_row, p.s_blk = s_blk, p.s_stride = s_stride;
-    const uint64_t at = reinterpret_cast<uintptr_t>(q) | (uint64_t)ldq | (uint64_t)q_stride;  // multiples of a power of two?
-    if (reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * size % 16 == 0 && x_stride * size % 16 == 0)
-        p.vec = at % 16 == 0 ? 2 : at % 8 == 0 ? 1 : 0;
+    p.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * size % 16 == 0 && x_stride * size % 16 == 0 &&
+            reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0 && q_stride % 8 == 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (x_dtype == UMSX_DTYPE_F32) launch_quant<float>(p, block_rows, sms, s);
     else if (x_dtype == UMSX_DTYPE_BF16) launch_quant<__nv_bfloat16>(p, block_rows, sms, s);
