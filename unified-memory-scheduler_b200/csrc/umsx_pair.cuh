@@ -182,29 +182,6 @@ __device__ __forceinline__ void arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// ---- stores through shared memory -----------------------------------------------------------------
-//
-// A box of a tensor map from shared memory; asynchronous, in groups of the issuing thread.  (One untiled bulk copy per
-// row instead costs about 30 cycles each to issue: 4 K a tile.)
-__device__ __forceinline__ void tma_store_2d(const void *tmap, int x, int y, uint32_t src) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(tmap), "r"(x), "r"(y), "r"(src)
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-// This thread's groups have read their sources.
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-
-// A barrier among 128 threads, and one that also tells whether any of them says so.
-__device__ __forceinline__ void bar_128(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ bool bar_any_128(int id, bool v) {
-    uint32_t r;
-    asm volatile("{ .reg .pred p, q; setp.ne.u32 q, %1, 0; bar.red.or.pred p, %2, 128, q; selp.u32 %0, 1, 0, p; }"
-                 : "=r"(r)
-                 : "r"((uint32_t)v), "r"(id)
-                 : "memory");
-    return r != 0;
-}
-
 // True in one lane of a converged warp.  The copies and MMAs are issued under it and not under a test of the
 // lane: their operands then stay in uniform registers (four MMAs took 490 cycles to issue under `lane == 0`).
 __device__ __forceinline__ bool elect_one() {

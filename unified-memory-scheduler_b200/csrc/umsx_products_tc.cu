@@ -49,7 +49,7 @@ constexpr int kSegment = 8;  // stages that share an accumulator where the outpu
 constexpr int kStageRow = 80;  // bytes of a staged output row: 64 of data; 80 spreads eight rows over all banks
 
 struct TcParams {
-    int groups, features, contraction, out_rows, out_dtype, fmt, vec, bulk, segment;
+    int groups, features, contraction, out_rows, out_dtype, fmt, vec, segment;
     int64_t rows;
     const int32_t *offsets;
     void *out;
@@ -157,10 +157,9 @@ __device__ __forceinline__ uint32_t pack16(uint32_t lo, uint32_t hi) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
-// 16 rows of 32 16-bit features from v (fragment order) to shared memory, row by row: rows of kStageRow bytes, or rows of 128
-// swizzled bytes of which the warp's features are chunks `chunk` to chunk + 3 (`to` at a multiple of eight rows).
-template <bool BF16, bool SWIZZLED>
-__device__ __forceinline__ void stage16(uint8_t *to, int chunk, int lane, const uint32_t (&v)[16]) {
+// 16 rows of 32 16-bit features from v (fragment order) to shared memory, row by row.
+template <bool BF16>
+__device__ __forceinline__ void stage16(uint8_t *to, int lane, const uint32_t (&v)[16]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         uint32_t m[4];
@@ -169,9 +168,7 @@ __device__ __forceinline__ void stage16(uint8_t *to, int chunk, int lane, const 
             const int e = 8 * (q >> 1) + 4 * i + 2 * (q & 1);
             m[q] = pack16<BF16>(v[e], v[e + 1]);
         }
-        const int row = 8 * i + (lane & 7);
-        tc::stmatrix_trans4(SWIZZLED ? to + row * 128 + ((chunk + (lane >> 3)) ^ (lane & 7)) * 16 : to + row * kStageRow + (lane >> 3) * 16,
-                            m[0], m[1], m[2], m[3]);
+        tc::stmatrix_trans4(to + (8 * i + (lane & 7)) * kStageRow + (lane >> 3) * 16, m[0], m[1], m[2], m[3]);
     }
 }
 
@@ -192,8 +189,8 @@ __device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, in
         return;
     }
     __syncwarp();  // the previous rows have been read out of the staging
-    if (o.dtype == UMSX_DTYPE_BF16) stage16<true, false>(stage, 0, lane, v);
-    else stage16<false, false>(stage, 0, lane, v);
+    if (o.dtype == UMSX_DTYPE_BF16) stage16<true>(stage, lane, v);
+    else stage16<false>(stage, lane, v);
     __syncwarp();
     uint16_t *p = static_cast<uint16_t *>(o.out) + o.at;
 #pragma unroll
@@ -469,34 +466,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
 // out[r][f] = sum_b xs[r][b] ws[f / 128][b] D_b[r][f] with D_b the product over block b of the contraction.  A stage
 // is one block: its MMAs start a fresh accumulator, and the epilogue warps add it, times the scales, to fp32
 // sums in registers.  The scale is one per column of the accumulator (a row of x) and CTA (128 features: one
-// block of w), so warps 2-3 put xs * ws of a stage's rows into shared memory and a thread multiplies
+// block of w), so warp 2 puts xs * ws of a stage's rows into shared memory and a thread multiplies
 // pairs of columns with one packed FMA.
 //
-// A tile's rows are two halves, each with MMAs, accumulators (two of 128 columns), a scale warp and four promotion
+// A tile's rows are two halves, each with accumulators (two of 128 columns), an issuing warp (1 and 3) and four promotion
 // warps of its own, so that one half's waits and tile changes run under the other's arithmetic; with both halves in
-// one accumulator the eight warps waited together, 250 of a block's 850 cycles at 128 rows.  The promotion bounds wide
+// one accumulator the eight warps waited together, 250 of a block's 850 cycles at 128 rows, and one warp that issues for
+// both halves takes 900 cycles a block for its waits, eight MMAs and three commits.  The promotion bounds wide
 // tiles: the accumulator leaves TMEM at about 230 bytes a cycle, 256 columns in 570 cycles, their MMAs take 512.  What it
 // needs: the number of column chunks a compile-time constant (a test per chunk costs 350 cycles a block) and, at 128
 // columns, 16 columns a load (with 32 the sums spill).
 //
-// 16-bit outputs leave through a staging of the whole tile and TMA stores of 32 or 8 rows, which drain under the next
-// tile's blocks; the last rows of a group, fewer than eight, are stored by the warps, since a box would overwrite the next
-// group's.  Stored by the promotion warps alone, all SMs at once, tiles took 5 K of their 23 K cycles (16 blocks) for it.
+// Single CTAs, not pairs: the promotion, not the operands' traffic, bounds the tiles, and a pair's CTAs wait for one
+// another's eight warps at every block (4096 x 4 rows, 128 experts of 5760 x 2880: 553 us in pairs, 485 alone).  The warps
+// store their sums themselves; a staging for TMA stores takes a stage and two barriers a tile and was slower (560 us).
 
 constexpr int kThreadsF8 = 384, kHalfCols = 128, kSlots = 4, kHalfWarps = 4;
-
-// A staged tile: two halves of 64 features, a row of a half is 128 bytes with the swizzle of the tensor map (16-byte
-// chunk c of row r at c ^ (r & 7)).
-constexpr int kHalfTile = kRowsMax * 128;
 
 // Half h of a tile: columns [at, at + n) of its n, and its accumulators: slot h + 2 * (block & 1).
 struct Half {
     int at, n;
 };
-template <int CG>
 __device__ __forceinline__ Half tile_half(int n, int h) {
-    constexpr int kStep = 16 * CG;
-    const int first = (n / 2 + kStep - 1) / kStep * kStep;
+    const int first = (n / 2 + 15) / 16 * 16;
     return h ? Half{first, n - first} : Half{0, first};
 }
 
@@ -506,16 +498,12 @@ struct F8Params {
     int64_t xs_row, xs_blk, ws_row, ws_blk, ws_group;
 };
 
-template <int CG>
 struct ShapeF8 {
     static constexpr int kBC8 = 128;  // contraction per stage, in bytes too
-    static constexpr int kBytesF = kBF * kBC8, kBytesR = kRowsMax / CG * kBC8, kBytesHalf = kBytesR / 2;
+    static constexpr int kBytesF = kBF * kBC8, kBytesR = kRowsMax * kBC8, kBytesHalf = kBytesR / 2;
     static constexpr int kStages = 4;
     static constexpr size_t kOperands = (size_t)kStages * (kBytesF + kBytesR);
-    // a pair's half stages leave room for a tile; a single CTA's (outputs of at most 128 features) do not
-    static constexpr bool kBulk = CG == 2;
-    static constexpr size_t kStaging = kBulk ? 2 * kHalfTile : kEpilogueWarps * 16 * kStageRow;
-    static constexpr size_t kSmem = 1024 + kOperands + kSlots * kHalfCols * sizeof(float) + kStaging;
+    static constexpr size_t kSmem = 1024 + kOperands + kSlots * kHalfCols * sizeof(float) + kEpilogueWarps * 16 * kStageRow;
 };
 
 __device__ __forceinline__ uint64_t pack2(uint32_t lo, uint32_t hi) { return (uint64_t)lo | ((uint64_t)hi << 32); }
@@ -528,12 +516,11 @@ struct F8Sync {
     uint32_t d_full, d_empty, sc_empty, gave_up;  // shared-memory addresses
     uint32_t lanes;                               // TMEM address of the warp's lanes
     const float *scales;
-    uint8_t *staging;  // 1024-byte aligned
-    const CUtensorMap *out32, *out8;  // boxes of 64 features x 32 and x 8 rows
+    uint8_t *stage;  // the warp's
 };
 
 // Half `part` of a tile by one promotion warp: NCH chunks of 32 columns.  `it`: blocks of this half so far.
-template <int CG, int NCH>
+template <int NCH>
 __device__ __forceinline__ void promote_half(const F8Sync &y, uint32_t &it, const TcParams &p, const Tile &x, const Half &half,
                                              int f, int kb, int part, int lane) {
     uint64_t acc[2 * NCH][8];  // 16 columns, pairs of columns in fragment order: 0.0f
@@ -570,131 +557,62 @@ __device__ __forceinline__ void promote_half(const F8Sync &y, uint32_t &it, cons
         tc::fence_before_sync();
         __syncwarp();
         if (lane < 2)  // one lane per barrier
-            tc::arrive_at(lane ? y.sc_empty + 8 * slot : CG == 1 ? y.d_empty + 8 * slot : tc::leader_addr(y.d_empty + 8 * slot));
+            tc::arrive((lane ? y.sc_empty : y.d_empty) + 8 * slot);
     }
-    auto sums = [&](int h, uint32_t (&v)[16]) {
+    // a half ends at a multiple of 16, its last chunk may not
+    const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, min(x.rows, half.at + half.n), p.vec != 0};
+#pragma unroll
+    for (int h = 0; h < 2 * NCH; ++h) {
+        uint32_t v[16];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             v[2 * i] = (uint32_t)acc[h][i];
             v[2 * i + 1] = (uint32_t)(acc[h][i] >> 32);
         }
-    };
-    const int quad = (threadIdx.x >> 5) & 3;
-    if (ShapeF8<CG>::kBulk && p.bulk) {
-        tc::bulk_wait_read();
-        tc::bar_128(1 + part);  // all four warps' copies of the last tile have read the staging
-        uint8_t *to = y.staging + (quad >> 1) * kHalfTile;
-        const int chunk = (quad & 1) * 4;  // of this warp's 32 features in a row of the half
-        if (p.out_dtype == UMSX_DTYPE_BF16) {
-#pragma unroll
-            for (int h = 0; h < 2 * NCH; ++h) {
-                uint32_t v[16];
-                sums(h, v);
-                stage16<true, true>(to + (half.at + 16 * h) * 128, chunk, lane, v);
-            }
-        } else {
-#pragma unroll
-            for (int h = 0; h < 2 * NCH; ++h) {
-                uint32_t v[16];
-                sums(h, v);
-                stage16<false, true>(to + (half.at + 16 * h) * 128, chunk, lane, v);
-            }
-        }
-        tc::fence_proxy_async();
-        tc::bar_128(1 + part);
-        const int even = x.rows & ~7, left = x.rows - even;  // rows in boxes, rows behind them
-        if (quad == 0) {
-            if (tc::elect_one()) {
-                const int f0 = f;  // of the tile's 128
-#pragma unroll
-                for (int c = 0; c < NCH; ++c)
-                    for (int s = 0; s < 2 && f0 + 64 * s < p.features; ++s) {
-                        const int r = half.at + 32 * c;
-                        const uint32_t src = smem_u32(y.staging) + s * kHalfTile;
-                        if (r + 32 <= even) tc::tma_store_2d(y.out32, f0 + 64 * s, x.row0 + r, src + r * 128);
-                        else
-                            for (int q = r; q < even && q < r + 32; q += 8)
-                                tc::tma_store_2d(y.out8, f0 + 64 * s, x.row0 + q, src + q * 128);
-                    }
-                tc::bulk_commit();
-            }
-            __syncwarp();
-        }
-        if (left && even >= half.at && even < half.at + half.n) {  // in this half: four lanes to a row
-            const int row = even + (lane >> 2), fl = 8 * (lane & 3);
-            if (row < x.rows && f + fl < p.features) {
-                const uint4 w = *reinterpret_cast<const uint4 *>(to + row * 128 + ((chunk + (lane & 3)) ^ (row & 7)) * 16);
-                uint16_t *d = static_cast<uint16_t *>(p.out) + (int64_t)(x.row0 + row) * p.ldo + f + fl;
-                if (f + fl + 8 <= p.features) {
-                    *reinterpret_cast<uint4 *>(d) = w;
-                } else {
-                    const uint16_t *e = reinterpret_cast<const uint16_t *>(&w);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (f + fl + j < p.features) d[j] = e[j];
-                }
-            }
-        }
-        return;
-    }
-    // a half ends at a multiple of 16 (of 32 in a pair), its last chunk may not
-    const OutTile o{p.out, (int64_t)x.row0 * p.ldo + f, p.ldo, p.out_dtype, p.features - f, min(x.rows, half.at + half.n), p.vec != 0};
-    uint8_t *own = y.staging + (quad + 4 * part) * 16 * kStageRow;
-#pragma unroll
-    for (int h = 0; h < 2 * NCH; ++h) {
-        uint32_t v[16];
-        sums(h, v);
-        store_chunk(o, own, lane, half.at + 16 * h, v);
+        store_chunk(o, y.stage, lane, half.at + 16 * h, v);
     }
 }
 
-template <int CG>
 __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_constant__ CUtensorMap map_f,
-                                                              const __grid_constant__ CUtensorMap map_r,
-                                                              const __grid_constant__ CUtensorMap map_o32,
-                                                              const __grid_constant__ CUtensorMap map_o8, const F8Params fp) {
-    using S = ShapeF8<CG>;
+                                                              const __grid_constant__ CUtensorMap map_r, const F8Params fp) {
+    using S = ShapeF8;
     const TcParams &p = fp.t;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     uint8_t *sF = smem, *sR = smem + S::kStages * S::kBytesF;  // a stage of R: the rows of half 0, from its middle those of half 1
-    uint8_t *staging = smem + S::kOperands;  // 1024-byte aligned
-    float *scales = reinterpret_cast<float *>(staging + S::kStaging);  // [slot][column]: xs * ws
-    // d_full: a slot's MMAs and its scales; d_empty: read by both CTAs' warps; sc_empty: by this one's
+    float *scales = reinterpret_cast<float *>(smem + S::kOperands);  // [slot][column]: xs * ws
+    uint8_t *staging = smem + S::kOperands + kSlots * kHalfCols * sizeof(float);
+    // d_full: a slot's MMAs and its scales; d_empty, sc_empty: both read by the four warps of its half
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[kSlots], d_empty[kSlots], sc_empty[kSlots], last;
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up;
     __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
 
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-    const uint32_t rank = CG == 1 ? 0 : tc::cluster_rank();
-    const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
-
     for (int g = tid; g < p.groups; g += kThreadsF8) group_bounds(p.offsets, g, p.rows, bounds[2 * g], bounds[2 * g + 1]);
     if (tid == 0) {
         gave_up = 0;
-        mbar_init(&last, 1);
+        mbar_init(&last, 2);
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(&full[s], 1);
-            mbar_init(&empty[s], 1);
+            mbar_init(&empty[s], 2);
         }
         for (int s = 0; s < kSlots; ++s) {
             mbar_init(&d_full[s], 2);
-            mbar_init(&d_empty[s], CG * kHalfWarps);
+            mbar_init(&d_empty[s], kHalfWarps);
             mbar_init(&sc_empty[s], kHalfWarps);
         }
     }
-    if (warp == 1) tc::pair_tmem_alloc<CG>(&tmem_s, kTmemCols);
+    if (warp == 1) tc::pair_tmem_alloc<1>(&tmem_s, kTmemCols);
     __syncthreads();
-    const int f_tiles = (p.features + kBF * CG - 1) / (kBF * CG);
-    if (warp == 0) tile_prefix<CG, kForward>(bounds, prefix, p.groups, f_tiles, p.out_rows, lane);
+    const int f_tiles = (p.features + kBF - 1) / kBF;
+    if (warp == 0) tile_prefix<1, kForward>(bounds, prefix, p.groups, f_tiles, p.out_rows, lane);
     tc::fence_before_sync();
-    if constexpr (CG == 1) __syncthreads();
-    else tc::cluster_sync_all();
+    __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = __shfl_sync(kFull, tmem_s, 0);
     const int total = __shfl_sync(kFull, prefix[p.groups], 0), kb = (p.contraction + S::kBC8 - 1) / S::kBC8;
-    const Tiles<CG, kForward> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
+    const Tiles<1, kForward> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
     const uint32_t up = smem_u32(&gave_up), aF = smem_u32(sF), aR = smem_u32(sR);
     const uint32_t b_full = smem_u32(full), b_empty = smem_u32(empty), b_dfull = smem_u32(d_full), b_dempty = smem_u32(d_empty),
@@ -705,28 +623,25 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
         tc::Ring<S::kStages> r;
         uint32_t used = 0;  // stages in use
         int group = 0;
-        for (int t = cluster; t < total && !stop(); t += clusters) {
+        for (int t = blockIdx.x; t < total && !stop(); t += gridDim.x) {
             const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
-            const Half h0 = tile_half<CG>(x.n, 0), h1 = tile_half<CG>(x.n, 1);
-            const int rows0 = h0.n / CG, rows1 = h1.n / CG;  // this CTA's rows of each half
-            const int boxes0 = (rows0 + kRowBox - 1) / kRowBox, boxes1 = (rows1 + kRowBox - 1) / kRowBox;
+            const Half h0 = tile_half(x.n, 0), h1 = tile_half(x.n, 1);
+            const int boxes0 = (h0.n + kRowBox - 1) / kRowBox, boxes1 = (h1.n + kRowBox - 1) / kRowBox;
             const uint32_t bytes = S::kBytesF + (boxes0 + boxes1) * kRowBox * S::kBC8;
-            const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * rows0, r1 = x.row0 + h1.at + (int)rank * rows1;
             for (int kk = 0; kk < kb; ++kk, r.next()) {
                 tc::wait(b_empty + 8 * r.s, r.phase ^ 1u, up);
                 used |= 1u << r.s;
                 if (tc::elect_one()) {
-                    uint32_t bar = b_full + 8 * r.s;
-                    if (rank == 0) tc::expect_tx(bar, CG * bytes);
-                    if (CG > 1) bar = tc::leader_addr(bar);
+                    const uint32_t bar = b_full + 8 * r.s;
+                    tc::expect_tx(bar, bytes);
                     const int c = kk * S::kBC8;
                     const uint32_t dR = aR + r.s * S::kBytesR;
-                    tc::pair_tma_3d<CG>(aF + r.s * S::kBytesF, &map_f, c, f0, x.g, bar);
+                    tc::pair_tma_3d<1>(aF + r.s * S::kBytesF, &map_f, c, x.f0, x.g, bar);
                     for (int b = 0; b < boxes0; ++b)
-                        tc::pair_tma_2d<CG>(dR + b * kRowBox * S::kBC8, &map_r, c, r0 + kRowBox * b, bar);
+                        tc::pair_tma_2d<1>(dR + b * kRowBox * S::kBC8, &map_r, c, x.row0 + kRowBox * b, bar);
                     for (int b = 0; b < boxes1; ++b)
-                        tc::pair_tma_2d<CG>(dR + S::kBytesHalf + b * kRowBox * S::kBC8, &map_r, c, r1 + kRowBox * b, bar);
+                        tc::pair_tma_2d<1>(dR + S::kBytesHalf + b * kRowBox * S::kBC8, &map_r, c, x.row0 + h1.at + kRowBox * b, bar);
                 }
                 __syncwarp();
             }
@@ -735,67 +650,64 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
             if (!(used >> s & 1u)) continue;
             const uint32_t last_phase = r.phase ^ (s >= r.s ? 1u : 0u);
             mbar_wait_bounded(&empty[s], last_phase, tc::kPairWaitCycles / 8);
-            if (stop() && rank == 0) mbar_wait_bounded(&full[s], last_phase, tc::kPairWaitCycles / 8);
+            if (stop()) mbar_wait_bounded(&full[s], last_phase, tc::kPairWaitCycles / 8);
         }
-    } else if (warp == 1) {
-        if (rank == 0) {
-            tc::Ring<S::kStages> r;
-            uint32_t it[2] = {0, 0};  // blocks of each half so far
-            int group = 0;
-            for (int t = cluster; t < total && !stop(); t += clusters) {
-                const Tile x = tiles.get(t, group, lane);
-                if (!x.rows) continue;
-                const int n0 = tile_half<CG>(x.n, 0).n, n1 = tile_half<CG>(x.n, 1).n;
-                const uint32_t idesc0 = tc::operand_idesc(0, false, false, kBF * CG, n0);
-                const uint32_t idesc1 = tc::operand_idesc(0, false, false, kBF * CG, n1);
-                for (int kk = 0; kk < kb; ++kk, r.next()) {
-                    const uint64_t df = tc::operand_desc(aF + r.s * S::kBytesF, false, 0);
-                    const uint64_t dr = tc::operand_desc(aR + r.s * S::kBytesR, false, 0);
-                    const int left = p.contraction - kk * S::kBC8;
-                    tc::wait(b_full + 8 * r.s, r.phase, up);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        if (h && !n1) break;
-                        const int slot = h + 2 * (int)(it[h] & 1u);
-                        tc::wait(b_dempty + 8 * slot, ((it[h] >> 1) & 1u) ^ 1u, up);
-                        tc::fence_after_sync();
-                        if (tc::elect_one()) {
-#pragma unroll
-                            for (int j = 0; j < S::kBC8 / 32; ++j)
-                                if (32 * j < left)
-                                    tc::pair_mma<CG, tc::kKindF8>(tmem + slot * kHalfCols, df + 2 * j,
-                                                                  dr + h * (S::kBytesHalf >> 4) + 2 * j, h ? idesc1 : idesc0, j != 0);
-                            tc::pair_commit<CG>(b_dfull + 8 * slot);
-                            if (h || !n1) tc::pair_commit<CG>(b_empty + 8 * r.s);
-                        }
-                        __syncwarp();
-                        ++it[h];
-                    }
-                }
-            }
-            if (tc::elect_one()) tc::leader_commit<CG>(smem_u32(&last));  // nor under MMAs in flight
-            mbar_wait_bounded(&last, 0, tc::kPairWaitCycles / 8);
-        }
-    } else if (warp < 4) {
-        // ---- scales of half warp - 2, two blocks ahead ----------------------------------------------------
-        const int h = warp - 2;
-        uint32_t it = 0;
+    } else if (warp == 1 || warp == 3) {
+        const int h = warp >> 1;
+        tc::Ring<S::kStages> r;
+        uint32_t it = 0;  // blocks of this half so far
         int group = 0;
-        for (int t = cluster; t < total && !stop(); t += clusters) {
+        for (int t = blockIdx.x; t < total && !stop(); t += gridDim.x) {
             const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
-            const Half half = tile_half<CG>(x.n, h);
-            if (!half.n) continue;
-            const int f0 = x.f0 + (int)rank * kBF, first = half.at + lane;
-            const float *ws = fp.ws + x.g * fp.ws_group + (int64_t)(f0 / kScaleBlock) * fp.ws_row;
-            const float *xs = fp.xs + (int64_t)(x.row0 + first) * fp.xs_row;
-            const bool on = f0 < p.features;  // the pair's second half may lie behind the last feature
-            float v[2][4], w[2];
-            auto fetch = [&](int kk, float (&v)[4], float &w) {
-                w = on && kk < kb ? __ldg(ws + kk * fp.ws_blk) : 0.0f;
+            const int n = tile_half(x.n, h).n;
+            const uint32_t idesc = tc::operand_idesc(0, false, false, kBF, n);
+            for (int kk = 0; kk < kb; ++kk, r.next()) {
+                tc::wait(b_full + 8 * r.s, r.phase, up);
+                const int slot = h + 2 * (int)(it & 1u);
+                if (n) tc::wait(b_dempty + 8 * slot, ((it >> 1) & 1u) ^ 1u, up);
+                tc::fence_after_sync();
+                if (tc::elect_one()) {
+                    if (n) {
+                        const uint64_t df = tc::operand_desc(aF + r.s * S::kBytesF, false, 0);
+                        const uint64_t dr = tc::operand_desc(aR + r.s * S::kBytesR + h * S::kBytesHalf, false, 0);
+                        const int left = p.contraction - kk * S::kBC8;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    v[i] = kk < kb && first + 32 * i < x.rows ? __ldg(xs + (int64_t)(32 * i) * fp.xs_row + kk * fp.xs_blk) : 0.0f;
+                        for (int j = 0; j < S::kBC8 / 32; ++j)
+                            if (32 * j < left)
+                                tc::pair_mma<1, tc::kKindF8>(tmem + slot * kHalfCols, df + 2 * j, dr + 2 * j, idesc, j != 0);
+                        tc::pair_commit<1>(b_dfull + 8 * slot);
+                    }
+                    tc::pair_commit<1>(b_empty + 8 * r.s);
+                }
+                __syncwarp();
+                if (n) ++it;
+            }
+        }
+        if (tc::elect_one()) tc::leader_commit<1>(smem_u32(&last));  // nor under MMAs in flight
+        mbar_wait_bounded(&last, 0, tc::kPairWaitCycles / 8);
+    } else if (warp == 2) {
+        // ---- scales, two blocks ahead: registers [block & 1][half][32 columns] ------------------------------
+        uint32_t it[2] = {0, 0};
+        int group = 0;
+        for (int t = blockIdx.x; t < total && !stop(); t += gridDim.x) {
+            const Tile x = tiles.get(t, group, lane);
+            if (!x.rows) continue;
+            const Half h1 = tile_half(x.n, 1);
+            const float *ws = fp.ws + x.g * fp.ws_group + (int64_t)(x.f0 / kScaleBlock) * fp.ws_row;
+            const float *xs[2] = {fp.xs + (int64_t)(x.row0 + lane) * fp.xs_row, fp.xs + (int64_t)(x.row0 + h1.at + lane) * fp.xs_row};
+            const int first[2] = {lane, h1.at + lane};
+            const int valid[2] = {min(x.rows, h1.at), x.rows};
+            float v[2][2][4], w[2];
+            auto fetch = [&](int kk, float (&v)[2][4], float &w) {
+                w = kk < kb ? __ldg(ws + kk * fp.ws_blk) : 0.0f;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        v[h][i] = kk < kb && first[h] + 32 * i < valid[h]
+                                      ? __ldg(xs[h] + (int64_t)(32 * i) * fp.xs_row + kk * fp.xs_blk)
+                                      : 0.0f;
             };
             fetch(0, v[0], w[0]);
             fetch(1, v[1], w[1]);
@@ -803,46 +715,49 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {
                     if (k0 + d >= kb) break;
-                    const int slot = h + 2 * (int)(it & 1u);
-                    float s4[4];
+                    float s[2][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s4[i] = v[d][i] * w[d];
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[h][i] = v[d][h][i] * w[d];
                     fetch(k0 + d + 2, v[d], w[d]);
-                    tc::wait(b_sempty + 8 * slot, ((it >> 1) & 1u) ^ 1u, up);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) scales[slot * kHalfCols + lane + 32 * i] = s4[i];
-                    __syncwarp();
-                    if (lane == 0) tc::arrive(b_dfull + 8 * slot);
-                    ++it;
+                    for (int h = 0; h < 2; ++h) {
+                        if (h && !h1.n) break;
+                        const int slot = h + 2 * (int)(it[h] & 1u);
+                        tc::wait(b_sempty + 8 * slot, ((it[h] >> 1) & 1u) ^ 1u, up);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) scales[slot * kHalfCols + lane + 32 * i] = s[h][i];
+                        __syncwarp();
+                        if (lane == 0) tc::arrive(b_dfull + 8 * slot);
+                        ++it[h];
+                    }
                 }
         }
     } else {
         const int quad = warp & 3, part = (warp - 4) >> 2;  // TMEM lanes 32 * quad.., half
         const F8Sync y{b_dfull, b_dempty, b_sempty, up, tmem + ((uint32_t)(quad * 32) << 16), scales,
-                       staging, &map_o32, &map_o8};
+                       staging + (warp - 4) * 16 * kStageRow};
         uint32_t it = 0;
         int group = 0;
-        for (int t = cluster; t < total; t += clusters) {
-            if (tc::bar_any_128(1 + part, stop())) break;  // the four warps of a half meet at barriers: they stop together
+        for (int t = blockIdx.x; t < total && !stop(); t += gridDim.x) {
             const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
-            const Half half = tile_half<CG>(x.n, part);
-            const int f = x.f0 + (int)rank * kBF + quad * 32, chunks = (half.n + 31) / 32;
+            const Half half = tile_half(x.n, part);
+            const int f = x.f0 + quad * 32, chunks = (half.n + 31) / 32;
             if (chunks == 0) continue;
-            if (chunks == 1) promote_half<CG, 1>(y, it, p, x, half, f, kb, part, lane);
-            else if (chunks == 2) promote_half<CG, 2>(y, it, p, x, half, f, kb, part, lane);
-            else if (chunks == 3) promote_half<CG, 3>(y, it, p, x, half, f, kb, part, lane);
-            else promote_half<CG, 4>(y, it, p, x, half, f, kb, part, lane);
+            if (chunks == 1) promote_half<1>(y, it, p, x, half, f, kb, part, lane);
+            else if (chunks == 2) promote_half<2>(y, it, p, x, half, f, kb, part, lane);
+            else if (chunks == 3) promote_half<3>(y, it, p, x, half, f, kb, part, lane);
+            else promote_half<4>(y, it, p, x, half, f, kb, part, lane);
         }
-        tc::bulk_wait_read();  // the copies read this CTA's shared memory
     }
     if (stop() && lane == 0) atomicOr(&g_product_err, 1u);
     __syncwarp();
     tc::fence_before_sync();
-    if constexpr (CG == 1) __syncthreads();
-    else tc::cluster_sync_all();
+    __syncthreads();
     tc::fence_after_sync();
-    if (warp == 1) tc::pair_tmem_dealloc<CG>(tmem, kTmemCols);
+    if (warp == 1) tc::pair_tmem_dealloc<1>(tmem, kTmemCols);
 }
 
 using EncodeTiled = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
@@ -908,25 +823,11 @@ int launch_mode(const Product &p, const CUtensorMap &mf, const CUtensorMap &mr, 
     return launch<CG, kGradWeight>(mf, mr, t, ft * rt, sms, s);
 }
 
-template <int CG>
-int launch_f8(const CUtensorMap &mf, const CUtensorMap &mr, const CUtensorMap (&mo)[2], const F8Params &fp, int sms,
-              cudaStream_t s) {
-    auto *kernel = k_product_f8<CG>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ShapeF8<CG>::kSmem) != cudaSuccess) return -1;
-    const int64_t ft = (fp.t.features + kBF * CG - 1) / (kBF * CG);
-    const int64_t rt = fp.t.rows / kRowsMax + std::min<int64_t>(fp.t.groups, fp.t.rows);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(CG * std::max<int64_t>(1, std::min<int64_t>(ft * rt, sms / CG))));
-    cfg.blockDim = dim3(kThreadsF8);
-    cfg.dynamicSmemBytes = ShapeF8<CG>::kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CG;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, mf, mr, mo[0], mo[1], fp) == cudaSuccess ? 1 : -1;
+int launch_f8(const CUtensorMap &mf, const CUtensorMap &mr, const F8Params &fp, int sms, cudaStream_t s) {
+    if (cudaFuncSetAttribute(k_product_f8, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ShapeF8::kSmem) != cudaSuccess) return -1;
+    const int64_t tiles = (int64_t)((fp.t.features + kBF - 1) / kBF) * (fp.t.rows / kRowsMax + std::min<int64_t>(fp.t.groups, fp.t.rows));
+    k_product_f8<<<(unsigned)std::min<int64_t>(tiles, sms), kThreadsF8, ShapeF8::kSmem, s>>>(mf, mr, fp);
+    return 1;
 }
 
 bool aligned(const void *p, int64_t stride, int size) {
@@ -971,14 +872,9 @@ int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
     t.out_group = p.out_stride;
     t.vec = aligned(p.out, p.ldo, 2) && p.out_stride % 8 == 0;
     t.segment = p.out_dtype == UMSX_DTYPE_F32 ? kSegment : 0x7fffffff;
-    t.bulk = t.vec && p.out_dtype != UMSX_DTYPE_F32;
     if (p.dtype == UMSX_DTYPE_E4M3) {
         const F8Params fp{t, p.xs, p.ws, p.xs_row, p.xs_blk, p.ws_row, p.ws_blk, p.ws_group};
-        CUtensorMap mo[2] = {};  // of the output, where it can have one: boxes of 32 and of 8 rows
-        if (t.bulk && (!encode(&mo[0], p.out_dtype, p.out, 2, p.n, p.rows, 1, p.ldo * 2, 0, 32) ||
-                       !encode(&mo[1], p.out_dtype, p.out, 2, p.n, p.rows, 1, p.ldo * 2, 0, 8)))
-            return -1;
-        return p.features() > kBF ? launch_f8<2>(mf, mr, mo, fp, sms, s) : launch_f8<1>(mf, mr, mo, fp, sms, s);
+        return launch_f8(mf, mr, fp, sms, s);
     }
     // CG = 2 for wide outputs
     return p.features() > kBF ? launch_mode<2>(p, mf, mr, t, sms, s) : launch_mode<1>(p, mf, mr, t, sms, s);
