@@ -496,6 +496,118 @@ def test_captured_and_replayed():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("tokens", [400, 20000])
+def test_captured_and_replayed_at_length(tokens):
+    """The same for the prompt's kernels (tcgen05, clusters of sixteen)."""
+    E, n, k, K = 7, 264, 128, 2
+    g = _gen(18)
+    ids = torch.randint(0, E, (tokens, K), generator=g, device="cuda", dtype=torch.int32)
+    x, w = _rand(g, tokens, k), _rand(g, E, n, k)
+    wq, ws = U.fp8_quantize(w, 128)
+
+    def step():
+        off, tok, job = U.group_rows(ids, E)
+        xr = x[tok]
+        y = U.grouped_mm(xr, w, off)
+        dx = U.grouped_mm_dx(y, w, off)
+        dw = U.grouped_mm_dw(y, xr, off)
+        return [off, tok, job, y, dx, dw, U.fp8_grouped_mm(*U.fp8_quantize(xr), wq, ws, off)]
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for seed in (1, 2):
+        ids.copy_(torch.randint(0, E, (tokens, K), generator=_gen(seed), device="cuda", dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step()):
+            assert torch.equal(a, b)
+
+
+def test_two_threads_at_once():
+    """Calls of two host threads on streams of their own give what they give alone."""
+    import threading
+    cases = [_case([200, 3, 90], 0, 0, 256, 512, BF16, seed=s) for s in (1, 2)]
+
+    def work(c, stream=None):
+        x, dy, w, off = c
+        return [U.grouped_mm(x, w, off, stream=stream), U.grouped_mm_dx(dy, w, off, stream=stream),
+                U.grouped_mm_dw(dy, x, off, stream=stream), *U.fp8_quantize(x, stream=stream)]
+
+    alone = [work(c) for c in cases]
+    torch.cuda.synchronize()
+    got = [None, None]
+
+    def run(i):
+        s = torch.cuda.Stream()
+        for _ in range(20):
+            got[i] = work(cases[i], s)
+        s.synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for a, b in zip(alone, got):
+        for p, q in zip(a, b):
+            assert torch.equal(p.float(), q.float())
+
+
+def test_given_stream_orders_new_outputs():
+    """Outputs that a call makes for a given stream (a torch stream or its number) are that stream's."""
+    x, dy, w, off = _case([300, 41], 0, 0, 256, 384, BF16, seed=6)
+    want = U.grouped_mm(x, w, off)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for s in (side, side.cuda_stream):
+        y = U.grouped_mm(x, w, off, stream=s)
+        z = U.grouped_mm_dx(y, w, off, stream=s)
+        side.synchronize()
+        assert torch.equal(y, want) and torch.equal(z, U.grouped_mm_dx(want, w, off))
+
+
+@pytest.mark.parametrize("n,k", [(256, 2048), (136, 4096), (96, 8200)])
+def test_long_contractions_in_fp32(n, k):
+    """fp32 outputs of the tensor cores add 512 of the contraction at a time, 16 to an addition: each of the at most 32
+    truncated additions of a part costs up to an ulp (2^-23 of the part's sum of magnitudes), the parts are added with
+    rounding."""
+    x, dy, w, off = _case([200, 60], 0, 0, n, k, BF16, seed=k)
+    y, parts = U.grouped_mm(x, w, off, out_dtype=F32), -(-k // 512)
+    for e, (i, j) in _spans(off):
+        xe, we = x[i:j].double(), w[e].double()
+        size = xe.abs() @ we.abs().T
+        off_by = (y[i:j].double() - xe @ we.T).abs()
+        assert (off_by <= (33 * 2.0 ** -23 + parts * 2.0 ** -24) * size).all()
+
+
+def test_every_row_to_one_of_many_experts():
+    """Few rows an expert on average, all of them with one: the choice of a kernel goes by the average."""
+    for rows in (33, 200):
+        counts = [0] * 64
+        counts[37] = rows
+        _check_all(counts, 0, 0, 272, 160, BF16, BF16, seed=rows)
+        x, xs, w, ws, off = _fp8_case(counts, 0, 0, 272, 160, seed=rows)
+        want, size = _fp8_want(x, xs, w[37], ws[37])
+        _close(U.fp8_grouped_mm(x, xs, w, ws, off, out_dtype=F32), want, size, 160, "y")
+
+
+@pytest.mark.parametrize("rows", [1, 17, 1024, 1025])
+def test_one_expert_is_the_dense_product(rows):
+    x, xs, w, ws, off = _fp8_case([rows], 0, 0, 200, 256, seed=rows)
+    assert torch.equal(U.fp8_grouped_mm(x, xs, w, ws, off), U.fp8_mm(x, xs, w[0], ws[0]))
+
+
+def test_status_is_clear_after_use():
+    x, dy, w, off = _case([300, 41], 0, 0, 256, 384, BF16, seed=6)
+    U.grouped_mm(x, w, off)
+    U.products_status()
+
+
 def test_launches_are_counted():
     x, dy, w, off = _case([3], 0, 0, 64, 64, BF16, seed=1)
     before = U.kernel_launches()

@@ -195,9 +195,9 @@ umsx_status run_product(const Product &p, umsx_stream stream) {
     if (e != cudaSuccess) return fail(UMSX_EDEVICE, std::string("device query: ") + cudaGetErrorString(e));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int n = product_few_takes(p, sms) ? launch_product_few(p, sms, s) : product_tc_takes(p) ? launch_product_tc(p, sms, s) : launch_product_any(p, sms, s);
-    if (n < 0) return fail(UMSX_EDEVICE, "the product's kernel could not be set up");
-    record_launches((uint64_t)n);
     e = cudaGetLastError();
+    if (n < 0) return fail(UMSX_EDEVICE, std::string("the product's kernel could not be set up: ") + cudaGetErrorString(e));
+    record_launches((uint64_t)n);
     if (e != cudaSuccess) return fail(UMSX_EDEVICE, std::string("product launch: ") + cudaGetErrorString(e));
     return UMSX_OK;
 }

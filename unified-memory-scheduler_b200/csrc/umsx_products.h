@@ -39,16 +39,16 @@ struct Product {
 };
 
 #ifdef __CUDACC__
-// Rows [a, b) of group g.  Offsets are clamped to the matrix, so that wrong ones cannot lead outside it.
+// First row of group g, and for g = groups the row behind the last one.  Offsets are clamped to the matrix, so that wrong
+// ones cannot lead outside it; a group whose end lies before its start is empty.
+__device__ __forceinline__ int group_start(const int32_t *offsets, int g, int64_t rows) {
+    if (!offsets) return g ? (int)rows : 0;
+    return min(max(__ldg(offsets + g), 0), (int)rows);
+}
+// Rows [a, b) of group g.
 __device__ __forceinline__ void group_bounds(const int32_t *offsets, int g, int64_t rows, int &a, int &b) {
-    if (!offsets) {
-        a = 0;
-        b = (int)rows;
-        return;
-    }
-    const int top = (int)rows;
-    a = min(max(__ldg(offsets + g), 0), top);
-    b = min(max(__ldg(offsets + g + 1), a), top);
+    a = group_start(offsets, g, rows);
+    b = max(a, group_start(offsets, g + 1, rows));
 }
 #endif
 

@@ -229,9 +229,8 @@ void launch(const FewParams &p, int nt, int64_t chunks, cudaStream_t s) {
 static int few_tiles(const Product &p, int sms) {
     const double mean = (double)p.rows / p.groups;
     const int64_t tiles = std::min<int64_t>(p.groups, p.rows) * ((p.n + 255) / 256);
-    if (p.rows > 32768) return 0;
-    if (mean <= 4) return 1;
-    return mean <= 32 && tiles <= sms / 2 ? (mean <= 8 ? 1 : 2) : 0;
+    if (mean <= 4 && p.rows <= 1024) return 1;  // 1024: one expert may have got them all, and is then read rows / 8 times
+    return mean <= 32 && p.rows <= 1024 && tiles <= sms / 2 ? (mean <= 8 ? 1 : 2) : 0;
 }
 
 bool product_few_takes(const Product &p, int sms) {

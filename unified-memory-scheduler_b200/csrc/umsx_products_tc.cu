@@ -72,7 +72,7 @@ struct Tile {
 
 template <int CG, int MODE>
 struct Tiles {
-    const int *start, *prefix;  // shared memory: bounds of the groups (start, end interleaved), tiles before group g
+    const int *start, *prefix;  // shared memory: first row of group g (and behind the last), tiles before group g
     int groups, f_tiles, features, contraction, out_rows;
 
     __device__ static int row_tiles(int rows) { return (rows + kRowsMax - 1) / kRowsMax; }
@@ -88,7 +88,7 @@ struct Tiles {
         // descriptors made of them then live in uniform registers, where the MMAs and copies want them.
         const auto uniform = [](int v) { return __shfl_sync(kFull, v, 0); };
         lo = uniform(lo);
-        const int a = uniform(start[2 * lo]), m = uniform(start[2 * lo + 1]) - a;
+        const int a = uniform(start[lo]), m = max(0, uniform(start[lo + 1]) - a);
         const int all = MODE == kGradWeight ? out_rows : m, rt = row_tiles(all);
         const int local = t - uniform(prefix[lo]);
         int i = 0, j = local, each = all;
@@ -116,13 +116,13 @@ struct Tiles {
 
 // Tiles before every group, by one warp.
 template <int CG, int MODE>
-__device__ __forceinline__ void tile_prefix(const int *bounds, int *prefix, int groups, int f_tiles, int out_rows, int lane) {
+__device__ __forceinline__ void tile_prefix(const int *start, int *prefix, int groups, int f_tiles, int out_rows, int lane) {
     int carry = 0;
     for (int g0 = 0; g0 < groups; g0 += 32) {
         const int g = g0 + lane;
         int tiles = 0;
         if (g < groups)
-            tiles = f_tiles * Tiles<CG, MODE>::row_tiles(MODE == kGradWeight ? out_rows : bounds[2 * g + 1] - bounds[2 * g]);
+            tiles = f_tiles * Tiles<CG, MODE>::row_tiles(MODE == kGradWeight ? out_rows : max(0, start[g + 1] - start[g]));
         int incl = tiles;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -222,13 +222,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     __shared__ __align__(8) uint64_t tail[S::kStages], fixed[S::kStages], last;
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up;
-    __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
+    __shared__ int start[kMaxGroups + 1], prefix[kMaxGroups + 1];
 
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
     const uint32_t rank = CG == 1 ? 0 : tc::cluster_rank();
     const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
 
-    for (int g = tid; g < p.groups; g += kThreads) group_bounds(p.offsets, g, p.rows, bounds[2 * g], bounds[2 * g + 1]);
+    for (int g = tid; g <= p.groups; g += kThreads) start[g] = group_start(p.offsets, g, p.rows);
     if (tid == 0) {
         gave_up = 0;
         for (int s = 0; s < S::kStages; ++s) {
@@ -246,14 +246,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     if (warp == 1) tc::pair_tmem_alloc<CG>(&tmem_s, kTmemCols);
     __syncthreads();
     const int f_tiles = (p.features + kBF * CG - 1) / (kBF * CG);
-    if (warp == 0) tile_prefix<CG, MODE>(bounds, prefix, p.groups, f_tiles, p.out_rows, lane);
+    if (warp == 0) tile_prefix<CG, MODE>(start, prefix, p.groups, f_tiles, p.out_rows, lane);
     tc::fence_before_sync();
     if constexpr (CG == 1) __syncthreads();
     else tc::cluster_sync_all();  // barriers are initialised before the peer's copies and arrivals reach them
     tc::fence_after_sync();
     const uint32_t tmem = __shfl_sync(kFull, tmem_s, 0);
     const int total = __shfl_sync(kFull, prefix[p.groups], 0);
-    const Tiles<CG, MODE> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
+    const Tiles<CG, MODE> tiles{start, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
     const uint32_t up = smem_u32(&gave_up), aF = smem_u32(sF), aR = smem_u32(sR);
     const uint32_t b_full = smem_u32(full), b_empty = smem_u32(empty), b_dfull = smem_u32(d_full), b_dempty = smem_u32(d_empty),
@@ -586,10 +586,10 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[kSlots], d_empty[kSlots], sc_empty[kSlots], last;
     __shared__ uint32_t tmem_s;
     __shared__ int gave_up;
-    __shared__ int bounds[2 * kMaxGroups], prefix[kMaxGroups + 1];
+    __shared__ int start[kMaxGroups + 1], prefix[kMaxGroups + 1];
 
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-    for (int g = tid; g < p.groups; g += kThreadsF8) group_bounds(p.offsets, g, p.rows, bounds[2 * g], bounds[2 * g + 1]);
+    for (int g = tid; g <= p.groups; g += kThreadsF8) start[g] = group_start(p.offsets, g, p.rows);
     if (tid == 0) {
         gave_up = 0;
         mbar_init(&last, 2);
@@ -606,13 +606,13 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     if (warp == 1) tc::pair_tmem_alloc<1>(&tmem_s, kTmemCols);
     __syncthreads();
     const int f_tiles = (p.features + kBF - 1) / kBF;
-    if (warp == 0) tile_prefix<1, kForward>(bounds, prefix, p.groups, f_tiles, p.out_rows, lane);
+    if (warp == 0) tile_prefix<1, kForward>(start, prefix, p.groups, f_tiles, p.out_rows, lane);
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = __shfl_sync(kFull, tmem_s, 0);
     const int total = __shfl_sync(kFull, prefix[p.groups], 0), kb = (p.contraction + S::kBC8 - 1) / S::kBC8;
-    const Tiles<1, kForward> tiles{bounds, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
+    const Tiles<1, kForward> tiles{start, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
     const uint32_t up = smem_u32(&gave_up), aF = smem_u32(sF), aR = smem_u32(sR);
     const uint32_t b_full = smem_u32(full), b_empty = smem_u32(empty), b_dfull = smem_u32(d_full), b_dempty = smem_u32(d_empty),

@@ -237,6 +237,10 @@ def route_static(x, router_w, router_b, experts: int, top_k: int, routing: int, 
 
 
 # ---- products over caller-owned expert weights --------------------------------------------------------
+#
+# Plain functions of CUDA tensors: they take no part in autograd (the gradients are functions of their own) and
+# write new tensors or the `out` given, on the current stream of the tensors' device or on `stream` (a torch stream or a
+# cudaStream_t).
 
 _CODES = {}  # torch dtype -> UMSX_DTYPE_*, filled on first use (torch is imported lazily)
 _TORCH = None
@@ -294,20 +298,27 @@ def _ld(t, dim=-2):
     return t.shape[-1] if dim == -2 else t.shape[-1] + (t.shape[-2] - 1) * _ld(t)
 
 
-def _new(shape, dtype, device):
-    """torch.empty for two or three dimensions; with the strides given it costs half as much."""
-    strides = (shape[1], 1) if len(shape) == 2 else (shape[1] * shape[2], shape[2], 1)
-    return _TORCH.empty_strided(shape, strides, dtype=dtype, device=device)
+def _new(shape, dtype, device, stream, strides=None):
+    """A tensor that is written on `stream` (None: the current one) first: what torch frees on one stream it may hand out
+    on that one only.  torch.empty for a given stream; with strides it costs half as much."""
+    if strides is None:
+        strides = (1,) if len(shape) == 1 else (shape[1], 1) if len(shape) == 2 else (shape[1] * shape[2], shape[2], 1)
+    if stream is None:
+        return _TORCH.empty_strided(shape, strides, dtype=dtype, device=device)
+    if isinstance(stream, int):
+        stream = _TORCH.cuda.ExternalStream(stream, device=device)
+    with _TORCH.cuda.stream(stream):
+        return _TORCH.empty_strided(shape, strides, dtype=dtype, device=device)
 
 
-def _out_arg(name, out, shape, dtype, like, default):
+def _out_arg(name, out, shape, dtype, like, default, stream):
     """`out`, checked, or a new tensor of `dtype` (`default` where that is None); and its type's code."""
     if out is None:
         dtype = default if dtype is None else dtype
         code = _CODES.get(dtype, -1)
         if code not in _OUT:
             _refuse(f"{name} cannot have type {dtype}")
-        return _new(shape, dtype, like.device), code
+        return _new(shape, dtype, like.device, stream), code
     if dtype is not None and dtype != out.dtype:
         _refuse(f"{name} has type {out.dtype}, not {dtype}")
     code = _matrix(name, out, len(shape), _OUT, like)
@@ -316,16 +327,21 @@ def _out_arg(name, out, shape, dtype, like, default):
     return out, code
 
 
-def _call(entry, t, stream, *args):
-    """entry(*args, stream) on t's device, which is the current one for the call; the stream given, or that device's
-    current one."""
-    index = t.device.index
+def _call(entry, tensors, stream, *args):
+    """entry(*args, stream) on the tensors' device, which is the current one for the call; the stream given, or that
+    device's current one.  A stream that is given is one more that uses the tensors: their memory is not handed out again
+    before it is done with them."""
+    index = tensors[0].device.index
     cuda = _TORCH.cuda
     before = cuda.current_device()
     if stream is None:
         s = _RAW_STREAM(index)
     else:
-        s = stream if isinstance(stream, int) else stream.cuda_stream
+        if isinstance(stream, int):
+            stream = cuda.ExternalStream(stream, device=index)
+        s = stream.cuda_stream
+        for t in tensors:
+            t.record_stream(stream)
     if before == index:
         status = entry(*args, s)
     else:
@@ -350,11 +366,11 @@ def group_rows(ids, experts: int, stream=None):
         _refuse("experts must be 1..1024")
     tokens, top_k = ids.shape
     dev, i32 = ids.device, torch.int32
-    offsets = torch.empty_strided((experts + 1,), (1,), dtype=i32, device=dev)
-    row_token = torch.empty_strided((tokens * top_k,), (1,), dtype=i32, device=dev)
-    row_of_job = torch.empty_strided((tokens, top_k), (top_k, 1), dtype=i32, device=dev)
-    _call(lib().umsx_group_rows, ids, stream, ids.data_ptr(), tokens, top_k, experts, offsets.data_ptr(),
-          row_token.data_ptr(), row_of_job.data_ptr())
+    offsets = _new((experts + 1,), i32, dev, stream)
+    row_token = _new((tokens * top_k,), i32, dev, stream)
+    row_of_job = _new((tokens, top_k), i32, dev, stream)
+    _call(lib().umsx_group_rows, (ids, offsets, row_token, row_of_job), stream, ids.data_ptr(), tokens, top_k, experts,
+          offsets.data_ptr(), row_token.data_ptr(), row_of_job.data_ptr())
     return offsets, row_token, row_of_job
 
 
@@ -370,9 +386,9 @@ def grouped_mm(x, w, offsets, out=None, out_dtype=None, stream=None):
     if x.shape[1] != k:
         _refuse(f"x has {x.shape[1]} columns, w has {k}")
     _offsets_arg(offsets, experts, x)
-    out, oc = _out_arg("out", out, (rows, n), out_dtype, x, x.dtype)
-    _call(lib().umsx_grouped_mm, x, stream, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ld(w, -3), offsets.data_ptr(),
-          experts, rows, n, k, code, out.data_ptr(), _ld(out), oc)
+    out, oc = _out_arg("out", out, (rows, n), out_dtype, x, x.dtype, stream)
+    _call(lib().umsx_grouped_mm, (x, w, offsets, out), stream, x.data_ptr(), _ld(x), w.data_ptr(), _ld(w), _ld(w, -3),
+          offsets.data_ptr(), experts, rows, n, k, code, out.data_ptr(), _ld(out), oc)
     return out
 
 
@@ -387,8 +403,8 @@ def grouped_mm_dx(dy, w, offsets, out=None, out_dtype=None, stream=None):
     if dy.shape[1] != n:
         _refuse(f"dy has {dy.shape[1]} columns, w has {n} rows")
     _offsets_arg(offsets, experts, dy)
-    out, oc = _out_arg("out", out, (rows, k), out_dtype, dy, dy.dtype)
-    _call(lib().umsx_grouped_mm_dx, dy, stream, dy.data_ptr(), _ld(dy), w.data_ptr(), _ld(w), _ld(w, -3),
+    out, oc = _out_arg("out", out, (rows, k), out_dtype, dy, dy.dtype, stream)
+    _call(lib().umsx_grouped_mm_dx, (dy, w, offsets, out), stream, dy.data_ptr(), _ld(dy), w.data_ptr(), _ld(w), _ld(w, -3),
           offsets.data_ptr(), experts, rows, n, k, code, out.data_ptr(), _ld(out), oc)
     return out
 
@@ -407,9 +423,9 @@ def grouped_mm_dw(dy, x, offsets, out=None, out_dtype=None, stream=None):
     if experts < 1:
         _refuse("offsets must hold at least two values")
     _offsets_arg(offsets, experts, dy)
-    out, oc = _out_arg("out", out, (experts, n, k), out_dtype, dy, torch.float32)
-    _call(lib().umsx_grouped_mm_dw, dy, stream, dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x), offsets.data_ptr(), experts,
-          rows, n, k, code, out.data_ptr(), _ld(out), _ld(out, -3), oc)
+    out, oc = _out_arg("out", out, (experts, n, k), out_dtype, dy, torch.float32, stream)
+    _call(lib().umsx_grouped_mm_dw, (dy, x, offsets, out), stream, dy.data_ptr(), _ld(dy), x.data_ptr(), _ld(x),
+          offsets.data_ptr(), experts, rows, n, k, code, out.data_ptr(), _ld(out), _ld(out, -3), oc)
     return out
 
 
@@ -432,7 +448,7 @@ def fp8_quantize(x, block_rows: int = 1, q=None, scales=None, stream=None):
     br, bc = -(-rows // block_rows), -(-cols // SCALE_BLOCK)
     dev = x.device
     if q is None:
-        q = _new((rows, cols) if dim == 2 else (matrices, rows, cols), torch.float8_e4m3fn, dev)
+        q = _new((rows, cols) if dim == 2 else (matrices, rows, cols), torch.float8_e4m3fn, dev, stream)
         ldq, qm = cols, rows * cols
     else:
         _matrix("q", q, dim, (DTYPE_E4M3,), x)
@@ -442,16 +458,16 @@ def fp8_quantize(x, block_rows: int = 1, q=None, scales=None, stream=None):
     if scales is None:
         s_row, s_blk, sm = (1, br, br * bc) if block_rows == 1 else (bc, 1, br * bc)
         if dim == 2:
-            scales = torch.empty_strided((br, bc), (s_row, s_blk), dtype=torch.float32, device=dev)
+            scales = _new((br, bc), torch.float32, dev, stream, (s_row, s_blk))
         else:
-            scales = torch.empty_strided((matrices, br, bc), (sm, s_row, s_blk), dtype=torch.float32, device=dev)
+            scales = _new((matrices, br, bc), torch.float32, dev, stream, (sm, s_row, s_blk))
     else:
         want = (br, bc) if dim == 2 else (matrices, br, bc)
         if scales.device != dev or scales.dtype != torch.float32 or scales.shape != want:
             _refuse(f"scales must be float32, on x's device and of shape {want}")
         s_row, s_blk, sm = scales.stride(-2), scales.stride(-1), scales.stride(0) if dim == 3 else 0
-    _call(lib().umsx_fp8_quantize, x, stream, x.data_ptr(), _ld(x), x.stride(0) if dim == 3 else 0, code, matrices, rows,
-          cols, block_rows, q.data_ptr(), ldq, qm, scales.data_ptr(), s_row, s_blk, sm)
+    _call(lib().umsx_fp8_quantize, (x, q, scales), stream, x.data_ptr(), _ld(x), x.stride(0) if dim == 3 else 0, code,
+          matrices, rows, cols, block_rows, q.data_ptr(), ldq, qm, scales.data_ptr(), s_row, s_blk, sm)
     return q, scales
 
 
@@ -477,8 +493,9 @@ def _fp8_product(x, xs, w, ws, offsets, out, out_dtype, stream):
         at = offsets.data_ptr()
     else:
         experts, wm, sm, at = 1, 0, 0, None
-    out, oc = _out_arg("out", out, (rows, n), out_dtype, x, torch.bfloat16)
-    _call(lib().umsx_fp8_grouped_mm, x, stream, x.data_ptr(), _ld(x), xs.data_ptr(), xs.stride(0), xs.stride(1),
+    out, oc = _out_arg("out", out, (rows, n), out_dtype, x, torch.bfloat16, stream)
+    tensors = (x, xs, w, ws, out, offsets) if grouped else (x, xs, w, ws, out)
+    _call(lib().umsx_fp8_grouped_mm, tensors, stream, x.data_ptr(), _ld(x), xs.data_ptr(), xs.stride(0), xs.stride(1),
           w.data_ptr(), _ld(w), wm, ws.data_ptr(), ws.stride(-2), ws.stride(-1), sm, at, experts, rows, n, k,
           out.data_ptr(), _ld(out), oc)
     return out
