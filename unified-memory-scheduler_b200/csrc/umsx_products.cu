@@ -22,15 +22,17 @@ umsx_status fail(umsx_status s, const std::string &msg) {
 
 // ---- any shape ---------------------------------------------------------------------------
 //
-// out[r][f] = sum_c R[r][c] F[f][c] in 64 x 64 tiles with fp32 FMAs, element loads and bounds
-// checks everywhere.  It takes what the tensor-core kernels cannot address: TMA wants bases
-// and row strides that are multiples of 16 bytes.  e4m3 operands are dequantised as they are
-// staged (code * scale, one rounding).
+// out[r][f] = sum_c R[r][c] F[f][c] for every stride and alignment: what the tcgen05 kernel cannot address, since TMA wants
+// bases and row strides that are multiples of 16 bytes (odd widths, slices that start anywhere).  Tiles of 64 rows x 128
+// features, 32 of the contraction a step: single-element loads, neighbouring lanes along the axis that is contiguous in
+// memory, one step ahead in registers; from shared memory into mma.sync.  e4m3 codes become f16 (exact); the sums of
+// a block of 128 are scaled once and added in fp32.  Bound by the issue of those loads (bf16 4096 x 4096 x 2049: 573 us,
+// 120 TFLOP/s; fp32 FMAs in place of mma.sync took 3441 us, 64-bit addresses per element instead of a step per thread 1295).
 
-constexpr int kTile = 64, kStep = 16;
+constexpr int kAnyRows = 64, kAnyF = 128, kStep = 32, kLine = kStep + 8;  // kLine: 80 bytes spread eight lines over all banks
 
 struct AnyParams {
-    int dtype, out_dtype, groups, mode;
+    int out_dtype, groups, mode;
     int64_t rows;
     int features, contraction;  // contraction: forward k, dx n (dw: the group's rows)
     int out_rows;               // dw: n
@@ -43,13 +45,60 @@ struct AnyParams {
     int64_t ldo, out_group;
 };
 
-__device__ __forceinline__ float load_el(const void *p, int64_t i, int dtype) {
-    if (dtype == UMSX_DTYPE_E4M3) {
-        const __nv_fp8_e4m3 v = static_cast<const __nv_fp8_e4m3 *>(p)[i];
-        return (float)v;
+// LINES x kStep elements of an operand, held by 256 threads between their load and their store: element i of a thread.
+template <int DTYPE, int LINES>
+struct Elements {
+    static constexpr int kPer = LINES * kStep / 256;
+    uint16_t v[kPer];
+
+    // Neighbouring threads lie along c where that is contiguous, along the lines otherwise; a thread's next element is a fixed
+    // step further in memory either way.
+    __device__ __forceinline__ void load(const void *p, int64_t s_line, int64_t s_c, int lines, int steps) {
+        constexpr int kSize = DTYPE == UMSX_DTYPE_E4M3 ? 1 : 2;
+        const bool along_c = s_c == 1;
+        const int l = along_c ? threadIdx.x / kStep : threadIdx.x % LINES, c = along_c ? threadIdx.x % kStep : threadIdx.x / LINES;
+        const int64_t by = (along_c ? 256 / kStep * s_line : 256 / LINES * s_c) * kSize;
+        const uint8_t *at = static_cast<const uint8_t *>(p) + (l * s_line + c * s_c) * kSize;
+        // elements of this thread that lie inside: the other coordinate is fixed
+        const int in = along_c ? (c < steps ? (lines - l + 256 / kStep - 1) / (256 / kStep) : 0)
+                               : (l < lines ? (steps - c + 256 / LINES - 1) / (256 / LINES) : 0);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i, at += by) {
+            if constexpr (kSize == 1) v[i] = i < in ? __ldg(at) : 0;
+            else v[i] = i < in ? __ldg(reinterpret_cast<const unsigned short *>(at)) : 0;
+        }
     }
-    const uint32_t h = __ldg(static_cast<const unsigned short *>(p) + i);
-    return dtype == UMSX_DTYPE_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+    __device__ __forceinline__ void store(uint16_t *to, bool along_c) const {
+        const int l = along_c ? threadIdx.x / kStep : threadIdx.x % LINES, c = along_c ? threadIdx.x % kStep : threadIdx.x / LINES;
+        uint16_t *at = to + l * kLine + c;
+        const int by = along_c ? 256 / kStep * kLine : 256 / LINES;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            uint16_t h = v[i];
+            if constexpr (DTYPE == UMSX_DTYPE_E4M3) h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)h, __NV_E4M3).x;
+            at[i * by] = h;
+        }
+    }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const uint16_t *p) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(smem_u32(p)));
+}
+
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ void store_el(void *p, int64_t i, int dtype, float v) {
@@ -58,80 +107,96 @@ __device__ __forceinline__ void store_el(void *p, int64_t i, int dtype, float v)
     else static_cast<__half *>(p)[i] = __float2half_rn(v);
 }
 
-__global__ void __launch_bounds__(256) k_product_any(const AnyParams p) {
-    __shared__ float sR[kStep][kTile + 4], sF[kStep][kTile + 4];
-    __shared__ int s_group, s_tile;
-    const int tid = threadIdx.x, f0 = blockIdx.x * kTile;
+template <int DTYPE>
+__global__ void __launch_bounds__(256, 2) k_product_any(const AnyParams p) {
+    constexpr bool kF8 = DTYPE == UMSX_DTYPE_E4M3;
+    constexpr int kSize = kF8 ? 1 : 2;
+    __shared__ __align__(16) uint16_t sR[kAnyRows * kLine], sF[kAnyF * kLine];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, f0 = blockIdx.x * kAnyF;
+    const int wr = (warp & 1) * 32, wf = (warp >> 1) * 32;  // the warp's 32 x 32 of the tile
+    const bool r_along = p.r_c == 1, f_along = p.f_c == 1;
     // row tiles of all groups in order; this CTA takes every gridDim.y-th
     for (int t = blockIdx.y;; t += gridDim.y) {
         __syncthreads();
-        if (tid == 0) {
-            int left = t, g = 0;
-            for (; g < p.groups; ++g) {
-                int a, b;
-                group_bounds(p.offsets, g, p.rows, a, b);
-                const int tiles = p.mode == kGradWeight ? (p.out_rows + kTile - 1) / kTile : (b - a + kTile - 1) / kTile;
-                if (left < tiles) break;
-                left -= tiles;
-            }
-            s_group = g;
-            s_tile = left;
+        int g = 0, tile = 0;
+        if (p.mode == kGradWeight) {
+            const int each = (p.out_rows + kAnyRows - 1) / kAnyRows;
+            g = t / each;
+            tile = t % each;
+            if (g >= p.groups) return;
+        } else if (!find_tile(p.offsets, p.groups, p.rows, kAnyRows, t, g, tile)) {
+            return;
         }
-        __syncthreads();
-        if (s_group == p.groups) return;
         int a, b;
-        group_bounds(p.offsets, s_group, p.rows, a, b);
+        group_bounds(p.offsets, g, p.rows, a, b);
         const bool dw = p.mode == kGradWeight;
-        const int r0 = s_tile * kTile, nr = dw ? p.out_rows : b - a, nc = dw ? b - a : p.contraction;
-        const int64_t r_base = dw ? (int64_t)a * p.r_c : (int64_t)a * p.r_row;
-        const int64_t f_base = dw ? (int64_t)a * p.f_c : (int64_t)s_group * p.f_group;
-        float acc[4][4] = {};
+        const int r0 = tile * kAnyRows, nr = min(kAnyRows, (dw ? p.out_rows : b - a) - r0), nf = min(kAnyF, p.features - f0);
+        const int nc = dw ? b - a : p.contraction;
+        const uint8_t *R = static_cast<const uint8_t *>(p.R) + (a * (dw ? p.r_c : p.r_row) + r0 * p.r_row) * kSize;
+        const uint8_t *F = static_cast<const uint8_t *>(p.F) + (dw ? a * p.f_c : g * p.f_group) * kSize + f0 * p.f_feat * kSize;
+        Elements<DTYPE, kAnyRows> er;
+        Elements<DTYPE, kAnyF> ef;
+        er.load(R, p.r_row, p.r_c, nr, nc);
+        ef.load(F, p.f_feat, p.f_c, nf, nc);
+        float acc[2][4][4] = {}, blk[2][4][4] = {};  // [16 rows][8 features]; blk: e4m3, of the present block of 128
         for (int c0 = 0; c0 < nc; c0 += kStep) {
-            for (int i = tid; i < kTile * kStep; i += 256) {
-                // neighbouring threads along the axis that is contiguous in memory
-                int rr = p.r_c == 1 ? i / kStep : i % kTile, cc = p.r_c == 1 ? i % kStep : i / kTile;
-                float v = 0.0f;
-                if (r0 + rr < nr && c0 + cc < nc) {
-                    v = load_el(p.R, r_base + (int64_t)(r0 + rr) * p.r_row + (int64_t)(c0 + cc) * p.r_c, p.dtype);
-                    if (p.rs) v *= __ldg(p.rs + (int64_t)(a + r0 + rr) * p.rs_row + (int64_t)((c0 + cc) / kScaleBlock) * p.rs_blk);
-                }
-                sR[cc][rr] = v;
-                rr = p.f_c == 1 ? i / kStep : i % kTile, cc = p.f_c == 1 ? i % kStep : i / kTile;
-                v = 0.0f;
-                if (f0 + rr < p.features && c0 + cc < nc) {
-                    v = load_el(p.F, f_base + (int64_t)(f0 + rr) * p.f_feat + (int64_t)(c0 + cc) * p.f_c, p.dtype);
-                    if (p.fs)
-                        v *= __ldg(p.fs + s_group * p.fs_group + (int64_t)((f0 + rr) / kScaleBlock) * p.fs_row +
-                                   (int64_t)((c0 + cc) / kScaleBlock) * p.fs_blk);
-                }
-                sF[cc][rr] = v;
-            }
+            __syncthreads();  // the previous step has been read
+            er.store(sR, r_along);
+            ef.store(sF, f_along);
             __syncthreads();
+            if (c0 + kStep < nc) {
+                er.load(R + (c0 + kStep) * p.r_c * kSize, p.r_row, p.r_c, nr, nc - c0 - kStep);
+                ef.load(F + (c0 + kStep) * p.f_c * kSize, p.f_feat, p.f_c, nf, nc - c0 - kStep);
+            }
 #pragma unroll
-            for (int cc = 0; cc < kStep; ++cc) {
-                float x[4], y[4];
+            for (int k = 0; k < kStep; k += 16) {
+                uint32_t x[2][4], y[2][4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    x[i] = sR[cc][(tid >> 4) * 4 + i];
-                    y[i] = sF[cc][(tid & 15) * 4 + i];
+                for (int i = 0; i < 2; ++i) {
+                    // rows x contraction: 8 x 8 matrices (0, 0), (8, 0), (0, 8), (8, 8); features: (0, 0), (0, 8), (8, 0), (8, 8)
+                    ldmatrix4(x[i], sR + (wr + 16 * i + (lane & 15)) * kLine + k + 8 * (lane >> 4));
+                    ldmatrix4(y[i], sF + (wf + 16 * i + (lane & 7) + 8 * (lane >> 4)) * kLine + k + 8 * ((lane >> 3) & 1));
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(x[i], y[j], acc[i][j]);
+                    for (int j = 0; j < 4; ++j)
+                        mma16816<DTYPE == UMSX_DTYPE_BF16>(kF8 ? blk[i][j] : acc[i][j], x[i], y[j >> 1][2 * (j & 1)], y[j >> 1][2 * (j & 1) + 1]);
             }
-            __syncthreads();
-        }
-        for (int i = 0; i < 4; ++i) {
-            const int r = r0 + (tid >> 4) * 4 + i;
-            if (r >= nr) break;
-            for (int j = 0; j < 4; ++j) {
-                const int f = f0 + (tid & 15) * 4 + j;
-                if (f >= p.features) break;
-                const int64_t o = dw ? s_group * p.out_group + (int64_t)r * p.ldo + f : (int64_t)(a + r) * p.ldo + f;
-                store_el(p.out, o, p.out_dtype, acc[i][j]);
+            if (kF8 && (c0 % kScaleBlock == kScaleBlock - kStep || c0 + kStep >= nc)) {
+                const int cb = c0 / kScaleBlock;
+                const float w = __ldg(p.fs + g * p.fs_group + (int64_t)(f0 / kScaleBlock) * p.fs_row + cb * p.fs_blk);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = wr + 16 * i + 8 * h + (lane >> 2);
+                        const float sc = r < nr ? w * __ldg(p.rs + (int64_t)(a + r0 + r) * p.rs_row + cb * p.rs_blk) : 0.0f;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                acc[i][j][2 * h + q] = fmaf(sc, blk[i][j][2 * h + q], acc[i][j][2 * h + q]);
+                                blk[i][j][2 * h + q] = 0.0f;
+                            }
+                    }
             }
         }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = wr + 16 * i + 8 * h + (lane >> 2);
+                if (r >= nr) continue;
+                const int64_t at = (dw ? g * p.out_group + (int64_t)(r0 + r) * p.ldo : (int64_t)(a + r0 + r) * p.ldo) + f0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int f = wf + 8 * j + 2 * (lane & 3) + q;
+                        if (f < nf) store_el(p.out, at + f, p.out_dtype, acc[i][j][2 * h + q]);
+                    }
+            }
     }
 }
 
@@ -139,7 +204,6 @@ __global__ void __launch_bounds__(256) k_product_any(const AnyParams p) {
 
 int launch_product_any(const Product &p, int sms, cudaStream_t s) {
     AnyParams a{};
-    a.dtype = p.dtype;
     a.out_dtype = p.out_dtype;
     a.groups = p.groups;
     a.mode = p.mode;
@@ -168,10 +232,12 @@ int launch_product_any(const Product &p, int sms, cudaStream_t s) {
         a.R = p.dy, a.r_row = 1, a.r_c = p.lddy;
         a.F = p.x, a.f_feat = 1, a.f_c = p.ldx;
     }
-    const int64_t tiles = p.mode == kGradWeight ? (int64_t)p.groups * ((p.n + kTile - 1) / kTile)
-                                                : (p.rows + kTile - 1) / kTile + p.groups;
-    const dim3 grid((unsigned)((a.features + kTile - 1) / kTile), (unsigned)std::min<int64_t>(tiles, 32 * sms));
-    k_product_any<<<grid, 256, 0, s>>>(a);
+    const int64_t tiles = p.mode == kGradWeight ? (int64_t)p.groups * ((p.n + kAnyRows - 1) / kAnyRows)
+                                                : p.rows / kAnyRows + std::min<int64_t>(p.groups, p.rows);
+    const dim3 grid((unsigned)((a.features + kAnyF - 1) / kAnyF), (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, 32 * sms)));
+    if (p.dtype == UMSX_DTYPE_BF16) k_product_any<UMSX_DTYPE_BF16><<<grid, 256, 0, s>>>(a);
+    else if (p.dtype == UMSX_DTYPE_F16) k_product_any<UMSX_DTYPE_F16><<<grid, 256, 0, s>>>(a);
+    else k_product_any<UMSX_DTYPE_E4M3><<<grid, 256, 0, s>>>(a);
     return 1;
 }
 

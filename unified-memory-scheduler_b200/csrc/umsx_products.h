@@ -50,6 +50,43 @@ __device__ __forceinline__ void group_bounds(const int32_t *offsets, int g, int6
     a = group_start(offsets, g, rows);
     b = max(a, group_start(offsets, g + 1, rows));
 }
+// The index-th tile of `per` rows, counted over the groups, by all threads of a CTA of 256 (a barrier in front of the next
+// call); false behind the last.
+__device__ __forceinline__ bool find_tile(const int32_t *offsets, int groups, int64_t rows, int per, int index, int &group,
+                                          int &tile) {
+    __shared__ int s_group, s_tile, s_sum[8];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int g0 = 0; g0 < groups; g0 += 256) {
+        const int g = g0 + tid;
+        int a = 0, b = 0;
+        if (g < groups) group_bounds(offsets, g, rows, a, b);
+        const int tiles = (b - a + per - 1) / per;
+        int incl = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) s_sum[warp] = incl;
+        if (tid == 0) s_group = -1;
+        __syncthreads();
+        int before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+            if (w < warp) before += s_sum[w];
+            all += s_sum[w];
+        }
+        const int first = before + incl - tiles;
+        if (index >= first && index < first + tiles) s_group = g, s_tile = index - first;
+        __syncthreads();
+        group = s_group;
+        tile = s_tile;
+        if (group >= 0) return true;
+        index -= all;
+        __syncthreads();  // s_sum is written again
+    }
+    return false;
+}
 #endif
 
 // Each returns the number of kernels launched, -1 when the driver refuses something.

@@ -23,7 +23,7 @@
 namespace umsx {
 namespace {
 
-constexpr int kWarps = 8, kFewF = 16;
+constexpr int kWarps = 8, kFewF = 16;  // kWarps: find_tile's CTA
 
 struct FewParams {
     int groups, n, k, out_dtype;
@@ -87,43 +87,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_product_few(const FewParams 
     constexpr int kRows = 8 * NT;
     constexpr bool kF8 = DTYPE == UMSX_DTYPE_E4M3;
     __shared__ float part[kWarps][kFewF * kRows];
-    __shared__ int s_group, s_chunk, s_sum[kWarps];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gl = lane >> 2, tl = lane & 3;
 
     // the blockIdx.y-th chunk of kRows rows, counted over the groups
     int group = 0, chunk = blockIdx.y, a = 0, b = (int)p.rows;
     if (p.offsets) {
-        int left = blockIdx.y;
-        bool found = false;
-        for (int g0 = 0; g0 < p.groups && !found; g0 += kWarps * 32) {
-            const int g = g0 + tid;
-            int lo = 0, hi = 0;
-            if (g < p.groups) group_bounds(p.offsets, g, p.rows, lo, hi);
-            const int chunks = (hi - lo + kRows - 1) / kRows;
-            int incl = chunks;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(kFull, incl, o);
-                if (lane >= o) incl += v;
-            }
-            if (lane == 31) s_sum[warp] = incl;
-            if (tid == 0) s_group = -1;
-            __syncthreads();
-            int before = 0, all = 0;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                if (w < warp) before += s_sum[w];
-                all += s_sum[w];
-            }
-            const int first = before + incl - chunks;
-            if (left >= first && left < first + chunks) s_group = g, s_chunk = left - first;
-            __syncthreads();
-            found = s_group >= 0;
-            left -= all;
-        }
-        if (!found) return;
-        group = s_group;
-        chunk = s_chunk;
+        if (!find_tile(p.offsets, p.groups, p.rows, kRows, blockIdx.y, group, chunk)) return;
         group_bounds(p.offsets, group, p.rows, a, b);
     }
     const int row0 = a + chunk * kRows, rows = min(kRows, b - row0);
