@@ -335,6 +335,16 @@ def test_group_rows(tokens, top_k, experts, kind):
         assert torch.equal(a.cpu().long(), b), name
 
 
+@pytest.mark.parametrize("jobs", [512, 513, 1536, 1537, 2048, 4095, 4096, 4097, 65536, 65537, 1048577])
+@pytest.mark.parametrize("experts", [7, 255, 256, 1024])
+def test_group_rows_around_its_launch_shapes(jobs, experts):
+    g = _gen(jobs + experts)
+    ids = torch.randint(-1, experts, (jobs, 1), generator=g, device="cuda", dtype=torch.int32)
+    got = U.group_rows(ids, experts)
+    for name, a, b in zip(("offsets", "row_token", "row_of_job"), got, _group_want(ids, experts)):
+        assert torch.equal(a.cpu().long(), b), name
+
+
 # ---- use -------------------------------------------------------------------------------------------------
 
 

@@ -3,12 +3,13 @@
 // A stable counting sort of T*k jobs by expert in ONE launch without global scratch: a cluster of
 // up to sixteen CTAs splits the jobs into one contiguous piece per warp; each warp counts its piece
 // per expert (lanes of equal expert find one another with a ballot per bit, so no atomics and one fixed
-// order; a ballot takes an SM 5 cycles and match_any 50), the counts are scanned over the warps of a CTA, over the CTAs through distributed shared
-// memory and over the experts, and a second walk over the piece gives every job its row.
+// order; a ballot takes an SM 5 cycles and match_any 50), the counts are scanned over the warps of a CTA, over the CTAs
+// through distributed shared memory and over the experts, and a second walk over the piece gives every job its row.
 // The second walk sorts a CTA's jobs in shared memory, so that row_token is written in runs: 32 lanes that
 // store to 32 rows take the SM 32 cycles, which was most of the kernel's time.
-// Bound: the ballots, eight or eleven per 32 jobs at 5 cycles each (131072 jobs on 16 SMs: 10 K cycles), which is why
-// the jobs are spread over the largest cluster there is; below that latency (three barriers, two dependent walks).
+// Bound: latency (the scans over warps, CTAs and experts, the barriers between them, two dependent walks): 4.5 us for 128
+// jobs, 14.3 for 16384, a launch in a graph.  Where there are many, the ballots too, eight or eleven per 32 jobs at 5
+// cycles each (131072 jobs on 16 SMs: 10 K cycles of 20 us), which is why they are spread over the largest cluster there is.
 // The ids are read once and 8 bytes per job written once, some MB that memory would take a microsecond for.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
@@ -27,6 +28,8 @@ namespace {
 
 constexpr int kBatch = 16;  // kBatch: steps of 32 ids a warp has in flight
 constexpr int kGroupSmemMax = 200 * 1024;
+
+constexpr int kWarpsMax = 16;
 
 // Shared memory: hist[warps][E], total[E], all[E], base[E], local[E], 32 partial sums, then `sorted` 16-bit job numbers.
 size_t group_smem(int warps, int experts, int64_t sorted) {
@@ -47,7 +50,7 @@ __device__ __forceinline__ unsigned same_expert(int e) {
 }
 
 template <int BITS>
-__global__ void __launch_bounds__(1024) k_group_rows(const int32_t *ids, int64_t jobs, int top_k, int E, int sort_local,
+__global__ void __launch_bounds__(32 * kWarpsMax) k_group_rows(const int32_t *ids, int64_t jobs, int top_k, int E, int sort_local,
                                                      int32_t *offsets, int32_t *row_token, int32_t *row_of_job) {
     extern __shared__ int smem[];
     cg::cluster_group cluster = cg::this_cluster();
@@ -199,13 +202,15 @@ extern "C" umsx_status umsx_group_rows(const int32_t *ids, int tokens, int top_k
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    // One CTA up to 1024 jobs (one step per warp): a cluster's two extra barriers cost more than they save there.  Sixteen
-    // CTAs are beyond the portable cluster size: asked for where they halve the time, and only if the device can hold them.
-    int ctas = jobs <= 1024 ? 1 : 8;
-    if (jobs > 16384 && e == cudaSuccess) {
+    // One CTA for few jobs, where a cluster's barriers cost more than its SMs save (us in one CTA, in eight; 128 experts: 512
+    // jobs 5.9, 9.3; 1024: 7.1, 9.8; 1536: 8.3, 9.8; 2048: 9.5, 8.9).  Sixteen CTAs, beyond the portable cluster size and
+    // only if the device can hold them, for many (in eight, in sixteen, with the warps of then; 2048: 9.0, 10.2; 4096
+    // jobs of 256 experts: 13.1, 12.5; 8192: 18.7, 13.4; 131072: 27.3, 23.1).
+    int ctas = jobs <= 1536 ? 1 : 8;
+    if (jobs >= 4096 && e == cudaSuccess) {
         int fit = 0;
         cfg.gridDim = dim3(16);
-        cfg.blockDim = dim3(1024);
+        cfg.blockDim = dim3(32 * kWarpsMax);
         cfg.dynamicSmemBytes = kGroupSmemMax;
         at[0].val.clusterDim.x = 16;
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
@@ -214,8 +219,11 @@ extern "C" umsx_status umsx_group_rows(const int32_t *ids, int tokens, int top_k
         else
             cudaGetLastError();  // not an error of this call
     }
-    // warps: no more than there are steps, no more than shared memory has counters for (E = 1024: 32 still fit)
-    const int warps = (int)std::min<int64_t>(32, std::max<int64_t>(4, (jobs + 32 * ctas - 1) / (32 * ctas)));
+    // Warps: each costs a row of the counters' scan, so sixteen at most (16384 jobs: 14.3 us, with 32 warps 19.3; 131072: 20.2,
+    // 23.1), a step of 32 jobs each in a cluster (4096: 12.5, with two steps a warp 17.8), four in a single CTA (512: 5.9, with
+    // one 7.8).
+    const int64_t share = 32 * ctas * (ctas == 1 ? 4 : 1);
+    const int warps = (int)std::min<int64_t>(kWarpsMax, std::max<int64_t>(4, (jobs + share - 1) / share));
     // one CTA's jobs, if their 16-bit numbers fit into shared memory (at 1024 experts up to 27 K of them)
     const int64_t piece = ((jobs + 31) / 32 + ctas * warps - 1) / (ctas * warps) * warps * 32;
     // (a single CTA's few jobs are written at once: its walk over the experts would take longer)
