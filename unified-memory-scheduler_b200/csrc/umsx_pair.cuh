@@ -33,22 +33,19 @@ __device__ __forceinline__ void pair_tmem_dealloc(uint32_t taddr, uint32_t ncols
     else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
 }
 
-enum MmaKind { kKindF16 = 0, kKindF8 = 1 };
-
-// D (+)= A * B^T for one slice of 32 bytes of K; issued by one thread (of the leader).
-template <int CG, MmaKind KIND>
-__device__ __forceinline__ void pair_mma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                         uint32_t accumulate) {
-#define UMSX_MMA(group, kind, mask)                                                                              \
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                               \
-                 "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), \
-                 "l"(b_desc), "r"(idesc), "r"(accumulate)                                                        \
-                 : "memory")
-    if constexpr (CG == 1 && KIND == kKindF16) UMSX_MMA("1", "f16", );
-    else if constexpr (CG == 2 && KIND == kKindF16) UMSX_MMA("2", "f16", );
-    else if constexpr (CG == 1) UMSX_MMA("1", "f8f6f4", );
-    else UMSX_MMA("2", "f8f6f4", );
-#undef UMSX_MMA
+// D (+)= A * B^T for one slice of 32 bytes of K; issued by one thread: 16-bit operands of a pair (by the leader) ...
+__device__ __forceinline__ void mma_f16_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc),
+                 "r"(idesc), "r"(accumulate)
+                 : "memory");
+}
+// ... and 8-bit operands of one CTA.
+__device__ __forceinline__ void mma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem), "l"(a_desc), "l"(b_desc),
+                 "r"(idesc), "r"(accumulate)
+                 : "memory");
 }
 
 // Arrive on `bar` (of both CTAs of a pair, at the same offset) once every MMA issued so far has completed.
@@ -70,12 +67,6 @@ __device__ __forceinline__ void leader_commit(uint32_t bar) {
     else asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
-// The leader's copy of a shared-memory object, as a shared::cluster address.
-__device__ __forceinline__ uint32_t leader_addr(const void *p) {
-    uint32_t a;
-    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
-    return a;
-}
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
@@ -122,7 +113,7 @@ __device__ __forceinline__ void pair_tma_3d(uint32_t dst, const void *tmap, int 
                      : "memory");
 }
 
-// The same for a barrier or buffer given by its address in this CTA.
+// The leader's copy of a shared-memory object of this CTA, as a shared::cluster address.
 __device__ __forceinline__ uint32_t leader_addr(uint32_t p) {
     uint32_t a;
     asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(p));

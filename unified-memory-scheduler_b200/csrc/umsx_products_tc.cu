@@ -1,7 +1,7 @@
 // Ragged products of 16-bit operands on the tensor cores (tcgen05), forward and both gradients.
 //
 // out[r][f] = sum_c R[r][c] F[f][c] with the FEATURES as the MMA's M (128 per CTA, TMEM lanes) and the
-// group's ROWS as its N.  N goes in steps of 16 (a CTA pair: 32), so a group of 140 rows costs 144 and not 256:
+// group's ROWS as its N.  N goes in steps of 32, so a group of 140 rows costs 160 and not 256:
 // with the rows as M, ragged groups would be padded to 128.  The rows of a group are split into equal
 // tiles of at most 256.
 //
@@ -9,13 +9,15 @@
 //   dx       F = w (MN-major: k is contiguous), R = dy  contraction n
 //   dw       F = x, R = dy, both MN-major               contraction: the group's rows
 //
-// One persistent CTA (pair) per SM (pair); CTA i takes tiles i, i + grid, ... of the list (group, feature
+// One persistent CTA pair per two SMs; pair i takes tiles i, i + pairs, ... of the list (group, feature
 // tile, row tile), which every CTA derives from the offsets, so there is no scheduler state and the order of
-// sums is fixed.  Roles: warp 0 TMA, warp 1 MMA, warps 2-9 epilogue, warp 10 (dw) the group's ragged end.
+// sums is fixed.  A pair's CTA reads half the rows' operand; single CTAs with tiles of 128 x 256 took 406, 401 and 500 us
+// for forward, dx and dw where pairs take 356, 388 and 426 (bf16, 32 experts of 512 rows, 5760 x 2880), and were no
+// faster for 128 features or fewer either (16 x 1024 rows, 128 x 2048: both 27 to 31 us).  Roles: warp 0 TMA, warp 1 MMA, warps 2-9 epilogue, warp 10 (dw) the group's ragged end.
 // Two accumulators of 256 columns: the epilogue drains one while the MMA fills the other.
 //
-// The tensor cores add to an fp32 accumulator by truncation, whose error grows with the number of additions (2.5e-6 of the
-// result at a contraction of 2048, against 0.8e-6 of rounded fp32 sums).  Outputs in fp32 therefore get a fresh accumulator
+// An accumulator of the tensor cores is less exact than rounded fp32 additions, the more so the longer it is added to (error
+// 2.5e-6 of the result at a contraction of 2048, against 0.8e-6).  Outputs in fp32 therefore get a fresh accumulator
 // every kSegment stages, which the epilogue adds up in registers; in 16-bit outputs the last rounding hides it.
 //
 // dw's contraction ends inside a block of 64 rows; the rows behind it belong to the next group.  Warp
@@ -41,6 +43,7 @@ __device__ uint32_t g_product_err;  // a bounded wait gave up (umsx_products_sta
 namespace {
 
 constexpr int kBF = 128, kBC = 64;  // features per CTA, contraction per stage
+constexpr int kPair = 2;            // CTAs that share a tile of the 16-bit kernel
 constexpr int kRowsMax = 256;       // rows of a tile (of a pair: 128 in each CTA)
 constexpr int kRowBox = 32;         // rows of one K-major TMA box
 constexpr int kThreads = 352, kEpilogueWarps = 8;
@@ -56,15 +59,15 @@ struct TcParams {
     int64_t ldo, out_group;
 };
 
-template <int CG, int MODE>
+template <int MODE>
 struct Shape {
     static constexpr bool kFMn = MODE != kForward, kRMn = MODE == kGradWeight;
-    static constexpr int kBytesF = kBF * kBC * 2, kBytesR = kRowsMax / CG * kBC * 2;
-    static constexpr int kStages = CG == 1 ? 4 : 6;
+    static constexpr int kBytesF = kBF * kBC * 2, kBytesR = kRowsMax / kPair * kBC * 2;
+    static constexpr int kStages = 6;
     static constexpr size_t kSmem = 1024 + (size_t)kStages * (kBytesF + kBytesR) + kEpilogueWarps * 16 * kStageRow;
 };
 
-// One tile of the list: rows [row0, row0 + rows) x features [f0, f0 + 128 * CG) of group g.
+// One tile of the list: rows [row0, row0 + rows) x features [f0, f0 + 128 * CG) of group g; CG: CTAs that share it.
 struct Tile {
     int g, f0, row0, rows, c0, c_len;  // c0: first contraction index (dw: a row of x and dy)
     int n;                             // rows rounded up to the MMA's N
@@ -210,10 +213,10 @@ __device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, in
     }
 }
 
-template <int CG, int MODE>
+template <int MODE>
 __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constant__ CUtensorMap map_f,
                                                             const __grid_constant__ CUtensorMap map_r, const TcParams p) {
-    using S = Shape<CG, MODE>;
+    using S = Shape<MODE>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = smem_raw + (-smem_u32(smem_raw) & 1023u);
     uint8_t *sF = smem, *sR = smem + S::kStages * S::kBytesF;
@@ -225,8 +228,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     __shared__ int start[kMaxGroups + 1], prefix[kMaxGroups + 1];
 
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
-    const uint32_t rank = CG == 1 ? 0 : tc::cluster_rank();
-    const int cluster = blockIdx.x / CG, clusters = gridDim.x / CG;
+    const uint32_t rank = tc::cluster_rank();
+    const int cluster = blockIdx.x / kPair, clusters = gridDim.x / kPair;
 
     for (int g = tid; g <= p.groups; g += kThreads) start[g] = group_start(p.offsets, g, p.rows);
     if (tid == 0) {
@@ -234,26 +237,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&tail[s], 1);
-            mbar_init(&fixed[s], CG);
+            mbar_init(&fixed[s], kPair);
             mbar_init(&empty[s], 1);
         }
         mbar_init(&last, 1);
         for (int b = 0; b < 2; ++b) {
             mbar_init(&d_full[b], 1);
-            mbar_init(&d_empty[b], CG * kEpilogueWarps);
+            mbar_init(&d_empty[b], kPair * kEpilogueWarps);
         }
     }
-    if (warp == 1) tc::pair_tmem_alloc<CG>(&tmem_s, kTmemCols);
+    if (warp == 1) tc::pair_tmem_alloc<kPair>(&tmem_s, kTmemCols);
     __syncthreads();
-    const int f_tiles = (p.features + kBF * CG - 1) / (kBF * CG);
-    if (warp == 0) tile_prefix<CG, MODE>(start, prefix, p.groups, f_tiles, p.out_rows, lane);
+    const int f_tiles = (p.features + kBF * kPair - 1) / (kBF * kPair);
+    if (warp == 0) tile_prefix<kPair, MODE>(start, prefix, p.groups, f_tiles, p.out_rows, lane);
     tc::fence_before_sync();
-    if constexpr (CG == 1) __syncthreads();
-    else tc::cluster_sync_all();  // barriers are initialised before the peer's copies and arrivals reach them
+    tc::cluster_sync_all();  // barriers are initialised before the peer's copies and arrivals reach them
     tc::fence_after_sync();
     const uint32_t tmem = __shfl_sync(kFull, tmem_s, 0);
     const int total = __shfl_sync(kFull, prefix[p.groups], 0);
-    const Tiles<CG, MODE> tiles{start, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
+    const Tiles<kPair, MODE> tiles{start, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
     const uint32_t up = smem_u32(&gave_up), aF = smem_u32(sF), aR = smem_u32(sR);
     const uint32_t b_full = smem_u32(full), b_empty = smem_u32(empty), b_dfull = smem_u32(d_full), b_dempty = smem_u32(d_empty),
@@ -268,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             const Tile x = tiles.get(t, group, lane);
             const int kb = (x.c_len + kBC - 1) / kBC;
             if (!x.rows) continue;
-            const int half = x.n / CG;  // rows of this CTA's part of R
+            const int half = x.n / kPair;  // rows of this CTA's part of R
             const int boxes = S::kRMn ? (half + 63) / 64 : (half + kRowBox - 1) / kRowBox;
             const uint32_t bytes = S::kBytesF + boxes * (S::kRMn ? 64 : kRowBox) * kBC * 2;
             const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
@@ -284,23 +286,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                         tc::expect_tx(bar, bytes);  // each CTA's own, for its warp 10
                         if (rank == 0) tc::arrive(b_full + 8 * r.s);
                     } else {
-                        if (rank == 0) tc::expect_tx(bar, CG * bytes);
-                        if (CG > 1) bar = tc::leader_addr(bar);
+                        if (rank == 0) tc::expect_tx(bar, kPair * bytes);
+                        bar = tc::leader_addr(bar);
                     }
                     const int c = x.c0 + kk * kBC;
                     const uint32_t dF = aF + r.s * S::kBytesF, dR = aR + r.s * S::kBytesR;
                     if constexpr (MODE == kForward) {
-                        tc::pair_tma_3d<CG>(dF, &map_f, c, f0, x.g, bar);
+                        tc::pair_tma_3d<kPair>(dF, &map_f, c, f0, x.g, bar);
                     } else {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            if constexpr (MODE == kGradInput) tc::pair_tma_3d<CG>(dF + h * 8192, &map_f, f0 + 64 * h, c, x.g, bar);
-                            else tc::pair_tma_2d<CG>(dF + h * 8192, &map_f, f0 + 64 * h, c, bar);
+                            if constexpr (MODE == kGradInput) tc::pair_tma_3d<kPair>(dF + h * 8192, &map_f, f0 + 64 * h, c, x.g, bar);
+                            else tc::pair_tma_2d<kPair>(dF + h * 8192, &map_f, f0 + 64 * h, c, bar);
                         }
                     }
                     for (int b = 0; b < boxes; ++b) {
-                        if constexpr (S::kRMn) tc::pair_tma_2d<CG>(dR + b * 8192, &map_r, r0 + 64 * b, c, bar);
-                        else tc::pair_tma_2d<CG>(dR + b * kRowBox * 128, &map_r, c, r0 + kRowBox * b, bar);
+                        if constexpr (S::kRMn) tc::pair_tma_2d<kPair>(dR + b * 8192, &map_r, r0 + 64 * b, c, bar);
+                        else tc::pair_tma_2d<kPair>(dR + b * kRowBox * 128, &map_r, c, r0 + kRowBox * b, bar);
                     }
                 }
                 __syncwarp();
@@ -325,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                 const Tile x = tiles.get(t, group, lane);
                 const int kb = (x.c_len + kBC - 1) / kBC;
                 if (!x.rows || !kb) continue;
-                const uint32_t idesc = tc::operand_idesc(p.fmt, S::kFMn, S::kRMn, kBF * CG, x.n);
+                const uint32_t idesc = tc::operand_idesc(p.fmt, S::kFMn, S::kRMn, kBF * kPair, x.n);
                 uint32_t buf = 0, d_tm = 0;
                 for (int kk = 0, in_seg = 0; kk < kb; ++kk, r.next()) {
                     if (in_seg == 0) {
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                     }
                     tc::wait(b_full + 8 * r.s, r.phase, up);
                     if (MODE == kGradWeight && kk == kb - 1 && (x.c_len & 15)) {
-                        tc::wait<(CG > 1)>(b_fixed + 8 * r.s, fixed_phase >> r.s & 1u, up);
+                        tc::wait<true>(b_fixed + 8 * r.s, fixed_phase >> r.s & 1u, up);
                         fixed_phase ^= 1u << r.s;
                     }
                     tc::fence_after_sync();
@@ -347,17 +349,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
 #pragma unroll
                         for (int j = 0; j < kBC / 16; ++j)
                             if (16 * j < left)
-                                tc::pair_mma<CG, tc::kKindF16>(d_tm, df + j * (S::kFMn ? 128 : 2), dr + j * (S::kRMn ? 128 : 2), idesc,
+                                tc::mma_f16_pair(d_tm, df + j * (S::kFMn ? 128 : 2), dr + j * (S::kRMn ? 128 : 2), idesc,
                                                                (in_seg | j) != 0);
-                        tc::pair_commit<CG>(b_empty + 8 * r.s);
-                        if (kk == kb - 1 || in_seg == p.segment - 1) tc::pair_commit<CG>(b_dfull + 8 * buf);
+                        tc::pair_commit<kPair>(b_empty + 8 * r.s);
+                        if (kk == kb - 1 || in_seg == p.segment - 1) tc::pair_commit<kPair>(b_dfull + 8 * buf);
                     }
                     __syncwarp();
                     if (++in_seg == p.segment) in_seg = 0;
                 }
             }
             // nor under MMAs in flight
-            if (tc::elect_one()) tc::leader_commit<CG>(smem_u32(&last));
+            if (tc::elect_one()) tc::leader_commit<kPair>(smem_u32(&last));
             mbar_wait_bounded(&last, 0, tc::kPairWaitCycles / 8);
         }
     } else if (warp < 2 + kEpilogueWarps) {
@@ -384,10 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             auto give = [&](uint32_t buf) {
                 tc::fence_before_sync();
                 __syncwarp();
-                if (lane == 0) {
-                    if constexpr (CG == 1) tc::arrive(b_dempty + 8 * buf);
-                    else tc::arrive_at(tc::leader_addr(b_dempty + 8 * buf));
-                }
+                if (lane == 0) tc::arrive_at(tc::leader_addr(b_dempty + 8 * buf));
             };
             if (segments <= 1) {
                 const uint32_t buf = segments ? take() : 0;
@@ -434,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             if (!x.rows) continue;
             it += kb;
             if (!(x.c_len & 15)) continue;
-            const int boxes = (x.n / CG + 63) / 64, s = (it - 1) % S::kStages;
+            const int boxes = (x.n / kPair + 63) / 64, s = (it - 1) % S::kStages;
             tc::wait(b_tail + 8 * s, tail_phase >> s & 1u, up);
             tail_phase ^= 1u << s;
             // lines (one contraction row each) from `valid` up to the last multiple of 16 that the MMAs read
@@ -446,19 +445,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             }
             tc::fence_proxy_async();
             __syncwarp();
-            if (lane == 0) {
-                if constexpr (CG == 1) tc::arrive(b_fixed + 8 * s);
-                else tc::publish_at(tc::leader_addr(b_fixed + 8 * s));
-            }
+            if (lane == 0) tc::publish_at(tc::leader_addr(b_fixed + 8 * s));
         }
     }
     if (stop() && lane == 0) atomicOr(&g_product_err, 1u);
     __syncwarp();
     tc::fence_before_sync();
-    if constexpr (CG == 1) __syncthreads();
-    else tc::cluster_sync_all();  // the peer's shared and tensor memory are no longer in use
+    tc::cluster_sync_all();  // the peer's shared and tensor memory are no longer in use
     tc::fence_after_sync();
-    if (warp == 1) tc::pair_tmem_dealloc<CG>(tmem, kTmemCols);
+    if (warp == 1) tc::pair_tmem_dealloc<kPair>(tmem, kTmemCols);
 }
 
 // ---- e4m3 operands with a scale per block of 128 -------------------------------------------------
@@ -471,11 +466,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
 //
 // A tile's rows are two halves, each with accumulators (two of 128 columns), an issuing warp (1 and 3) and four promotion
 // warps of its own, so that one half's waits and tile changes run under the other's arithmetic; with both halves in
-// one accumulator the eight warps waited together, 250 of a block's 850 cycles at 128 rows, and one warp that issues for
-// both halves takes 900 cycles a block for its waits, eight MMAs and three commits.  The promotion bounds wide
-// tiles: the accumulator leaves TMEM at about 230 bytes a cycle, 256 columns in 570 cycles, their MMAs take 512.  What it
-// needs: the number of column chunks a compile-time constant (a test per chunk costs 350 cycles a block) and, at 128
-// columns, 16 columns a load (with 32 the sums spill).
+// one accumulator the eight warps waited together.  2048 x 10944 x 2048 takes 68 us, 1.47 K cycles for each of a CTA's 80
+// blocks (start and tile changes included) where the MMAs take 512 (tensor pipe 38 %).  No single part bounds it: copies that
+// left one out took 61 (MMAs), 59 (TMEM loads), 66 (scale loads), 72 (stores) and 82 us (FMAs).  At 256 rows shared
+// memory carries 112 KB a block, 875 cycles at 128 bytes a cycle, the floor of this tiling.  The promotion
+// needs the number of column chunks as a compile-time constant and, at 128 columns, 16 columns a load (with 32
+// the sums spill).
 //
 // Single CTAs, not pairs: the promotion, not the operands' traffic, bounds the tiles, and a pair's CTAs wait for one
 // another's eight warps at every block (4096 x 4 rows, 128 experts of 5760 x 2880: 553 us in pairs, 485 alone).  The warps
@@ -675,7 +671,7 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
 #pragma unroll
                         for (int j = 0; j < S::kBC8 / 32; ++j)
                             if (32 * j < left)
-                                tc::pair_mma<1, tc::kKindF8>(tmem + slot * kHalfCols, df + 2 * j, dr + 2 * j, idesc, j != 0);
+                                tc::mma_e4m3(tmem + slot * kHalfCols, df + 2 * j, dr + 2 * j, idesc, j != 0);
                         tc::pair_commit<1>(b_dfull + 8 * slot);
                     }
                     tc::pair_commit<1>(b_empty + 8 * r.s);
@@ -794,33 +790,32 @@ bool encode(CUtensorMap *m, int dtype, const void *base, int rank, uint64_t inne
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int CG, int MODE>
+template <int MODE>
 int launch(const CUtensorMap &mf, const CUtensorMap &mr, const TcParams &t, int64_t tiles_most, int sms, cudaStream_t s) {
-    auto *kernel = k_product_tc<CG, MODE>;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<CG, MODE>::kSmem) != cudaSuccess)
+    auto *kernel = k_product_tc<MODE>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE>::kSmem) != cudaSuccess)
         return -1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(CG * std::max<int64_t>(1, std::min<int64_t>(tiles_most, sms / CG))));
+    cfg.gridDim = dim3((unsigned)(kPair * std::max<int64_t>(1, std::min<int64_t>(tiles_most, sms / kPair))));
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Shape<CG, MODE>::kSmem;
+    cfg.dynamicSmemBytes = Shape<MODE>::kSmem;
     cfg.stream = s;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = CG;
+    at[0].val.clusterDim.x = kPair;
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, mf, mr, t) == cudaSuccess ? 1 : -1;
 }
 
-template <int CG>
 int launch_mode(const Product &p, const CUtensorMap &mf, const CUtensorMap &mr, const TcParams &t, int sms, cudaStream_t s) {
-    const int64_t ft = (p.features() + kBF * CG - 1) / (kBF * CG);
+    const int64_t ft = (p.features() + kBF * kPair - 1) / (kBF * kPair);
     const int64_t rt = p.mode == kGradWeight ? (int64_t)p.groups * ((p.n + kRowsMax - 1) / kRowsMax)
                                              : p.rows / kRowsMax + std::min<int64_t>(p.groups, p.rows);
-    if (p.mode == kForward) return launch<CG, kForward>(mf, mr, t, ft * rt, sms, s);
-    if (p.mode == kGradInput) return launch<CG, kGradInput>(mf, mr, t, ft * rt, sms, s);
-    return launch<CG, kGradWeight>(mf, mr, t, ft * rt, sms, s);
+    if (p.mode == kForward) return launch<kForward>(mf, mr, t, ft * rt, sms, s);
+    if (p.mode == kGradInput) return launch<kGradInput>(mf, mr, t, ft * rt, sms, s);
+    return launch<kGradWeight>(mf, mr, t, ft * rt, sms, s);
 }
 
 int launch_f8(const CUtensorMap &mf, const CUtensorMap &mr, const F8Params &fp, int sms, cudaStream_t s) {
@@ -876,8 +871,7 @@ int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
         const F8Params fp{t, p.xs, p.ws, p.xs_row, p.xs_blk, p.ws_row, p.ws_blk, p.ws_group};
         return launch_f8(mf, mr, fp, sms, s);
     }
-    // CG = 2 for wide outputs
-    return p.features() > kBF ? launch_mode<2>(p, mf, mr, t, sms, s) : launch_mode<1>(p, mf, mr, t, sms, s);
+    return launch_mode(p, mf, mr, t, sms, s);
 }
 
 uint32_t *product_err_word() {
