@@ -382,7 +382,9 @@ umsx_status umsx_moe_create_gguf(const umsx_moe_desc *desc, const char *first_sh
  * nothing between calls, synchronise nothing and can be captured into a graph.  Calls on several
  * streams or threads do not disturb one another.  Strides count elements; the last dimension of every
  * matrix is contiguous.  Bases and strides that are multiples of 16 bytes run on the tensor cores, any
- * others on a slower kernel.  An output must not overlap an input.
+ * others on a slower kernel.  An output must not overlap an input or another output: such calls are
+ * refused, and so are buffers that interleave other than as columns of one row stride or rows of one
+ * matrix stride.
  *
  * Rows are grouped by expert: rows offsets[e] .. offsets[e+1] - 1 belong to expert e (offsets: int32
  * [experts + 1], on the device, ascending; values outside 0..rows are clamped to it).  Groups may be

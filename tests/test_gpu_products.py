@@ -450,6 +450,35 @@ def test_layer_of_16_bit_weights_with_gradients():
     assert n == T * K - 1
 
 
+def test_operand_and_output_in_one_buffer():
+    """Columns of one buffer lie beside one another and are allowed; the same memory is refused, and left as it was."""
+    x, dy, w, off = _case([70, 5, 33], 0, 2, 96, 96, BF16, seed=8)
+    rows = x.shape[0]
+
+    def same(a, b):  # bit by bit: x has rows of NaN
+        return torch.equal(a.contiguous().view(torch.int16), b.contiguous().view(torch.int16))
+
+    buf = torch.zeros(rows, 192, dtype=BF16, device="cuda")
+    buf[:, :96] = x
+    want = torch.zeros_like(dy)
+    U.grouped_mm(x, w, off, out=want)
+    U.grouped_mm(buf[:, :96], w, off, out=buf[:, 96:])
+    assert same(buf[:, :96], x) and same(buf[:, 96:], want)
+    for out in (buf[:, :96], buf[:, 8:104]):
+        with pytest.raises(U.UmsxError, match="overlaps"):
+            U.grouped_mm(buf[:, :96], w, off, out=out)
+    assert same(buf[:, :96], x) and same(buf[:, 96:], want)
+
+
+def test_the_legacy_stream_by_its_number():
+    x, dy, w, off = _case([20, 3], 0, 0, 64, 64, F16, seed=9)
+    want = U.grouped_mm(x, w, off)
+    torch.cuda.synchronize()
+    got = U.grouped_mm(x, w, off, stream=0)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+
+
 def test_same_bits_twice_and_on_another_stream():
     x, dy, w, off = _case([300, 0, 41, 77], 0, 3, 256, 384, BF16, seed=6)
     xq, xs, wq, ws, _ = _fp8_case([300, 0, 41, 77], 0, 3, 256, 384, seed=6)

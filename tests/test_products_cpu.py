@@ -111,3 +111,35 @@ def test_e4m3_rounding_rule():
     mid = (grid[:-1] + grid[1:]) / 2
     near = torch.from_numpy(mid.astype(np.float32)).to(torch.float8_e4m3fn).float().numpy()
     assert np.all((near == grid[:-1]) | (near == grid[1:]))
+
+
+def _at(byte):
+    return ctypes.c_void_p(byte)
+
+
+BASE = 1 << 20
+# x [10][64], w [4][32][64], dy [10][32] and their results far from one another; what the overlapping calls move.
+FAR = {_mm: dict(x=_at(BASE), w=_at(2 * BASE), offsets=_at(3 * BASE), out=_at(4 * BASE)),
+       _dx: dict(dy=_at(BASE), w=_at(2 * BASE), offsets=_at(3 * BASE), dx=_at(4 * BASE)),
+       _dw: dict(dy=_at(BASE), x=_at(2 * BASE), offsets=_at(3 * BASE), dw=_at(4 * BASE)),
+       _fp8: dict(x=_at(BASE), xs=_at(2 * BASE), w=_at(3 * BASE), ws=_at(4 * BASE), offsets=_at(5 * BASE), out=_at(6 * BASE)),
+       _quant: dict(x=_at(BASE), q=_at(2 * BASE), scales=_at(3 * BASE)),
+       _group: dict(ids=_at(BASE), offsets=_at(2 * BASE), row_token=_at(3 * BASE), row_of_job=_at(4 * BASE))}
+
+
+@pytest.mark.parametrize("call,over", [
+    (_mm, dict(out=_at(BASE))), (_mm, dict(out=_at(BASE + 10 * 64 * 2 - 2))), (_mm, dict(out=_at(2 * BASE + 4 * 32 * 64 * 2 - 2))),
+    (_mm, dict(out=_at(BASE - 10 * 32 * 4 + 4))), (_mm, dict(out=_at(3 * BASE + 16))),
+    (_mm, dict(ldx=96, out=_at(BASE + 126), ldo=96, out_dtype=U.DTYPE_BF16)),  # columns 63.. beside columns ..63
+    (_mm, dict(ldx=96, out=_at(BASE + 128), ldo=48)),                          # equal strides in bytes, the rows are 128 wide
+    (_mm, dict(ldx=128, out=_at(BASE + 128), ldo=100, out_dtype=U.DTYPE_BF16)),
+    (_dx, dict(dx=_at(BASE))), (_dx, dict(dx=_at(2 * BASE + 64))), (_dx, dict(dx=_at(3 * BASE))),
+    (_dw, dict(dw=_at(BASE))), (_dw, dict(dw=_at(2 * BASE + 8))), (_dw, dict(dw=_at(3 * BASE + 4))),
+    (_fp8, dict(out=_at(BASE + 639))), (_fp8, dict(out=_at(2 * BASE))), (_fp8, dict(out=_at(3 * BASE))),
+    (_fp8, dict(out=_at(4 * BASE))), (_fp8, dict(out=_at(5 * BASE))),
+    (_quant, dict(q=_at(BASE))), (_quant, dict(scales=_at(BASE + 4))), (_quant, dict(scales=_at(2 * BASE + 4))),
+    (_group, dict(row_of_job=_at(BASE))), (_group, dict(row_token=_at(BASE + 28))), (_group, dict(offsets=_at(BASE))),
+    (_group, dict(row_token=_at(4 * BASE))), (_group, dict(row_of_job=_at(2 * BASE + 4)))])
+def test_overlapping_outputs_are_refused(call, over):
+    assert call(**{**FAR[call], **over}) == U.EINVAL
+    assert b"overlaps" in U.lib().umsx_last_error()

@@ -289,6 +289,11 @@ extern "C" umsx_status umsx_fp8_quantize(const void *x, int64_t ldx, int64_t x_s
         return fail(UMSX_EINVAL, "a stride is shorter than a row");
     if (matrices == 0 || rows == 0) return UMSX_OK;
     if (!x || !q || !scales) return fail(UMSX_EINVAL, "null buffer");
+    const int64_t br = (rows + block_rows - 1) / block_rows, bc = (cols + kScaleBlock - 1) / kScaleBlock;
+    const Region rx = region(x, x_dtype == UMSX_DTYPE_F32 ? 4 : 2, cols, rows, ldx, matrices, x_stride),
+                 rq = region(q, 1, cols, rows, ldq, matrices, q_stride),
+                 rs = region(scales, 4, (matrices - 1) * s_stride + (br - 1) * s_row + (bc - 1) * s_blk + 1, 1, 0);
+    if (overlap(rq, rx) || overlap(rs, rx) || overlap(rs, rq)) return fail(UMSX_EINVAL, "an output overlaps the input or the other output");
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

@@ -194,6 +194,11 @@ extern "C" umsx_status umsx_group_rows(const int32_t *ids, int tokens, int top_k
         return fail(UMSX_EINVAL, "group_rows takes tokens >= 0, top_k >= 1, experts 1..1024 and fewer than 2^31 - 16 jobs");
     if (!offsets || (tokens && (!ids || !row_token || !row_of_job))) return fail(UMSX_EINVAL, "null buffer");
     const int64_t jobs = (int64_t)tokens * top_k;
+    const Region r[4] = {region(ids, 4, jobs, 1, 0), region(offsets, 4, experts + 1, 1, 0), region(row_token, 4, jobs, 1, 0),
+                         region(row_of_job, 4, jobs, 1, 0)};
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < i; ++j)
+            if (overlap(r[i], r[j])) return fail(UMSX_EINVAL, "an output overlaps the ids or another output");
     const auto kernel = experts < 256 ? k_group_rows<8> : k_group_rows<11>;  // bits of 0..experts
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupSmemMax);
     cudaLaunchConfig_t cfg{};

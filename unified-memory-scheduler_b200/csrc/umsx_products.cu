@@ -254,7 +254,22 @@ umsx_status check_product(const Product &p) {
     return UMSX_OK;
 }
 
+// The kernels write while other CTAs still read: an output inside an operand would race.
+bool out_overlaps(const Product &p) {
+    const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2, out_size = p.out_dtype == UMSX_DTYPE_F32 ? 4 : 2;
+    const bool dw = p.mode == kGradWeight;
+    const Region out = dw ? region(p.out, out_size, p.k, p.n, p.ldo, p.groups, p.out_stride)
+                          : region(p.out, out_size, p.features(), p.rows, p.ldo);
+    const int64_t kb = (p.k + kScaleBlock - 1) / kScaleBlock, nb = (p.n + kScaleBlock - 1) / kScaleBlock;
+    return (p.rows && (overlap(out, region(p.x, size, p.k, p.rows, p.ldx)) || overlap(out, region(p.dy, size, p.n, p.rows, p.lddy)) ||
+                       overlap(out, region(p.xs, 4, (p.rows - 1) * p.xs_row + (kb - 1) * p.xs_blk + 1, 1, 0)))) ||
+           overlap(out, region(p.w, size, p.k, p.n, p.ldw, p.groups, p.w_stride)) ||
+           overlap(out, region(p.ws, 4, (p.groups - 1) * p.ws_group + (nb - 1) * p.ws_row + (kb - 1) * p.ws_blk + 1, 1, 0)) ||
+           overlap(out, region(p.offsets, 4, p.groups + 1, 1, 0));
+}
+
 umsx_status run_product(const Product &p, umsx_stream stream) {
+    if (out_overlaps(p)) return fail(UMSX_EINVAL, "the output overlaps an input");
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

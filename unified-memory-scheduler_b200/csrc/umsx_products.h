@@ -38,6 +38,33 @@ struct Product {
     int features() const { return mode == kForward ? n : k; }
 };
 
+// Where a tensor lies: `blocks` blocks, `block` bytes apart, of `lines` lines of `width` bytes, `line` bytes apart.
+struct Region {
+    const void *base;
+    int64_t width, lines, line, blocks, block;
+    int64_t extent() const { return (blocks - 1) * block + (lines - 1) * line + width; }
+};
+// A matrix or a stack of them, strides in elements of `size` bytes.
+inline Region region(const void *base, int size, int64_t width, int64_t lines, int64_t line, int64_t blocks = 1, int64_t block = 0) {
+    return {base, width * size, lines, lines > 1 ? line * size : 0, blocks, blocks > 1 ? block * size : 0};
+}
+// Whether the two may share a byte.  Slices of one buffer that lie beside one another share none although their ranges
+// do: columns of equal line stride, or lines of equal block stride.
+inline bool overlap(const Region &a, const Region &b) {
+    if (!a.base || !b.base || a.extent() <= 0 || b.extent() <= 0) return false;
+    const int64_t at = (int64_t)((uintptr_t)b.base - (uintptr_t)a.base);
+    if (at >= a.extent() || -at >= b.extent()) return false;
+    const auto beside = [at](int64_t period, int64_t wa, int64_t wb) {
+        if (period <= 0) return false;
+        const int64_t r = (at % period + period) % period;
+        return r >= wa && r + wb <= period;
+    };
+    const auto whole = [](const Region &x, int64_t period) { return x.blocks == 1 || x.block % period == 0; };
+    if (a.line == b.line && a.line > 0 && whole(a, a.line) && whole(b, a.line) && beside(a.line, a.width, b.width)) return false;
+    const int64_t ba = (a.lines - 1) * a.line + a.width, bb = (b.lines - 1) * b.line + b.width;
+    return !(a.block == b.block && beside(a.block, ba, bb));
+}
+
 #ifdef __CUDACC__
 // First row of group g, and for g = groups the row behind the last one.  Offsets are clamped to the matrix, so that wrong
 // ones cannot lead outside it; a group whose end lies before its start is empty.

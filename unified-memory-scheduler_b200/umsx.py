@@ -377,7 +377,8 @@ def group_rows(ids, experts: int, stream=None):
 def grouped_mm(x, w, offsets, out=None, out_dtype=None, stream=None):
     """out[r] = x[r] @ w[e].T for the rows r of every expert e (umsx_grouped_mm): x [rows, k] and w
     [experts, n, k] both bfloat16 or both float16, offsets int32 [experts + 1]; out [rows, n] float32,
-    bfloat16 or float16 (default: x's type).  Rows outside the groups are not written."""
+    bfloat16 or float16 (default: x's type).  Rows outside the groups are not written.  As in its gradients and the
+    e4m3 products, an `out` that overlaps an operand is refused."""
     _torch()
     code = _matrix("x", x, 2, _SIXTEEN)
     _matrix("w", w, 3, (code,), x)
