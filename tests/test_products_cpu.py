@@ -143,3 +143,14 @@ FAR = {_mm: dict(x=_at(BASE), w=_at(2 * BASE), offsets=_at(3 * BASE), out=_at(4 
 def test_overlapping_outputs_are_refused(call, over):
     assert call(**{**FAR[call], **over}) == U.EINVAL
     assert b"overlaps" in U.lib().umsx_last_error()
+
+
+@pytest.mark.parametrize("call,over", [
+    (_mm, dict(x=_at(BASE + 1))), (_mm, dict(w=_at(2 * BASE + 1))), (_mm, dict(out=_at(4 * BASE + 2))),
+    (_mm, dict(offsets=_at(3 * BASE + 2))), (_dx, dict(dy=_at(BASE + 1))), (_dx, dict(dx=_at(4 * BASE + 1))),
+    (_dw, dict(x=_at(2 * BASE + 1))), (_dw, dict(dw=_at(4 * BASE + 2))), (_fp8, dict(xs=_at(2 * BASE + 2))),
+    (_fp8, dict(ws=_at(4 * BASE + 1))), (_fp8, dict(out=_at(6 * BASE + 1))), (_quant, dict(x=_at(BASE + 1))),
+    (_quant, dict(scales=_at(3 * BASE + 2))), (_group, dict(ids=_at(BASE + 2))), (_group, dict(row_token=_at(3 * BASE + 1)))])
+def test_buffers_between_elements_are_refused(call, over):
+    assert call(**{**FAR[call], **over}) == U.EINVAL
+    assert b"aligned" in U.lib().umsx_last_error()

@@ -294,6 +294,8 @@ extern "C" umsx_status umsx_fp8_quantize(const void *x, int64_t ldx, int64_t x_s
                  rq = region(q, 1, cols, rows, ldq, matrices, q_stride),
                  rs = region(scales, 4, (matrices - 1) * s_stride + (br - 1) * s_row + (bc - 1) * s_blk + 1, 1, 0);
     if (overlap(rq, rx) || overlap(rs, rx) || overlap(rs, rq)) return fail(UMSX_EINVAL, "an output overlaps the input or the other output");
+    if (reinterpret_cast<uintptr_t>(x) % (x_dtype == UMSX_DTYPE_F32 ? 4 : 2) || reinterpret_cast<uintptr_t>(scales) % 4)
+        return fail(UMSX_EINVAL, "a buffer is not aligned to its elements");
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);

@@ -199,6 +199,9 @@ extern "C" umsx_status umsx_group_rows(const int32_t *ids, int tokens, int top_k
     for (int i = 0; i < 4; ++i)
         for (int j = 0; j < i; ++j)
             if (overlap(r[i], r[j])) return fail(UMSX_EINVAL, "an output overlaps the ids or another output");
+    for (const void *q : {static_cast<const void *>(ids), static_cast<const void *>(offsets), static_cast<const void *>(row_token),
+                          static_cast<const void *>(row_of_job)})
+        if (reinterpret_cast<uintptr_t>(q) % 4) return fail(UMSX_EINVAL, "a buffer is not aligned to its elements");
     const auto kernel = experts < 256 ? k_group_rows<8> : k_group_rows<11>;  // bits of 0..experts
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kGroupSmemMax);
     cudaLaunchConfig_t cfg{};

@@ -24,67 +24,152 @@ umsx_status fail(umsx_status s, const std::string &msg) {
 //
 // out[r][f] = sum_c R[r][c] F[f][c] for every stride and alignment: what the tcgen05 kernel cannot address, since TMA wants
 // bases and row strides that are multiples of 16 bytes (odd widths, slices that start anywhere).  Tiles of 64 rows x 128
-// features, 32 of the contraction a step: single-element loads, neighbouring lanes along the axis that is contiguous in
-// memory, one step ahead in registers; from shared memory into mma.sync.  e4m3 codes become f16 (exact); the sums of
-// a block of 128 are scaled once and added in fp32.  Bound by the issue of those loads (bf16 4096 x 4096 x 2049: 573 us,
-// 120 TFLOP/s; fp32 FMAs in place of mma.sync took 3441 us, 64-bit addresses per element instead of a step per thread 1295).
+// features; a step takes 128 bytes of every line, as it lies in memory (along c, or along the rows or features for the
+// gradients), one step ahead in registers.  A lane loads the aligned word that holds its first byte and shifts its four out of
+// that and the next lane's; a line's alignment is the same in every step.  From shared memory into mma.sync, by ldmatrix
+// with or without a transposition.  e4m3 codes become f16 (exact); a step is a block of 128, scaled once and added in fp32.
+// The sums go through shared memory, so that a warp stores 32 neighbours.
+// Bound by the latency of a step where there are few tiles (e4m3 511 x 308 x 1323: 24 tiles, 37 us; with steps of 32 values
+// 80), by issue where there are many: bf16 4096 x 4096 x 2049 takes 481 us forward (143 TFLOP/s), 522 for dx, 514 for dw, e4m3
+// 446; with single-element loads 573, 784, 891 and 1116, and with a test in front of every load and shift 778 forward.
 
-constexpr int kAnyRows = 64, kAnyF = 128, kStep = 32, kLine = kStep + 8;  // kLine: 80 bytes spread eight lines over all banks
+constexpr int kAnyRows = 64, kAnyF = 128, kLineBytes = 128, kAnyWarps = 8;
+constexpr int kSumLine = kAnyF + 4;
+
+template <int DTYPE>
+struct AnyShape {
+    static constexpr int kSize = DTYPE == UMSX_DTYPE_E4M3 ? 1 : 2;
+    static constexpr int kC = kLineBytes / kSize;  // contraction a step
+    static_assert(kSize == 2 || kC == kScaleBlock, "a step of e4m3 codes is a block");
+    static constexpr int kLine = kC + 8;           // 16-bit values from line to line: eight lines spread over all banks
+    static constexpr int kOperands = (kAnyRows + kAnyF) * kLine * 2, kSums = kAnyRows * kSumLine * 4;
+    static constexpr int kSmem = kOperands > kSums ? kOperands : kSums;
+};
 
 struct AnyParams {
-    int out_dtype, groups, mode;
+    int out_dtype, groups;
     int64_t rows;
     int features, contraction;  // contraction: forward k, dx n (dw: the group's rows)
     int out_rows;               // dw: n
     const int32_t *offsets;
-    const void *R, *F;
-    int64_t r_row, r_c, f_feat, f_c, f_group;  // element strides
+    const uint8_t *R, *F, *R_end, *F_end;  // first byte, and behind the last
+    int64_t r_pitch, f_pitch, f_group;     // bytes: between lines in memory, F's from group to group
     const float *rs, *fs;
     int64_t rs_row, rs_blk, fs_row, fs_blk, fs_group;
     void *out;
     int64_t ldo, out_group;
 };
 
-// LINES x kStep elements of an operand, held by 256 threads between their load and their store: element i of a thread.
-template <int DTYPE, int LINES>
-struct Elements {
-    static constexpr int kPer = LINES * kStep / 256;
-    uint16_t v[kPer];
+// The bytes of an aligned word that lie in [begin, end).
+__device__ __noinline__ uint32_t edge_word(const uint8_t *at, const uint8_t *begin, const uint8_t *end) {
+    uint32_t v = 0;
+    for (int i = 0; i < 4; ++i)
+        if (at + i >= begin && at + i < end) v |= (uint32_t)__ldg(at + i) << 8 * i;
+    return v;
+}
 
-    // Neighbouring threads lie along c where that is contiguous, along the lines otherwise; a thread's next element is a fixed
-    // step further in memory either way.
-    __device__ __forceinline__ void load(const void *p, int64_t s_line, int64_t s_c, int lines, int steps) {
-        constexpr int kSize = DTYPE == UMSX_DTYPE_E4M3 ? 1 : 2;
-        const bool along_c = s_c == 1;
-        const int l = along_c ? threadIdx.x / kStep : threadIdx.x % LINES, c = along_c ? threadIdx.x % kStep : threadIdx.x / LINES;
-        const int64_t by = (along_c ? 256 / kStep * s_line : 256 / LINES * s_c) * kSize;
-        const uint8_t *at = static_cast<const uint8_t *>(p) + (l * s_line + c * s_c) * kSize;
-        // elements of this thread that lie inside: the other coordinate is fixed
-        const int in = along_c ? (c < steps ? (lines - l + 256 / kStep - 1) / (256 / kStep) : 0)
-                               : (l < lines ? (steps - c + 256 / LINES - 1) / (256 / LINES) : 0);
+// One step of an operand of LINES rows or features, held by 256 threads between its load and its store.  ALONG: lines in memory
+// run along the contraction, LINES of them; otherwise along the rows or features, 64 of them in LINES / 64 parts of 128 bytes.
+// Warp w takes lines w, w + 8, ..., lane j their word j; lane i also the word behind the i-th.
+template <bool ALONG, int LINES>
+struct Words {
+    static constexpr int kPer = LINES / kAnyWarps, kParts = ALONG ? 1 : LINES / 64;
+    uint32_t w[kPer], behind;
+    int bytes;  // of a line that are inside
+
+    __device__ __forceinline__ void load(const uint8_t *p, int64_t pitch, int lines, int line_bytes, const uint8_t *begin,
+                                         const uint8_t *end) {
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        bytes = line_bytes;
+        if (lines <= 0 || line_bytes <= 0) lines = 0;
+        const uint8_t *line = p + warp * pitch;
+        const int skew = (int)(reinterpret_cast<uintptr_t>(line) & 3);
+        const uint8_t *at = line - skew + 4 * lane;
+        const int i_b = lane / kParts, part_b = lane % kParts;
+        const uint8_t *at_b = line - skew + kLineBytes + (int64_t)i_b * kAnyWarps * pitch + part_b * kLineBytes;
+        const bool in_b = skew && lane < kPer && warp + kAnyWarps * i_b < lines &&
+                          kLineBytes - skew < min(kLineBytes, bytes - part_b * kLineBytes);
+        // words may reach over the operand's first or last byte in the tiles there
+        const uint8_t *low = p - (reinterpret_cast<uintptr_t>(p) & 3);
+        const uint8_t *high = p + (lines - 1) * pitch + bytes;
+        high += -reinterpret_cast<uintptr_t>(high) & 3;
+        const bool inside = low >= begin && high <= end;
+        if (inside && lines >= (ALONG ? LINES : 64) && bytes >= kParts * kLineBytes) {  // no test in front of any load
+            const uint8_t *q = at;
+            const int64_t down = kAnyWarps * pitch;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i, at += by) {
-            if constexpr (kSize == 1) v[i] = i < in ? __ldg(at) : 0;
-            else v[i] = i < in ? __ldg(reinterpret_cast<const unsigned short *>(at)) : 0;
+            for (int i = 0; i < kPer; ++i) {
+                w[i] = __ldg(reinterpret_cast<const uint32_t *>(q + i % kParts * kLineBytes));
+                if ((i + 1) % kParts == 0) q += down;
+            }
+            behind = in_b ? __ldg(reinterpret_cast<const uint32_t *>(at_b)) : 0;
+            return;
         }
-    }
-    __device__ __forceinline__ void store(uint16_t *to, bool along_c) const {
-        const int l = along_c ? threadIdx.x / kStep : threadIdx.x % LINES, c = along_c ? threadIdx.x % kStep : threadIdx.x / LINES;
-        uint16_t *at = to + l * kLine + c;
-        const int by = along_c ? 256 / kStep * kLine : 256 / LINES;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
-            uint16_t h = v[i];
-            if constexpr (DTYPE == UMSX_DTYPE_E4M3) h = __nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)h, __NV_E4M3).x;
-            at[i * by] = h;
+            const int part = i % kParts, l = warp + kAnyWarps * (i / kParts);
+            const bool in = l < lines && 4 * lane - skew < min(kLineBytes, bytes - part * kLineBytes);
+            const uint8_t *q = at + (int64_t)(i / kParts) * kAnyWarps * pitch + part * kLineBytes;
+            w[i] = in && inside ? __ldg(reinterpret_cast<const uint32_t *>(q)) : 0;
+        }
+        behind = in_b && inside ? __ldg(reinterpret_cast<const uint32_t *>(at_b)) : 0;
+        if (inside) return;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int part = i % kParts, l = warp + kAnyWarps * (i / kParts);
+            const bool in = l < lines && 4 * lane - skew < min(kLineBytes, bytes - part * kLineBytes);
+            if (in) w[i] = edge_word(at + (int64_t)(i / kParts) * kAnyWarps * pitch + part * kLineBytes, begin, end);
+        }
+        if (in_b) behind = edge_word(at_b, begin, end);
+    }
+
+    // To lines of `kLine` 16-bit values (not ALONG: part after part); zero behind the end, where a NaN may lie.
+    template <int DTYPE>
+    __device__ __forceinline__ void store(uint16_t *to, const uint8_t *p, int64_t pitch) const {
+        constexpr int kLine = AnyShape<DTYPE>::kLine;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        const int skew = (int)(reinterpret_cast<uintptr_t>(p + warp * pitch) & 3);
+        uint32_t mask[kParts];
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+            const int left = bytes - part * kLineBytes - 4 * lane;
+            mask[part] = left >= 4 ? ~0u : left > 0 ? (1u << 8 * left) - 1u : 0u;
+        }
+        uint16_t *d = to + warp * kLine + (DTYPE == UMSX_DTYPE_E4M3 ? 4 : 2) * lane;
+        const auto put = [&](int i, uint32_t v) {
+            uint16_t *at = d + (i % kParts * 64 + kAnyWarps * (i / kParts)) * kLine;
+            v &= mask[i % kParts];
+            if constexpr (DTYPE == UMSX_DTYPE_E4M3) {
+                const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v & 0xffffu), __NV_E4M3),
+                                  hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(v >> 16), __NV_E4M3);
+                *reinterpret_cast<uint2 *>(at) = make_uint2(lo.x | (uint32_t)lo.y << 16, hi.x | (uint32_t)hi.y << 16);
+            } else {
+                *reinterpret_cast<uint32_t *>(at) = v;
+            }
+        };
+        if (skew) {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const uint32_t next = __shfl_down_sync(kFull, w[i], 1), last = __shfl_sync(kFull, behind, i);
+                put(i, __funnelshift_r(w[i], lane == 31 ? last : next, 8 * skew));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) put(i, w[i]);
         }
     }
 };
 
+template <bool TRANS>
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], const uint16_t *p) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-                 : "r"(smem_u32(p)));
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(smem_u32(p)));
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(smem_u32(p)));
 }
 
 template <bool BF16>
@@ -107,19 +192,22 @@ __device__ __forceinline__ void store_el(void *p, int64_t i, int dtype, float v)
     else static_cast<__half *>(p)[i] = __float2half_rn(v);
 }
 
-template <int DTYPE>
-__global__ void __launch_bounds__(256, 2) k_product_any(const AnyParams p) {
-    constexpr bool kF8 = DTYPE == UMSX_DTYPE_E4M3;
-    constexpr int kSize = kF8 ? 1 : 2;
-    __shared__ __align__(16) uint16_t sR[kAnyRows * kLine], sF[kAnyF * kLine];
+template <int DTYPE, int MODE>
+__global__ void __launch_bounds__(32 * kAnyWarps, 2) k_product_any(const AnyParams p) {
+    using S = AnyShape<DTYPE>;
+    constexpr bool kF8 = DTYPE == UMSX_DTYPE_E4M3, dw = MODE == kGradWeight;
+    constexpr bool kRAlong = !dw, kFAlong = MODE == kForward;
+    constexpr int kSize = S::kSize, kC = S::kC, kLine = S::kLine;
+    extern __shared__ __align__(16) uint8_t any_smem[];
+    uint16_t *sR = reinterpret_cast<uint16_t *>(any_smem), *sF = sR + kAnyRows * kLine;
+    float *sums = reinterpret_cast<float *>(any_smem);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, f0 = blockIdx.x * kAnyF;
     const int wr = (warp & 1) * 32, wf = (warp >> 1) * 32;  // the warp's 32 x 32 of the tile
-    const bool r_along = p.r_c == 1, f_along = p.f_c == 1;
     // row tiles of all groups in order; this CTA takes every gridDim.y-th
     for (int t = blockIdx.y;; t += gridDim.y) {
         __syncthreads();
         int g = 0, tile = 0;
-        if (p.mode == kGradWeight) {
+        if (dw) {
             const int each = (p.out_rows + kAnyRows - 1) / kAnyRows;
             g = t / each;
             tile = t % each;
@@ -129,41 +217,53 @@ __global__ void __launch_bounds__(256, 2) k_product_any(const AnyParams p) {
         }
         int a, b;
         group_bounds(p.offsets, g, p.rows, a, b);
-        const bool dw = p.mode == kGradWeight;
         const int r0 = tile * kAnyRows, nr = min(kAnyRows, (dw ? p.out_rows : b - a) - r0), nf = min(kAnyF, p.features - f0);
         const int nc = dw ? b - a : p.contraction;
-        const uint8_t *R = static_cast<const uint8_t *>(p.R) + (a * (dw ? p.r_c : p.r_row) + r0 * p.r_row) * kSize;
-        const uint8_t *F = static_cast<const uint8_t *>(p.F) + (dw ? a * p.f_c : g * p.f_group) * kSize + f0 * p.f_feat * kSize;
-        Elements<DTYPE, kAnyRows> er;
-        Elements<DTYPE, kAnyF> ef;
-        er.load(R, p.r_row, p.r_c, nr, nc);
-        ef.load(F, p.f_feat, p.f_c, nf, nc);
-        float acc[2][4][4] = {}, blk[2][4][4] = {};  // [16 rows][8 features]; blk: e4m3, of the present block of 128
-        for (int c0 = 0; c0 < nc; c0 += kStep) {
+        // the tile's first line, and from step to step
+        const uint8_t *R = p.R + (dw ? a * p.r_pitch + (int64_t)r0 * kSize : (int64_t)(a + r0) * p.r_pitch);
+        const uint8_t *F = p.F + g * p.f_group + (kFAlong ? f0 * p.f_pitch : (int64_t)f0 * kSize + (dw ? a * p.f_pitch : 0));
+        const int64_t r_step = kRAlong ? kLineBytes : kC * p.r_pitch, f_step = kFAlong ? kLineBytes : kC * p.f_pitch;
+        Words<kRAlong, kAnyRows> er;
+        Words<kFAlong, kAnyF> ef;
+        const auto load = [&](int c0) {
+            const int left = min(kC, nc - c0);
+            const uint8_t *r = R + c0 / kC * r_step, *f = F + c0 / kC * f_step;
+            er.load(r, p.r_pitch, kRAlong ? nr : left, (kRAlong ? left : nr) * kSize, p.R, p.R_end);
+            ef.load(f, p.f_pitch, kFAlong ? nf : left, (kFAlong ? left : nf) * kSize, p.F, p.F_end);
+        };
+        if (nc > 0) load(0);
+        float acc[2][4][4] = {};  // [16 rows][8 features]
+        for (int c0 = 0; c0 < nc; c0 += kC) {
             __syncthreads();  // the previous step has been read
-            er.store(sR, r_along);
-            ef.store(sF, f_along);
+            er.template store<DTYPE>(sR, R, p.r_pitch);
+            ef.template store<DTYPE>(sF, F, p.f_pitch);
             __syncthreads();
-            if (c0 + kStep < nc) {
-                er.load(R + (c0 + kStep) * p.r_c * kSize, p.r_row, p.r_c, nr, nc - c0 - kStep);
-                ef.load(F + (c0 + kStep) * p.f_c * kSize, p.f_feat, p.f_c, nf, nc - c0 - kStep);
-            }
+            const int left = nc - c0;
+            if (c0 + kC < nc) load(c0 + kC);
+            float blk[2][4][4] = {};  // e4m3: of this block
 #pragma unroll
-            for (int k = 0; k < kStep; k += 16) {
+            for (int k = 0; k < kC; k += 16) {
+                if (k >= left) break;
                 uint32_t x[2][4], y[2][4];
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     // rows x contraction: 8 x 8 matrices (0, 0), (8, 0), (0, 8), (8, 8); features: (0, 0), (0, 8), (8, 0), (8, 8)
-                    ldmatrix4(x[i], sR + (wr + 16 * i + (lane & 15)) * kLine + k + 8 * (lane >> 4));
-                    ldmatrix4(y[i], sF + (wf + 16 * i + (lane & 7) + 8 * (lane >> 4)) * kLine + k + 8 * ((lane >> 3) & 1));
+                    const int r = wr + 16 * i, f = wf + 16 * i;
+                    if constexpr (kRAlong) ldmatrix4<false>(x[i], sR + (r + (lane & 15)) * kLine + k + 8 * (lane >> 4));
+                    else ldmatrix4<true>(x[i], sR + (k + (lane & 7) + 8 * (lane >> 4)) * kLine + r + 8 * ((lane >> 3) & 1));
+                    if constexpr (kFAlong)
+                        ldmatrix4<false>(y[i], sF + (f + (lane & 7) + 8 * (lane >> 4)) * kLine + k + 8 * ((lane >> 3) & 1));
+                    else
+                        ldmatrix4<true>(y[i], sF + ((f & 64) + k + (lane & 7) + 8 * ((lane >> 3) & 1)) * kLine + (f & 63) + 8 * (lane >> 4));
                 }
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        mma16816<DTYPE == UMSX_DTYPE_BF16>(kF8 ? blk[i][j] : acc[i][j], x[i], y[j >> 1][2 * (j & 1)], y[j >> 1][2 * (j & 1) + 1]);
+                        mma16816<DTYPE == UMSX_DTYPE_BF16>(kF8 ? blk[i][j] : acc[i][j], x[i], y[j >> 1][2 * (j & 1)],
+                                                           y[j >> 1][2 * (j & 1) + 1]);
             }
-            if (kF8 && (c0 % kScaleBlock == kScaleBlock - kStep || c0 + kStep >= nc)) {
+            if constexpr (kF8) {
                 const int cb = c0 / kScaleBlock;
                 const float w = __ldg(p.fs + g * p.fs_group + (int64_t)(f0 / kScaleBlock) * p.fs_row + cb * p.fs_blk);
 #pragma unroll
@@ -175,38 +275,52 @@ __global__ void __launch_bounds__(256, 2) k_product_any(const AnyParams p) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
 #pragma unroll
-                            for (int q = 0; q < 2; ++q) {
+                            for (int q = 0; q < 2; ++q)
                                 acc[i][j][2 * h + q] = fmaf(sc, blk[i][j][2 * h + q], acc[i][j][2 * h + q]);
-                                blk[i][j][2 * h + q] = 0.0f;
-                            }
                     }
             }
         }
+        __syncthreads();  // the operands have been read
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int r = wr + 16 * i + 8 * h + (lane >> 2);
-                if (r >= nr) continue;
-                const int64_t at = (dw ? g * p.out_group + (int64_t)(r0 + r) * p.ldo : (int64_t)(a + r0 + r) * p.ldo) + f0;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
+                    *reinterpret_cast<float2 *>(sums + (wr + 16 * i + 8 * h + (lane >> 2)) * kSumLine + wf + 8 * j + 2 * (lane & 3)) =
+                        make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
+        __syncthreads();
+        for (int r = warp; r < nr; r += kAnyWarps) {
+            const int64_t at = (dw ? g * p.out_group + (int64_t)(r0 + r) * p.ldo : (int64_t)(a + r0 + r) * p.ldo) + f0;
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int f = wf + 8 * j + 2 * (lane & 3) + q;
-                        if (f < nf) store_el(p.out, at + f, p.out_dtype, acc[i][j][2 * h + q]);
-                    }
-            }
+            for (int f = lane; f < kAnyF; f += 32)
+                if (f < nf) store_el(p.out, at + f, p.out_dtype, sums[r * kSumLine + f]);
+        }
     }
+}
+
+template <int DTYPE, int MODE>
+int launch_any(const AnyParams &a, dim3 grid, cudaStream_t s) {
+    auto *kernel = k_product_any<DTYPE, MODE>;
+    constexpr int kSmem = AnyShape<DTYPE>::kSmem;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess) return -1;
+    kernel<<<grid, 32 * kAnyWarps, kSmem, s>>>(a);
+    return 1;
+}
+template <int DTYPE>
+int launch_any(const AnyParams &a, ProductMode mode, dim3 grid, cudaStream_t s) {
+    if (mode == kForward) return launch_any<DTYPE, kForward>(a, grid, s);
+    return mode == kGradInput ? launch_any<DTYPE, kGradInput>(a, grid, s) : launch_any<DTYPE, kGradWeight>(a, grid, s);
 }
 
 }  // namespace
 
 int launch_product_any(const Product &p, int sms, cudaStream_t s) {
+    const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2;
+    const auto bytes = [](const void *q) { return static_cast<const uint8_t *>(q); };
     AnyParams a{};
     a.out_dtype = p.out_dtype;
     a.groups = p.groups;
-    a.mode = p.mode;
     a.rows = p.rows;
     a.offsets = p.offsets;
     a.features = p.features();
@@ -222,23 +336,20 @@ int launch_product_any(const Product &p, int sms, cudaStream_t s) {
     a.fs_row = p.ws_row;
     a.fs_blk = p.ws_blk;
     a.fs_group = p.ws_group;
-    if (p.mode == kForward) {
-        a.R = p.x, a.r_row = p.ldx, a.r_c = 1;
-        a.F = p.w, a.f_feat = p.ldw, a.f_c = 1, a.f_group = p.w_stride;
-    } else if (p.mode == kGradInput) {
-        a.R = p.dy, a.r_row = p.lddy, a.r_c = 1;
-        a.F = p.w, a.f_feat = 1, a.f_c = p.ldw, a.f_group = p.w_stride;
-    } else {
-        a.R = p.dy, a.r_row = 1, a.r_c = p.lddy;
-        a.F = p.x, a.f_feat = 1, a.f_c = p.ldx;
-    }
-    const int64_t tiles = p.mode == kGradWeight ? (int64_t)p.groups * ((p.n + kAnyRows - 1) / kAnyRows)
-                                                : p.rows / kAnyRows + std::min<int64_t>(p.groups, p.rows);
+    const bool fwd = p.mode == kForward, dw = p.mode == kGradWeight;
+    a.R = bytes(fwd ? p.x : p.dy);
+    a.r_pitch = (fwd ? p.ldx : p.lddy) * size;
+    a.R_end = a.R + (p.rows - 1) * a.r_pitch + (int64_t)(fwd ? p.k : p.n) * size;
+    a.F = bytes(dw ? p.x : p.w);
+    a.f_pitch = (dw ? p.ldx : p.ldw) * size;
+    a.f_group = dw ? 0 : p.groups > 1 ? p.w_stride * size : 0;
+    a.F_end = a.F + (p.groups - 1) * a.f_group + ((dw ? p.rows : p.n) - 1) * a.f_pitch + (int64_t)p.k * size;
+    const int64_t tiles = dw ? (int64_t)p.groups * ((p.n + kAnyRows - 1) / kAnyRows)
+                             : p.rows / kAnyRows + std::min<int64_t>(p.groups, p.rows);
     const dim3 grid((unsigned)((a.features + kAnyF - 1) / kAnyF), (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, 32 * sms)));
-    if (p.dtype == UMSX_DTYPE_BF16) k_product_any<UMSX_DTYPE_BF16><<<grid, 256, 0, s>>>(a);
-    else if (p.dtype == UMSX_DTYPE_F16) k_product_any<UMSX_DTYPE_F16><<<grid, 256, 0, s>>>(a);
-    else k_product_any<UMSX_DTYPE_E4M3><<<grid, 256, 0, s>>>(a);
-    return 1;
+    if (p.dtype == UMSX_DTYPE_BF16) return launch_any<UMSX_DTYPE_BF16>(a, p.mode, grid, s);
+    if (p.dtype == UMSX_DTYPE_F16) return launch_any<UMSX_DTYPE_F16>(a, p.mode, grid, s);
+    return launch_any<UMSX_DTYPE_E4M3, kForward>(a, grid, s);
 }
 
 namespace {
@@ -268,8 +379,14 @@ bool out_overlaps(const Product &p) {
            overlap(out, region(p.offsets, 4, p.groups + 1, 1, 0));
 }
 
+bool misaligned(const void *p, int size) { return reinterpret_cast<uintptr_t>(p) % size; }
+
 umsx_status run_product(const Product &p, umsx_stream stream) {
     if (out_overlaps(p)) return fail(UMSX_EINVAL, "the output overlaps an input");
+    const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2, out_size = p.out_dtype == UMSX_DTYPE_F32 ? 4 : 2;
+    if (misaligned(p.x, size) || misaligned(p.dy, size) || misaligned(p.w, size) || misaligned(p.out, out_size) ||
+        misaligned(p.xs, 4) || misaligned(p.ws, 4) || misaligned(p.offsets, 4))
+        return fail(UMSX_EINVAL, "a buffer is not aligned to its elements");
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
