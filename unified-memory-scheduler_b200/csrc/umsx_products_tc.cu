@@ -175,7 +175,11 @@ __device__ __forceinline__ void stage16(uint8_t *to, int lane, const uint32_t (&
     }
 }
 
-// Rows c0 .. c0 + 15 of the tile from v (fragment order), through the warp's staging of 16 rows.
+// Rows c0 .. c0 + 15 of the tile from v (fragment order), through the warp's staging of 16 rows.  RUNS: where 16-byte
+// stores cannot be used, a store of 32 neighbours for each row, not eight elements of a row by each lane (bf16 5759 x 2880, 32
+// experts of 512 rows: 365 us, 600; e4m3 346, 668).  Not for dw, whose width is odd only where an operand is too, unless that
+// is padded: the code's registers cost its fp32 outputs 5 %.
+template <bool RUNS>
 __device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, int lane, int c0, const uint32_t (&v)[16]) {
     if (o.dtype == UMSX_DTYPE_F32) {
         float *p = static_cast<float *>(o.out) + o.at + (int64_t)(c0 + 2 * (lane & 3)) * o.ldo + (lane >> 2);
@@ -196,13 +200,23 @@ __device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, in
     else stage16<false>(stage, lane, v);
     __syncwarp();
     uint16_t *p = static_cast<uint16_t *>(o.out) + o.at;
+    if (RUNS && !o.vec) {
+        const int rows = min(16, o.rows - c0);
+        if (lane < o.features) {
+            p += (int64_t)c0 * o.ldo + lane;
+#pragma unroll
+            for (int r = 0; r < 16; ++r, p += o.ldo)
+                if (r < rows) *p = *reinterpret_cast<const uint16_t *>(stage + r * kStageRow + lane * 2);
+        }
+        return;
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int row = 8 * i + (lane >> 2), f = 8 * (lane & 3);
         if (c0 + row >= o.rows || f >= o.features) continue;
         const uint4 w = *reinterpret_cast<const uint4 *>(stage + row * kStageRow + f * 2);
         uint16_t *d = p + (int64_t)(c0 + row) * o.ldo + f;
-        if (o.vec && f + 8 <= o.features) {
+        if ((RUNS || o.vec) && f + 8 <= o.features) {
             *reinterpret_cast<uint4 *>(d) = w;
         } else {
             const uint16_t *h = reinterpret_cast<const uint16_t *>(&w);
@@ -393,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                 for (int c0 = part * 16; c0 < x.rows; c0 += 32) {
                     uint32_t v[16] = {};  // an expert without rows: dw is zero
                     if (segments) tc::tmem_ld_frag(lanes + buf * kRowsMax + c0, v);
-                    store_chunk(o, stage, lane, c0, v);
+                    store_chunk<MODE != kGradWeight>(o, stage, lane, c0, v);
                 }
                 if (segments) give(buf);
                 continue;
@@ -421,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                     uint32_t v[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(acc[c][j]);
-                    store_chunk(o, stage, lane, 32 * c + part * 16, v);
+                    store_chunk<MODE != kGradWeight>(o, stage, lane, 32 * c + part * 16, v);
                 }
         }
     } else if (MODE == kGradWeight) {
@@ -565,7 +579,7 @@ __device__ __forceinline__ void promote_half(const F8Sync &y, uint32_t &it, cons
             v[2 * i] = (uint32_t)acc[h][i];
             v[2 * i + 1] = (uint32_t)(acc[h][i] >> 32);
         }
-        store_chunk(o, y.stage, lane, half.at + 16 * h, v);
+        store_chunk<true>(o, y.stage, lane, half.at + 16 * h, v);
     }
 }
 
