@@ -450,6 +450,45 @@ def test_layer_of_16_bit_weights_with_gradients():
     assert n == T * K - 1
 
 
+# Either side of what decides between the kernels: 1024 rows, 2^17 outputs (features in steps of 16), 4 and 8 rows an expert,
+# 16-byte strides; long contractions of few tiles.
+@pytest.mark.parametrize("counts,n,k", [([1024], 128, 64), ([1025], 128, 64), ([512], 256, 96), ([513], 256, 96), ([511], 241, 96),
+                                        ([57], 640, 4096), ([4] * 9, 48, 160), ([5] * 9, 48, 160), ([8, 9, 0, 7], 512, 2080),
+                                        ([9, 9, 0, 9], 512, 2080), ([300, 0, 3], 136, 1040), ([7, 500], 17, 1041)])
+@pytest.mark.parametrize("out", [BF16, F32])
+def test_around_the_choice_of_kernel(counts, n, k, out):
+    _check_all(counts, 2, 3, n, k, BF16, out, seed=n + k)
+    x, xs, w, ws, off = _fp8_case(counts, 2, 3, n, k, seed=n + k)
+    y = torch.full((x.shape[0], n), 5.0, dtype=out, device="cuda")
+    U.fp8_grouped_mm(x, xs, w, ws, off, out=y)
+    assert (y[:2] == 5).all() and (y[-3:] == 5).all()
+    for e, (i, j) in _spans(off):
+        want, size = _fp8_want(x[i:j], xs[i:j], w[e], ws[e])
+        _close(y[i:j], want, size, k, f"expert {e}")
+
+
+# Operands that begin and end at any element of an allocation's first and last words, in every direction.
+@pytest.mark.parametrize("shift", [0, 1, 2, 3])
+@pytest.mark.parametrize("n,k", [(1, 1), (3, 5), (63, 65), (129, 131), (257, 64)])
+def test_operands_at_the_ends_of_their_memory(shift, n, k):
+    counts = [3, 0, 66]
+    x, dy, w, off = _case(counts, 0, 0, n, k, BF16, seed=n * k)
+
+    def moved(t):  # the last bytes of their storage, `shift` elements from its start
+        buf = torch.full((t.numel() + shift,), float("nan"), dtype=t.dtype, device="cuda")
+        buf[shift:] = t.flatten()
+        return buf[shift:].view(t.shape)
+
+    xm, dym, wm = moved(x), moved(dy), moved(w)
+    for e, (i, j) in _spans(off):
+        _close(U.grouped_mm(xm, wm, off, out_dtype=F32)[i:j], x[i:j].double() @ w[e].double().T,
+               x[i:j].double().abs() @ w[e].double().abs().T, k, f"expert {e}")
+        _close(U.grouped_mm_dw(dym, xm, off)[e], dy[i:j].double().T @ x[i:j].double(),
+               dy[i:j].double().abs().T @ x[i:j].double().abs(), j - i, f"dw {e}")
+        _close(U.grouped_mm_dx(dym, wm, off, out_dtype=F32)[i:j], dy[i:j].double() @ w[e].double(),
+               dy[i:j].double().abs() @ w[e].double().abs(), n, f"dx {e}")
+
+
 def test_operand_and_output_in_one_buffer():
     """Columns of one buffer lie beside one another and are allowed; the same memory is refused, and left as it was."""
     x, dy, w, off = _case([70, 5, 33], 0, 2, 96, 96, BF16, seed=8)

@@ -392,7 +392,9 @@ umsx_status run_product(const Product &p, umsx_stream stream) {
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return fail(UMSX_EDEVICE, std::string("device query: ") + cudaGetErrorString(e));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int n = product_few_takes(p, sms) ? launch_product_few(p, sms, s) : product_tc_takes(p) ? launch_product_tc(p, sms, s) : launch_product_any(p, sms, s);
+    const int n = product_few_takes(p)  ? launch_product_few(p, sms, s)
+                  : product_tc_takes(p) ? launch_product_tc(p, sms, s)
+                                        : launch_product_any(p, sms, s);
     e = cudaGetLastError();
     if (n < 0) return fail(UMSX_EDEVICE, std::string("the product's kernel could not be set up: ") + cudaGetErrorString(e));
     record_launches((uint64_t)n);

@@ -121,7 +121,7 @@ int launch_product_any(const Product &p, int sms, cudaStream_t s);
 int launch_product_tc(const Product &p, int sms, cudaStream_t s);  // where product_tc_takes(p)
 bool product_tc_takes(const Product &p);
 int launch_product_few(const Product &p, int sms, cudaStream_t s);  // where product_few_takes(p)
-bool product_few_takes(const Product &p, int sms);
+bool product_few_takes(const Product &p);
 uint32_t *product_err_word();  // of the current device: nonzero after a bounded wait gave up
 
 }  // namespace umsx

@@ -9,8 +9,9 @@
 // lane t takes eight neighbours and feeds two MMAs with them.  e4m3 codes become f16 (exact) and the fp32 sums of a
 // block of 128 are scaled once.  The eight warps' sums are added in a fixed order.
 //
-// Bound: memory (e4m3, 96 rows over 64 experts of 2816 x 2048: 61 us, 4.9 TB/s, 75 % of a copy's rate).  The tcgen05 kernel's tiles of 128 or 256 features leave SMs without work here (8 experts of 1536
-// features: 48 tiles for 74 pairs) and go through a pipeline that costs more than the weights of one step.
+// Bound: memory (e4m3, 96 rows over 64 experts of 2816 x 2048: 61 us, 4.9 TB/s, 75 % of a copy's rate).  The tcgen05
+// kernel's tiles of 128 or 256 features leave SMs without work here (8 experts of 1536 features: 48 tiles for 74 pairs) and
+// go through a pipeline that costs more than the weights of one step.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -191,26 +192,28 @@ void launch(const FewParams &p, int nt, int64_t chunks, cudaStream_t s) {
 
 }  // namespace
 
-// Tiles of eight rows a CTA takes, or 0 where the tcgen05 kernel is to be used.  Measured with cold weights (2816 x 2048 e4m3,
-// 1536 x 2048 bf16), this kernel / the other: 3 rows an expert 82 / 78 us and 123 / 125, 6 rows 88 / 88, 8 rows (bf16) 160 / 147;
-// one matrix, which gives the other only n / 256 tiles: 8 rows 10.2 / 14.3, 32 rows 12.3 / 14.3 with two tiles of rows
-// (one: 14.3), 48 rows 14.3 / 14.3.
-static int few_tiles(const Product &p, int sms) {
+// Tiles of eight rows a CTA takes, or 0 where the tcgen05 kernel is to be used.  Decoding, up to four rows an expert on average:
+// the weights are all there is to read (2816 x 2048 e4m3, 1536 x 2048 bf16, this kernel / the other: 3 rows an expert 82 / 78 us
+// and 123 / 125, 6 rows 88 / 88, 8 rows in bf16 160 / 147).  Up to 2^17 outputs: the other has few tiles, each alone with its
+// contraction, which this one splits over eight warps (us, bf16; 57 rows of 640 x 9728: 19.5 / 39.9, 256 of 136 x 5648: 13.3 /
+// 35.8, 64 of 640 x 128: 8.2 / 10.2, 8 x 8 of 1536 x 2048: 18.5 / 22.6, 128 of 1024 x 4096: 21.5 / 23.6); with more of them it
+// reads the weights too often (8 x 32 of 1536 x 2048: 30.8 / 22.5, 128 of 2048 x 4096: 37.9 / 25.6).
+static int few_tiles(const Product &p) {
     const double mean = (double)p.rows / p.groups;
-    const int64_t tiles = std::min<int64_t>(p.groups, p.rows) * ((p.n + 255) / 256);
-    if (mean <= 4 && p.rows <= 1024) return 1;  // 1024: one expert may have got them all, and is then read rows / 8 times
-    return mean <= 32 && p.rows <= 1024 && tiles <= sms / 2 ? (mean <= 8 ? 1 : 2) : 0;
+    if (p.rows > 1024) return 0;  // one expert may have got them all, and is then read rows / 8 times
+    if (mean <= 4) return 1;
+    return p.rows * ((p.n + kFewF - 1) / kFewF * kFewF) <= 1 << 17 ? (mean <= 8 ? 1 : 2) : 0;
 }
 
-bool product_few_takes(const Product &p, int sms) {
+bool product_few_takes(const Product &p) {
     const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2;
     const auto ok = [&](const void *b, int64_t ld) { return reinterpret_cast<uintptr_t>(b) % 16 == 0 && ld * size % 16 == 0; };
     return p.mode == kForward && p.rows > 0 && p.k * size % 16 == 0 && ok(p.x, p.ldx) && ok(p.w, p.ldw) &&
-           (p.groups == 1 || p.w_stride * size % 16 == 0) && few_tiles(p, sms) > 0;
+           (p.groups == 1 || p.w_stride * size % 16 == 0) && few_tiles(p) > 0;
 }
 
 int launch_product_few(const Product &p, int sms, cudaStream_t s) {
-    const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2, nt = few_tiles(p, sms);
+    const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2, nt = few_tiles(p);
     FewParams f{};
     f.groups = p.groups, f.n = p.n, f.k = p.k, f.out_dtype = p.out_dtype;
     f.rows = p.rows, f.offsets = p.offsets;
