@@ -692,3 +692,44 @@ def test_launches_are_counted():
     U.grouped_mm(x, w, off)
     U.fp8_quantize(x)
     assert U.kernel_launches() >= before + 2
+
+
+# ---- bounded waits ---------------------------------------------------------------------------------------
+
+
+def _tcgen05_calls():
+    """Calls that run on the tcgen05 kernels (more than 1024 rows, aligned), name -> (function, reads of its result)."""
+    counts = [700, 0, 10, 413]
+    x, dy, w, off = _case(counts, 0, 0, 256, 512, BF16, seed=31)
+    xs16, dys16, _, off16 = _case([64, 1056], 0, 0, 256, 512, BF16, seed=32)
+    xt, dyt, _, offt = _case([10, 1100], 0, 0, 256, 512, BF16, seed=33)  # the first tile's only stage ends raggedly
+    xq, xs, wq, ws, offq = _fp8_case(counts, 0, 0, 256, 512, seed=34)
+    return {"forward": lambda: U.grouped_mm(x, w, off), "forward in fp32": lambda: U.grouped_mm(x, w, off, out_dtype=F32),
+            "dx": lambda: U.grouped_mm_dx(dy, w, off), "dw": lambda: U.grouped_mm_dw(dys16, xs16, off16),
+            "dw of ragged groups": lambda: U.grouped_mm_dw(dyt, xt, offt), "e4m3": lambda: U.fp8_grouped_mm(xq, xs, wq, ws, offq)}
+
+
+@pytest.mark.parametrize("call", ["forward", "forward in fp32", "dx", "dw", "dw of ragged groups", "e4m3"])
+@pytest.mark.parametrize("cta", [0, 1])
+def test_a_wait_that_runs_out_is_reported(call, cta):
+    """A CTA's first copies never start, so that the waits behind them run out (a millisecond here): the kernel ends, the
+    status says so once, and the next call gives its usual bits.  CTA 1 is the second of a pair in the 16-bit products."""
+    fn = _tcgen05_calls()[call]
+    want = fn()
+    U.products_status()
+    U.products_inject_fault(cta, wait_limit_cycles=2_000_000)
+    fn()
+    with pytest.raises(U.UmsxError) as e:
+        U.products_status()
+    assert e.value.status == U.ETIMEOUT
+    U.products_status()
+    assert torch.equal(fn(), want)
+    U.products_status()
+
+
+def test_a_fault_beyond_the_grid_injects_nothing():
+    for fn in _tcgen05_calls().values():
+        want = fn()
+        U.products_inject_fault(1 << 20, wait_limit_cycles=200_000_000)
+        assert torch.equal(fn(), want)
+        U.products_status()

@@ -183,31 +183,60 @@ __device__ __forceinline__ bool elect_one() {
 
 // ---- bounded waits -----------------------------------------------------------------------------
 //
-// A wait that has not ended after about a second marks its CTA as given up (`gave_up`, shared memory): every other
-// wait of the CTA then returns at once, so that the kernel ends; its loops look at the mark once per tile.  One asm
-// block without results: as a function with a verdict, tested and voted on after every call, a wait for a complete
-// phase took 250 cycles instead of 50.
-constexpr long long kPairWaitCycles = 2000000000ll;
+// A wait that has not ended after the CTA's limit marks the CTA as given up; every other wait of the CTA whose phase is not
+// complete then ends too, and the loops look at the mark once per tile.  One asm block each (a function with a loop in it took
+// 250 cycles where a phase was complete, a block 50); mark and limit lie in shared memory, where only a wait that is not over
+// at once looks at them.
+constexpr long long kPairWaitCycles = 2000000000ll;       // the usual limit, about a second
+constexpr long long kDrainCycles = kPairWaitCycles / 64;  // for copies and MMAs in flight at the end, which take microseconds
+
+struct GiveUp {
+    int given_up;
+    long long limit;  // SM cycles
+};
 
 #define UMSX_WAIT(sem)                                                                                            \
     asm volatile(                                                                                                 \
-        "{\n\t.reg .pred p, q;\n\t.reg .b32 g;\n\t.reg .b64 t0, t;\n\t"                                          \
-        "mbarrier.try_wait.parity" sem ".shared::cta.b64 p, [%0], %1;\n\t"                                        \
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 g;\n\t.reg .b64 t0, t, m;\n\tmov.u32 %0, 0;\n\t"                      \
+        "mbarrier.try_wait.parity" sem ".shared::cta.b64 p, [%1], %2;\n\t"                                        \
         "@p bra DONE;\n\tmov.u64 t0, %%clock64;\n"                                                               \
-        "AGAIN:\n\tmbarrier.try_wait.parity" sem ".shared::cta.b64 p, [%0], %1;\n\t"                             \
-        "@p bra DONE;\n\tld.volatile.shared.b32 g, [%2];\n\tsetp.ne.b32 q, g, 0;\n\t@q bra DONE;\n\t"            \
-        "mov.u64 t, %%clock64;\n\tsub.s64 t, t, t0;\n\tsetp.lt.s64 q, t, %3;\n\t@q bra AGAIN;\n\t"              \
-        "st.volatile.shared.b32 [%2], 1;\nDONE:\n\t}" ::"r"(bar), "r"(parity), "r"(gave_up), "l"(kPairWaitCycles) \
+        "AGAIN:\n\tmbarrier.try_wait.parity" sem ".shared::cta.b64 p, [%1], %2;\n\t"                             \
+        "@p bra DONE;\n\tld.volatile.shared.b32 g, [%3];\n\tsetp.ne.b32 q, g, 0;\n\t@q bra LOST;\n\t"            \
+        "ld.shared.b64 m, [%3+8];\n\tmov.u64 t, %%clock64;\n\tsub.s64 t, t, t0;\n\t"                            \
+        "setp.lt.s64 q, t, m;\n\t@q bra AGAIN;\n\tst.volatile.shared.b32 [%3], 1;\n"                            \
+        "LOST:\n\tmov.u32 %0, 1;\nDONE:\n\t}"                                                                  \
+        : "=&r"(lost)                                                                                             \
+        : "r"(bar), "r"(parity), "r"(give_up)                                                                     \
         : "memory")
 
-// bar, gave_up: shared-memory addresses.  ACROSS: the barrier hands over what the other CTA's threads wrote
-// (publish_at); an acquire of cluster scope costs about 200 cycles more, so the other waits stay at this CTA's scope.
+// Whether all lanes of the (converged) warp saw the phase complete.  Where they did not, the warp leaves its loops before it
+// arrives with expected bytes, copies or multiplies any more: a barrier that it has not seen free would get a second
+// arrival in a phase that awaits one.  bar, give_up: shared-memory addresses.  ACROSS: the barrier hands over what the
+// other CTA's threads wrote (publish_at); an acquire of cluster scope costs about 200 cycles more, so the other waits
+// stay at this CTA's scope.
 template <bool ACROSS = false>
-__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, uint32_t gave_up) {
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, uint32_t give_up) {
+    uint32_t lost;
     if constexpr (ACROSS) UMSX_WAIT(".acquire.cluster");
     else UMSX_WAIT("");
+    return !__any_sync(kFull, lost);
 }
 #undef UMSX_WAIT
+
+// The same without a verdict, whose vote costs the e4m3 kernel 8 %, for warps that may run on to the end of their tile: their
+// reads give garbage, which the mark says, and their plain arrivals only end phases early.  In a CTA that has given up it ends
+// at once, as the first look at the barrier does not block.
+__device__ __forceinline__ void wait_or_run_on(uint32_t bar, uint32_t parity, uint32_t give_up) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t.reg .b32 g;\n\t.reg .b64 t0, t, m;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%0], %1;\n\t@p bra DONE;\n\tmov.u64 t0, %%clock64;\n"
+        "AGAIN:\n\tld.volatile.shared.b32 g, [%2];\n\tsetp.ne.b32 q, g, 0;\n\t@q bra DONE;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t@p bra DONE;\n\t"
+        "ld.shared.b64 m, [%2+8];\n\tmov.u64 t, %%clock64;\n\tsub.s64 t, t, t0;\n\t"
+        "setp.lt.s64 q, t, m;\n\t@q bra AGAIN;\n\tst.volatile.shared.b32 [%2], 1;\nDONE:\n\t}" ::"r"(bar),
+        "r"(parity), "r"(give_up)
+        : "memory");
+}
 
 // A ring position: stage and the parity of its next use.
 template <int STAGES>

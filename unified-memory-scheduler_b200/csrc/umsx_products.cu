@@ -381,7 +381,14 @@ bool out_overlaps(const Product &p) {
 
 bool misaligned(const void *p, int size) { return reinterpret_cast<uintptr_t>(p) % size; }
 
-umsx_status run_product(const Product &p, umsx_stream stream) {
+// What umsx_products_inject_fault left for the calling thread's next product on the tcgen05 kernels.
+struct Fault {
+    int cta = -1;
+    long long wait_limit = 0;
+};
+thread_local Fault g_fault;
+
+umsx_status run_product(Product &p, umsx_stream stream) {
     if (out_overlaps(p)) return fail(UMSX_EINVAL, "the output overlaps an input");
     const int size = p.dtype == UMSX_DTYPE_E4M3 ? 1 : 2, out_size = p.out_dtype == UMSX_DTYPE_F32 ? 4 : 2;
     if (misaligned(p.x, size) || misaligned(p.dy, size) || misaligned(p.w, size) || misaligned(p.out, out_size) ||
@@ -392,9 +399,11 @@ umsx_status run_product(const Product &p, umsx_stream stream) {
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return fail(UMSX_EDEVICE, std::string("device query: ") + cudaGetErrorString(e));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int n = product_few_takes(p)  ? launch_product_few(p, sms, s)
-                  : product_tc_takes(p) ? launch_product_tc(p, sms, s)
-                                        : launch_product_any(p, sms, s);
+    const bool few = product_few_takes(p), tc = !few && product_tc_takes(p);
+    if (tc) p.fault_cta = g_fault.cta, p.wait_limit = g_fault.wait_limit, g_fault = Fault{};
+    const int n = few ? launch_product_few(p, sms, s)
+                  : tc ? launch_product_tc(p, sms, s)
+                       : launch_product_any(p, sms, s);
     e = cudaGetLastError();
     if (n < 0) return fail(UMSX_EDEVICE, std::string("the product's kernel could not be set up: ") + cudaGetErrorString(e));
     record_launches((uint64_t)n);
@@ -493,6 +502,12 @@ umsx_status umsx_products_status(umsx_stream stream) {
     if (e == cudaSuccess && v) e = cudaMemsetAsync(word, 0, sizeof v, s);
     if (e != cudaSuccess) return fail(UMSX_EDEVICE, std::string("products status: ") + cudaGetErrorString(e));
     return v ? fail(UMSX_ETIMEOUT, "a bounded wait of a product's kernel gave up: its output is not complete") : UMSX_OK;
+}
+
+umsx_status umsx_products_inject_fault(int cta, int64_t wait_limit_cycles) {
+    if (cta < 0 || wait_limit_cycles < 1) return fail(UMSX_EINVAL, "cta must not be negative, wait_limit_cycles must be positive");
+    g_fault = {cta, wait_limit_cycles};
+    return UMSX_OK;
 }
 
 }  // extern "C"

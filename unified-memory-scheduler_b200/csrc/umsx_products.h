@@ -34,6 +34,8 @@ struct Product {
     int64_t xs_row, xs_blk, ws_row, ws_blk, ws_group;
     void *out;  // forward [rows][n], dx [rows][k], dw [groups][n][k]
     int64_t ldo, out_stride;
+    int fault_cta;         // CTA that withholds its first copies (umsx_products_inject_fault), -1: none
+    long long wait_limit;  // SM cycles of a bounded wait, 0: the usual ones
 
     int features() const { return mode == kForward ? n : k; }
 };

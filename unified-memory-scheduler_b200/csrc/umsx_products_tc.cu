@@ -57,6 +57,8 @@ struct TcParams {
     const int32_t *offsets;
     void *out;
     int64_t ldo, out_group;
+    int fault_cta;
+    long long wait_limit;
 };
 
 template <int MODE>
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     // dw, a tile's ragged last stage: its copies to this CTA, and both CTAs' zeroing
     __shared__ __align__(8) uint64_t tail[S::kStages], fixed[S::kStages], last;
     __shared__ uint32_t tmem_s;
-    __shared__ int gave_up;
+    __shared__ tc::GiveUp give_up;
     __shared__ int start[kMaxGroups + 1], prefix[kMaxGroups + 1];
 
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
@@ -247,7 +249,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
 
     for (int g = tid; g <= p.groups; g += kThreads) start[g] = group_start(p.offsets, g, p.rows);
     if (tid == 0) {
-        gave_up = 0;
+        give_up.given_up = 0;
+        give_up.limit = p.wait_limit;
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&tail[s], 1);
@@ -271,16 +274,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
     const int total = __shfl_sync(kFull, prefix[p.groups], 0);
     const Tiles<kPair, MODE> tiles{start, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
-    const uint32_t up = smem_u32(&gave_up), aF = smem_u32(sF), aR = smem_u32(sR);
+    const uint32_t up = smem_u32(&give_up), aF = smem_u32(sF), aR = smem_u32(sR);
     const uint32_t b_full = smem_u32(full), b_empty = smem_u32(empty), b_dfull = smem_u32(d_full), b_dempty = smem_u32(d_empty),
                    b_tail = smem_u32(tail), b_fixed = smem_u32(fixed);
-    const auto stop = [&] { return __shfl_sync(kFull, *const_cast<volatile int *>(&gave_up), 0) != 0; };
+    const auto stop = [&] { return __shfl_sync(kFull, *const_cast<volatile int *>(&give_up.given_up), 0) != 0; };
 
     if (warp == 0) {
         tc::Ring<S::kStages> r;
         uint32_t tails = 0, tail_phase = 0, used = 0;  // bit s: stage s holds a ragged end; uses of tail[s], mod 2; stages in use
         int group = 0;
-        for (int t = cluster; t < total && !stop(); t += clusters) {
+        bool withhold = (int)blockIdx.x == p.fault_cta, on = true;
+        for (int t = cluster; on && t < total && !stop(); t += clusters) {
             const Tile x = tiles.get(t, group, lane);
             const int kb = (x.c_len + kBC - 1) / kBC;
             if (!x.rows) continue;
@@ -289,7 +293,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             const uint32_t bytes = S::kBytesF + boxes * (S::kRMn ? 64 : kRowBox) * kBC * 2;
             const int f0 = x.f0 + (int)rank * kBF, r0 = x.row0 + (int)rank * half;
             for (int kk = 0; kk < kb; ++kk, r.next()) {
-                tc::wait(b_empty + 8 * r.s, r.phase ^ 1u, up);
+                if (!(on = tc::wait(b_empty + 8 * r.s, r.phase ^ 1u, up))) break;
+                if (withhold) {
+                    withhold = false;
+                    continue;
+                }
                 const bool ragged = MODE == kGradWeight && kk == kb - 1 && (x.c_len & 15);
                 used |= 1u << r.s;
                 if (ragged) tails |= 1u << r.s, tail_phase ^= 1u << r.s;
@@ -323,21 +331,22 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             }
         }
         // A CTA must not exit before the last arrivals at its barriers, nor, where a wait gave up and the MMAs did not
-        // read them, under copies in flight.
+        // read them, under copies in flight: those of the odd CTA complete on the leader's barrier, and land long before
+        // its own wait here has run out.
         for (uint32_t s = 0; s < (uint32_t)S::kStages; ++s) {
             if (!(used >> s & 1u)) continue;
             const uint32_t last_phase = r.phase ^ (s >= r.s ? 1u : 0u);
-            mbar_wait_bounded(&empty[s], last_phase, tc::kPairWaitCycles / 8);
-            if (!stop()) continue;
-            if (tails >> s & 1u) mbar_wait_bounded(&tail[s], (tail_phase >> s & 1u) ^ 1u, tc::kPairWaitCycles / 8);
-            else if (rank == 0) mbar_wait_bounded(&full[s], last_phase, tc::kPairWaitCycles / 8);
+            if (mbar_wait_bounded(&empty[s], last_phase, tc::kDrainCycles)) continue;
+            if (tails >> s & 1u) mbar_wait_bounded(&tail[s], (tail_phase >> s & 1u) ^ 1u, tc::kDrainCycles);
+            else if (rank == 0) mbar_wait_bounded(&full[s], last_phase, tc::kDrainCycles);
         }
     } else if (warp == 1) {
         if (rank == 0) {
             tc::Ring<S::kStages> r;
             uint32_t n_item = 0, fixed_phase = 0;
             int group = 0;
-            for (int t = cluster; t < total && !stop(); t += clusters) {
+            bool on = true;
+            for (int t = cluster; on && t < total && !stop(); t += clusters) {
                 const Tile x = tiles.get(t, group, lane);
                 const int kb = (x.c_len + kBC - 1) / kBC;
                 if (!x.rows || !kb) continue;
@@ -346,12 +355,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                 for (int kk = 0, in_seg = 0; kk < kb; ++kk, r.next()) {
                     if (in_seg == 0) {
                         buf = n_item & 1u, d_tm = tmem + buf * kRowsMax;
-                        tc::wait(b_dempty + 8 * buf, ((n_item >> 1) & 1u) ^ 1u, up);
+                        if (!(on = tc::wait(b_dempty + 8 * buf, ((n_item >> 1) & 1u) ^ 1u, up))) break;
                         ++n_item;
                     }
-                    tc::wait(b_full + 8 * r.s, r.phase, up);
+                    if (!(on = tc::wait(b_full + 8 * r.s, r.phase, up))) break;
                     if (MODE == kGradWeight && kk == kb - 1 && (x.c_len & 15)) {
-                        tc::wait<true>(b_fixed + 8 * r.s, fixed_phase >> r.s & 1u, up);
+                        if (!(on = tc::wait<true>(b_fixed + 8 * r.s, fixed_phase >> r.s & 1u, up))) break;
                         fixed_phase ^= 1u << r.s;
                     }
                     tc::fence_after_sync();
@@ -374,14 +383,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             }
             // nor under MMAs in flight
             if (tc::elect_one()) tc::leader_commit<kPair>(smem_u32(&last));
-            mbar_wait_bounded(&last, 0, tc::kPairWaitCycles / 8);
+            mbar_wait_bounded(&last, 0, tc::kDrainCycles);
         }
     } else if (warp < 2 + kEpilogueWarps) {
         const int quad = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes 32 * quad.., columns in turns of 16
         uint8_t *stage = smem + S::kStages * (S::kBytesF + S::kBytesR) + (warp - 2) * 16 * kStageRow;
         uint32_t n_item = 0;
         int group = 0;
-        for (int t = cluster; t < total && !stop(); t += clusters) {
+        bool on = true;
+        for (int t = cluster; on && t < total && !stop(); t += clusters) {
             const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
             const int f = x.f0 + (int)rank * kBF + quad * 32;
@@ -392,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             // The next accumulator, and its return.
             auto take = [&] {
                 const uint32_t buf = n_item & 1u;
-                tc::wait(b_dfull + 8 * buf, (n_item >> 1) & 1u, up);
+                on = tc::wait(b_dfull + 8 * buf, (n_item >> 1) & 1u, up);
                 tc::fence_after_sync();
                 ++n_item;
                 return buf;
@@ -404,6 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             };
             if (segments <= 1) {
                 const uint32_t buf = segments ? take() : 0;
+                if (!on) break;
                 for (int c0 = part * 16; c0 < x.rows; c0 += 32) {
                     uint32_t v[16] = {};  // an expert without rows: dw is zero
                     if (segments) tc::tmem_ld_frag(lanes + buf * kRowsMax + c0, v);
@@ -419,6 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                 for (int j = 0; j < 16; ++j) acc[c][j] = 0.0f;
             for (int g = 0; g < segments; ++g) {
                 const uint32_t buf = take();
+                if (!on) break;
 #pragma unroll
                 for (int c = 0; c < kRowsMax / 32; ++c)
                     if (32 * c + part * 16 < x.rows) {
@@ -429,6 +441,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                     }
                 give(buf);
             }
+            if (!on) break;
 #pragma unroll
             for (int c = 0; c < kRowsMax / 32; ++c)
                 if (32 * c + part * 16 < x.rows) {
@@ -448,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
             it += kb;
             if (!(x.c_len & 15)) continue;
             const int boxes = (x.n / kPair + 63) / 64, s = (it - 1) % S::kStages;
-            tc::wait(b_tail + 8 * s, tail_phase >> s & 1u, up);
+            if (!tc::wait(b_tail + 8 * s, tail_phase >> s & 1u, up)) break;
             tail_phase ^= 1u << s;
             // lines (one contraction row each) from `valid` up to the last multiple of 16 that the MMAs read
             const int valid = x.c_len - (kb - 1) * kBC, lines = 16 - (valid & 15);
@@ -523,7 +536,7 @@ __device__ __forceinline__ void fma2(uint64_t &acc, uint64_t a, uint64_t b) {
 
 // What a promotion warp needs of its CTA.
 struct F8Sync {
-    uint32_t d_full, d_empty, sc_empty, gave_up;  // shared-memory addresses
+    uint32_t d_full, d_empty, sc_empty, give_up;  // shared-memory addresses
     uint32_t lanes;                               // TMEM address of the warp's lanes
     const float *scales;
     uint8_t *stage;  // the warp's
@@ -541,7 +554,7 @@ __device__ __forceinline__ void promote_half(const F8Sync &y, uint32_t &it, cons
     constexpr int kTogether = NCH <= 2 ? 2 * NCH : 1;  // loads of 16 columns under one wait
     for (int kk = 0; kk < kb; ++kk, ++it) {
         const int slot = part + 2 * (int)(it & 1u);
-        tc::wait(y.d_full + 8 * slot, (it >> 1) & 1u, y.gave_up);
+        tc::wait_or_run_on(y.d_full + 8 * slot, (it >> 1) & 1u, y.give_up);
         tc::fence_after_sync();
         const float *sc = y.scales + slot * kHalfCols + 2 * (lane & 3);
         const uint32_t src = y.lanes + slot * kHalfCols;
@@ -595,13 +608,14 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     // d_full: a slot's MMAs and its scales; d_empty, sc_empty: both read by the four warps of its half
     __shared__ __align__(8) uint64_t full[S::kStages], empty[S::kStages], d_full[kSlots], d_empty[kSlots], sc_empty[kSlots], last;
     __shared__ uint32_t tmem_s;
-    __shared__ int gave_up;
+    __shared__ tc::GiveUp give_up;
     __shared__ int start[kMaxGroups + 1], prefix[kMaxGroups + 1];
 
     const int tid = threadIdx.x, warp = __shfl_sync(kFull, tid >> 5, 0), lane = tid & 31;
     for (int g = tid; g <= p.groups; g += kThreadsF8) start[g] = group_start(p.offsets, g, p.rows);
     if (tid == 0) {
-        gave_up = 0;
+        give_up.given_up = 0;
+        give_up.limit = p.wait_limit;
         mbar_init(&last, 2);
         for (int s = 0; s < S::kStages; ++s) {
             mbar_init(&full[s], 1);
@@ -624,23 +638,28 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
     const int total = __shfl_sync(kFull, prefix[p.groups], 0), kb = (p.contraction + S::kBC8 - 1) / S::kBC8;
     const Tiles<1, kForward> tiles{start, prefix, p.groups, f_tiles, p.features, p.contraction, p.out_rows};
 
-    const uint32_t up = smem_u32(&gave_up), aF = smem_u32(sF), aR = smem_u32(sR);
+    const uint32_t up = smem_u32(&give_up), aF = smem_u32(sF), aR = smem_u32(sR);
     const uint32_t b_full = smem_u32(full), b_empty = smem_u32(empty), b_dfull = smem_u32(d_full), b_dempty = smem_u32(d_empty),
                    b_sempty = smem_u32(sc_empty);
-    const auto stop = [&] { return __shfl_sync(kFull, *const_cast<volatile int *>(&gave_up), 0) != 0; };
+    const auto stop = [&] { return __shfl_sync(kFull, *const_cast<volatile int *>(&give_up.given_up), 0) != 0; };
 
     if (warp == 0) {
         tc::Ring<S::kStages> r;
         uint32_t used = 0;  // stages in use
         int group = 0;
-        for (int t = blockIdx.x; t < total && !stop(); t += gridDim.x) {
+        bool withhold = (int)blockIdx.x == p.fault_cta, on = true;
+        for (int t = blockIdx.x; on && t < total && !stop(); t += gridDim.x) {
             const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
             const Half h0 = tile_half(x.n, 0), h1 = tile_half(x.n, 1);
             const int boxes0 = (h0.n + kRowBox - 1) / kRowBox, boxes1 = (h1.n + kRowBox - 1) / kRowBox;
             const uint32_t bytes = S::kBytesF + (boxes0 + boxes1) * kRowBox * S::kBC8;
             for (int kk = 0; kk < kb; ++kk, r.next()) {
-                tc::wait(b_empty + 8 * r.s, r.phase ^ 1u, up);
+                if (!(on = tc::wait(b_empty + 8 * r.s, r.phase ^ 1u, up))) break;
+                if (withhold) {
+                    withhold = false;
+                    continue;
+                }
                 used |= 1u << r.s;
                 if (tc::elect_one()) {
                     const uint32_t bar = b_full + 8 * r.s;
@@ -656,26 +675,26 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
                 __syncwarp();
             }
         }
-        for (uint32_t s = 0; s < (uint32_t)S::kStages; ++s) {  // as in k_product_tc: no exit before the last arrivals
+        for (uint32_t s = 0; s < (uint32_t)S::kStages; ++s) {  // as in k_product_tc: no exit before the last arrivals and copies
             if (!(used >> s & 1u)) continue;
             const uint32_t last_phase = r.phase ^ (s >= r.s ? 1u : 0u);
-            mbar_wait_bounded(&empty[s], last_phase, tc::kPairWaitCycles / 8);
-            if (stop()) mbar_wait_bounded(&full[s], last_phase, tc::kPairWaitCycles / 8);
+            if (!mbar_wait_bounded(&empty[s], last_phase, tc::kDrainCycles)) mbar_wait_bounded(&full[s], last_phase, tc::kDrainCycles);
         }
     } else if (warp == 1 || warp == 3) {
         const int h = warp >> 1;
         tc::Ring<S::kStages> r;
         uint32_t it = 0;  // blocks of this half so far
         int group = 0;
-        for (int t = blockIdx.x; t < total && !stop(); t += gridDim.x) {
+        bool on = true;
+        for (int t = blockIdx.x; on && t < total && !stop(); t += gridDim.x) {
             const Tile x = tiles.get(t, group, lane);
             if (!x.rows) continue;
             const int n = tile_half(x.n, h).n;
             const uint32_t idesc = tc::operand_idesc(0, false, false, kBF, n);
             for (int kk = 0; kk < kb; ++kk, r.next()) {
-                tc::wait(b_full + 8 * r.s, r.phase, up);
+                if (!(on = tc::wait(b_full + 8 * r.s, r.phase, up))) break;
                 const int slot = h + 2 * (int)(it & 1u);
-                if (n) tc::wait(b_dempty + 8 * slot, ((it >> 1) & 1u) ^ 1u, up);
+                if (n && !(on = tc::wait(b_dempty + 8 * slot, ((it >> 1) & 1u) ^ 1u, up))) break;
                 tc::fence_after_sync();
                 if (tc::elect_one()) {
                     if (n) {
@@ -695,7 +714,7 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
             }
         }
         if (tc::elect_one()) tc::leader_commit<1>(smem_u32(&last));  // nor under MMAs in flight
-        mbar_wait_bounded(&last, 0, tc::kPairWaitCycles / 8);
+        mbar_wait_bounded(&last, 0, tc::kDrainCycles);
     } else if (warp == 2) {
         // ---- scales, two blocks ahead: registers [block & 1][half][32 columns] ------------------------------
         uint32_t it[2] = {0, 0};
@@ -735,7 +754,7 @@ __global__ void __launch_bounds__(kThreadsF8, 1) k_product_f8(const __grid_const
                     for (int h = 0; h < 2; ++h) {
                         if (h && !h1.n) break;
                         const int slot = h + 2 * (int)(it[h] & 1u);
-                        tc::wait(b_sempty + 8 * slot, ((it[h] >> 1) & 1u) ^ 1u, up);
+                        tc::wait_or_run_on(b_sempty + 8 * slot, ((it[h] >> 1) & 1u) ^ 1u, up);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) scales[slot * kHalfCols + lane + 32 * i] = s[h][i];
                         __syncwarp();
@@ -880,6 +899,8 @@ int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
     t.ldo = p.ldo;
     t.out_group = p.out_stride;
     t.vec = aligned(p.out, p.ldo, 2) && p.out_stride % 8 == 0;
+    t.fault_cta = p.fault_cta;
+    t.wait_limit = p.wait_limit ? p.wait_limit : tc::kPairWaitCycles;
     t.segment = p.out_dtype == UMSX_DTYPE_F32 ? kSegment : 0x7fffffff;
     if (p.dtype == UMSX_DTYPE_E4M3) {
         const F8Params fp{t, p.xs, p.ws, p.xs_row, p.xs_blk, p.ws_row, p.ws_blk, p.ws_group};

@@ -49,7 +49,7 @@ EXPORTS = ["umsx_moe_create", "umsx_moe_create_synthetic", "umsx_moe_destroy", "
            "umsx_ep_prefill_status", "umsx_ep_prefill_destroy",
            "umsx_gguf_load_experts", "umsx_gguf_experts_free", "umsx_moe_create_gguf",
            "umsx_group_rows", "umsx_grouped_mm", "umsx_grouped_mm_dx", "umsx_grouped_mm_dw", "umsx_fp8_quantize",
-           "umsx_fp8_grouped_mm", "umsx_products_status",
+           "umsx_fp8_grouped_mm", "umsx_products_status", "umsx_products_inject_fault",
            "umsx_kernel_launches", "umsx_last_error", "umsx_version"]
 
 
@@ -147,6 +147,7 @@ def lib():
         "umsx_fp8_grouped_mm": (i32, [vp, i64, vp, i64, i64, vp, i64, i64, vp, i64, i64, i64, vp, i32, i64, i32, i32,
                                       vp, i64, i32, vp]),
         "umsx_products_status": (i32, [vp]),
+        "umsx_products_inject_fault": (i32, [i32, i64]),
         "umsx_kernel_launches": (u64, []),
         "umsx_last_error": (C.c_char_p, []),
         "umsx_version": (i32, []),
@@ -522,6 +523,12 @@ def products_status(stream=None):
     """Raises UmsxError (ETIMEOUT) if a bounded wait inside one of the products' kernels gave up on the current
     device since the last query (umsx_products_status); synchronises the stream."""
     check(lib().umsx_products_status(_stream(stream)))
+
+
+def products_inject_fault(cta: int = 0, wait_limit_cycles: int = 2_000_000):
+    """Test hook (umsx_products_inject_fault): this thread's next product on the tcgen05 kernels loses CTA `cta`'s first
+    copies, with every wait bounded by wait_limit_cycles; products_status then raises UmsxError (ETIMEOUT)."""
+    check(lib().umsx_products_inject_fault(int(cta), int(wait_limit_cycles)))
 
 
 def load_gguf_experts(first_shard: str, layer: int, ids, dequantize: bool = True) -> dict:
