@@ -389,7 +389,7 @@ umsx_status umsx_moe_create_gguf(const umsx_moe_desc *desc, const char *first_sh
  * Rows are grouped by expert: rows offsets[e] .. offsets[e+1] - 1 belong to expert e (offsets: int32
  * [experts + 1], on the device, ascending; values outside 0..rows are clamped to it).  Groups may be
  * empty; rows before the first and behind the last group are neither read nor written.
- * experts <= 1024; n, k <= 2^24; rows <= 2^31 - 16.
+ * experts <= 1024; n, k <= 2^24; rows <= 2^31 - 512.
  *
  * umsx_group_rows: the grouping of a router's picks.  ids [tokens][top_k] as umsx_route gives them; ids
  * outside 0..experts-1 (the -1 of masked picks) belong to no group.  The sort is stable (rows of one

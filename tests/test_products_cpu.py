@@ -159,3 +159,11 @@ def test_buffers_between_elements_are_refused(call, over):
 @pytest.mark.parametrize("cta,limit", [(-1, 1000), (0, 0), (0, -5)])
 def test_bad_fault_injections_are_refused(cta, limit):
     assert U.lib().umsx_products_inject_fault(cta, limit) == U.EINVAL
+
+
+@pytest.mark.parametrize("call", [_mm, _dx, _dw, _fp8])
+@pytest.mark.parametrize("rows", [2 ** 31 - 511, 2 ** 31 - 256, 2 ** 31 - 16, 2 ** 32])
+def test_rows_that_the_index_arithmetic_does_not_hold_are_refused(call, rows):
+    """A row index plus a tile of 256 rows, or a step of 128 of the contraction, has to fit into 32 bits."""
+    assert call(rows=rows) == U.EINVAL
+    assert b"rows must be" in U.lib().umsx_last_error()

@@ -360,7 +360,7 @@ bool out_ok(int t) { return t == UMSX_DTYPE_F32 || t == UMSX_DTYPE_BF16 || t == 
 umsx_status check_product(const Product &p) {
     if (p.groups < 1 || p.groups > kMaxGroups) return fail(UMSX_EINVAL, "experts must be 1..1024");
     if (p.n < 1 || p.k < 1 || p.n > (1 << 24) || p.k > (1 << 24)) return fail(UMSX_EINVAL, "n and k must be 1..2^24");
-    if (p.rows < 0 || p.rows > 0x7ffffff0) return fail(UMSX_EINVAL, "rows must be 0..2^31 - 16");
+    if (p.rows < 0 || p.rows > kMaxRows) return fail(UMSX_EINVAL, "rows must be 0..2^31 - 512");
     if (!out_ok(p.out_dtype)) return fail(UMSX_EINVAL, "the output's type must be F32, BF16 or F16");
     return UMSX_OK;
 }

@@ -18,6 +18,7 @@ namespace umsx {
 enum ProductMode { kForward = 0, kGradInput = 1, kGradWeight = 2 };
 
 constexpr int kMaxGroups = 1024;
+constexpr int64_t kMaxRows = (1ll << 31) - 512;  // a row plus a tile of rows, or a step of the contraction, is an int
 constexpr int kScaleBlock = 128;  // values that share one scale of an e4m3 operand
 
 struct Product {
