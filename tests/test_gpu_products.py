@@ -733,3 +733,50 @@ def test_a_fault_beyond_the_grid_injects_nothing():
         U.products_inject_fault(1 << 20, wait_limit_cycles=200_000_000)
         assert torch.equal(fn(), want)
         U.products_status()
+
+
+# ---- long contractions -----------------------------------------------------------------------------------
+#
+# Operands between 0.5 and 1.5, so that a partial sum grows steadily and what an addition cuts off does not average out.
+# A tensor-core addition of 16 products to a sum may cut each of the products and the result off, at one and a half units in the
+# last place at worst.  Over the 32 additions of a part of 512 the sum grows linearly, 16.5 times the part's own size in all:
+# at most 25 units (2^-23) of it.  The parts are added with rounding, half a unit each, and the result is rounded once to its
+# type.  One accumulator for the whole contraction loses about 0.3 units an addition on average.
+
+
+def _grows(gen, *shape, dtype=BF16):
+    return (torch.rand(shape, generator=gen, device="cuda") + 0.5).to(dtype)
+
+
+def _long_close(got, want, part, parts, what):
+    """want: fp64, of positive terms.  part: of the contraction in one accumulator; parts: roundings of fp32 sums."""
+    half = torch.finfo(got.dtype).eps / 2
+    tol = (25 * (part / 512) * 2.0 ** -23 + parts * 2.0 ** -24 + half) * want * (1 + half)
+    off = (got.double() - want).abs()
+    assert (off <= tol).all(), f"{what}: {float((off / want).max()):.3g} of the value off"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_long_contractions_of_any_alignment(dtype):
+    """The kernel for odd widths, fp32 out: 65,537 of the contraction in every direction; and the last of them in 16 bits, where an
+    accumulator takes 4,096."""
+    g, c = _gen(51), 65537
+    off = _offsets([70])
+    x, w = _grows(g, 70, c, dtype=dtype), _grows(g, 1, 65, c, dtype=dtype)
+    _long_close(U.grouped_mm(x, w, off, out_dtype=F32), x.double() @ w[0].double().T, 512, 129, "y")
+    dy, w = _grows(g, 70, c, dtype=dtype), _grows(g, 1, c, 65, dtype=dtype)
+    _long_close(U.grouped_mm_dx(dy, w, off, out_dtype=F32), dy.double() @ w[0].double(), 512, 129, "dx")
+    dy, x, off = _grows(g, c, 67, dtype=dtype), _grows(g, c, 65, dtype=dtype), _offsets([c])
+    _long_close(U.grouped_mm_dw(dy, x, off)[0], dy.double().T @ x.double(), 512, 129, "dw")
+    x = x * 2.0 ** -6  # the sum stays an f16
+    _long_close(U.grouped_mm_dw(dy, x, off, out_dtype=dtype)[0], dy.double().T @ x.double(), 4096, 17, "dw in 16 bits")
+
+
+@pytest.mark.parametrize("rows", [2, 8, 60])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_long_contractions_of_few_rows(rows, dtype):
+    """The streaming kernel, fp32 out: eight warps share 65,536 of the contraction and add at most 256 in one accumulator."""
+    g, c = _gen(52), 65536
+    x, w = _grows(g, rows, c, dtype=dtype), _grows(g, 1, 48, c, dtype=dtype)
+    y = U.grouped_mm(x, w, _offsets([rows]), out_dtype=F32)
+    _long_close(y, x.double() @ w[0].double().T, 256, c // (8 * 128) + 8, "y")

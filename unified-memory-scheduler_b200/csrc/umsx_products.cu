@@ -28,13 +28,15 @@ umsx_status fail(umsx_status s, const std::string &msg) {
 // gradients), one step ahead in registers.  A lane loads the aligned word that holds its first byte and shifts its four out of
 // that and the next lane's; a line's alignment is the same in every step.  From shared memory into mma.sync, by ldmatrix
 // with or without a transposition.  e4m3 codes become f16 (exact); a step is a block of 128, scaled once and added in fp32.
-// The sums go through shared memory, so that a warp stores 32 neighbours.
+// 16-bit operands get a fresh accumulator every 512 of the contraction (kAccumulate16 of it for 16-bit outputs), added up in fp32
+// in shared memory: the tensor cores add less exactly than fp32 additions round, the more so the longer they add.  From there a
+// warp stores 32 neighbours.
 // Bound by the latency of a step where there are few tiles (e4m3 511 x 308 x 1323: 24 tiles, 37 us; with steps of 32 values
 // 80), by issue where there are many: bf16 4096 x 4096 x 2049 takes 481 us forward (143 TFLOP/s), 522 for dx, 514 for dw, e4m3
 // 446; with single-element loads 573, 784, 891 and 1116, and with a test in front of every load and shift 778 forward.
 
 constexpr int kAnyRows = 64, kAnyF = 128, kLineBytes = 128, kAnyWarps = 8;
-constexpr int kSumLine = kAnyF + 4;
+constexpr int kSumLine = kAnyF + 8;  // a half warp's pairs of sums lie in different banks
 
 template <int DTYPE>
 struct AnyShape {
@@ -43,11 +45,11 @@ struct AnyShape {
     static_assert(kSize == 2 || kC == kScaleBlock, "a step of e4m3 codes is a block");
     static constexpr int kLine = kC + 8;           // 16-bit values from line to line: eight lines spread over all banks
     static constexpr int kOperands = (kAnyRows + kAnyF) * kLine * 2, kSums = kAnyRows * kSumLine * 4;
-    static constexpr int kSmem = kOperands > kSums ? kOperands : kSums;
+    static constexpr int kSmem = kOperands + kSums;
 };
 
 struct AnyParams {
-    int out_dtype, groups;
+    int out_dtype, groups, segment;  // segment: contraction that shares an accumulator
     int64_t rows;
     int features, contraction;  // contraction: forward k, dx n (dw: the group's rows)
     int out_rows;               // dw: n
@@ -200,7 +202,7 @@ __global__ void __launch_bounds__(32 * kAnyWarps, 2) k_product_any(const AnyPara
     constexpr int kSize = S::kSize, kC = S::kC, kLine = S::kLine;
     extern __shared__ __align__(16) uint8_t any_smem[];
     uint16_t *sR = reinterpret_cast<uint16_t *>(any_smem), *sF = sR + kAnyRows * kLine;
-    float *sums = reinterpret_cast<float *>(any_smem);
+    float *sums = reinterpret_cast<float *>(any_smem + S::kOperands);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, f0 = blockIdx.x * kAnyF;
     const int wr = (warp & 1) * 32, wf = (warp >> 1) * 32;  // the warp's 32 x 32 of the tile
     // row tiles of all groups in order; this CTA takes every gridDim.y-th
@@ -232,63 +234,69 @@ __global__ void __launch_bounds__(32 * kAnyWarps, 2) k_product_any(const AnyPara
             ef.load(f, p.f_pitch, kFAlong ? nf : left, (kFAlong ? left : nf) * kSize, p.F, p.F_end);
         };
         if (nc > 0) load(0);
-        float acc[2][4][4] = {};  // [16 rows][8 features]
-        for (int c0 = 0; c0 < nc; c0 += kC) {
-            __syncthreads();  // the previous step has been read
-            er.template store<DTYPE>(sR, R, p.r_pitch);
-            ef.template store<DTYPE>(sF, F, p.f_pitch);
-            __syncthreads();
-            const int left = nc - c0;
-            if (c0 + kC < nc) load(c0 + kC);
-            float blk[2][4][4] = {};  // e4m3: of this block
+        int c0 = 0;
+        do {  // at least once: the sums of nothing are zero
+            const int end = c0 + (kF8 ? nc : min(nc - c0, p.segment));
+            const bool first = c0 == 0;
+            float acc[2][4][4] = {};  // [16 rows][8 features]
+            for (; c0 < end; c0 += kC) {
+                __syncthreads();  // the previous step has been read
+                er.template store<DTYPE>(sR, R, p.r_pitch);
+                ef.template store<DTYPE>(sF, F, p.f_pitch);
+                __syncthreads();
+                const int left = nc - c0;
+                if (c0 + kC < nc) load(c0 + kC);
+                float blk[2][4][4] = {};  // e4m3: of this block
 #pragma unroll
-            for (int k = 0; k < kC; k += 16) {
-                if (k >= left) break;
-                uint32_t x[2][4], y[2][4];
+                for (int k = 0; k < kC; k += 16) {
+                    if (k >= left) break;
+                    uint32_t x[2][4], y[2][4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    // rows x contraction: 8 x 8 matrices (0, 0), (8, 0), (0, 8), (8, 8); features: (0, 0), (0, 8), (8, 0), (8, 8)
-                    const int r = wr + 16 * i, f = wf + 16 * i;
-                    if constexpr (kRAlong) ldmatrix4<false>(x[i], sR + (r + (lane & 15)) * kLine + k + 8 * (lane >> 4));
-                    else ldmatrix4<true>(x[i], sR + (k + (lane & 7) + 8 * (lane >> 4)) * kLine + r + 8 * ((lane >> 3) & 1));
-                    if constexpr (kFAlong)
-                        ldmatrix4<false>(y[i], sF + (f + (lane & 7) + 8 * (lane >> 4)) * kLine + k + 8 * ((lane >> 3) & 1));
-                    else
-                        ldmatrix4<true>(y[i], sF + ((f & 64) + k + (lane & 7) + 8 * ((lane >> 3) & 1)) * kLine + (f & 63) + 8 * (lane >> 4));
-                }
+                    for (int i = 0; i < 2; ++i) {
+                        // rows x contraction: 8 x 8 matrices (0, 0), (8, 0), (0, 8), (8, 8); features: (0, 0), (0, 8), (8, 0), (8, 8)
+                        const int r = wr + 16 * i, f = wf + 16 * i;
+                        if constexpr (kRAlong) ldmatrix4<false>(x[i], sR + (r + (lane & 15)) * kLine + k + 8 * (lane >> 4));
+                        else ldmatrix4<true>(x[i], sR + (k + (lane & 7) + 8 * (lane >> 4)) * kLine + r + 8 * ((lane >> 3) & 1));
+                        if constexpr (kFAlong)
+                            ldmatrix4<false>(y[i], sF + (f + (lane & 7) + 8 * (lane >> 4)) * kLine + k + 8 * ((lane >> 3) & 1));
+                        else
+                            ldmatrix4<true>(y[i], sF + ((f & 64) + k + (lane & 7) + 8 * ((lane >> 3) & 1)) * kLine + (f & 63) + 8 * (lane >> 4));
+                    }
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        mma16816<DTYPE == UMSX_DTYPE_BF16>(kF8 ? blk[i][j] : acc[i][j], x[i], y[j >> 1][2 * (j & 1)],
-                                                           y[j >> 1][2 * (j & 1) + 1]);
-            }
-            if constexpr (kF8) {
-                const int cb = c0 / kScaleBlock;
-                const float w = __ldg(p.fs + g * p.fs_group + (int64_t)(f0 / kScaleBlock) * p.fs_row + cb * p.fs_blk);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int r = wr + 16 * i + 8 * h + (lane >> 2);
-                        const float sc = r < nr ? w * __ldg(p.rs + (int64_t)(a + r0 + r) * p.rs_row + cb * p.rs_blk) : 0.0f;
+                    for (int i = 0; i < 2; ++i)
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
+                            mma16816<DTYPE == UMSX_DTYPE_BF16>(kF8 ? blk[i][j] : acc[i][j], x[i], y[j >> 1][2 * (j & 1)],
+                                                               y[j >> 1][2 * (j & 1) + 1]);
+                }
+                if constexpr (kF8) {
+                    const int cb = c0 / kScaleBlock;
+                    const float w = __ldg(p.fs + g * p.fs_group + (int64_t)(f0 / kScaleBlock) * p.fs_row + cb * p.fs_blk);
 #pragma unroll
-                            for (int q = 0; q < 2; ++q)
-                                acc[i][j][2 * h + q] = fmaf(sc, blk[i][j][2 * h + q], acc[i][j][2 * h + q]);
-                    }
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int r = wr + 16 * i + 8 * h + (lane >> 2);
+                            const float sc = r < nr ? w * __ldg(p.rs + (int64_t)(a + r0 + r) * p.rs_row + cb * p.rs_blk) : 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                                for (int q = 0; q < 2; ++q)
+                                    acc[i][j][2 * h + q] = fmaf(sc, blk[i][j][2 * h + q], acc[i][j][2 * h + q]);
+                        }
+                }
             }
-        }
-        __syncthreads();  // the operands have been read
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    *reinterpret_cast<float2 *>(sums + (wr + 16 * i + 8 * h + (lane >> 2)) * kSumLine + wf + 8 * j + 2 * (lane & 3)) =
-                        make_float2(acc[i][j][2 * h], acc[i][j][2 * h + 1]);
+                    for (int j = 0; j < 4; ++j) {
+                        float2 *to = reinterpret_cast<float2 *>(sums + (wr + 16 * i + 8 * h + (lane >> 2)) * kSumLine + wf + 8 * j + 2 * (lane & 3));
+                        const float2 had = first ? make_float2(0.0f, 0.0f) : *to;
+                        *to = make_float2(had.x + acc[i][j][2 * h], had.y + acc[i][j][2 * h + 1]);
+                    }
+        } while (c0 < nc);
         __syncthreads();
         for (int r = warp; r < nr; r += kAnyWarps) {
             const int64_t at = (dw ? g * p.out_group + (int64_t)(r0 + r) * p.ldo : (int64_t)(a + r0 + r) * p.ldo) + f0;
@@ -321,6 +329,7 @@ int launch_product_any(const Product &p, int sms, cudaStream_t s) {
     AnyParams a{};
     a.out_dtype = p.out_dtype;
     a.groups = p.groups;
+    a.segment = (p.out_dtype == UMSX_DTYPE_F32 ? kAccumulate32 : kAccumulate16);
     a.rows = p.rows;
     a.offsets = p.offsets;
     a.features = p.features();

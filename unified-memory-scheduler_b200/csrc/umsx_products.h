@@ -19,6 +19,9 @@ enum ProductMode { kForward = 0, kGradInput = 1, kGradWeight = 2 };
 
 constexpr int kMaxGroups = 1024;
 constexpr int64_t kMaxRows = (1ll << 31) - 512;  // a row plus a tile of rows, or a step of the contraction, is an int
+// Contraction of 16-bit operands that shares a tensor-core accumulator, for fp32 and for 16-bit outputs, whose last rounding hides
+// an error of 2^-15 of the value (25 units of 2^-23 for each 512 at worst, half an f16's unit is 2^-11).
+constexpr int kAccumulate32 = 512, kAccumulate16 = 4096;
 constexpr int kScaleBlock = 128;  // values that share one scale of an e4m3 operand
 
 struct Product {

@@ -7,7 +7,8 @@
 // Each lane loads 16 bytes of a weight row straight into the registers of mma.sync, U steps ahead.  A fragment wants
 // elements (2t, 2t+1, 2t+8, 2t+9) of 16; any other eight of the contraction do as well if both operands use the same ones, so
 // lane t takes eight neighbours and feeds two MMAs with them.  e4m3 codes become f16 (exact) and the fp32 sums of a
-// block of 128 are scaled once.  The eight warps' sums are added in a fixed order.
+// block of 128 are scaled once; 16-bit operands get a fresh accumulator every U steps (at most 256 of the contraction), added up
+// in fp32, since the tensor cores add less exactly than fp32 additions round.  The eight warps' sums are added in a fixed order.
 //
 // Bound: memory (e4m3, 96 rows over 64 experts of 2816 x 2048: 61 us, 4.9 TB/s, 75 % of a copy's rate).  The tcgen05
 // kernel's tiles of 128 or 256 features leave SMs without work here (8 experts of 1536 features: 48 tiles for 74 pairs) and
@@ -140,6 +141,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_product_few(const FewParams 
                         xs[u][t][j] = __ldg(p.xs + (int64_t)(row0 + min(8 * t + 2 * tl + j, rows - 1)) * p.xs_row + blk * p.xs_blk);
             }
         }
+        float seg[NT][4] = {};  // 16-bit: of these steps
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -156,9 +158,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2) k_product_few(const FewParams 
                     acc[t][3] = fmaf(d[3], c1, acc[t][3]);
                 } else {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) multiply<DTYPE>(acc[t], wa[u][h], wb[u][h], xv[u][t][h]);
+                    for (int h = 0; h < 2; ++h) multiply<DTYPE>(seg[t], wa[u][h], wb[u][h], xv[u][t][h]);
                 }
             }
+        if constexpr (!kF8)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][i] += seg[t][i];
     }
     // part[warp][row][feature]
 #pragma unroll
