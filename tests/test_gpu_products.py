@@ -780,3 +780,16 @@ def test_long_contractions_of_few_rows(rows, dtype):
     x, w = _grows(g, rows, c, dtype=dtype), _grows(g, 1, 48, c, dtype=dtype)
     y = U.grouped_mm(x, w, _offsets([rows]), out_dtype=F32)
     _long_close(y, x.double() @ w[0].double().T, 256, c // (8 * 128) + 8, "y")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_long_contractions_of_16_bit_outputs(dtype):
+    """The tcgen05 kernel with 16-bit outputs: 4,096 of the contraction in one accumulator, in every direction."""
+    g, c = _gen(53), 1 << 20
+    dy, x, off = _grows(g, c, 64, dtype=dtype), _grows(g, c, 64, dtype=dtype) * 2.0 ** -8, _offsets([c])
+    _long_close(U.grouped_mm_dw(dy, x, off, out_dtype=dtype)[0], dy.double().T @ x.double(), 4096, c // 4096, "dw")
+    c, off = 1 << 17, _offsets([1100])
+    x, w = _grows(g, 1100, c, dtype=dtype) * 2.0 ** -6, _grows(g, 1, 128, c, dtype=dtype)
+    _long_close(U.grouped_mm(x, w, off), x.double() @ w[0].double().T, 4096, c // 4096, "y")
+    dy, w = _grows(g, 1100, c, dtype=dtype) * 2.0 ** -6, _grows(g, 1, c, 128, dtype=dtype)
+    _long_close(U.grouped_mm_dx(dy, w, off), dy.double() @ w[0].double(), 4096, c // 4096, "dx")

@@ -18,7 +18,8 @@
 //
 // An accumulator of the tensor cores is less exact than rounded fp32 additions, the more so the longer it is added to (error
 // 2.5e-6 of the result at a contraction of 2048, against 0.8e-6).  Outputs in fp32 therefore get a fresh accumulator
-// every kSegment stages, which the epilogue adds up in registers; in 16-bit outputs the last rounding hides it.
+// every 512 of the contraction (kAccumulate32), which the epilogue adds up in registers.  In 16-bit outputs the last
+// rounding hides 4096 of it (kAccumulate16), not any length: in one accumulator an f16 dw of 2^20 rows was 6.4e-3 of the value off.
 //
 // dw's contraction ends inside a block of 64 rows; the rows behind it belong to the next group.  Warp
 // 10 zeroes them in both operands (a zero in one would leave 0 * NaN) up to the next multiple of 16, where
@@ -48,7 +49,6 @@ constexpr int kRowsMax = 256;       // rows of a tile (of a pair: 128 in each CT
 constexpr int kRowBox = 32;         // rows of one K-major TMA box
 constexpr int kThreads = 352, kEpilogueWarps = 8;
 constexpr uint32_t kTmemCols = 512;
-constexpr int kSegment = 8;  // stages that share an accumulator where the output is fp32: 512 of the contraction
 constexpr int kStageRow = 80;  // bytes of a staged output row: 64 of data; 80 spreads eight rows over all banks
 
 struct TcParams {
@@ -901,7 +901,7 @@ int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
     t.vec = aligned(p.out, p.ldo, 2) && p.out_stride % 8 == 0;
     t.fault_cta = p.fault_cta;
     t.wait_limit = p.wait_limit ? p.wait_limit : tc::kPairWaitCycles;
-    t.segment = p.out_dtype == UMSX_DTYPE_F32 ? kSegment : 0x7fffffff;
+    t.segment = (p.out_dtype == UMSX_DTYPE_F32 ? kAccumulate32 : kAccumulate16) / kBC;
     if (p.dtype == UMSX_DTYPE_E4M3) {
         const F8Params fp{t, p.xs, p.ws, p.xs_row, p.xs_blk, p.ws_row, p.ws_blk, p.ws_group};
         return launch_f8(mf, mr, fp, sms, s);
