@@ -793,3 +793,20 @@ def test_long_contractions_of_16_bit_outputs(dtype):
     _long_close(U.grouped_mm(x, w, off), x.double() @ w[0].double().T, 4096, c // 4096, "y")
     dy, w = _grows(g, 1100, c, dtype=dtype) * 2.0 ** -6, _grows(g, 1, c, 128, dtype=dtype)
     _long_close(U.grouped_mm_dx(dy, w, off), dy.double() @ w[0].double(), 4096, c // 4096, "dx")
+
+
+def test_a_ragged_end_far_ahead_is_waited_for():
+    """A weight gradient whose groups end at multiples of 16 rows but for the last: the warp that zeroes a ragged end waits for it
+    from the start, for several times the limit of 0.1 ms (200,000 cycles), to which no other wait comes near."""
+    counts = [64] * 1023 + [30]
+    x, dy, _, off = _case(counts, 0, 0, 1024, 1024, BF16, seed=41)
+    want = U.grouped_mm_dw(dy, x, off)
+    U.products_status()
+    start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    U.products_inject_fault(1 << 20, wait_limit_cycles=200_000)
+    start.record()
+    got = U.grouped_mm_dw(dy, x, off)
+    end.record()
+    U.products_status()
+    assert torch.equal(got, want)
+    assert start.elapsed_time(end) > 0.3, "the call was too short to show anything"

@@ -195,18 +195,18 @@ struct GiveUp {
     long long limit;  // SM cycles
 };
 
-#define UMSX_WAIT(sem)                                                                                            \
+#define UMSX_WAIT(sem, scale, ...)                                                                                \
     asm volatile(                                                                                                 \
         "{\n\t.reg .pred p, q;\n\t.reg .b32 g;\n\t.reg .b64 t0, t, m;\n\tmov.u32 %0, 0;\n\t"                      \
         "mbarrier.try_wait.parity" sem ".shared::cta.b64 p, [%1], %2;\n\t"                                        \
         "@p bra DONE;\n\tmov.u64 t0, %%clock64;\n"                                                               \
         "AGAIN:\n\tmbarrier.try_wait.parity" sem ".shared::cta.b64 p, [%1], %2;\n\t"                             \
         "@p bra DONE;\n\tld.volatile.shared.b32 g, [%3];\n\tsetp.ne.b32 q, g, 0;\n\t@q bra LOST;\n\t"            \
-        "ld.shared.b64 m, [%3+8];\n\tmov.u64 t, %%clock64;\n\tsub.s64 t, t, t0;\n\t"                            \
+        "ld.shared.b64 m, [%3+8];\n\t" scale "mov.u64 t, %%clock64;\n\tsub.s64 t, t, t0;\n\t"                  \
         "setp.lt.s64 q, t, m;\n\t@q bra AGAIN;\n\tst.volatile.shared.b32 [%3], 1;\n"                            \
         "LOST:\n\tmov.u32 %0, 1;\nDONE:\n\t}"                                                                  \
         : "=&r"(lost)                                                                                             \
-        : "r"(bar), "r"(parity), "r"(give_up)                                                                     \
+        : "r"(bar), "r"(parity), "r"(give_up) __VA_ARGS__                                                         \
         : "memory")
 
 // Whether all lanes of the (converged) warp saw the phase complete.  Where they did not, the warp leaves its loops before it
@@ -217,8 +217,14 @@ struct GiveUp {
 template <bool ACROSS = false>
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, uint32_t give_up) {
     uint32_t lost;
-    if constexpr (ACROSS) UMSX_WAIT(".acquire.cluster");
-    else UMSX_WAIT("");
+    if constexpr (ACROSS) UMSX_WAIT(".acquire.cluster", "");
+    else UMSX_WAIT("", "");
+    return !__any_sync(kFull, lost);
+}
+// The same for `times` limits.
+__device__ __forceinline__ bool wait_long(uint32_t bar, uint32_t parity, uint32_t give_up, uint32_t times) {
+    uint32_t lost;
+    UMSX_WAIT("", ".reg .b64 n;\n\tcvt.u64.u32 n, %4;\n\tmul.lo.s64 m, m, n;\n\t", , "r"(times));
     return !__any_sync(kFull, lost);
 }
 #undef UMSX_WAIT

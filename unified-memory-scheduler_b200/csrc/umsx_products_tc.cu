@@ -452,17 +452,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_product_tc(const __grid_constan
                 }
         }
     } else if (MODE == kGradWeight) {
-        uint32_t it = 0, tail_phase = 0;
+        // This warp passes over tiles without a ragged end and waits for the next one that has one, however far ahead; the
+        // epilogue waits for every accumulator up to there, so it may wait for as many limits.
+        uint32_t s_next = 0, tail_phase = 0, limits = 1;
         int group = 0;
         for (int t = cluster; t < total && !stop(); t += clusters) {
             const Tile x = tiles.get(t, group, lane);
             const int kb = (x.c_len + kBC - 1) / kBC;
             if (!x.rows) continue;
-            it += kb;
+            s_next = (s_next + kb) % S::kStages;
+            limits += (kb - 1) / p.segment + 1;
             if (!(x.c_len & 15)) continue;
-            const int boxes = (x.n / kPair + 63) / 64, s = (it - 1) % S::kStages;
-            if (!tc::wait(b_tail + 8 * s, tail_phase >> s & 1u, up)) break;
+            const int boxes = (x.n / kPair + 63) / 64, s = (s_next + S::kStages - 1) % S::kStages;
+            if (!tc::wait_long(b_tail + 8 * s, tail_phase >> s & 1u, up, limits)) break;
             tail_phase ^= 1u << s;
+            limits = 1;
             // lines (one contraction row each) from `valid` up to the last multiple of 16 that the MMAs read
             const int valid = x.c_len - (kb - 1) * kBC, lines = 16 - (valid & 15);
             for (int i = lane; i < (2 + boxes) * lines * 8; i += 32) {
