@@ -810,3 +810,104 @@ def test_a_ragged_end_far_ahead_is_waited_for():
     U.products_status()
     assert torch.equal(got, want)
     assert start.elapsed_time(end) > 0.3, "the call was too short to show anything"
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_long_contractions_in_fp32_on_tcgen05(dtype):
+    """The tcgen05 kernel with fp32 outputs (more than 1024 rows, or a gradient): 512 of the contraction in one accumulator."""
+    g, c = _gen(54), 1 << 16
+    off = _offsets([700, 400])
+    x, w = _grows(g, 1100, c, dtype=dtype), _grows(g, 2, 128, c, dtype=dtype)
+    y = U.grouped_mm(x, w, off, out_dtype=F32)
+    dy, v = _grows(g, 1100, c, dtype=dtype), _grows(g, 2, c, 128, dtype=dtype)
+    dx = U.grouped_mm_dx(dy, v, off, out_dtype=F32)
+    for e, (i, j) in _spans(off):
+        _long_close(y[i:j], x[i:j].double() @ w[e].double().T, 512, c // 512, "y")
+        _long_close(dx[i:j], dy[i:j].double() @ v[e].double(), 512, c // 512, "dx")
+    dy, x, off = _grows(g, 2 * c, 72, dtype=dtype), _grows(g, 2 * c, 136, dtype=dtype), _offsets([c - 37, c + 37])
+    dw = U.grouped_mm_dw(dy, x, off)
+    for e, (i, j) in _spans(off):
+        _long_close(dw[e], dy[i:j].double().T @ x[i:j].double(), 512, c // 512 + 1, "dw")
+
+
+# ---- the prompt's kernels: more than 1024 rows, aligned ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("out", [F32, BF16, F16])
+@pytest.mark.parametrize("pad", [0, 8])
+def test_types_and_strides_of_prompts(dtype, out, pad):
+    _check_all([640, 0, 5, 500], 1, 2, 192, 320, dtype, out, seed=17, pad=pad)
+
+
+def test_non_finite_values_stay_in_their_rows_of_prompts():
+    """One row of a tile of 256 with a NaN or an infinity, and an expert of NaN between two others, in all three directions."""
+    counts = [600, 700, 7]
+    x, dy, w, off = _case(counts, 0, 0, 128, 256, BF16, seed=12)
+    clean, clean_dx, clean_dw = U.grouped_mm(x, w, off), U.grouped_mm_dx(dy, w, off), U.grouped_mm_dw(dy, x, off)
+    x2, dy2 = x.clone(), dy.clone()
+    x2[605, 3], x2[1299, 0] = float("nan"), float("inf")
+    dy2[605, 5], dy2[1299, 0] = float("nan"), float("inf")
+    y, dx = U.grouped_mm(x2, w, off), U.grouped_mm_dx(dy2, w, off)
+    rows = [r for r in range(x.shape[0]) if r not in (605, 1299)]
+    for got, want in ((y, clean), (dx, clean_dx)):
+        assert torch.equal(got[rows], want[rows]) and torch.isnan(got[605]).all() and not torch.isfinite(got[1299]).any()
+    dw = U.grouped_mm_dw(dy, x2, off)
+    assert torch.equal(dw[0], clean_dw[0]) and torch.equal(dw[2], clean_dw[2])
+    assert torch.isnan(dw[1][:, 3]).all() and torch.equal(dw[1][:, 4:], clean_dw[1][:, 4:])
+    w2 = w.clone()
+    w2[1] = float("nan")
+    for got, want in ((U.grouped_mm(x, w2, off), clean), (U.grouped_mm_dx(dy, w2, off), clean_dx)):
+        assert torch.equal(got[:600], want[:600]) and torch.equal(got[1300:], want[1300:]) and torch.isnan(got[600:1300]).all()
+
+
+def test_fp8_non_finite_codes_stay_in_their_rows_of_prompts():
+    x, xs, w, ws, off = _fp8_case([600, 700, 7], 0, 0, 128, 256, seed=12)
+    clean = U.fp8_grouped_mm(x, xs, w, ws, off)
+    bad = x.view(torch.uint8).clone()
+    bad[605, 3], bad[1299, 200] = 0x7F, 0xFF
+    y = U.fp8_grouped_mm(bad.view(E4M3), xs, w, ws, off)
+    rows = [r for r in range(x.shape[0]) if r not in (605, 1299)]
+    assert torch.equal(y[rows], clean[rows]) and torch.isnan(y[605]).all() and torch.isnan(y[1299]).all()
+    bad = w.view(torch.uint8).clone()
+    bad[1] = 0x7F
+    y = U.fp8_grouped_mm(x, xs, bad.view(E4M3), ws, off)
+    assert torch.equal(y[:600], clean[:600]) and torch.equal(y[1300:], clean[1300:]) and torch.isnan(y[600:1300]).all()
+
+
+def test_same_bits_twice_and_on_other_streams_of_prompts():
+    counts = [900, 0, 341, 77]
+    x, dy, w, off = _case(counts, 0, 3, 256, 1024, BF16, seed=16)
+    xq, xs, wq, ws, _ = _fp8_case(counts, 0, 3, 256, 1024, seed=16)
+
+    def run(stream=None):
+        y = torch.zeros(x.shape[0], 256, dtype=F32, device="cuda")
+        z = torch.zeros_like(y)
+        torch.cuda.synchronize()
+        return (U.grouped_mm(x, w, off, out=y, stream=stream), U.fp8_grouped_mm(xq, xs, wq, ws, off, out=z, stream=stream))
+
+    first = run()
+    side, side2 = torch.cuda.Stream(), torch.cuda.Stream()
+    a, b = run(side), run(side2)  # two calls at once
+    torch.cuda.synchronize()
+    for p, q, r in zip(first, a, b):
+        assert torch.equal(p, q) and torch.equal(p, r)
+
+
+def test_given_stream_orders_new_outputs_of_prompts():
+    x, dy, w, off = _case([700, 441], 0, 0, 256, 384, BF16, seed=26)
+    want = U.grouped_mm(x, w, off)
+    want_dx = U.grouped_mm_dx(want, w, off)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for s in (side, side.cuda_stream):
+        y = U.grouped_mm(x, w, off, stream=s)
+        z = U.grouped_mm_dx(y, w, off, stream=s)
+        side.synchronize()
+        assert torch.equal(y, want) and torch.equal(z, want_dx)
+
+
+def test_status_is_clear_after_prompts():
+    for fn in _tcgen05_calls().values():
+        fn()
+        U.products_status()

@@ -167,3 +167,14 @@ def test_rows_that_the_index_arithmetic_does_not_hold_are_refused(call, rows):
     """A row index plus a tile of 256 rows, or a step of 128 of the contraction, has to fit into 32 bits."""
     assert call(rows=rows) == U.EINVAL
     assert b"rows must be" in U.lib().umsx_last_error()
+
+
+def test_e4m3_ties_go_to_the_even_code():
+    """Halfway between two neighbours of the grid the code with an even last bit is taken, on either side of zero."""
+    codes = torch.arange(256, dtype=torch.uint8)
+    value = codes.view(torch.float8_e4m3fn).float().numpy()
+    for sign in (0, 0x80):
+        for c in range(126):  # 0x7F is NaN
+            mid = np.float32((value[sign + c] + value[sign + c + 1]) / 2)
+            got = int(torch.tensor([mid]).to(torch.float8_e4m3fn).view(torch.uint8)[0])
+            assert got == sign + c + (c & 1), (sign, c)
