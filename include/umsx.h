@@ -420,7 +420,8 @@ umsx_status umsx_grouped_mm_dw(const void *dy, int64_t lddy, const void *x, int6
  * scale = max(amax / 448, 2^-126) with amax over the block's finite values, code = the e4m3 value nearest
  * to x / scale (ties to even); inf and NaN become the NaN code.  x [matrices][rows][cols] (F32, BF16 or
  * F16), q the same shape, one byte each; scale of block (i, j) of matrix m at scales[m * s_stride +
- * i * s_row + j * s_blk]. */
+ * i * s_row + j * s_blk]; strides that give two blocks one address, or interleave other than one dimension inside another, are
+ * refused. */
 umsx_status umsx_fp8_quantize(const void *x, int64_t ldx, int64_t x_stride, int x_dtype, int matrices, int64_t rows,
                               int cols, int block_rows, void *q, int64_t ldq, int64_t q_stride, float *scales,
                               int64_t s_row, int64_t s_blk, int64_t s_stride, umsx_stream stream);

@@ -911,3 +911,21 @@ def test_status_is_clear_after_prompts():
     for fn in _tcgen05_calls().values():
         fn()
         U.products_status()
+
+
+def test_scales_of_any_nested_layout():
+    """Blocks of columns first, rows first, matrices innermost, with gaps; a broadcast one is refused and nothing is written."""
+    x = _rand(_gen(61), 3, 20, 300)
+    q0, s0 = U.fp8_quantize(x)
+    for order in ((0, 1, 2), (0, 2, 1), (1, 2, 0), (2, 1, 0)):
+        shape = [s0.shape[i] for i in order]
+        store = torch.zeros([2 * n for n in shape], device="cuda")
+        view = store[:shape[0], :shape[1], :shape[2]].permute([order.index(i) for i in range(3)])
+        q, s = U.fp8_quantize(x, scales=view)
+        assert torch.equal(s, s0) and torch.equal(q.float(), q0.float())
+    shared = torch.zeros(1, 1, 1, device="cuda")
+    with pytest.raises(U.UmsxError, match="one address"):
+        U.fp8_quantize(x, scales=shared.expand(3, 20, 3))
+    torch.cuda.synchronize()
+    assert not shared.any()
+    U.fp8_quantize(x[0, :1, :100], scales=torch.zeros(1, device="cuda").expand(1, 1))  # one block: no stride counts

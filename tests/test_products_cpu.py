@@ -178,3 +178,12 @@ def test_e4m3_ties_go_to_the_even_code():
             mid = np.float32((value[sign + c] + value[sign + c + 1]) / 2)
             got = int(torch.tensor([mid]).to(torch.float8_e4m3fn).view(torch.uint8)[0])
             assert got == sign + c + (c & 1), (sign, c)
+
+
+@pytest.mark.parametrize("over", [dict(s_row=0), dict(s_row=1, s_blk=9, cols=200, ldx=200, ldq=200, x_stride=2000, q_stride=2000),
+                                  dict(s_stride=0), dict(s_stride=9), dict(s_row=2, s_stride=18), dict(block_rows=128, s_stride=0),
+                                  dict(s_row=0, s_blk=0, s_stride=0, rows=1, matrices=1, cols=129, ldx=129, ldq=129)])
+def test_scales_that_share_an_address_are_refused(over):
+    """matrices 2 x 10 rows x 64 columns unless given otherwise: each block's scale needs an address of its own."""
+    assert _quant(**{**FAR[_quant], **over}) == U.EINVAL
+    assert b"one address" in U.lib().umsx_last_error()

@@ -14,8 +14,10 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <array>
 #include <string>
 #include <type_traits>
+#include <utility>
 
 #include "umsx_device.cuh"
 #include "umsx_internal.h"
@@ -265,6 +267,18 @@ void launch_quant(QuantParams p, int block_rows, int sms, cudaStream_t s) {
     }
 }
 
+// Whether an array's strides give each element an address of its own: from the shortest on, each spans the shorter ones.
+bool distinct(std::array<std::pair<int64_t, int64_t>, 3> dims) {  // (stride, length)
+    std::sort(dims.begin(), dims.end());
+    int64_t span = 0;  // from the first element to the last
+    for (const auto &[stride, length] : dims) {
+        if (length <= 1) continue;
+        if (stride <= span) return false;
+        span += (length - 1) * stride;
+    }
+    return true;
+}
+
 umsx_status fail(umsx_status s, const std::string &msg) {
     record_error(msg.c_str());
     return s;
@@ -290,6 +304,7 @@ extern "C" umsx_status umsx_fp8_quantize(const void *x, int64_t ldx, int64_t x_s
     if (matrices == 0 || rows == 0) return UMSX_OK;
     if (!x || !q || !scales) return fail(UMSX_EINVAL, "null buffer");
     const int64_t br = (rows + block_rows - 1) / block_rows, bc = (cols + kScaleBlock - 1) / kScaleBlock;
+    if (!distinct({{{s_stride, matrices}, {s_row, br}, {s_blk, bc}}})) return fail(UMSX_EINVAL, "the strides of the scales give two blocks one address");
     const Region rx = region(x, x_dtype == UMSX_DTYPE_F32 ? 4 : 2, cols, rows, ldx, matrices, x_stride),
                  rq = region(q, 1, cols, rows, ldq, matrices, q_stride),
                  rs = region(scales, 4, (matrices - 1) * s_stride + (br - 1) * s_row + (bc - 1) * s_blk + 1, 1, 0);
