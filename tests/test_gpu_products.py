@@ -929,3 +929,20 @@ def test_scales_of_any_nested_layout():
     torch.cuda.synchronize()
     assert not shared.any()
     U.fp8_quantize(x[0, :1, :100], scales=torch.zeros(1, device="cuda").expand(1, 1))  # one block: no stride counts
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_tiny_blocks(dtype, block_rows):
+    """Block maxima from 2^-110 to 2^-70, on both sides of where the quotient's residual stops being exact, values down to
+    2^-22 of them: scales and codes as the formula gives them with one rounding each."""
+    g = _gen(71)
+    top = torch.arange(-110, -69, device="cuda").repeat_interleave(128).double()
+    x = torch.exp2(top[:, None] - 22 * torch.rand(top.numel(), 128, generator=g, device="cuda").double())
+    x = (x * torch.where(torch.rand(x.shape, generator=g, device="cuda") < 0.5, -1.0, 1.0)).to(dtype)
+    q, s = U.fp8_quantize(x, block_rows)
+    amax = x.double().abs().view(-1, block_rows, 128).amax((1, 2))
+    want = torch.clamp(amax / 448.0, min=2.0 ** -126).float()
+    assert torch.equal(s[:, 0], want)
+    quotient = (x.double() / want.double().repeat_interleave(block_rows)[:, None]).float()
+    assert torch.equal(q.float(), _round_e4m3(quotient.double()).float())

@@ -114,7 +114,9 @@ __device__ __forceinline__ float quotient(float x, float d, float y) {
     const float q = __fmul_rn(x, y);
     return __fmaf_rn(__fmaf_rn(-q, d, x), y, q);
 }
-constexpr float kPlain = 0x1p-90f;  // smallest block maximum for it
+// Smallest block maximum for it.  The residual is exact down to |x| = 2^-102 (the last bit of q d is at least 2^-149 there);
+// below, x / d is at most 2^-102 * 448 * 2^80 < 2^-13, which no error of an ulp lifts to the 2^-10 where codes begin.
+constexpr float kPlain = 0x1p-80f;
 
 // The same for two values at once (packed fp32 operations); yy, dd: y and -d in both halves.
 __device__ __forceinline__ uint64_t twice(float v) { return (uint64_t)__float_as_uint(v) << 32 | __float_as_uint(v); }
@@ -134,8 +136,7 @@ __device__ __forceinline__ float block_scale(float amax) {
     return fmaxf(__fdiv_rn(amax, 448.0f), 0x1p-126f);
 }
 
-// Codes of a lane's values.  plain: every value is finite and the block's maximum at least kPlain; a value far below
-// it may have a subnormal residual, but then rounds to the code zero either way.
+// Codes of a lane's values.  plain: every value is finite and the block's maximum at least kPlain.
 template <class T>
 __device__ __forceinline__ void store_codes(uint8_t *row, int b, int l, int cols, bool vec, const Values<T> &v, float scale, bool plain) {
     uint32_t w[8];
