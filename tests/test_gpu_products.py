@@ -946,3 +946,18 @@ def test_quantize_tiny_blocks(dtype, block_rows):
     assert torch.equal(s[:, 0], want)
     quotient = (x.double() / want.double().repeat_interleave(block_rows)[:, None]).float()
     assert torch.equal(q.float(), _round_e4m3(quotient.double()).float())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("top", [1.0, 2.0 ** -14, 0.0])
+def test_quantize_keeps_the_sign_of_zero(dtype, block_rows, top):
+    """x / scale of a zero has the zero's sign, and so has a quotient that rounds to zero; in a block of zeros too."""
+    x = torch.zeros(128, 256, device="cuda", dtype=dtype)
+    x[:, 1::2] = -0.0
+    x[:, 0] = x[:, 128] = top
+    x[:, 2], x[:, 3] = top * 2.0 ** -10 / 448, -top * 2.0 ** -11 / 448  # half the smallest code, but for x's own rounding; less
+    q, s = U.fp8_quantize(x, block_rows)
+    value = _round_e4m3((x.double().abs() / max(top / 448, 2.0 ** -126)).float().double()).to(E4M3).view(torch.uint8)
+    sign = torch.where(torch.signbit(x.float()), 0x80, 0).to(torch.uint8)
+    assert torch.equal(q.view(torch.uint8), value | sign)

@@ -118,7 +118,8 @@ __device__ __forceinline__ float quotient(float x, float d, float y) {
 // below, x / d is at most 2^-102 * 448 * 2^80 < 2^-13, which no error of an ulp lifts to the 2^-10 where codes begin.
 constexpr float kPlain = 0x1p-80f;
 
-// The same for two values at once (packed fp32 operations); yy, dd: y and -d in both halves.
+// -x / d for two values at once (packed fp32 operations); yy, dd: -y and d in both halves.  The negative, because a sum of
+// opposite zeros is +0: x = -0 meets one on the way, and its code is to keep the sign.
 __device__ __forceinline__ uint64_t twice(float v) { return (uint64_t)__float_as_uint(v) << 32 | __float_as_uint(v); }
 __device__ __forceinline__ float2 quotients(float a, float b, uint64_t dd, uint64_t yy) {
     uint64_t x, q, r;
@@ -141,13 +142,13 @@ template <class T>
 __device__ __forceinline__ void store_codes(uint8_t *row, int b, int l, int cols, bool vec, const Values<T> &v, float scale, bool plain) {
     uint32_t w[8];
     if (plain) {
-        const uint64_t yy = twice(__frcp_rn(scale)), dd = twice(-scale);
+        const uint64_t yy = twice(-__frcp_rn(scale)), dd = twice(scale);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float2 a = quotients(v.value(4 * i), v.value(4 * i + 1), dd, yy);
             const float2 b = quotients(v.value(4 * i + 2), v.value(4 * i + 3), dd, yy);
-            w[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
-                   (uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16;
+            w[i] = ((uint32_t)__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3) |
+                    (uint32_t)__nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3) << 16) ^ 0x80808080u;
         }
     } else {
 #pragma unroll
