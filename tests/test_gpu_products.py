@@ -961,3 +961,58 @@ def test_quantize_keeps_the_sign_of_zero(dtype, block_rows, top):
     value = _round_e4m3((x.double().abs() / max(top / 448, 2.0 ** -126)).float().double()).to(E4M3).view(torch.uint8)
     sign = torch.where(torch.signbit(x.float()), 0x80, 0).to(torch.uint8)
     assert torch.equal(q.view(torch.uint8), value | sign)
+
+
+# ---- autograd --------------------------------------------------------------------------------------------
+
+
+def test_a_gradient_that_would_be_lost_is_warned_about():
+    import warnings
+    x, dy, w, off = _case([3, 4], 0, 0, 64, 32, BF16, seed=1)
+    xq, xs, wq, ws, _ = _fp8_case([3, 4], 0, 0, 64, 32, seed=1)
+    need = [t.clone().requires_grad_() for t in (x, w, dy, xs)]
+    calls = [lambda: U.grouped_mm(need[0], w, off), lambda: U.grouped_mm(x, need[1], off), lambda: U.grouped_mm_dx(need[2], w, off),
+             lambda: U.grouped_mm_dw(need[2], x, off), lambda: U.fp8_quantize(need[0])[0],
+             lambda: U.fp8_grouped_mm(xq, need[3], wq, ws, off), lambda: U.fp8_mm(xq, need[3], wq[0], ws[0])]
+    for call in calls:
+        with pytest.warns(UserWarning, match="autograd"):
+            got = call()
+        assert not got.requires_grad
+        with warnings.catch_warnings(), torch.no_grad():
+            warnings.simplefilter("error")
+            assert torch.equal(call().float(), got.float())
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        U.grouped_mm(x, w, off)
+
+
+class _GroupedMM(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, off):
+        ctx.save_for_backward(x, w, off)
+        return U.grouped_mm(x, w, off, out=x.new_zeros(x.shape[0], w.shape[1]))
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, w, off = ctx.saved_tensors
+        dy = dy.contiguous()
+        return U.grouped_mm_dx(dy, w, off, out=torch.zeros_like(x)), U.grouped_mm_dw(dy, x, off, out_dtype=w.dtype), None
+
+
+def test_products_joined_in_an_autograd_function():
+    import warnings
+    x, dy, w, off = _case([30, 0, 41], 0, 0, 64, 96, BF16, seed=81)
+    x = torch.cat([x, _rand(_gen(82), 5, 96)])  # five rows of no group
+    dy = torch.cat([dy, _rand(_gen(83), 5, 64)])
+    x.requires_grad_(), w.requires_grad_()
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        y = _GroupedMM.apply(x, w, off)
+        y.backward(dy)
+    assert not y[71:].any() and not x.grad[71:].any()
+    x, w, dx, dw = x.detach().double(), w.detach().double(), x.grad, w.grad
+    for e, (i, j) in _spans(off):
+        dye = dy[i:j].double()
+        _close(y[i:j].detach(), x[i:j] @ w[e].T, x[i:j].abs() @ w[e].abs().T, 96, "y")
+        _close(dx[i:j], dye @ w[e], dye.abs() @ w[e].abs(), 64, "dx")
+        _close(dw[e], dye.T @ x[i:j], dye.abs().T @ x[i:j].abs(), j - i, "dw")

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import warnings
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(PKG, "libumsx.so")
@@ -239,9 +240,9 @@ def route_static(x, router_w, router_b, experts: int, top_k: int, routing: int, 
 
 # ---- products over caller-owned expert weights --------------------------------------------------------
 #
-# Plain functions of CUDA tensors: they take no part in autograd (the gradients are functions of their own) and
-# write new tensors or the `out` given, on the current stream of the tensors' device or on `stream` (a torch stream or a
-# cudaStream_t).
+# Plain functions of CUDA tensors: they take no part in autograd (the gradients are functions of their own, and an
+# operand that requires one is warned about) and write new tensors or the `out` given, on the current stream of the
+# tensors' device or on `stream` (a torch stream or a cudaStream_t).
 
 _CODES = {}  # torch dtype -> UMSX_DTYPE_*, filled on first use (torch is imported lazily)
 _TORCH = None
@@ -331,9 +332,15 @@ def _out_arg(name, out, shape, dtype, like, default, stream):
 def _call(entry, tensors, stream, *args):
     """entry(*args, stream) on the tensors' device, which is the current one for the call; the stream given, or that
     device's current one.  A stream that is given is one more that uses the tensors: their memory is not handed out again
-    before it is done with them."""
+    before it is done with them.  A gradient that would be lost here is warned about."""
     index = tensors[0].device.index
     cuda = _TORCH.cuda
+    for t in tensors:
+        if t.requires_grad and _TORCH.is_grad_enabled():
+            warnings.warn("a tensor given requires a gradient, but the products take no part in autograd: the result is detached "
+                          "(grouped_mm_dx and grouped_mm_dw are grouped_mm's gradients; torch.no_grad() or detach() says that "
+                          "none is wanted)", stacklevel=3)
+            break
     before = cuda.current_device()
     if stream is None:
         s = _RAW_STREAM(index)
@@ -379,7 +386,8 @@ def grouped_mm(x, w, offsets, out=None, out_dtype=None, stream=None):
     """out[r] = x[r] @ w[e].T for the rows r of every expert e (umsx_grouped_mm): x [rows, k] and w
     [experts, n, k] both bfloat16 or both float16, offsets int32 [experts + 1]; out [rows, n] float32,
     bfloat16 or float16 (default: x's type).  Rows outside the groups are not written.  As in its gradients and the
-    e4m3 products, an `out` that overlaps an operand is refused."""
+    e4m3 products, an `out` that overlaps an operand is refused.  The result is detached from autograd: an autograd.Function
+    that calls this forward, and grouped_mm_dx and grouped_mm_dw backward, gives it its gradients."""
     _torch()
     code = _matrix("x", x, 2, _SIXTEEN)
     _matrix("w", w, 3, (code,), x)
