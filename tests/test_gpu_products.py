@@ -1016,3 +1016,25 @@ def test_products_joined_in_an_autograd_function():
         _close(y[i:j].detach(), x[i:j] @ w[e].T, x[i:j].abs() @ w[e].abs().T, 96, "y")
         _close(dx[i:j], dye @ w[e], dye.abs() @ w[e].abs(), 64, "dx")
         _close(dw[e], dye.T @ x[i:j], dye.abs().T @ x[i:j].abs(), j - i, "dw")
+
+
+def test_an_error_is_reported_by_its_own_call_only():
+    """A call that fails in the CUDA runtime (a status query, which synchronises, on a stream that is being captured) leaves
+    nothing that a later, sound one reports."""
+    rt = pytest.importorskip("cuda.bindings.runtime")
+    x, dy, w, off = _case([3, 4], 0, 0, 64, 32, BF16, seed=1)
+    ids = torch.zeros(4, 2, dtype=torch.int32, device="cuda")
+    xb, rw = _rand(_gen(2), 4, 64), torch.zeros(8, 64, device="cuda")
+    calls = [lambda: U.grouped_mm(x, w, off), lambda: U.grouped_mm_dx(dy, w, off), lambda: U.fp8_quantize(x),
+             lambda: U.group_rows(ids, 4), lambda: U.route_static(xb, rw, None, 8, 2, U.ROUTE_SOFTMAX_TOPK_NORM)]
+    for call in calls:
+        call()
+        side = torch.cuda.Stream()
+        assert int(rt.cudaStreamBeginCapture(side.cuda_stream, rt.cudaStreamCaptureMode.cudaStreamCaptureModeThreadLocal)[0]) == 0
+        with pytest.raises(U.UmsxError) as e:
+            U.products_status(side)
+        assert e.value.status == U.EDEVICE
+        rt.cudaStreamEndCapture(side.cuda_stream)  # the capture is void
+        call()
+    torch.cuda.synchronize()
+    U.products_status()

@@ -31,7 +31,10 @@ umsx_status fail(umsx_status s, const std::string &msg) {
 #define UMSX_CUDA(call)                                                                        \
     do {                                                                                       \
         cudaError_t err_ = (call);                                                             \
-        if (err_ != cudaSuccess) return fail(UMSX_EDEVICE, std::string(#call) + ": " + cudaGetErrorString(err_)); \
+        if (err_ != cudaSuccess) {                                                             \
+            (void)cudaGetLastError(); /* reported here, not by the next launch's check */      \
+            return fail(UMSX_EDEVICE, std::string(#call) + ": " + cudaGetErrorString(err_));   \
+        }                                                                                      \
     } while (0)
 
 #define UMSX_LAUNCHED(n)                                                                       \

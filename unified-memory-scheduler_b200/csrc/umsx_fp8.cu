@@ -326,6 +326,7 @@ extern "C" umsx_status umsx_fp8_quantize(const void *x, int64_t ldx, int64_t x_s
     p.vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && ldx * size % 16 == 0 && x_stride * size % 16 == 0 &&
             reinterpret_cast<uintptr_t>(q) % 8 == 0 && ldq % 8 == 0 && q_stride % 8 == 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    (void)cudaGetLastError();  // an earlier call's error is not this launch's
     if (x_dtype == UMSX_DTYPE_F32) launch_quant<float>(p, block_rows, sms, s);
     else if (x_dtype == UMSX_DTYPE_BF16) launch_quant<__nv_bfloat16>(p, block_rows, sms, s);
     else launch_quant<__half>(p, block_rows, sms, s);

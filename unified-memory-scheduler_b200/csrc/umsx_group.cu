@@ -245,7 +245,10 @@ extern "C" umsx_status umsx_group_rows(const int32_t *ids, int tokens, int top_k
         at[0].val.clusterDim.x = ctas;
         e = cudaLaunchKernelEx(&cfg, kernel, ids, jobs, top_k, experts, (int)sort_local, offsets, row_token, row_of_job);
     }
-    if (e != cudaSuccess) return fail(UMSX_EDEVICE, std::string("group_rows launch: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();  // reported here, not by the next launch's check
+        return fail(UMSX_EDEVICE, std::string("group_rows launch: ") + cudaGetErrorString(e));
+    }
     record_launches(1);
     return UMSX_OK;
 }

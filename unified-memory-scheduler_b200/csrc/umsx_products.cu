@@ -408,6 +408,7 @@ umsx_status run_product(Product &p, umsx_stream stream) {
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return fail(UMSX_EDEVICE, std::string("device query: ") + cudaGetErrorString(e));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    (void)cudaGetLastError();  // an earlier call's error is not this launch's
     const bool few = product_few_takes(p), tc = !few && product_tc_takes(p);
     if (tc) p.fault_cta = g_fault.cta, p.wait_limit = g_fault.wait_limit, g_fault = Fault{};
     const int n = few ? launch_product_few(p, sms, s)
@@ -509,7 +510,10 @@ umsx_status umsx_products_status(umsx_stream stream) {
     cudaError_t e = cudaMemcpyAsync(&v, word, sizeof v, cudaMemcpyDeviceToHost, s);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s);
     if (e == cudaSuccess && v) e = cudaMemsetAsync(word, 0, sizeof v, s);
-    if (e != cudaSuccess) return fail(UMSX_EDEVICE, std::string("products status: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess) {
+        (void)cudaGetLastError();  // reported here, not by the next launch's check
+        return fail(UMSX_EDEVICE, std::string("products status: ") + cudaGetErrorString(e));
+    }
     return v ? fail(UMSX_ETIMEOUT, "a bounded wait of a product's kernel gave up: its output is not complete") : UMSX_OK;
 }
 
