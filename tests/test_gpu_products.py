@@ -1038,3 +1038,54 @@ def test_an_error_is_reported_by_its_own_call_only():
         call()
     torch.cuda.synchronize()
     U.products_status()
+
+
+# ---- odd widths in padded buffers -------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("counts", [[640, 0, 5, 500], [3, 0, 7, 1], [70, 9]])
+@pytest.mark.parametrize("out", [F32, F16])
+def test_odd_widths_with_aligned_rows(counts, out):
+    """Rows that start at multiples of 16 bytes but end between them: the tensor cores' kernels take them, and NaN in the padding
+    reaches nothing.  Outputs are columns of a wider buffer too, whose padding stays as it was."""
+    for n, k in ((193, 321), (33, 65), (17, 129)):
+        x, dy, w, off = _case(counts, 1, 2, n, k, F16, seed=n, pad=7)  # rows of n + 7 and k + 7
+        w._base[:, :, k:] = float("nan")
+        rows = x.shape[0]
+        stores = [torch.full(s, 9.0, dtype=out, device="cuda") for s in ((rows, n + 7), (rows, k + 7), (len(counts), n, k + 7))]
+        y, dx, dw = stores[0][:, :n], stores[1][:, :k], stores[2][:, :, :k]
+        U.grouped_mm(x, w, off, out=y)
+        U.grouped_mm_dx(dy, w, off, out=dx)
+        U.grouped_mm_dw(dy, x, off, out=dw)
+        assert (stores[0][:, n:] == 9).all() and (stores[1][:, k:] == 9).all() and (stores[2][:, :, k:] == 9).all()
+        a, b = 1, 1 + sum(counts)
+        for t in stores[:2]:
+            assert (t[:a] == 9).all() and (t[b:] == 9).all()
+        for e, (i, j) in _spans(off):
+            xe, dye, we = x[i:j].double(), dy[i:j].double(), w[e].double()
+            _close(y[i:j], xe @ we.T, xe.abs() @ we.abs().T, k, "y")
+            _close(dx[i:j], dye @ we, dye.abs() @ we.abs(), n, "dx")
+            _close(dw[e], dye.T @ xe, dye.abs().T @ xe.abs(), j - i, "dw")
+
+
+@pytest.mark.parametrize("counts", [[640, 0, 5, 500], [3, 0, 7, 1], [70, 9]])
+@pytest.mark.parametrize("out", [F32, BF16])
+def test_fp8_odd_widths_with_aligned_rows(counts, out):
+    for n, k in ((193, 321), (130, 129), (17, 145)):
+        x, xs, w, ws, off = _fp8_case(counts, 1, 2, n, k, seed=n, pad=-k % 16)
+        torch.as_strided(w.view(torch.uint8), (len(counts), n, k + -k % 16), w.stride())[:, :, k:] = 0x7F  # NaN
+        store = torch.full((x.shape[0], n + 7), 9.0, dtype=out, device="cuda")
+        U.fp8_grouped_mm(x, xs, w, ws, off, out=store[:, :n])
+        assert (store[:, n:] == 9).all() and (store[:1] == 9).all() and (store[-2:] == 9).all()
+        for e, (i, j) in _spans(off):
+            want, size = _fp8_want(x[i:j], xs[i:j], w[e], ws[e])
+            _close(store[i:j, :n], want, size, k, f"expert {e}")
+
+
+def test_quantize_takes_one_matrix_for_all():
+    """A matrix that is broadcast over the first dimension is read in place."""
+    x = _rand(_gen(91), 1, 30, 200)
+    q0, s0 = U.fp8_quantize(x[0], 128)
+    q, s = U.fp8_quantize(x.expand(3, 30, 200), 128)
+    for i in range(3):
+        assert torch.equal(q[i].float(), q0.float()) and torch.equal(s[i], s0)
