@@ -211,7 +211,9 @@ extern "C" umsx_status umsx_group_rows(const int32_t *ids, int tokens, int top_k
     cfg.attrs = at;
     cfg.numAttrs = 1;
     // One CTA for few jobs, where a cluster's barriers cost more than its SMs save (us in one CTA, in eight; 128 experts: 512
-    // jobs 5.9, 9.3; 1024: 7.1, 9.8; 1536: 8.3, 9.8; 2048: 9.5, 8.9).  Sixteen CTAs, beyond the portable cluster size and
+    // jobs 5.9, 9.3; 1024: 7.1, 9.8; 1536: 8.3, 9.8; 2048: 9.5, 8.9).  The border is that of 128 experts: the counters' scan grows
+    // with the experts and eight CTAs repeat it, so 2048 jobs of 64 experts take 9.5, 7.6, of 256 10.9, 12.0 and of 1024 12.9, 23.4.
+    // Sixteen CTAs, beyond the portable cluster size and
     // only if the device can hold them, for many (in eight, in sixteen, with the warps of then; 2048: 9.0, 10.2; 4096
     // jobs of 256 experts: 13.1, 12.5; 8192: 18.7, 13.4; 131072: 27.3, 23.1).
     int ctas = jobs <= 1536 ? 1 : 8;

@@ -1,5 +1,5 @@
-// Entry points of the ragged products (umsx_grouped_mm and its gradients, umsx_fp8_mm,
-// umsx_fp8_grouped_mm), and the kernel that takes every shape, stride and alignment.
+// Entry points of the ragged products (umsx_grouped_mm and its gradients, umsx_fp8_grouped_mm), and the kernel that takes
+// every shape, stride and alignment.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -32,8 +32,8 @@ umsx_status fail(umsx_status s, const std::string &msg) {
 // in shared memory: the tensor cores add less exactly than fp32 additions round, the more so the longer they add.  From there a
 // warp stores 32 neighbours.
 // Bound by the latency of a step where there are few tiles (e4m3 511 x 308 x 1323: 24 tiles, 37 us; with steps of 32 values
-// 80), by issue where there are many: bf16 4096 x 4096 x 2049 takes 481 us forward (143 TFLOP/s), 522 for dx, 514 for dw, e4m3
-// 446; with single-element loads 573, 784, 891 and 1116, and with a test in front of every load and shift 778 forward.
+// 80), by issue where there are many: bf16 4096 x 4096 x 2049 takes 483 us forward (142 TFLOP/s), 522 for dx, 508 for dw
+// (500, 523 for fp32 outputs, forward and dw), e4m3 446; with single-element loads 573, 784, 891 and 1116, and with a test in front of every load and shift 778 forward.
 
 constexpr int kAnyRows = 64, kAnyF = 128, kLineBytes = 128, kAnyWarps = 8;
 constexpr int kSumLine = kAnyF + 8;  // a half warp's pairs of sums lie in different banks

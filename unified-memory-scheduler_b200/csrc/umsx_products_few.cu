@@ -204,7 +204,10 @@ void launch(const FewParams &p, int nt, int64_t chunks, cudaStream_t s) {
 // and 123 / 125, 6 rows 88 / 88, 8 rows in bf16 160 / 147).  Up to 2^17 outputs: the other has few tiles, each alone with its
 // contraction, which this one splits over eight warps (us, bf16; 57 rows of 640 x 9728: 19.5 / 39.9, 256 of 136 x 5648: 13.3 /
 // 35.8, 64 of 640 x 128: 8.2 / 10.2, 8 x 8 of 1536 x 2048: 18.5 / 22.6, 128 of 1024 x 4096: 21.5 / 23.6); with more of them it
-// reads the weights too often (8 x 32 of 1536 x 2048: 30.8 / 22.5, 128 of 2048 x 4096: 37.9 / 25.6).
+// reads the weights too often (8 x 32 of 1536 x 2048: 30.8 / 22.5, 128 of 2048 x 4096: 37.9 / 25.6).  e4m3, with half the bytes,
+// changes over a little later (the same seven: 18.5 / 43.0, 12.3 / 36.9, 8.2 / 10.3, 16.4 / 16.4, 19.5 / 28.7, then
+// 26.6 / 18.4 and 30.7 / 26.6; between them 256 of 640 x 9728, 160 K outputs: 38.9 / 55.3, in bf16 47.1 / 55.3).  The rows of the longest group are not known on
+// the host: where one of many experts gets them all, its weights are read once for every eight or sixteen.
 static int few_tiles(const Product &p) {
     const double mean = (double)p.rows / p.groups;
     if (p.rows > 1024) return 0;  // one expert may have got them all, and is then read rows / 8 times

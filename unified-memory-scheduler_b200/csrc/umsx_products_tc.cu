@@ -12,8 +12,9 @@
 // One persistent CTA pair per two SMs; pair i takes tiles i, i + pairs, ... of the list (group, feature
 // tile, row tile), which every CTA derives from the offsets, so there is no scheduler state and the order of
 // sums is fixed.  A pair's CTA reads half the rows' operand; single CTAs with tiles of 128 x 256 took 406, 401 and 500 us
-// for forward, dx and dw where pairs take 356, 388 and 426 (bf16, 32 experts of 512 rows, 5760 x 2880), and were no
-// faster for 128 features or fewer either (16 x 1024 rows, 128 x 2048: both 27 to 31 us).  Roles: warp 0 TMA, warp 1 MMA, warps 2-9 epilogue, warp 10 (dw) the group's ragged end.
+// for forward, dx and dw where pairs took 356, 388 and 426 (bf16, 32 experts of 512 rows, 5760 x 2880; now, on another card,
+// 363, 397 and 437), and were no faster for 128 features or fewer either (16 x 1024 rows, 128 x 2048: both 27 to 31 us).
+// Roles: warp 0 TMA, warp 1 MMA, warps 2-9 epilogue, warp 10 (dw) the group's ragged end.
 // Two accumulators of 256 columns: the epilogue drains one while the MMA fills the other.
 //
 // An accumulator of the tensor cores is less exact than rounded fp32 additions, the more so the longer it is added to (error
@@ -179,7 +180,7 @@ __device__ __forceinline__ void stage16(uint8_t *to, int lane, const uint32_t (&
 
 // Rows c0 .. c0 + 15 of the tile from v (fragment order), through the warp's staging of 16 rows.  RUNS: where 16-byte
 // stores cannot be used, a store of 32 neighbours for each row, not eight elements of a row by each lane (bf16 5759 x 2880, 32
-// experts of 512 rows: 365 us, 600; e4m3 346, 668).  Not for dw, whose width is odd only where an operand is too, unless that
+// experts of 512 rows: 365 us, now 377, and 600; e4m3 346, 668).  Not for dw, whose width is odd only where an operand is too, unless that
 // is padded: the code's registers cost its fp32 outputs 5 %.
 template <bool RUNS>
 __device__ __forceinline__ void store_chunk(const OutTile &o, uint8_t *stage, int lane, int c0, const uint32_t (&v)[16]) {
