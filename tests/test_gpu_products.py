@@ -1089,3 +1089,24 @@ def test_quantize_takes_one_matrix_for_all():
     q, s = U.fp8_quantize(x.expand(3, 30, 200), 128)
     for i in range(3):
         assert torch.equal(q[i].float(), q0.float()) and torch.equal(s[i], s0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("block_rows", [1, 128])
+def test_quantize_ties_go_to_the_even_code(dtype, block_rows):
+    """Every midpoint of two neighbouring e4m3 values, beside a 448 that makes the scale one, and the same times 2^-5."""
+    value = torch.arange(127, dtype=torch.uint8, device="cuda").view(E4M3).float()
+    x = torch.zeros(4, 128, device="cuda")
+    x[:, 0] = 448.0
+    x[0, 1:127] = (value[:-1] + value[1:]) / 2
+    x[1, 1:127] = -x[0, 1:127]
+    x[2:] = x[:2] * 2.0 ** -5
+    code = torch.arange(126, dtype=torch.uint8, device="cuda")
+    even = code + (code & 1)
+    for rows in ((0, 2), (2, 4)):
+        xr = x[rows[0]:rows[1]].to(dtype)
+        assert torch.equal(xr.float(), x[rows[0]:rows[1]])  # exact in every type
+        q, s = U.fp8_quantize(xr, block_rows)
+        assert (s == xr[0, 0].float() / 448).all()
+        q = q.view(torch.uint8)
+        assert torch.equal(q[0, 1:127], even) and torch.equal(q[1, 1:127], even | 0x80)
