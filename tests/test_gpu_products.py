@@ -1110,3 +1110,17 @@ def test_quantize_ties_go_to_the_even_code(dtype, block_rows):
         assert (s == xr[0, 0].float() / 448).all()
         q = q.view(torch.uint8)
         assert torch.equal(q[0, 1:127], even) and torch.equal(q[1, 1:127], even | 0x80)
+
+
+@pytest.mark.parametrize("rows,n,k,pad", [(1100, 128, 1 << 16, 0), (8, 128, 1 << 16, 0), (60, 128, 1 << 16, 0), (70, 65, (1 << 16) + 1, 2)])
+def test_long_contractions_of_e4m3(rows, n, k, pad):
+    """e4m3 in fp32 on the tcgen05 kernel, the streaming one (one and two tiles of eight rows) and that for any alignment: a block
+    of 128 in one accumulator, then a product of two scales and one multiply-add for each block, each rounded once."""
+    g = _gen(95)
+    x = torch.empty(rows, k + pad, dtype=torch.uint8, device="cuda")[:, :k].view(E4M3)
+    x.copy_((torch.rand(rows, k, generator=g, device="cuda") + 0.5).to(E4M3))
+    w = torch.empty(n, k + pad, dtype=torch.uint8, device="cuda")[:, :k].view(E4M3)
+    w.copy_((torch.rand(n, k, generator=g, device="cuda") + 0.5).to(E4M3))
+    xs, ws = _grows(g, _blocks(k), rows, dtype=F32).t(), _grows(g, _blocks(n), _blocks(k), dtype=F32)
+    want, _ = _fp8_want(x, xs, w, ws)
+    _long_close(U.fp8_mm(x, xs, w, ws, out_dtype=F32), want, 128, _blocks(k) + 8 + 1, "y")
