@@ -442,7 +442,7 @@ umsx_status umsx_products_status(umsx_stream stream);
 
 /* Fault injection for failure-detection tests, as umsx_stack_inject_fault: the calling thread's next product that runs on
  * the tcgen05 kernels (umsx_grouped_mm and its gradients, umsx_fp8_grouped_mm; aligned, not a few rows) runs with CTA `cta`
- * withholding its first copies and every wait bounded by wait_limit_cycles SM cycles, so the waits run out, the kernel ends,
+ * withholding its first copies and every wait bounded by wait_limit_cycles SM cycles (at most 2e9), so the waits run out, the kernel ends,
  * its output is not complete and umsx_products_status reports UMSX_ETIMEOUT.  One call only; a CTA without a tile, or beyond
  * the grid, injects nothing, and only the limit counts. */
 umsx_status umsx_products_inject_fault(int cta, int64_t wait_limit_cycles);

@@ -156,7 +156,7 @@ def test_buffers_between_elements_are_refused(call, over):
     assert b"aligned" in U.lib().umsx_last_error()
 
 
-@pytest.mark.parametrize("cta,limit", [(-1, 1000), (0, 0), (0, -5)])
+@pytest.mark.parametrize("cta,limit", [(-1, 1000), (0, 0), (0, -5), (0, 2_000_000_001)])
 def test_bad_fault_injections_are_refused(cta, limit):
     assert U.lib().umsx_products_inject_fault(cta, limit) == U.EINVAL
 

@@ -187,8 +187,7 @@ __device__ __forceinline__ bool elect_one() {
 // complete then ends too, and the loops look at the mark once per tile.  One asm block each (a function with a loop in it took
 // 250 cycles where a phase was complete, a block 50); mark and limit lie in shared memory, where only a wait that is not over
 // at once looks at them.
-constexpr long long kPairWaitCycles = 2000000000ll;       // the usual limit, about a second
-constexpr long long kDrainCycles = kPairWaitCycles / 64;  // for copies and MMAs in flight at the end, which take microseconds
+constexpr long long kDrainCycles = 1ll << 25;  // 17 ms, for copies and MMAs in flight at the end, which take microseconds
 
 struct GiveUp {
     int given_up;

@@ -518,7 +518,8 @@ umsx_status umsx_products_status(umsx_stream stream) {
 }
 
 umsx_status umsx_products_inject_fault(int cta, int64_t wait_limit_cycles) {
-    if (cta < 0 || wait_limit_cycles < 1) return fail(UMSX_EINVAL, "cta must not be negative, wait_limit_cycles must be positive");
+    if (cta < 0 || wait_limit_cycles < 1 || wait_limit_cycles > kWaitCycles)  // a wait may be for many limits: no overflow
+        return fail(UMSX_EINVAL, "cta must not be negative, wait_limit_cycles must be 1..2000000000");
     g_fault = {cta, wait_limit_cycles};
     return UMSX_OK;
 }

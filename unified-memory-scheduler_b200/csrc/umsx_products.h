@@ -22,6 +22,7 @@ constexpr int64_t kMaxRows = (1ll << 31) - 512;  // a row plus a tile of rows, o
 // Contraction of 16-bit operands that shares a tensor-core accumulator, for fp32 and for 16-bit outputs, whose last rounding hides
 // an error of 2^-15 of the value (25 units of 2^-23 for each 512 at worst, half an f16's unit is 2^-11).
 constexpr int kAccumulate32 = 512, kAccumulate16 = 4096;
+constexpr long long kWaitCycles = 2000000000ll;  // limit of a bounded wait, about a second
 constexpr int kScaleBlock = 128;  // values that share one scale of an e4m3 operand
 
 struct Product {

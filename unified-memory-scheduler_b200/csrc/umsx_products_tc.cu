@@ -905,7 +905,7 @@ int launch_product_tc(const Product &p, int sms, cudaStream_t s) {
     t.out_group = p.out_stride;
     t.vec = aligned(p.out, p.ldo, 2) && p.out_stride % 8 == 0;
     t.fault_cta = p.fault_cta;
-    t.wait_limit = p.wait_limit ? p.wait_limit : tc::kPairWaitCycles;
+    t.wait_limit = p.wait_limit ? p.wait_limit : kWaitCycles;
     t.segment = (p.out_dtype == UMSX_DTYPE_F32 ? kAccumulate32 : kAccumulate16) / kBC;
     if (p.dtype == UMSX_DTYPE_E4M3) {
         const F8Params fp{t, p.xs, p.ws, p.xs_row, p.xs_blk, p.ws_row, p.ws_blk, p.ws_group};
